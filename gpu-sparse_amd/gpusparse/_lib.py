@@ -24,7 +24,7 @@ GS_SEARCH_PHASES = 8
 NOALLOC_SCRATCH_BYTES = 256 << 20   # GS_NOALLOC_SCRATCH_BYTES
 PHASE_NAMES = ("query_prep", "heavy_terms", "threshold_seed", "scoring", "candidate_select", "fp64_rescore",
                "final_sort")
-ABI_VERSION = 10
+ABI_VERSION = 11
 
 WTYPE_OF_DTYPE = {torch.float32: GS_W_F32, torch.float16: GS_W_F16, torch.uint8: GS_W_U8}
 
@@ -124,6 +124,46 @@ class GsSynthSpec(C.Structure):
     ]
 
 
+GS_H_F32, GS_H_F16, GS_H_BF16 = 0, 1, 2
+GS_REDUCE_NONE, GS_REDUCE_MEAN, GS_REDUCE_SUM = 0, 1, 2
+HTYPE_OF_DTYPE = {torch.float32: GS_H_F32, torch.float16: GS_H_F16, torch.bfloat16: GS_H_BF16}
+
+
+class GsVocabHead(C.Structure):
+    """Mirror of ``struct gs_vocab_head``."""
+
+    _fields_ = [
+        ("hidden_d", C.c_void_p),
+        ("hidden_text_stride", C.c_int64),
+        ("hidden_row_stride", C.c_int64),
+        ("hidden_dim_stride", C.c_int64),
+        ("weight_d", C.c_void_p),
+        ("weight_row_stride", C.c_int64),
+        ("weight_dim_stride", C.c_int64),
+        ("bias_d", C.c_void_p),
+        ("type", C.c_int32),
+        ("bias_type", C.c_int32),
+        ("texts", C.c_int32),
+        ("length", C.c_int32),
+        ("dim", C.c_int32),
+        ("vocab", C.c_int32),
+    ]
+
+
+class GsVocabTargets(C.Structure):
+    """Mirror of ``struct gs_vocab_targets``."""
+
+    _fields_ = [
+        ("targets_d", C.c_void_p),
+        ("ignore_index", C.c_int64),
+        ("teacher_ids_d", C.c_void_p),
+        ("teacher_logits_d", C.c_void_p),
+        ("teacher_type", C.c_int32),
+        ("top", C.c_int32),
+        ("temperature", C.c_float),
+    ]
+
+
 _P = C.c_void_p
 _I32, _I64, _SZ = C.c_int32, C.c_int64, C.c_size_t
 
@@ -180,6 +220,14 @@ SIGNATURES = {
     "gs_compacted_topk": (C.c_int, [_P, _I64, _I32, _I64, _P, _I32, _I32, _P, _P, _P, _P, _SZ, _P]),
     "gs_scatter_add": (C.c_int, [C.POINTER(GsIndex), _P, _P, _P, _P, _I32, _I32, _P, _I64, _I64, _I64,
                                  _I32, _P]),
+    "gs_term_weights_workspace": (C.c_int, [C.POINTER(GsVocabHead), _I32, C.POINTER(_SZ), C.POINTER(_SZ)]),
+    "gs_term_weights": (C.c_int, [C.POINTER(GsVocabHead), _P, _P, _P, _P, _SZ, _P]),
+    "gs_term_weights_grad": (C.c_int, [C.POINTER(GsVocabHead), _P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
+    "gs_vocab_loss_workspace": (C.c_int, [C.POINTER(GsVocabHead), C.POINTER(GsVocabTargets), C.POINTER(_SZ),
+                                          C.POINTER(_SZ), C.POINTER(_SZ)]),
+    "gs_vocab_loss": (C.c_int, [C.POINTER(GsVocabHead), C.POINTER(GsVocabTargets), _I32, _P, _P, _SZ, _P, _SZ, _P]),
+    "gs_vocab_loss_grad": (C.c_int, [C.POINTER(GsVocabHead), C.POINTER(GsVocabTargets), _I32, _P, _P, _SZ, _P, _P, _P,
+                                     _P, _SZ, _P]),
 }
 
 SYNTH_SIGNATURES = {

@@ -1,0 +1,243 @@
+"""The vocabulary head of a learned sparse encoder, and the losses it is trained with.
+
+An index holds what such an encoder answers with: a non-negative weight per
+vocabulary term and text.  Its last layer is one product, hidden states times the
+vocabulary's rows, ``l = hidden @ weight.T + bias``; the operators here are that
+product with what follows it, without the ``[tokens, vocab]`` logits in memory:
+
+- :func:`term_weights`: ``log(1 + relu(max of l over a text's kept tokens))``, the
+  rows an index is built from and the queries it is searched with;
+- :func:`vocab_loss`: softmax cross entropy over the vocabulary;
+- :func:`distill_loss`: distillation from a teacher's top logits.
+
+All three work with autograd (first derivatives).  Tensors are float32, float16 or
+bfloat16, hidden states and weight of one type; sums and softmaxes are in 32 bits, and
+gradients of 16-bit tensors are rounded to their type.  Hidden states and weight may
+have any strides and sizes; a weight whose rows are 16-byte aligned and a multiple of 32
+values wide is read where it is, others are laid out once per call.  Work is queued on
+the current stream of the tensors' device; results are deterministic.
+"""
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+
+C = _lib.C
+REDUCTIONS = {"none": _lib.GS_REDUCE_NONE, "mean": _lib.GS_REDUCE_MEAN, "sum": _lib.GS_REDUCE_SUM}
+MAX_TOP = 1024  # most teacher logits per row
+
+
+def _check_head(hidden, weight, bias, dims: str) -> torch.device:
+    for name, t in (("hidden", hidden), ("weight", weight)) + ((("bias", bias),) if bias is not None else ()):
+        if not isinstance(t, torch.Tensor):
+            raise ValueError(f"{name} must be a tensor, got {type(t).__name__}")
+        if t.dtype not in _lib.HTYPE_OF_DTYPE:
+            raise ValueError(f"{name} must be float32, float16 or bfloat16, got {t.dtype}")
+    if weight.dim() != 2:
+        raise ValueError(f"weight must be [vocab, dim], got {tuple(weight.shape)}")
+    if hidden.dtype != weight.dtype:
+        raise ValueError(f"hidden ({hidden.dtype}) and weight ({weight.dtype}) must be of one type")
+    if hidden.shape[-1] != weight.shape[1]:
+        raise ValueError(f"hidden must be {dims} with dim {weight.shape[1]}, got {tuple(hidden.shape)}")
+    if bias is not None and tuple(bias.shape) != (weight.shape[0],):
+        raise ValueError(f"bias must be [{weight.shape[0]}], got {tuple(bias.shape)}")
+    dev = _lib.require_gpu(hidden.device)
+    _same_device(dev, weight=weight, bias=bias)
+    return dev
+
+
+def _same_device(dev, **tensors):
+    for name, t in tensors.items():
+        if t is not None and t.device != dev:
+            raise ValueError(f"{name} is on {t.device}, hidden on {dev}")
+
+
+def _head(hidden, weight, bias) -> _lib.GsVocabHead:
+    """The C struct of hidden [texts, length, dim], weight [vocab, dim] and a contiguous bias."""
+    s = hidden.stride()
+    return _lib.GsVocabHead(hidden.data_ptr(), s[0], s[1], s[2], weight.data_ptr(), weight.stride(0), weight.stride(1),
+                            _lib.ptr(bias), _lib.HTYPE_OF_DTYPE[hidden.dtype],
+                            _lib.GS_H_F32 if bias is None else _lib.HTYPE_OF_DTYPE[bias.dtype], hidden.shape[0],
+                            hidden.shape[1], hidden.shape[2], weight.shape[0])
+
+
+def _bytes(n: int, dev) -> torch.Tensor:
+    return torch.empty(int(n), dtype=torch.uint8, device=dev)
+
+
+def _grads(ctx, hidden, weight, bias):
+    """Empty gradients of the inputs that need one (hidden, weight, bias)."""
+    return [torch.empty(t.shape, dtype=t.dtype, device=t.device) if need else None
+            for t, need in zip((hidden, weight, bias), ctx.needs_input_grad[:3])]
+
+
+class _TermWeights(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, weight, bias, mask, want_tokens):
+        dev = hidden.device
+        texts, vocab = hidden.shape[0], weight.shape[0]
+        track = any(ctx.needs_input_grad[:3])
+        weights = torch.empty((texts, vocab), dtype=torch.float32, device=dev)
+        tokens = torch.empty((texts, vocab), dtype=torch.int32, device=dev) if want_tokens or track else None
+        L, head = _lib.lib(), _head(hidden, weight, bias)
+        need, grad_need = C.c_size_t(), C.c_size_t()
+        with torch.cuda.device(dev):
+            _lib.check(L.gs_term_weights_workspace(C.byref(head), tokens is not None, C.byref(need), C.byref(grad_need)),
+                       "gs_term_weights_workspace")
+            ws = _bytes(need.value, dev)
+            _lib.check(L.gs_term_weights(C.byref(head), _lib.ptr(mask), weights.data_ptr(), _lib.ptr(tokens), ws.data_ptr(),
+                                         ws.numel(), _lib.stream_ptr(dev)), "gs_term_weights")
+        if track:
+            ctx.save_for_backward(hidden, weight, bias, weights, tokens)
+            ctx.grad_bytes = grad_need.value
+        if tokens is None:
+            return weights, None
+        ctx.mark_non_differentiable(tokens)
+        return weights, tokens
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad, _):
+        hidden, weight, bias, weights, tokens = ctx.saved_tensors
+        dev = hidden.device
+        dh, dw, db = _grads(ctx, hidden, weight, bias)
+        L, head = _lib.lib(), _head(hidden, weight, bias)
+        grad = grad.to(torch.float32).contiguous()
+        with torch.cuda.device(dev):
+            ws = _bytes(ctx.grad_bytes, dev)
+            _lib.check(L.gs_term_weights_grad(C.byref(head), grad.data_ptr(), weights.data_ptr(), tokens.data_ptr(),
+                                              _lib.ptr(dh), _lib.ptr(dw), _lib.ptr(db), ws.data_ptr(), ws.numel(),
+                                              _lib.stream_ptr(dev)), "gs_term_weights_grad")
+        return dh, dw, db, None, None
+
+
+def term_weights(hidden, weight, bias=None, *, mask=None, return_tokens: bool = False):
+    """Term weights of texts from an encoder's hidden states: float32 [texts, vocab],
+    ``log(1 + relu(max over the text's kept tokens of hidden @ weight.T + bias))``.
+
+    hidden: [texts, length, dim].  weight: [vocab, dim].  bias: [vocab] or None.
+    mask: [texts, length], nonzero for the tokens that count (None: all do); the hidden
+    states of the others are never read, and a text without any has weights 0.
+    return_tokens: also the int32 [texts, vocab] lowest token that reaches the maximum
+    (-1 where the weight is 0), through which the gradient flows."""
+    if not isinstance(hidden, torch.Tensor) or hidden.dim() != 3:
+        raise ValueError("hidden must be [texts, length, dim]")
+    dev = _check_head(hidden, weight, bias, "[texts, length, dim]")
+    if mask is not None:
+        if not isinstance(mask, torch.Tensor) or tuple(mask.shape) != tuple(hidden.shape[:2]):
+            raise ValueError(f"mask must be a tensor of shape {tuple(hidden.shape[:2])}")
+        _same_device(dev, mask=mask)
+        if mask.dtype not in (torch.bool, torch.uint8):
+            mask = mask != 0
+        mask = mask.contiguous()
+    bias = None if bias is None else bias.contiguous()
+    weights, tokens = _TermWeights.apply(hidden, weight, bias, mask, bool(return_tokens))
+    return (weights, tokens) if return_tokens else weights
+
+
+class _VocabLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, weight, bias, ids, logits, ignore_index, temperature, reduction):
+        dev = hidden.device
+        rows = hidden.shape[1]
+        head = _head(hidden, weight, bias)
+        if logits is None:
+            targets = _lib.GsVocabTargets(_lib.ptr(ids), ignore_index, None, None, _lib.GS_H_F32, 0, 1.0)
+        else:
+            targets = _lib.GsVocabTargets(None, 0, _lib.ptr(ids), logits.data_ptr(), _lib.HTYPE_OF_DTYPE[logits.dtype],
+                                          logits.shape[1], temperature)
+        loss = torch.empty((rows,) if reduction == _lib.GS_REDUCE_NONE else (), dtype=torch.float32, device=dev)
+        L = _lib.lib()
+        need = [C.c_size_t() for _ in range(3)]
+        with torch.cuda.device(dev):
+            _lib.check(L.gs_vocab_loss_workspace(C.byref(head), C.byref(targets), *map(C.byref, need)),
+                       "gs_vocab_loss_workspace")
+            saved, ws = _bytes(need[0].value, dev), _bytes(need[1].value, dev)
+            _lib.check(L.gs_vocab_loss(C.byref(head), C.byref(targets), reduction, loss.data_ptr(), saved.data_ptr(),
+                                       saved.numel(), ws.data_ptr(), ws.numel(), _lib.stream_ptr(dev)), "gs_vocab_loss")
+        if any(ctx.needs_input_grad[:3]):
+            ctx.save_for_backward(hidden, weight, bias, ids, logits, saved)
+            ctx.targets, ctx.reduction, ctx.grad_bytes = targets, reduction, need[2].value
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        hidden, weight, bias, _, _, saved = ctx.saved_tensors
+        dev = hidden.device
+        dh, dw, db = _grads(ctx, hidden, weight, bias)
+        L, head = _lib.lib(), _head(hidden, weight, bias)
+        grad = grad.to(torch.float32).contiguous()
+        with torch.cuda.device(dev):
+            ws = _bytes(ctx.grad_bytes, dev)
+            _lib.check(L.gs_vocab_loss_grad(C.byref(head), C.byref(ctx.targets), ctx.reduction, grad.data_ptr(),
+                                            saved.data_ptr(), saved.numel(), _lib.ptr(dh), _lib.ptr(dw), _lib.ptr(db),
+                                            ws.data_ptr(), ws.numel(), _lib.stream_ptr(dev)), "gs_vocab_loss_grad")
+        return dh, dw, db, None, None, None, None, None
+
+
+def _loss(hidden, weight, bias, ids, logits, ignore_index, temperature, reduction):
+    lead = hidden.shape[:-1]
+    bias = None if bias is None else bias.contiguous()
+    flat = hidden.reshape(1, -1, hidden.shape[-1]) if hidden.numel() else hidden.new_empty((1, lead.numel(), hidden.shape[-1]))
+    out = _VocabLoss.apply(flat, weight, bias, ids, logits, ignore_index, temperature, REDUCTIONS[reduction])
+    return out.reshape(lead) if reduction == "none" else out
+
+
+def _check_rows(hidden, reduction):
+    if reduction not in REDUCTIONS:
+        raise ValueError(f"reduction must be one of {sorted(REDUCTIONS)}, got {reduction!r}")
+    if not isinstance(hidden, torch.Tensor) or hidden.dim() < 1:
+        raise ValueError("hidden must be [..., dim]")
+
+
+def _ids(t, shape, what, dev):
+    if not isinstance(t, torch.Tensor) or t.dtype not in (torch.int64, torch.int32):
+        raise ValueError(f"{what} must be an int64 or int32 tensor")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{what} must be {tuple(shape)}, got {tuple(t.shape)}")
+    _same_device(dev, **{what: t})
+    return t.to(torch.int64).contiguous()
+
+
+def vocab_loss(hidden, weight, targets, bias=None, *, ignore_index: int = -100, reduction: str = "mean"):
+    """Softmax cross entropy of ``hidden @ weight.T + bias`` over the vocabulary, without the logits.
+
+    hidden: [..., dim]; targets: [...] int64 or int32 term ids.  A row whose target is
+    ignore_index or outside the vocabulary is left out: its loss and gradient are 0, it does
+    not count in the mean, and its hidden state is never read.  reduction: "mean" over the rows
+    that count (0 when none does), "sum", or "none" (a loss per row).  float32."""
+    _check_rows(hidden, reduction)
+    dev = _check_head(hidden, weight, bias, "[..., dim]")
+    ids = _ids(targets, hidden.shape[:-1], "targets", dev)
+    return _loss(hidden, weight, bias, ids, None, int(ignore_index), 1.0, reduction)
+
+
+def distill_loss(hidden, weight, teacher_ids, teacher_logits, bias=None, *, temperature: float = 1.0,
+                 reduction: str = "mean"):
+    """Distillation from a teacher's top logits: ``temperature**2 * sum_k q_k (log q_k - log p[id_k])``
+    with ``q = softmax(teacher_logits / temperature)`` over a row's ids and
+    ``p = softmax(l / temperature)`` over the whole vocabulary, l = hidden @ weight.T + bias
+    never in memory.
+
+    hidden: [..., dim]; teacher_ids: [..., top] int64 or int32, teacher_logits: [..., top]
+    (float32, float16 or bfloat16), top <= 1024.  Ids outside the vocabulary (padding) are
+    skipped, equal ids add up; a row without any other id is left out as in :func:`vocab_loss`.
+    The teacher gets no gradient."""
+    _check_rows(hidden, reduction)
+    dev = _check_head(hidden, weight, bias, "[..., dim]")
+    if not isinstance(teacher_logits, torch.Tensor) or teacher_logits.dtype not in _lib.HTYPE_OF_DTYPE:
+        raise ValueError("teacher_logits must be a float32, float16 or bfloat16 tensor")
+    if teacher_logits.dim() != hidden.dim() or teacher_logits.shape[:-1] != hidden.shape[:-1]:
+        raise ValueError(f"teacher_logits must be {tuple(hidden.shape[:-1])} + (top,), got {tuple(teacher_logits.shape)}")
+    top = teacher_logits.shape[-1]
+    if not 1 <= top <= MAX_TOP:
+        raise ValueError(f"{top} teacher logits per row: 1 to {MAX_TOP} are supported")
+    if not 0.0 < float(temperature) < float("inf"):
+        raise ValueError(f"temperature must be positive and finite, got {temperature}")
+    ids = _ids(teacher_ids, teacher_logits.shape, "teacher_ids", dev)
+    _same_device(dev, teacher_logits=teacher_logits)
+    logits = teacher_logits.detach().reshape(-1, top).contiguous()
+    return _loss(hidden, weight, bias, ids.reshape(-1, top), logits, 0, float(temperature), reduction)

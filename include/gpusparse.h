@@ -25,7 +25,7 @@
 extern "C" {
 #endif
 
-#define GS_ABI_VERSION 10
+#define GS_ABI_VERSION 11
 
 #define GS_OK 0
 #define GS_EINVAL 1   /* bad argument or layout */
@@ -397,6 +397,70 @@ int gs_scatter_add(const gs_index *index, const int64_t *lo_d, const int64_t *hi
                    const int32_t *q_terms_d, const void *q_weights_d, int32_t B, int32_t T,
                    void *out_d, int64_t chunk_start, int64_t chunk_len, int64_t out_stride,
                    int32_t block_pl, void *stream);
+
+/* ------------------------------------------------------------ the vocabulary head
+ * No counterpart in the reference, which starts from the vectors these make: the last layer of a
+ * learned sparse encoder and the losses it is trained with.  All are one product,
+ *     l[t][v] = sum_d hidden[t][d] weight[v][d] + bias[v],
+ * whose [tokens][vocab] result is never written: it is consumed tile by tile.
+ *
+ * hidden is [texts][length][dim] with any element strides (rows of a loss: texts = 1), weight [vocab][dim] with
+ * any element strides; both of `type`.  bias is [vocab] of `bias_type`, or NULL.  Sums are fp32.
+ * texts * length <= 2^28, dim <= 32768, vocab <= 2^20. */
+#define GS_H_F32 0
+#define GS_H_F16 1
+#define GS_H_BF16 2
+
+typedef struct gs_vocab_head {
+    const void *hidden_d;
+    int64_t hidden_text_stride, hidden_row_stride, hidden_dim_stride;
+    const void *weight_d;
+    int64_t weight_row_stride, weight_dim_stride;
+    const void *bias_d;
+    int32_t type;       /* GS_H_* of hidden, weight and their gradients */
+    int32_t bias_type;  /* GS_H_* of bias and its gradient */
+    int32_t texts, length, dim, vocab;
+} gs_vocab_head;
+
+/* Term weights: weights_d fp32 [texts][vocab] = log(1 + relu(max over the text's kept tokens of l)); 0 for a text
+ * without one.  mask_d uint8 [texts][length], 0: the token is left out (its hidden state is never read); NULL: all are
+ * kept.  tokens_d int32 [texts][vocab] (or NULL): the lowest token whose l is the maximum, -1 where the weight is 0. */
+int gs_term_weights_workspace(const gs_vocab_head *head, int32_t tokens, size_t *bytes, size_t *grad_bytes);
+int gs_term_weights(const gs_vocab_head *head, const uint8_t *mask_d, float *weights_d, int32_t *tokens_d,
+                    void *workspace_d, size_t workspace_bytes, void *stream);
+/* Its gradient, given the weights, their tokens and grad_d fp32 [texts][vocab]; contiguous outputs of hidden's,
+ * weight's and bias's shapes, each NULL when not wanted.  Sums run in a fixed order. */
+int gs_term_weights_grad(const gs_vocab_head *head, const float *grad_d, const float *weights_d, const int32_t *tokens_d,
+                         void *dhidden_d, void *dweight_d, void *dbias_d, void *workspace_d, size_t workspace_bytes,
+                         void *stream);
+
+/* What each row's logits are compared with: one id per row (softmax cross entropy), or a teacher's top logits
+ * (distillation).  A target that is ignore_index or outside [0, vocab) leaves its row out; so does a teacher's row
+ * without an id in [0, vocab), and its other ids are skipped.  Rows left out have loss and gradient 0, their hidden
+ * states are never read, and they do not count in a mean. */
+typedef struct gs_vocab_targets {
+    const int64_t *targets_d;      /* [rows], or NULL */
+    int64_t ignore_index;
+    const int64_t *teacher_ids_d;  /* [rows][top], or NULL */
+    const void *teacher_logits_d;  /* [rows][top] of teacher_type */
+    int32_t teacher_type, top;     /* 1 <= top <= 1024 */
+    float temperature;             /* of both softmaxes; the loss carries its square */
+} gs_vocab_targets;
+
+#define GS_REDUCE_NONE 0  /* loss_d, grad_d: [rows] */
+#define GS_REDUCE_MEAN 1  /* one value, over the rows that count (0 when none does) */
+#define GS_REDUCE_SUM 2
+
+/* loss = lse(l) - l[target], or temperature^2 sum_k q_k (log q_k - log p[id_k]) with q = softmax(teacher logits /
+ * temperature) over the row's ids and p = softmax(l / temperature) over the vocabulary.  saved_d is what the gradient
+ * needs besides the weight (and the weight again when it is not laid out as the product reads it). */
+int gs_vocab_loss_workspace(const gs_vocab_head *head, const gs_vocab_targets *targets, size_t *saved_bytes,
+                            size_t *scratch_bytes, size_t *grad_bytes);
+int gs_vocab_loss(const gs_vocab_head *head, const gs_vocab_targets *targets, int32_t reduction, float *loss_d,
+                  void *saved_d, size_t saved_bytes, void *scratch_d, size_t scratch_bytes, void *stream);
+int gs_vocab_loss_grad(const gs_vocab_head *head, const gs_vocab_targets *targets, int32_t reduction,
+                       const float *grad_d, const void *saved_d, size_t saved_bytes, void *dhidden_d, void *dweight_d,
+                       void *dbias_d, void *scratch_d, size_t scratch_bytes, void *stream);
 
 #ifdef __cplusplus
 }
