@@ -103,6 +103,10 @@ __device__ __forceinline__ float wave_max(float v) {
     for (int d = 32; d >= 1; d >>= 1) v = fmaxf(v, __shfl_xor(v, d, GS_WAVE));
     return v;
 }
+// the larger one, NaN if either is
+__device__ __forceinline__ float maximum(float a, float b, float c) {
+    return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c);
+}
 template <int CTRL>
 __device__ __forceinline__ float dpp_add(float v) {
     return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, false));
@@ -110,41 +114,61 @@ __device__ __forceinline__ float dpp_add(float v) {
 // over the 16 lanes of a row of lanes
 __device__ __forceinline__ float sum16(float v) { return dpp_add<0x121>(dpp_add<0x122>(dpp_add<0x124>(dpp_add<0x128>(v)))); }
 
-// ---------------------------------------------------------------- kept rows
+// ---------------------------------------------------------------- setup
 
-// rows[i]: the i-th row with keep[row] != 0, ascending (keep NULL: all); inv[row]: its place or -1; *n: how many.
-// For texts of `length` rows, seg[i] is the row's text.  One workgroup, 16 rows per thread and turn.
-__global__ __launch_bounds__(1024) void k_kept_rows(const uint8_t *keep, int total, int length, int *rows, int *inv,
-                                                    int *seg, int *n) {
+// What decides whether a row is kept: a byte per row (NULL: all are), or a target per row.
+struct Keep {
+    const uint8_t *mask;
+    const int64_t *targets;
+    int64_t ignore;
+    int vocab;
+    int total;
+    // bit e: row r0 + e is kept
+    __device__ __forceinline__ uint32_t sixteen(int64_t r0) const {
+        if (r0 >= total) return 0;
+        const uint32_t in = r0 + 16 > total ? (1u << (total - r0)) - 1u : 0xFFFFu;
+        uint32_t m = 0;
+        if (targets) {
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                const int64_t t = targets[min(r0 + e, (int64_t)total - 1)];
+                m |= (t >= 0 && t < vocab && t != ignore ? 1u : 0u) << e;
+            }
+        } else if (!mask) {
+            m = 0xFFFF;
+        } else if ((reinterpret_cast<uintptr_t>(mask) & 15) == 0 && r0 + 16 <= total) {
+            const uint4 w = *reinterpret_cast<const uint4 *>(mask + r0);
+            const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int e = 0; e < 16; e++) m |= (((ws[e >> 2] >> (8 * (e & 3))) & 255u) ? 1u : 0u) << e;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 16; e++) m |= (mask[min(r0 + e, (int64_t)total - 1)] ? 1u : 0u) << e;
+        }
+        return m & in;
+    }
+};
+
+// rows[i]: the i-th kept row, ascending; inv[row]: its place or -1; *n: how many.  For texts of `length` rows, seg[i]
+// is the row's text, -1 for the rest of the last tile.  One workgroup of 1024, 16 rows per thread and turn.
+__device__ __forceinline__ void kept_rows(const Keep &keep, int length, int *rows, int *inv, int *seg, int *n) {
     __shared__ int part[16];
-    __shared__ int base_s;
     const int tid = threadIdx.x, lane = gs_lane(), wave = tid >> 6;
     int base = 0;
-    const bool vec = keep && (reinterpret_cast<uintptr_t>(keep) & 15) == 0;
-    for (int64_t at = 0; at < total; at += 16384) {
+    for (int64_t at = 0; at < keep.total; at += 16384) {
         const int64_t r0 = at + tid * 16;
-        uint32_t m = 0;
-        if (r0 < total) {
-            if (!keep) m = 0xFFFF;
-            else if (vec && r0 + 16 <= total) {
-                const uint4 w = *reinterpret_cast<const uint4 *>(keep + r0);
-                const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                for (int e = 0; e < 16; e++) m |= (((ws[e >> 2] >> (8 * (e & 3))) & 255u) ? 1u : 0u) << e;
-            } else {
-                for (int e = 0; e < 16 && r0 + e < total; e++) m |= (keep[r0 + e] ? 1u : 0u) << e;
-            }
-            if (r0 + 16 > total) m &= (1u << (total - r0)) - 1u;
-        }
+        const uint32_t m = keep.sixteen(r0);
         const uint32_t c = __popc(m);
         const uint32_t inc = gs_wave_incl_scan(c);
         if (lane == 63) part[wave] = (int)inc;
         __syncthreads();
         int before = base;
-        for (int w = 0; w < wave; w++) before += part[w];
-        if (tid == 1023) base_s = before + (int)inc;
+        for (int w = 0; w < 16; w++) {
+            if (w < wave) before += part[w];
+            base += part[w];
+        }
         int o = before + (int)(inc - c);
-        for (int e = 0; e < 16 && r0 + e < total; e++) {
+        for (int e = 0; e < 16 && r0 + e < keep.total; e++) {
             const bool k = (m >> e) & 1;
             const int row = (int)(r0 + e);
             if (inv) inv[row] = k ? o : -1;
@@ -155,10 +179,34 @@ __global__ __launch_bounds__(1024) void k_kept_rows(const uint8_t *keep, int tot
             }
         }
         __syncthreads();
-        base = base_s;
-        __syncthreads();
     }
+    if (seg)
+        for (int i = base + tid; i < round_up(base, kRowPad); i += 1024) seg[i] = -1;
     if (tid == 0) *n = base;
+}
+
+// First launch of a call.  Workgroup 0 lists the kept rows; the others write the bias in fp32 (0 without one, -inf for
+// the rows that pad the vocabulary: they drop out of every softmax and maximum) and clear what is added to later.
+__global__ __launch_bounds__(1024) void k_setup(Keep keep, int length, int *rows, int *inv, int *seg, int *n, const void *bias,
+                                                int bias_type, int vocab, int padded, float *bias_o, float *zero, int64_t zeros) {
+    if (blockIdx.x == 0) {
+        kept_rows(keep, length, rows, inv, seg, n);
+        return;
+    }
+    const int64_t by = (int64_t)(gridDim.x - 1) * 1024, at = (int64_t)(blockIdx.x - 1) * 1024 + threadIdx.x;
+    for (int64_t v = at; v < padded; v += by) {
+        float x = 0.f;
+        if (v >= vocab) x = -INFINITY;
+        else if (bias)
+            x = bias_type == GS_H_F32 ? ((const float *)bias)[v]
+                                      : bias_type == GS_H_F16 ? (float)((const _Float16 *)bias)[v] : (float)((const __bf16 *)bias)[v];
+        bias_o[v] = x;
+    }
+    for (int64_t i = at * 4; i < zeros; i += by * 4) {
+        if (i + 3 < zeros) *reinterpret_cast<f32x4 *>(zero + i) = f32x4{0.f, 0.f, 0.f, 0.f};
+        else
+            for (int e = 0; e < 4 && i + e < zeros; e++) zero[i + e] = 0.f;
+    }
 }
 
 // ---------------------------------------------------------------- packing
@@ -170,44 +218,27 @@ struct Source {
     int dim, vec;
 };
 
-// Rows of a strided matrix as contiguous 16-bit ones (fp32: three planes), zero to a multiple of kStep values.
 template <int HT, int NP>
-__global__ __launch_bounds__(256) void k_pack(Source s, const int *rows, const int *n_d, int n, int dimp, uint16_t *out) {
+__device__ __forceinline__ void pack_row(const Source &s, int row, int dimp, uint16_t *dst, int lane) {
     using T = typename HVal<HT>::t;
     using S = std::conditional_t<HT == GS_H_F16, _Float16, __bf16>;
-    if (n_d) n = min(n, *n_d);
-    const int lane = gs_lane();
-    for (int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); i < n; i += (int64_t)gridDim.x * 4) {
-        const int row = rows ? rows[i] : (int)i;
-        const T *src = (const T *)s.p + (int64_t)(row / s.length) * s.s0 + (int64_t)(row % s.length) * s.s1;
-        uint16_t *dst = out + i * (int64_t)NP * dimp;
-        for (int d = lane * 4; d < dimp; d += 256) store_planes4<S, NP>(dst, dimp, d, row4(src, s.sd, d, s.dim, s.vec));
+    const T *src = (const T *)s.p + (int64_t)(row / s.length) * s.s0 + (int64_t)(row % s.length) * s.s1;
+    for (int d = lane * 4; d < dimp; d += 256) store_planes4<S, NP>(dst, dimp, d, row4(src, s.sd, d, s.dim, s.vec));
+}
+
+// Rows of the kept hidden states and, where the product cannot read it in place (w_rows > 0), of the vocabulary as
+// contiguous 16-bit ones (fp32: three planes), zero to a multiple of kStep values.  One wave per row.
+template <int HT, int NP>
+__global__ __launch_bounds__(256) void k_pack(Source h, const int *rows, const int *n_d, uint16_t *h_out, Source w, int w_rows,
+                                              uint16_t *w_out, int dimp) {
+    const int n = *n_d, lane = gs_lane();
+    for (int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); i < (int64_t)n + w_rows; i += (int64_t)gridDim.x * 4) {
+        if (i < n) pack_row<HT, NP>(h, rows[i], dimp, h_out + i * (int64_t)NP * dimp, lane);
+        else pack_row<HT, NP>(w, (int)(i - n), dimp, w_out + (i - n) * (int64_t)NP * dimp, lane);
     }
 }
 
-// The bias in fp32 (0 without one), -inf for the rows that pad the vocabulary: they drop out of every softmax.
-__global__ void k_bias(const void *bias, int type, int vocab, int padded, float *out) {
-    const int v = blockIdx.x * blockDim.x + threadIdx.x;
-    if (v >= padded) return;
-    float x = 0.f;
-    if (v >= vocab) x = -INFINITY;
-    else if (bias)
-        x = type == GS_H_F32 ? ((const float *)bias)[v]
-                             : type == GS_H_F16 ? (float)((const _Float16 *)bias)[v] : (float)((const __bf16 *)bias)[v];
-    out[v] = x;
-}
-
 // ---------------------------------------------------------------- targets
-
-// One target per row: its id, and whether the row counts (an id outside the vocabulary does not, as in a search).
-__global__ void k_targets(const int64_t *targets, int64_t ignore, int rows, int vocab, int *ids, uint8_t *keep) {
-    const int r = blockIdx.x * blockDim.x + threadIdx.x;
-    if (r >= rows) return;
-    const int64_t t = targets[r];
-    const bool ok = t >= 0 && t < vocab && t != ignore;
-    ids[r] = ok ? (int)t : -1;
-    keep[r] = ok;
-}
 
 // A teacher's row: q = softmax(logits / tau) over its ids inside the vocabulary, sorted by id (equal ids stay apart,
 // in their order), ids beyond them INT_MAX; sum of q log q.  One workgroup per row; LDS holds the row.
@@ -268,68 +299,97 @@ __global__ __launch_bounds__(256) void k_teacher(const int64_t *ids, const void 
     }
 }
 
-// first[t][i]: where row rows[i]'s entries with ids >= t * width begin (K > 1 only)
-__global__ void k_entry_starts(const int *ids, int top, const int *rows, const int *n_d, int tiles, int width, int64_t ld,
-                               uint16_t *first) {
-    const int i = blockIdx.x * blockDim.x + threadIdx.x;
-    if (i >= *n_d) return;
-    const int *row = ids + (int64_t)rows[i] * top;
-    int k = 0;
-    for (int t = 0; t <= tiles; t++) {
-        const int64_t v = (int64_t)t * width;
-        while (k < top && row[k] < v) k++;
-        first[t * ld + i] = (uint16_t)k;
+// A teacher's entries by kept row, and first[t][i]: the first of kept row i's with an id of at least t * kRowPad, t up to
+// tiles.  One wave per row.
+__global__ __launch_bounds__(256) void k_entries(const int *ids, const float *share, int top, const int *rows, const int *n_d,
+                                                 int tiles, int64_t ld, int *ids_o, float *share_o, uint16_t *first) {
+    const int n = *n_d, lane = gs_lane();
+    for (int i = blockIdx.x * 4 + (threadIdx.x >> 6); i < n; i += gridDim.x * 4) {
+        const int64_t from = (int64_t)rows[i] * top, to = (int64_t)i * top;
+        for (int k = lane; k <= top; k += 64) {
+            // entry k is the first of the tiles past its predecessor's, up to its own
+            const int id = k < top ? ids[from + k] : 0x7FFFFFFF;
+            const int prev = k > 0 ? ids[from + k - 1] : -1;
+            if (k < top) {
+                ids_o[to + k] = id;
+                share_o[to + k] = share[from + k];
+            }
+            const int t1 = id == 0x7FFFFFFF ? tiles : id / kRowPad;
+            int t = prev < 0 ? 0 : prev == 0x7FFFFFFF ? tiles + 1 : prev / kRowPad + 1;
+            for (; t <= t1; t++) first[t * ld + i] = (uint16_t)k;
+        }
     }
 }
 
-// sum_k q_k l[id_k] of each kept row, from the unpacked values in fp32.  One wave per row, ids in turn.
+// Each kept row's target id, and its logit from the unpacked values in fp32.  One wave per row.
 template <int HT>
 __global__ __launch_bounds__(256) void k_target_logits(Source h, const void *weight, int64_t wr, int64_t wd, int wvec,
-                                                       const float *bias, const int *ids, const float *q, int top,
-                                                       const int *rows, const int *n_d, float *out) {
+                                                       const float *bias, const int64_t *targets, const int *rows,
+                                                       const int *n_d, int *ids, float *out) {
     using T = typename HVal<HT>::t;
     const int n = *n_d, lane = gs_lane();
     for (int i = blockIdx.x * 4 + (threadIdx.x >> 6); i < n; i += gridDim.x * 4) {
-        const int row = rows[i];
+        const int row = rows[i], id = (int)targets[row];
         const T *src = (const T *)h.p + (int64_t)(row / h.length) * h.s0 + (int64_t)(row % h.length) * h.s1;
-        float sum = 0.f;
-        for (int k0 = 0; k0 < top; k0 += 4) {
-            int id[4];
-            float qk[4], a[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int k = k0 + e;
-                id[e] = k < top ? ids[(int64_t)row * top + k] : 0x7FFFFFFF;
-                qk[e] = id[e] == 0x7FFFFFFF || id[e] < 0 ? 0.f : q ? q[(int64_t)row * top + k] : 1.f;
-                if (qk[e] == 0.f) id[e] = -1;
-            }
-            if ((id[0] & id[1] & id[2] & id[3]) < 0 && id[0] < 0 && id[1] < 0 && id[2] < 0 && id[3] < 0) continue;
-            for (int d = lane * 4; d < h.dim; d += 256) {
-                const f32x4 x = row4(src, h.sd, d, h.dim, h.vec);
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    if (id[e] < 0) continue;
-                    const f32x4 y = row4((const T *)weight + id[e] * wr, wd, d, h.dim, wvec);
-                    a[e] = fmaf(x[0], y[0], fmaf(x[1], y[1], fmaf(x[2], y[2], fmaf(x[3], y[3], a[e]))));
-                }
-            }
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-                if (id[e] >= 0) sum += qk[e] * (wave_sum(a[e]) + bias[id[e]]);
+        const T *w = (const T *)weight + id * wr;
+        float a = 0.f;
+        for (int d = lane * 4; d < h.dim; d += 256) {
+            const f32x4 x = row4(src, h.sd, d, h.dim, h.vec), y = row4(w, wd, d, h.dim, wvec);
+            a = fmaf(x[0], y[0], fmaf(x[1], y[1], fmaf(x[2], y[2], fmaf(x[3], y[3], a))));
         }
-        if (lane == 0) out[i] = sum;
+        a = wave_sum(a);
+        if (lane == 0) {
+            out[i] = a + bias[id];
+            ids[i] = id;
+        }
     }
 }
 
 // ---------------------------------------------------------------- epilogues
 
+// The target shares of the kept rows, ascending by id within a row.
+struct Entries {
+    const int *ids;         // [kept row][top]
+    const float *share;     // NULL: 1
+    const uint16_t *first;  // [vocabulary / kRowPad + 1][kept row] (top > 1)
+    int64_t ld;
+    int top;
+    // f(mine, share) for each entry of the lanes' tokens n among the wave's terms [wv, wv + 16 MR): in the lane that
+    // holds the entry's term in register `mine` = 4 i + e; other lanes get -1.
+    template <int MR, class F>
+    __device__ __forceinline__ void each(int n, bool on, int wv, int q, F &&f) const {
+        int64_t base = 0;
+        int k = 0, end = 0;
+        if (on) {
+            base = (int64_t)n * top;
+            end = 1;
+            if (top > 1) {
+                const int64_t t = (int64_t)(wv / kRowPad) * ld + n;
+                k = first[t];
+                end = first[t + ld];
+            }
+        }
+        while (__any(k < end)) {
+            const int lv = k < end ? ids[base + k] - wv : -1;
+            if (__any(lv >= 0 && lv < MR * 16)) {
+                const float s = k < end ? (share ? share[base + k] : 1.f) : 0.f;
+                f(lv >= 0 && lv < MR * 16 && ((lv >> 2) & 3) == q ? (lv >> 4) * 4 + (lv & 3) : -1, s);
+            }
+            k++;
+        }
+    }
+};
+
 // Softmax sums of a tile: per token the largest scaled logit and the sum of 2^(scaled logit - it), over each wave's
-// terms.  part[block of terms][token].
+// terms: part[block of terms][token]; with SHARES also the sum of share * logit: dots[block of terms][token].
+template <bool SHARES>
 struct EpiSums {
     const float *bias;
     float scale;  // log2(e) / temperature
     float2 *part;
+    float *dots;
     int64_t ld;
+    Entries entries;
     template <class TL>
     __device__ __forceinline__ void run(f32x4 (&acc)[TL::MR][TL::MC], const Place &at) const {
         const int q = at.lane >> 4;
@@ -342,25 +402,38 @@ struct EpiSums {
         const int64_t block = at.row0 / (TL::MR * 16);
 #pragma unroll
         for (int j = 0; j < TL::MC; j++) {
+            const int n = at.col0 + 16 * j + (at.lane & 15);
             float m = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < TL::MR; i++)
-                m = fmaxf(m, fmaxf(fmaxf(acc[i][j][0], acc[i][j][1]), fmaxf(acc[i][j][2], acc[i][j][3])));
+            for (int i = 0; i < TL::MR; i++) m = maximum(maximum(m, acc[i][j][0], acc[i][j][1]), acc[i][j][2], acc[i][j][3]);
             float mc = m * scale, s = 0.f;
             const float sub = m == -INFINITY ? 0.f : mc;
 #pragma unroll
             for (int i = 0; i < TL::MR; i++)
 #pragma unroll
                 for (int e = 0; e < 4; e++) s += __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], scale, -sub));
+            float dot = 0.f;
+            if (SHARES)
+                entries.each<TL::MR>(n, n < at.n_c, at.row0, q, [&](int mine, float share) {
+                    float x = 0.f;
+#pragma unroll
+                    for (int i = 0; i < TL::MR; i++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) x = mine == i * 4 + e ? acc[i][j][e] : x;
+                    if (share != 0.f) dot = fmaf(share, x, dot);
+                });
 #pragma unroll
             for (int d = 16; d <= 32; d <<= 1) {
                 const float mo = __shfl_xor(mc, d, GS_WAVE), so = __shfl_xor(s, d, GS_WAVE);
                 const float mn = fmaxf(mc, mo), by = mn == -INFINITY ? 0.f : mn;
                 s = s * __builtin_amdgcn_exp2f(mc - by) + so * __builtin_amdgcn_exp2f(mo - by);
                 mc = mn;
+                if (SHARES) dot += __shfl_xor(dot, d, GS_WAVE);
             }
-            const int n = at.col0 + 16 * j + (at.lane & 15);
-            if (q == 0 && n < at.n_c) part[block * ld + n] = make_float2(mc, s);
+            if (q == 0 && n < at.n_c) {
+                part[block * ld + n] = make_float2(mc, s);
+                if (SHARES) dots[block * ld + n] = dot;
+            }
         }
     }
 };
@@ -373,12 +446,7 @@ struct EpiLogitGrad {
     float scale;
     const float *lse2;     // log2 of the softmax sum, per kept row
     const float *factor;   // per kept row
-    const int *rows;       // kept row -> source row
-    const int *ids;        // [source row][top], ascending
-    const float *share;    // NULL: 1
-    const uint16_t *first; // [vocabulary / kRowPad][kept row] (top > 1)
-    int64_t first_ld;
-    int top;
+    Entries entries;
     int v0;                // first term of this piece
     uint16_t *out;
     int64_t ld, plane;
@@ -405,32 +473,12 @@ struct EpiLogitGrad {
             for (int i = 0; i < TL::MR; i++)
 #pragma unroll
                 for (int e = 0; e < 4; e++) acc[i][j][e] = __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], scale, -l));
-            // target shares: the lane that holds the entry's term takes them off
-            int64_t base = 0;
-            int k = 0, end = 0;
-            if (on) {
-                base = (int64_t)rows[n] * top;
-                end = top;
-                if (top > 1) {
-                    const int t = wv / kRowPad;
-                    k = first[t * first_ld + n];
-                    end = first[(t + 1) * first_ld + n];
-                }
-            }
-            int id = k < end ? ids[base + k] : 0x7FFFFFFF;
-            while (__any(k < end)) {
-                const int lv = id - wv;
-                if (__any(k < end && lv >= 0 && lv < TL::MR * 16)) {
-                    const float s = k < end ? (share ? share[base + k] : 1.f) : 0.f;
-                    const int mine = k < end && lv >= 0 && ((lv >> 2) & 3) == q ? (lv >> 4) * 4 + (lv & 3) : -1;
+            entries.each<TL::MR>(n, on, wv, q, [&](int mine, float share) {
 #pragma unroll
-                    for (int i = 0; i < TL::MR; i++)
+                for (int i = 0; i < TL::MR; i++)
 #pragma unroll
-                        for (int e = 0; e < 4; e++) acc[i][j][e] -= mine == i * 4 + e ? s : 0.f;
-                }
-                k++;
-                id = k < end ? ids[base + k] : 0x7FFFFFFF;
-            }
+                    for (int e = 0; e < 4; e++) acc[i][j][e] -= mine == i * 4 + e ? share : 0.f;
+            });
 #pragma unroll
             for (int i = 0; i < TL::MR; i++) {
                 acc[i][j] *= f;
@@ -505,140 +553,153 @@ struct EpiHiddenPart {
 
 // Largest logit of each text and term: rows are kept tokens (ascending by text), columns terms.  best[text][term]
 // takes the maximum of the positive ones' bits; with tokens, of (bits, ~kept row), so that the lowest token wins a
-// tie.  Maxima do not depend on the order of the atomics.
+// tie.  Maxima do not depend on the order of the atomics.  The bias is added to a maximum (rounding keeps order).
 template <bool TOK>
 struct EpiTextMax {
     const float *bias;
     const int *seg;   // text of each kept row, padded with -1 to a whole tile
     void *best;
     int vocab;
+
+    // Takes rows row .. row + 3's values into the lane's maximum (and where it is; the first of equal ones)
+    __device__ __forceinline__ static void take(f32x4 x, int row, float &top, int &tok) {
+        if (TOK) {
+            float t = top;
+            int k = tok;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                // a NaN is taken, and not given up for what follows
+                const bool up = !(x[e] <= t) && t == t;
+                t = up ? x[e] : t;
+                k = up ? row + e : k;
+            }
+            top = t, tok = k;
+        } else {
+            top = maximum(maximum(top, x[0], x[1]), x[2], x[3]);
+        }
+    }
+    template <int MC>
+    __device__ __forceinline__ void flush(int text, float (&top)[MC], int (&tok)[MC], const float (&b)[MC], const Place &at) const {
+        static_assert(MC <= 4, "a lane group writes one column block");
+        const int q = at.lane >> 4;
+        int mine = 0, row = 0;
+#pragma unroll
+        for (int j = 0; j < MC; j++) {
+            // as integers positive values order as they should, NaN above them, and the others are below 0
+            const float l = top[j] + b[j];
+            int x = l != l ? 0x7FC00000 : __float_as_int(l), r = tok[j];
+#pragma unroll
+            for (int d = 16; d <= 32; d <<= 1) {
+                const int xo = __shfl_xor(x, d, GS_WAVE);
+                if (TOK) {
+                    const int ro = __shfl_xor(r, d, GS_WAVE);
+                    r = xo > x || (xo == x && ro < r) ? ro : r;
+                }
+                x = max(x, xo);
+            }
+            if (j == q) mine = x, row = r;
+        }
+        const int v = at.col0 + 16 * q + (at.lane & 15);
+        if (q < MC && v < vocab && mine > 0) {
+            const int64_t o = (int64_t)text * vocab + v;
+            if (TOK)
+                atomicMax((unsigned long long *)best + o,
+                          (unsigned long long)(uint32_t)mine << 32 | (0xFFFFFFFFu - (uint32_t)row));
+            else
+                atomicMax((uint32_t *)best + o, (uint32_t)mine);
+        }
+    }
     template <class TL>
     __device__ __forceinline__ void run(f32x4 (&acc)[TL::MR][TL::MC], const Place &at) const {
-        static_assert(TL::MC <= 4, "a lane group flushes one column block");
         const int q = at.lane >> 4;
-        float b[TL::MC];
-#pragma unroll
-        for (int j = 0; j < TL::MC; j++) b[j] = bias[at.col0 + 16 * j + (at.lane & 15)];
-        int cur = -1;
-        float top[TL::MC];
+        if (at.row0 >= at.n_r) return;
+        float b[TL::MC], top[TL::MC];
         int tok[TL::MC];
-        auto flush = [&]() {
-            if (cur < 0) return;
-            float mine = 0.f;
-            int row = 0;
 #pragma unroll
-            for (int j = 0; j < TL::MC; j++) {
-                float x = top[j];
-                int r = tok[j];
+        for (int j = 0; j < TL::MC; j++) b[j] = bias[at.col0 + 16 * j + (at.lane & 15)], top[j] = -INFINITY, tok[j] = 0x7FFFFFFF;
+        int4 s[TL::MR];
 #pragma unroll
-                for (int d = 16; d <= 32; d <<= 1) {
-                    const float xo = __shfl_xor(x, d, GS_WAVE);
-                    if (TOK) {
-                        const int ro = __shfl_xor(r, d, GS_WAVE);
-                        const bool take = __float_as_int(xo) > __float_as_int(x) || (__float_as_int(xo) == __float_as_int(x) && ro < r);
-                        x = take ? xo : x;
-                        r = take ? ro : r;
-                    } else {
-                        x = __int_as_float(max(__float_as_int(x), __float_as_int(xo)));
-                    }
-                }
-                if (j == q) mine = x, row = r;
-            }
-            const int v = at.col0 + 16 * q + (at.lane & 15);
-            if (q < TL::MC && v < vocab && __float_as_int(mine) > 0) {
-                const int64_t o = (int64_t)cur * vocab + v;
-                if (TOK) {
-                    const unsigned long long key = (unsigned long long)__float_as_uint(mine) << 32 | (0xFFFFFFFFu - (uint32_t)row);
-                    atomicMax((unsigned long long *)best + o, key);
-                } else {
-                    atomicMax((uint32_t *)best + o, __float_as_uint(mine));
-                }
-            }
-        };
+        for (int i = 0; i < TL::MR; i++) s[i] = *reinterpret_cast<const int4 *>(seg + at.row0 + 16 * i + 4 * q);
+        int cur = __builtin_amdgcn_readlane(s[0].x, 0);
 #pragma unroll
         for (int i = 0; i < TL::MR; i++) {
             const int row = at.row0 + 16 * i + 4 * q;
-            const int4 s = *reinterpret_cast<const int4 *>(seg + row);
-            const int lo = __builtin_amdgcn_readlane(s.x, 0);
-            // as integers, positive values and NaN order as wanted and negative ones lie below the start, 0
-            const int sv[4] = {s.x, s.y, s.z, s.w};
+            const int lo = __builtin_amdgcn_readlane(s[i].x, 0), hi = __builtin_amdgcn_readlane(s[i].w, 48);
+            if (lo == cur && hi == cur) {  // all of one text
+#pragma unroll
+                for (int j = 0; j < TL::MC; j++) take(acc[i][j], row, top[j], tok[j]);
+                continue;
+            }
             int now = lo;
-            while (now >= 0) {
+            while (now >= 0) {  // rows past the last kept one are -1, and come last
                 if (now != cur) {
-                    flush();
+                    flush<TL::MC>(cur, top, tok, b, at);
                     cur = now;
 #pragma unroll
-                    for (int j = 0; j < TL::MC; j++) top[j] = 0.f, tok[j] = 0x7FFFFFFF;
+                    for (int j = 0; j < TL::MC; j++) top[j] = -INFINITY, tok[j] = 0x7FFFFFFF;
                 }
-#pragma unroll
-                for (int j = 0; j < TL::MC; j++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const float raw = acc[i][j][e] + b[j];
-                        const float x = sv[e] == now ? (raw != raw ? __int_as_float(0x7FC00000) : raw) : 0.f;
-                        if (TOK) {
-                            const bool take = __float_as_int(x) > __float_as_int(top[j]);
-                            top[j] = take ? x : top[j];
-                            tok[j] = take ? row + e : tok[j];
-                        } else {
-                            top[j] = __int_as_float(max(__float_as_int(top[j]), __float_as_int(x)));
-                        }
-                    }
-                // the next text in this block, if any
+                const int sv[4] = {s[i].x, s[i].y, s[i].z, s[i].w};
                 int next = 0x7FFFFFFF;
 #pragma unroll
                 for (int e = 0; e < 4; e++)
                     if (sv[e] > now) next = min(next, sv[e]);
+#pragma unroll
+                for (int j = 0; j < TL::MC; j++) {
+                    f32x4 x;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) x[e] = sv[e] == now ? acc[i][j][e] : -INFINITY;
+                    take(x, row, top[j], tok[j]);
+                }
                 next = min(next, __shfl_xor(next, 16, GS_WAVE));
                 next = min(next, __shfl_xor(next, 32, GS_WAVE));
                 next = gs_uniform(next);
                 now = next == 0x7FFFFFFF ? -1 : next;
             }
         }
-        flush();
+        flush<TL::MC>(cur, top, tok, b, at);
     }
 };
 
 // ---------------------------------------------------------------- losses' small kernels
 
 // log2 of each kept row's softmax sum, and its loss.  Sixteen rows per 256 threads.
-__global__ __launch_bounds__(256) void k_row_loss(const float2 *part, int64_t ld, int blocks, const int *rows, const int *n_d,
-                                                  const float *target, const float *ent, float tau, float *lse2_o,
+__global__ __launch_bounds__(256) void k_row_loss(const float2 *part, const float *dots, int64_t ld, int blocks,
+                                                  const int *rows, const int *n_d, const float *target, const float *ent, float tau, float *lse2_o,
                                                   float *loss_o, float *loss_rows) {
-    __shared__ float sm[16][17], ss[16][17];
+    __shared__ float sm[16][17], ss[16][17], sd[16][17];
     const int n = *n_d, x = threadIdx.x & 15, y = threadIdx.x >> 4;
     for (int64_t i0 = (int64_t)blockIdx.x * 16; i0 < n; i0 += (int64_t)gridDim.x * 16) {
         const int64_t i = i0 + x;
-        float m = -INFINITY, s = 0.f;
-        if (i < n)
+        float m = -INFINITY, s = 0.f, dot = 0.f;
+        auto add = [&](float mo, float so) {
+            const float mn = fmaxf(m, mo), by = mn == -INFINITY ? 0.f : mn;
+            s = s * __builtin_amdgcn_exp2f(m - by) + so * __builtin_amdgcn_exp2f(mo - by);
+            m = mn;
+        };
+        if (i < n) {
+#pragma unroll 4
             for (int b = y; b < blocks; b += 16) {
                 const float2 p = part[b * ld + i];
-                const float mn = fmaxf(m, p.x), by = mn == -INFINITY ? 0.f : mn;
-                s = s * __builtin_amdgcn_exp2f(m - by) + p.y * __builtin_amdgcn_exp2f(p.x - by);
-                m = mn;
+                if (dots) dot += dots[b * ld + i];
+                add(p.x, p.y);
             }
-        sm[y][x] = m;
-        ss[y][x] = s;
+        }
+        sm[y][x] = m, ss[y][x] = s, sd[y][x] = dot;
         __syncthreads();
         if (y == 0 && i < n) {
             for (int b = 1; b < 16; b++) {
-                const float mn = fmaxf(m, sm[b][x]), by = mn == -INFINITY ? 0.f : mn;
-                s = s * __builtin_amdgcn_exp2f(m - by) + ss[b][x] * __builtin_amdgcn_exp2f(sm[b][x] - by);
-                m = mn;
+                add(sm[b][x], ss[b][x]);
+                dot += sd[b][x];
             }
             const float l2 = m + log2f(s);
             const int row = rows[i];
-            const float loss = tau * tau * ((ent ? ent[row] : 0.f) + (l2 * kLn2 - target[i] / tau));
+            const float loss = tau * tau * ((ent ? ent[row] : 0.f) + (l2 * kLn2 - (target ? target[i] : dot) / tau));
             lse2_o[i] = l2;
             loss_o[i] = loss;
             if (loss_rows) loss_rows[row] = loss;
         }
         __syncthreads();
     }
-}
-
-__global__ void k_fill(float *p, int64_t n, float v) {
-    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) p[i] = v;
 }
 
 // Sum (or mean) of the kept rows' losses, in an order of its own; 0 where no row is kept.
@@ -695,26 +756,42 @@ __global__ __launch_bounds__(1024) void k_row_factor(const float *grad, int per_
 
 // dH of every source row from its parts (0 for rows that are not kept)
 template <class O>
-__global__ __launch_bounds__(256) void k_hidden_grad(const float *part, const int *inv, const int *n_d, int total, int dim,
-                                                     int dimp, int tr, int bc, int slots, int most,
-                                                     const float *scale, O *out) {
-    const int n = *n_d, lane = gs_lane();
-    const int split = parts_of(n, tr, bc, slots, most);
+__global__ __launch_bounds__(256) void k_hidden_grad(const float *part, const int *inv, const int *n_d, const int *parts_d,
+                                                     int total, int dim, int dimp, const float *scale, O *out) {
+    __shared__ f32x4 red[3][64];
+    const int n = *n_d, parts = *parts_d, lane = gs_lane(), wave = threadIdx.x >> 6;
     const float s = *scale;
     const bool vec = (dim & 3) == 0;
-    for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < total; r += (int64_t)gridDim.x * 4) {
-        const int i = inv[r];
-        for (int d = lane * 4; d < dim; d += 256) {
-            f32x4 x = f32x4{0.f, 0.f, 0.f, 0.f};
-            if (i >= 0)
-                for (int p = 0; p < split; p++) x += *reinterpret_cast<const f32x4 *>(part + ((int64_t)p * n + i) * dimp + d);
-            x *= s;
-            O *to = out + r * dim + d;
-            if (vec) store4(to, x);
-            else
-                for (int e = 0; e < 4; e++)
-                    if (d + e < dim) to[e] = (O)x[e];
+    const int chunks = (dim + 255) / 256;
+    const auto put = [&](int64_t r, int d, f32x4 x) {
+        x *= s;
+        O *to = out + r * dim + d;
+        if (vec) store4(to, x);
+        else
+            for (int e = 0; e < 4; e++)
+                if (d + e < dim) to[e] = (O)x[e];
+    };
+    // few parts: a wave per (row, 256 values); many: a workgroup, whose waves take parts in turn and are added in order
+    const int by = parts > 8 ? 1 : 4;
+    for (int64_t w0 = (int64_t)blockIdx.x * by; w0 < (int64_t)total * chunks; w0 += (int64_t)gridDim.x * by) {
+        const int64_t w = by == 4 ? w0 + wave : w0;
+        const int64_t r = w / chunks;
+        const int d = (int)(w - r * chunks) * 256 + lane * 4;
+        const int i = r < total ? inv[r] : -1;
+        f32x4 x = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (i >= 0 && d < dimp) {
+#pragma unroll 4
+            for (int p = by == 4 ? 0 : wave; p < parts; p += by == 4 ? 1 : 4)
+                x += *reinterpret_cast<const f32x4 *>(part + ((int64_t)p * n + i) * dimp + d);
         }
+        if (by == 4) {
+            if (r < total && d < dim) put(r, d, x);
+            continue;
+        }
+        if (wave) red[wave - 1][lane] = x;
+        __syncthreads();
+        if (wave == 0 && d < dim) put(r, d, x + red[0][lane] + red[1][lane] + red[2][lane]);
+        __syncthreads();
     }
 }
 
@@ -722,12 +799,21 @@ __global__ __launch_bounds__(256) void k_hidden_grad(const float *part, const in
 template <class O>
 __global__ __launch_bounds__(256) void k_bias_grad(const float *sums, int64_t ld, const int *n_d, int bc, int per_tile, int vocab,
                                                    const float *scale, O *out) {
-    const int v = blockIdx.x * 256 + threadIdx.x;
-    if (v >= vocab) return;
+    __shared__ float red[8][33];
+    const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
+    const int v = blockIdx.x * 32 + x;
     const int blocks = (*n_d + bc - 1) / bc * per_tile;
     float s = 0.f;
-    for (int b = 0; b < blocks; b++) s += sums[b * ld + v];
-    out[v] = (O)(s * *scale);
+    if (v < vocab) {
+#pragma unroll 4
+        for (int b = y; b < blocks; b += 8) s += sums[b * ld + v];
+    }
+    red[y][x] = s;
+    __syncthreads();
+    if (y == 0 && v < vocab) {
+        for (int i = 1; i < 8; i++) s += red[i][x];
+        out[v] = (O)(s * *scale);
+    }
 }
 
 // ---------------------------------------------------------------- term weights' small kernels
@@ -927,12 +1013,50 @@ __global__ __launch_bounds__(256) void k_entries_weight(Source h, const float *g
 
 // ---------------------------------------------------------------- host
 
-// Tiles: `Large` for whole batches (two workgroups of 4 waves per CU, three stages of 24 KiB, 128 x 64 per wave);
-// `Small` where the kept side is at most one tile of 64, and reading the vocabulary is what takes the time.
+// Tiles.  Two operands' tiles cross LDS once per wave that shares them, so the larger the wave's share the better the
+// matrix units are fed; but a tile needs work for every CU.
+//   Large  256 x 256, eight waves of 128 x 64, one workgroup per CU
+//   Mid    128 x 128, four waves of 64 x 64, two workgroups per CU: up to kMidRows rows
+//   Small  64 x 64, four waves of 32 x 32, four stages: up to kSmallRows rows, where reading the vocabulary is what
+//          takes the time
 template <class T, int NP, bool RK, bool CK>
-using Large = Tile<T, NP, 256, 128, 2, 2, 3, RK, CK>;
+using Large = Tile<T, NP, 256, 256, 2, 4, 2, 2, RK, CK>;
+template <class T, int NP, bool RK, bool CK>  // k-major operands: waves of 64 x 128, dW 880 -> 915 TFLOP/s
+using LargeK = Tile<T, NP, 256, 256, 4, 2, 2, 2, RK, CK>;
 template <class T, int NP, bool RK, bool CK>
-using Small = Tile<T, NP, 64, 64, 2, 2, 6, RK, CK>;
+using Mid = Tile<T, NP, 128, 128, 2, 2, 2, 2, RK, CK>;
+template <class T, int NP, bool RK, bool CK>
+using Small = Tile<T, NP, 64, 64, 2, 2, 4, 2, RK, CK>;
+
+constexpr int kSmallRows = 64, kMidRows = 1024;
+
+enum TileClass { kSmall, kMid, kLarge };
+TileClass class_of(int64_t rows) { return rows <= kSmallRows ? kSmall : rows <= kMidRows ? kMid : kLarge; }
+int edge_of(TileClass c) { return c == kSmall ? 64 : c == kMid ? 128 : 256; }
+int row_waves_of(TileClass) { return 2; }
+int col_waves_of(TileClass c) { return c == kLarge ? 4 : 2; }
+
+// CALL(tile template) for a class
+#define GSV_BY_CLASS(cls, CALL)   \
+    switch (cls) {                \
+        case kSmall: CALL(Small); break; \
+        case kMid: CALL(Mid); break;     \
+        default: CALL(Large); break;     \
+    }
+// CALL(operand type, planes) for a head's type
+#define GSV_BY_TYPE(type, CALL)              \
+    switch (type) {                          \
+        case GS_H_F32: CALL(Bf16, 3); break; \
+        case GS_H_F16: CALL(F16, 1); break;  \
+        default: CALL(Bf16, 1); break;       \
+    }
+// CALL(value type) for a type of values
+#define GSV_BY_VALUE(type, CALL)             \
+    switch (type) {                          \
+        case GS_H_F32: CALL(float); break;   \
+        case GS_H_F16: CALL(_Float16); break; \
+        default: CALL(__bf16); break;        \
+    }
 
 int cu_count(int *cus) {
     int dev = 0;
@@ -941,17 +1065,16 @@ int cu_count(int *cus) {
     return GS_OK;
 }
 
-int es_of(int type) { return type == GS_H_F32 ? 4 : 2; }
+bool known(int type) { return type == GS_H_F32 || type == GS_H_F16 || type == GS_H_BF16; }
 
 bool vec_ok(const void *p, int type, int64_t s0, int64_t s1, int64_t sd) {
-    return sd == 1 && s0 % 4 == 0 && s1 % 4 == 0 && (uintptr_t)p % (4 * es_of(type)) == 0;
+    return sd == 1 && s0 % 4 == 0 && s1 % 4 == 0 && (uintptr_t)p % (type == GS_H_F32 ? 16 : 8) == 0;
 }
 
 int check_head(const gs_vocab_head *h) {
     GS_REQUIRE(h, "head is NULL");
-    GS_REQUIRE(h->type == GS_H_F32 || h->type == GS_H_F16 || h->type == GS_H_BF16, "unknown hidden type %d", h->type);
-    GS_REQUIRE(h->bias_type == GS_H_F32 || h->bias_type == GS_H_F16 || h->bias_type == GS_H_BF16, "unknown bias type %d",
-               h->bias_type);
+    GS_REQUIRE(known(h->type), "unknown hidden type %d", h->type);
+    GS_REQUIRE(known(h->bias_type), "unknown bias type %d", h->bias_type);
     GS_REQUIRE(h->texts >= 0 && h->length >= 0, "negative texts or length");
     GS_REQUIRE((int64_t)h->texts * h->length <= (1 << 28), "%lld rows exceed 2^28", (long long)h->texts * h->length);
     GS_REQUIRE(h->dim >= 1 && h->dim <= 32768, "dim=%d outside [1, 32768]", h->dim);
@@ -959,9 +1082,10 @@ int check_head(const gs_vocab_head *h) {
     return GS_OK;
 }
 
-struct Layout {  // of what both losses and term weights keep in memory
+struct Layout {
     int rows, dimp, planes, vocabp;
     bool w_direct;
+    TileClass cls;
 };
 
 Layout layout_of(const gs_vocab_head *h) {
@@ -973,20 +1097,22 @@ Layout layout_of(const gs_vocab_head *h) {
     // the product reads the vocabulary's rows where they are if each is whole 16-byte pieces
     l.w_direct = l.planes == 1 && h->dim % kStep == 0 && h->weight_dim_stride == 1 && h->weight_row_stride % 8 == 0 &&
                  h->weight_row_stride >= h->dim && h->weight_row_stride < (1 << 20) && (uintptr_t)h->weight_d % 16 == 0;
+    l.cls = class_of(l.rows);
     return l;
 }
 
-struct Saved {
+// What every call makes first.
+struct Common {
     int *n, *rows, *inv, *seg;
     float *bias;
     uint16_t *hidden, *weight;
 };
 
-void take_saved(gs_arena &a, const Layout &l, const gs_vocab_head *h, bool seg, Saved *s) {
+void take_common(gs_arena &a, const Layout &l, const gs_vocab_head *h, bool texts, Common *s) {
     s->n = a.take<int>(64);
     s->rows = a.take<int>(l.rows);
-    s->inv = seg ? nullptr : a.take<int>(l.rows);
-    s->seg = seg ? a.take<int>(l.rows + kRowPad) : nullptr;
+    s->inv = texts ? nullptr : a.take<int>(l.rows);
+    s->seg = texts ? a.take<int>(l.rows + kRowPad) : nullptr;
     s->bias = a.take<float>(l.vocabp);
     s->hidden = a.take<uint16_t>((size_t)l.rows * l.planes * l.dimp);
     s->weight = l.w_direct ? nullptr : a.take<uint16_t>((size_t)h->vocab * l.planes * l.dimp);
@@ -1001,136 +1127,132 @@ Source weight_source(const gs_vocab_head *h) {
                   vec_ok(h->weight_d, h->type, 0, h->weight_row_stride, h->weight_dim_stride)};
 }
 
-Operand hidden_operand(const Layout &l, const Saved &s) {
+Operand hidden_operand(const Layout &l, const Common &s) {
     return Operand{s.hidden, (int64_t)l.planes * l.dimp, l.dimp, (int64_t)l.planes * l.dimp};
 }
-Operand weight_operand(const Layout &l, const Saved &s, const gs_vocab_head *h) {
+Operand weight_operand(const Layout &l, const Common &s, const gs_vocab_head *h) {
     if (l.w_direct) return Operand{(const uint16_t *)h->weight_d, h->weight_row_stride, 0, l.dimp};
     return Operand{s.weight, (int64_t)l.planes * l.dimp, l.dimp, (int64_t)l.planes * l.dimp};
 }
 
-int pack_rows(const gs_vocab_head *h, const Source &src, const int *rows, const int *n_d, int n, int dimp, uint16_t *out,
-              hipStream_t s) {
-    if (n <= 0) return GS_OK;
-    const unsigned g = gs_blocks(n, 4, 8192);
-    switch (h->type) {
-        case GS_H_F32: hipLaunchKernelGGL((k_pack<GS_H_F32, 3>), dim3(g), dim3(256), 0, s, src, rows, n_d, n, dimp, out); break;
-        case GS_H_F16: hipLaunchKernelGGL((k_pack<GS_H_F16, 1>), dim3(g), dim3(256), 0, s, src, rows, n_d, n, dimp, out); break;
-        default: hipLaunchKernelGGL((k_pack<GS_H_BF16, 1>), dim3(g), dim3(256), 0, s, src, rows, n_d, n, dimp, out); break;
-    }
+// Kept rows, bias, cleared memory, then hidden states and (where needed) vocabulary rows in the product's form.
+int prepare(const gs_vocab_head *h, const Layout &l, const Keep &keep, const Common &c, float *zero, int64_t zeros, hipStream_t s) {
+    hipLaunchKernelGGL(k_setup, dim3(1 + gs_blocks(l.vocabp + zeros / 4, 1024, 1024)), dim3(1024), 0, s, keep,
+                       h->length > 0 ? h->length : 1, c.rows, c.inv, c.seg, c.n, h->bias_d, h->bias_type, h->vocab, l.vocabp,
+                       c.bias, zero, zeros);
+    GS_CHECK_LAUNCH();
+    const int w_rows = l.w_direct ? 0 : h->vocab;
+    if (l.rows + w_rows == 0) return GS_OK;
+    const dim3 g(gs_blocks((int64_t)l.rows + w_rows, 4, 8192));
+    const Source hs = hidden_source(h), ws = weight_source(h);
+#define GSV_PACK(HT, NP) \
+    hipLaunchKernelGGL((k_pack<HT, NP>), g, dim3(256), 0, s, hs, c.rows, c.n, c.hidden, ws, w_rows, c.weight, l.dimp)
+    if (h->type == GS_H_F32) GSV_PACK(GS_H_F32, 3);
+    else if (h->type == GS_H_F16) GSV_PACK(GS_H_F16, 1);
+    else GSV_PACK(GS_H_BF16, 1);
+#undef GSV_PACK
     GS_CHECK_LAUNCH();
     return GS_OK;
 }
-
-// Kept rows, bias, hidden states and (where needed) vocabulary rows in the product's form.
-int prepare(const gs_vocab_head *h, const Layout &l, const uint8_t *keep, const Saved &sv, hipStream_t s) {
-    hipLaunchKernelGGL(k_kept_rows, dim3(1), dim3(1024), 0, s, keep, l.rows, h->length > 0 ? h->length : 1, sv.rows, sv.inv,
-                       sv.seg, sv.n);
-    GS_CHECK_LAUNCH();
-    hipLaunchKernelGGL(k_bias, dim3(gs_blocks(l.vocabp, 256)), dim3(256), 0, s, h->bias_d, h->bias_type, h->vocab, l.vocabp,
-                       sv.bias);
-    GS_CHECK_LAUNCH();
-    if (int rc = pack_rows(h, hidden_source(h), sv.rows, sv.n, l.rows, l.dimp, sv.hidden, s)) return rc;
-    if (!l.w_direct)
-        if (int rc = pack_rows(h, weight_source(h), nullptr, nullptr, h->vocab, l.dimp, sv.weight, s)) return rc;
-    return GS_OK;
-}
-
-// f.template operator()<T, NP>() for the head's type
-#define GSV_BY_TYPE(type, CALL)                  \
-    switch (type) {                              \
-        case GS_H_F32: CALL(Bf16, 3); break;     \
-        case GS_H_F16: CALL(F16, 1); break;      \
-        default: CALL(Bf16, 1); break;           \
-    }
-
-constexpr int kSmallRows = 64;
 
 // ---------------------------------------------------------------- losses
 
 struct LossPlan {
     Layout l;
-    int top, small;
-    int piece, pieces;     // terms per piece (a multiple of kRowPad)
-    int row_block;         // terms per softmax-sum block
-    int h_tr, h_bc, h_most, slots;
-    int64_t part_rows;     // rows of dH parts
+    int top;
+    int piece, pieces;   // terms per piece (a multiple of kRowPad)
+    int block, blocks;   // terms per softmax-sum block, and blocks
+    int most;            // parts of dH
+    int64_t part_rows;   // rows of all of dH's parts
+    int64_t sum_rows;    // rows of the bias's sums
 };
 
 LossPlan loss_plan(const gs_vocab_head *h, const gs_vocab_targets *t, int cus) {
     LossPlan p;
     p.l = layout_of(h);
     p.top = t->teacher_ids_d ? t->top : 1;
-    p.small = p.l.rows <= kSmallRows;
+    const int edge = edge_of(p.l.cls);
     const int64_t per = (int64_t)(p.l.rows > 0 ? p.l.rows : 1) * p.l.planes * 2;
     int64_t most = (int64_t)kPieceBytes / per / kRowPad * kRowPad;
     if (most < kRowPad) most = kRowPad;
     p.pieces = (int)((p.l.vocabp + most - 1) / most);
     p.piece = (int)round_up((p.l.vocabp + p.pieces - 1) / p.pieces, kRowPad);
     p.pieces = (p.l.vocabp + p.piece - 1) / p.piece;
-    p.row_block = p.small ? 32 : 128;
-    p.h_tr = (h->dim + (p.small ? 63 : 255)) / (p.small ? 64 : 256);
-    p.h_bc = p.small ? 64 : 128;
-    p.slots = 2 * cus;
-    p.h_most = p.piece / kStep / 8;
-    if (p.h_most < 1) p.h_most = 1;
-    // split(n) * n, split = slots / (h_tr * ceil(n / bc)): at most slots * bc / h_tr rows, or n
-    const int64_t wide = (int64_t)p.slots * p.h_bc / p.h_tr;
-    p.part_rows = p.l.rows > wide ? p.l.rows : wide;
+    p.block = edge / row_waves_of(p.l.cls);
+    p.blocks = (h->vocab + edge - 1) / edge * row_waves_of(p.l.cls);
+    p.most = p.piece / kStep / 8 < 64 ? p.piece / kStep / 8 : 64;
+    if (p.most < 1) p.most = 1;
+    // parts_of: parts that even out hold at most a piece's terms and the rows, parts that fill at most a tile's rows for
+    // each workgroup that runs at a time
+    const int tr = (h->dim + edge - 1) / edge;
+    const int64_t even = (int64_t)p.piece + p.l.rows, fill = (int64_t)2 * cus * edge / tr + p.l.rows;
+    const int64_t by_most = (int64_t)p.most * p.l.rows;
+    p.part_rows = even > fill ? even : fill;
+    if (p.part_rows > by_most) p.part_rows = by_most;
+    p.sum_rows = (int64_t)(p.l.rows + edge - 1) / edge * col_waves_of(p.l.cls);
     return p;
 }
 
 struct LossSaved {
-    Saved s;
+    Common c;
     float *lse2, *loss;
-    int *ids;
-    float *share, *ent;
+    int *ids;          // kept rows' entries
+    float *share;
+    uint16_t *first;
 };
 
 void take_loss_saved(gs_arena &a, const LossPlan &p, const gs_vocab_head *h, const gs_vocab_targets *t, LossSaved *s) {
-    take_saved(a, p.l, h, false, &s->s);
+    const bool teacher = t->teacher_ids_d != nullptr;
+    take_common(a, p.l, h, false, &s->c);
     s->lse2 = a.take<float>(p.l.rows);
     s->loss = a.take<float>(p.l.rows);
     s->ids = a.take<int>((size_t)p.l.rows * p.top);
-    s->share = t->teacher_ids_d ? a.take<float>((size_t)p.l.rows * p.top) : nullptr;
-    s->ent = t->teacher_ids_d ? a.take<float>(p.l.rows) : nullptr;
+    s->share = teacher ? a.take<float>((size_t)p.l.rows * p.top) : nullptr;
+    s->first = teacher ? a.take<uint16_t>((size_t)(p.l.vocabp / kRowPad + 1) * p.l.rows) : nullptr;
 }
 
 struct LossScratch {
     uint8_t *keep;
+    int *ids;          // source rows' entries of a teacher
+    float *share, *ent;
     float *target;
     float2 *part;
+    float *dots;
 };
-void take_loss_scratch(gs_arena &a, const LossPlan &p, LossScratch *s) {
-    s->keep = a.take<uint8_t>(p.l.rows);
-    s->target = a.take<float>(p.l.rows);
-    s->part = a.take<float2>((size_t)(p.l.vocabp / p.row_block) * p.l.rows);
+void take_loss_scratch(gs_arena &a, const LossPlan &p, const gs_vocab_targets *t, LossScratch *s) {
+    const bool teacher = t->teacher_ids_d != nullptr;
+    const size_t rows = p.l.rows, sums = (size_t)p.blocks * rows;
+    s->keep = teacher ? a.take<uint8_t>(rows) : nullptr;
+    s->ids = teacher ? a.take<int>(rows * p.top) : nullptr;
+    s->share = teacher ? a.take<float>(rows * p.top) : nullptr;
+    s->ent = teacher ? a.take<float>(rows) : nullptr;
+    s->target = teacher ? nullptr : a.take<float>(rows);
+    s->part = a.take<float2>(sums);
+    s->dots = teacher ? a.take<float>(sums) : nullptr;
 }
 
 struct GradScratch {
     float *factor, *scale, *sums, *part;
-    uint16_t *first, *dl;
-    int64_t sum_rows;
+    int *parts;
+    uint16_t *dl;
 };
 void take_grad_scratch(gs_arena &a, const LossPlan &p, GradScratch *s) {
-    const int bc = p.small ? 64 : 128;
     s->factor = a.take<float>(p.l.rows);
     s->scale = a.take<float>(64);
-    s->sum_rows = (p.l.rows + bc - 1) / bc * 2;
-    s->sums = a.take<float>((size_t)s->sum_rows * p.l.vocabp);
+    s->parts = a.take<int>(64);
+    s->sums = a.take<float>((size_t)p.sum_rows * p.l.vocabp);
     s->part = a.take<float>((size_t)p.part_rows * p.l.dimp);
-    s->first = p.top > 1 ? a.take<uint16_t>((size_t)(p.l.vocabp / kRowPad + 1) * p.l.rows) : nullptr;
     s->dl = a.take<uint16_t>((size_t)p.l.rows * p.l.planes * p.piece);
 }
 
 int check_targets(const gs_vocab_head *h, const gs_vocab_targets *t) {
     GS_REQUIRE(t, "targets are NULL");
-    GS_REQUIRE((t->targets_d != nullptr) != (t->teacher_ids_d != nullptr), "targets or a teacher's ids, not both or neither");
+    GS_REQUIRE((t->targets_d != nullptr) != (t->teacher_ids_d != nullptr) || (int64_t)h->texts * h->length == 0,
+               "targets or a teacher's ids, not both or neither");
     if (t->teacher_ids_d) {
         GS_REQUIRE(t->teacher_logits_d, "teacher ids without logits");
         GS_REQUIRE(t->top >= 1 && t->top <= kMaxTop, "top=%d outside [1, %d]", t->top, kMaxTop);
-        GS_REQUIRE(t->teacher_type == GS_H_F32 || t->teacher_type == GS_H_F16 || t->teacher_type == GS_H_BF16,
-                   "unknown teacher type %d", t->teacher_type);
+        GS_REQUIRE(known(t->teacher_type), "unknown teacher type %d", t->teacher_type);
         GS_REQUIRE(t->temperature > 0.f && t->temperature < INFINITY, "temperature=%g must be positive and finite",
                    (double)t->temperature);
     }
@@ -1139,49 +1261,56 @@ int check_targets(const gs_vocab_head *h, const gs_vocab_targets *t) {
 
 float tau_of(const gs_vocab_targets *t) { return t->teacher_ids_d ? t->temperature : 1.f; }
 
-// The tiles' k loop over a [k][x] operand moves its buffer by whole rows, so one row of logit gradients must stay
-// within a buffer's 2 GiB with its 32 rows: 32 rows * planes * piece * 2 bytes <= 2^31 holds for every piece here.
+Entries entries_of(const LossPlan &p, const LossSaved &s) { return Entries{s.ids, s.share, s.first, p.l.rows, p.top}; }
 
 template <class T, int NP>
-int run_sums(const gs_vocab_head *h, const LossPlan &p, const LossSaved &s, float2 *part, float scale, int cus, hipStream_t st) {
-    const Dims d{h->vocab, p.l.rows, p.l.dimp, s.s.n, 0, 1, 0, 1, 0, 0};
-    const Operand w = weight_operand(p.l, s.s, h), hid = hidden_operand(p.l, s.s);
-    const EpiSums e{s.s.bias, scale, part, p.l.rows};
-    if (p.small) return launch_product<Small<T, NP, false, false>>(w, hid, d, e, cus, st);
-    return launch_product<Large<T, NP, false, false>>(w, hid, d, e, cus, st);
+int run_sums(const gs_vocab_head *h, const LossPlan &p, const LossSaved &s, const LossScratch &x, float scale, int cus,
+             hipStream_t st) {
+    const Dims d{h->vocab, p.l.rows, p.l.dimp, s.c.n, 0, 1, 0};
+    const Operand w = weight_operand(p.l, s.c, h), hid = hidden_operand(p.l, s.c);
+#define GSV_SUMS(TL)                                                                                                     \
+    return s.share ? launch_product<TL<T, NP, false, false>>(                                                            \
+                         w, hid, d, EpiSums<true>{s.c.bias, scale, x.part, x.dots, p.l.rows, entries_of(p, s)}, cus, st)  \
+                   : launch_product<TL<T, NP, false, false>>(                                                            \
+                         w, hid, d, EpiSums<false>{s.c.bias, scale, x.part, x.dots, p.l.rows, entries_of(p, s)}, cus, st)
+    GSV_BY_CLASS(p.l.cls, GSV_SUMS)
+#undef GSV_SUMS
 }
 
 template <class T, int NP, class O>
-int run_grad(const gs_vocab_head *h, const LossPlan &p, const LossSaved &s, const GradScratch &g, float scale, bool dh, bool dw,
-             bool db, void *dw_d, int cus, hipStream_t st) {
+int run_grad(const gs_vocab_head *h, const LossPlan &p, const LossSaved &s, const GradScratch &g, float scale, bool want_dh,
+             bool want_db, void *dw_d, int cus, hipStream_t st) {
     using S = typename T::store_t;
-    const Operand w = weight_operand(p.l, s.s, h), hid = hidden_operand(p.l, s.s);
+    const Operand w = weight_operand(p.l, s.c, h), hid = hidden_operand(p.l, s.c);
     const Operand dl{g.dl, (int64_t)NP * p.piece, p.piece, (int64_t)NP * p.piece};
     for (int c = 0; c < p.pieces; c++) {
         const int v0 = c * p.piece, nv = min(p.piece, h->vocab - v0);
         if (nv <= 0) break;
         Operand wp = w;
         wp.p += (int64_t)v0 * w.stride;
-        const EpiLogitGrad<S> e{s.s.bias, scale, s.lse2, g.factor, s.s.rows, s.ids, s.share, g.first, p.l.rows, p.top, v0,
-                                g.dl, dl.stride, p.piece, db ? g.sums : nullptr, p.l.vocabp};
-        const Dims de{nv, p.l.rows, p.l.dimp, s.s.n, 0, 1, 0, 1, 0, 0};
-        int rc = p.small ? launch_product<Small<T, NP, false, false>>(wp, hid, de, e, cus, st)
-                         : launch_product<Large<T, NP, false, false>>(wp, hid, de, e, cus, st);
+        const EpiLogitGrad<S> e{s.c.bias, scale, s.lse2, g.factor, entries_of(p, s), v0, g.dl, dl.stride, p.piece,
+                                want_db ? g.sums : nullptr, p.l.vocabp};
+        const EpiHiddenPart eh{g.part, p.l.dimp, c > 0};
+        const EpiWeightGrad<O> ew{(O *)dw_d + (int64_t)v0 * h->dim, g.scale, h->dim, h->dim % 4 == 0};
+        const Dims de{nv, p.l.rows, p.l.dimp, s.c.n, 0, 1, 0};
+        const Dims dh{want_dh ? h->dim : 0, p.l.rows, nv, s.c.n, 0, 1, 0};
+        const Dims dw{dw_d ? h->dim : 0, nv, p.l.rows, s.c.n, 0, 0, 1};
+        int rc = GS_OK;
+#define GSV_GRAD(TL) rc = launch_product<TL<T, NP, false, false>>(wp, hid, de, e, cus, st)
+        GSV_BY_CLASS(p.l.cls, GSV_GRAD)
+#undef GSV_GRAD
         if (rc) return rc;
-        if (dh) {
-            const EpiHiddenPart eh{g.part, p.l.dimp, c > 0};
-            const Dims dd{h->dim, p.l.rows, nv, s.s.n, 0, 1, 0, 0, p.slots, p.h_most};
-            rc = p.small ? launch_product<Small<T, NP, true, false>>(wp, dl, dd, eh, cus, st)
-                         : launch_product<Large<T, NP, true, false>>(wp, dl, dd, eh, cus, st);
-            if (rc) return rc;
+        if (!want_dh && !dw_d) continue;
+#define GSV_PAIR(TL)                                                                                                  \
+    rc = launch_pair<TL<T, NP, true, false>, TL<T, NP, true, true>>(wp, dl, dh, eh, hid, dl, dw, ew, p.piece, p.most,  \
+                                                                    g.parts, cus, st)
+        switch (p.l.cls) {
+            case kSmall: GSV_PAIR(Small); break;
+            case kMid: GSV_PAIR(Mid); break;
+            default: GSV_PAIR(LargeK); break;
         }
-        if (dw) {
-            const EpiWeightGrad<O> ew{(O *)dw_d + (int64_t)v0 * h->dim, g.scale, h->dim, h->dim % 4 == 0};
-            const Dims dd{h->dim, nv, p.l.rows, s.s.n, 0, 0, 1, 1, 0, 0};
-            rc = p.small ? launch_product<Small<T, NP, true, true>>(hid, dl, dd, ew, cus, st)
-                         : launch_product<Large<T, NP, true, true>>(hid, dl, dd, ew, cus, st);
-            if (rc) return rc;
-        }
+#undef GSV_PAIR
+        if (rc) return rc;
     }
     return GS_OK;
 }
@@ -1195,7 +1324,7 @@ extern "C" int gs_vocab_loss_workspace(const gs_vocab_head *h, const gs_vocab_ta
     if (int rc = check_head(h)) return rc;
     if (int rc = check_targets(h, t)) return rc;
     GS_REQUIRE(saved_bytes && scratch_bytes && grad_bytes, "NULL size pointer");
-    int cus = 256;
+    int cus = 0;
     if (int rc = cu_count(&cus)) return rc;
     const LossPlan p = loss_plan(h, t, cus);
     LossSaved s;
@@ -1203,9 +1332,9 @@ extern "C" int gs_vocab_loss_workspace(const gs_vocab_head *h, const gs_vocab_ta
     GradScratch g;
     gs_arena a{nullptr, 0, 0}, b{nullptr, 0, 0}, c{nullptr, 0, 0};
     take_loss_saved(a, p, h, t, &s);
-    take_loss_scratch(b, p, &x);
+    take_loss_scratch(b, p, t, &x);
     take_grad_scratch(c, p, &g);
-    *saved_bytes = a.used + 256, *scratch_bytes = b.used + 256, *grad_bytes = c.used + 256;
+    *saved_bytes = a.used, *scratch_bytes = b.used, *grad_bytes = c.used;
     return GS_OK;
 }
 
@@ -1214,14 +1343,15 @@ extern "C" int gs_vocab_loss(const gs_vocab_head *h, const gs_vocab_targets *t, 
     if (int rc = check_head(h)) return rc;
     if (int rc = check_targets(h, t)) return rc;
     GS_REQUIRE(reduction >= GS_REDUCE_NONE && reduction <= GS_REDUCE_SUM, "unknown reduction %d", reduction);
-    int cus = 256;
+    GS_REQUIRE(saved_d && scratch_d && loss_d, "NULL loss or workspace");
+    int cus = 0;
     if (int rc = cu_count(&cus)) return rc;
     const LossPlan p = loss_plan(h, t, cus);
     LossSaved sv;
     LossScratch x;
     gs_arena a{(char *)saved_d, 0, saved_bytes}, b{(char *)scratch_d, 0, scratch_bytes};
     take_loss_saved(a, p, h, t, &sv);
-    take_loss_scratch(b, p, &x);
+    take_loss_scratch(b, p, t, &x);
     if (!a.ok() || !b.ok()) {
         gs_set_error("vocab_loss workspace too small: need %zu + %zu bytes, got %zu + %zu", a.used, b.used, saved_bytes,
                      scratch_bytes);
@@ -1230,46 +1360,42 @@ extern "C" int gs_vocab_loss(const gs_vocab_head *h, const gs_vocab_targets *t, 
     const hipStream_t s = gs_stream(stream);
     const int rows = p.l.rows;
     const float tau = tau_of(t);
-    if (reduction == GS_REDUCE_NONE && rows > 0) {
-        hipLaunchKernelGGL(k_fill, dim3(gs_blocks(rows, 256, 1024)), dim3(256), 0, s, loss_d, (int64_t)rows, 0.f);
+    const bool teacher = t->teacher_ids_d != nullptr;
+    if (teacher && rows > 0) {
+        const int th = t->top <= 64 ? 64 : t->top <= 128 ? 128 : 256;
+        hipLaunchKernelGGL(k_teacher, dim3(rows), dim3(th), 0, s, t->teacher_ids_d, t->teacher_logits_d, t->teacher_type, t->top,
+                           h->vocab, 1.f / tau, x.ids, x.share, x.ent, x.keep);
         GS_CHECK_LAUNCH();
     }
+    const Keep keep{x.keep, teacher ? nullptr : t->targets_d, t->ignore_index, h->vocab, rows};
+    if (int rc = prepare(h, p.l, keep, sv.c, loss_d, reduction == GS_REDUCE_NONE ? rows : 0, s)) return rc;
     if (rows > 0) {
-        if (t->teacher_ids_d) {
-            const int th = t->top <= 64 ? 64 : t->top <= 128 ? 128 : 256;
-            hipLaunchKernelGGL(k_teacher, dim3(rows), dim3(th), 0, s, t->teacher_ids_d, t->teacher_logits_d, t->teacher_type,
-                               t->top, h->vocab, 1.f / tau, sv.ids, sv.share, sv.ent, x.keep);
+        const dim3 g(gs_blocks(rows, 4, 4096));
+        if (teacher) {
+            hipLaunchKernelGGL(k_entries, g, dim3(256), 0, s, x.ids, x.share, p.top, sv.c.rows, sv.c.n, p.l.vocabp / kRowPad,
+                               (int64_t)rows, sv.ids, sv.share, sv.first);
         } else {
-            hipLaunchKernelGGL(k_targets, dim3(gs_blocks(rows, 256)), dim3(256), 0, s, t->targets_d, t->ignore_index, rows,
-                               h->vocab, sv.ids, x.keep);
+            const Source hs = hidden_source(h), ws = weight_source(h);
+#define GSV_TL(HT)                                                                                                         \
+    hipLaunchKernelGGL((k_target_logits<HT>), g, dim3(256), 0, s, hs, h->weight_d, h->weight_row_stride, h->weight_dim_stride, \
+                       ws.vec, sv.c.bias, t->targets_d, sv.c.rows, sv.c.n, sv.ids, x.target)
+            if (h->type == GS_H_F32) GSV_TL(GS_H_F32);
+            else if (h->type == GS_H_F16) GSV_TL(GS_H_F16);
+            else GSV_TL(GS_H_BF16);
+#undef GSV_TL
         }
         GS_CHECK_LAUNCH();
-    }
-    if (int rc = prepare(h, p.l, x.keep, sv.s, s)) return rc;
-    if (rows > 0) {
-        const Source hs = hidden_source(h), ws = weight_source(h);
-        const unsigned g = gs_blocks(rows, 4, 4096);
-#define GSV_TL(HT)                                                                                                        \
-    hipLaunchKernelGGL((k_target_logits<HT>), dim3(g), dim3(256), 0, s, hs, h->weight_d, h->weight_row_stride,             \
-                       h->weight_dim_stride, ws.vec, sv.s.bias, sv.ids, sv.share, p.top, sv.s.rows, sv.s.n, x.target)
-        if (h->type == GS_H_F32) GSV_TL(GS_H_F32);
-        else if (h->type == GS_H_F16) GSV_TL(GS_H_F16);
-        else GSV_TL(GS_H_BF16);
-#undef GSV_TL
-        GS_CHECK_LAUNCH();
         int rc = GS_OK;
-#define GSV_SUMS(T, NP) rc = run_sums<T, NP>(h, p, sv, x.part, kLog2e / tau, cus, s)
+#define GSV_SUMS(T, NP) rc = run_sums<T, NP>(h, p, sv, x, kLog2e / tau, cus, s)
         GSV_BY_TYPE(h->type, GSV_SUMS)
 #undef GSV_SUMS
         if (rc) return rc;
-        const int row_tile = p.small ? 64 : 256;
-        const int blocks = (h->vocab + row_tile - 1) / row_tile * (row_tile / p.row_block);
-        hipLaunchKernelGGL(k_row_loss, dim3(gs_blocks(rows, 16, 4096)), dim3(256), 0, s, x.part, (int64_t)rows, blocks, sv.s.rows,
-                           sv.s.n, x.target, sv.ent, tau, sv.lse2, sv.loss, reduction == GS_REDUCE_NONE ? loss_d : nullptr);
+        hipLaunchKernelGGL(k_row_loss, dim3(gs_blocks(rows, 16, 4096)), dim3(256), 0, s, x.part, x.dots, (int64_t)rows, p.blocks,
+                           sv.c.rows, sv.c.n, x.target, x.ent, tau, sv.lse2, sv.loss, reduction == GS_REDUCE_NONE ? loss_d : nullptr);
         GS_CHECK_LAUNCH();
     }
     if (reduction != GS_REDUCE_NONE) {
-        hipLaunchKernelGGL(k_loss_sum, dim3(1), dim3(1024), 0, s, sv.loss, sv.s.n, reduction == GS_REDUCE_MEAN, loss_d);
+        hipLaunchKernelGGL(k_loss_sum, dim3(1), dim3(1024), 0, s, sv.loss, sv.c.n, reduction == GS_REDUCE_MEAN, loss_d);
         GS_CHECK_LAUNCH();
     }
     return GS_OK;
@@ -1281,7 +1407,8 @@ extern "C" int gs_vocab_loss_grad(const gs_vocab_head *h, const gs_vocab_targets
     if (int rc = check_head(h)) return rc;
     if (int rc = check_targets(h, t)) return rc;
     GS_REQUIRE(reduction >= GS_REDUCE_NONE && reduction <= GS_REDUCE_SUM, "unknown reduction %d", reduction);
-    int cus = 256;
+    GS_REQUIRE(saved_d && scratch_d && grad_d, "NULL gradient or workspace");
+    int cus = 0;
     if (int rc = cu_count(&cus)) return rc;
     const LossPlan p = loss_plan(h, t, cus);
     LossSaved sv;
@@ -1297,45 +1424,29 @@ extern "C" int gs_vocab_loss_grad(const gs_vocab_head *h, const gs_vocab_targets
     const hipStream_t s = gs_stream(stream);
     const int rows = p.l.rows;
     const float tau = tau_of(t);
-    hipLaunchKernelGGL(k_row_factor, dim3(1), dim3(1024), 0, s, grad_d, reduction == GS_REDUCE_NONE, sv.s.rows, sv.s.n,
+    hipLaunchKernelGGL(k_row_factor, dim3(1), dim3(1024), 0, s, grad_d, reduction == GS_REDUCE_NONE, sv.c.rows, sv.c.n,
                        reduction == GS_REDUCE_MEAN, tau, h->type == GS_H_F16, g.factor, g.scale);
     GS_CHECK_LAUNCH();
-    if (p.top > 1 && rows > 0) {
-        hipLaunchKernelGGL(k_entry_starts, dim3(gs_blocks(rows, 64)), dim3(64), 0, s, sv.ids, p.top, sv.s.rows, sv.s.n,
-                           p.l.vocabp / kRowPad, kRowPad, (int64_t)rows, g.first);
-        GS_CHECK_LAUNCH();
-    }
     int rc = GS_OK;
-    const float scale = kLog2e / tau;
-    // with no rows every launch below is empty of tiles but for dW's, which writes its zeros
-    if (rows > 0 || dweight_d) {
-        if (h->type == GS_H_F32)
-            rc = run_grad<Bf16, 3, float>(h, p, sv, g, scale, dhidden_d, dweight_d, dbias_d, dweight_d, cus, s);
-        else if (h->type == GS_H_F16)
-            rc = run_grad<F16, 1, _Float16>(h, p, sv, g, scale, dhidden_d, dweight_d, dbias_d, dweight_d, cus, s);
-        else
-            rc = run_grad<Bf16, 1, __bf16>(h, p, sv, g, scale, dhidden_d, dweight_d, dbias_d, dweight_d, cus, s);
-        if (rc) return rc;
-    }
+    // without a kept row no launch has a tile but dW's, which writes its zeros
+    if (h->type == GS_H_F32) rc = run_grad<Bf16, 3, float>(h, p, sv, g, kLog2e / tau, dhidden_d, dbias_d, dweight_d, cus, s);
+    else if (h->type == GS_H_F16) rc = run_grad<F16, 1, _Float16>(h, p, sv, g, kLog2e / tau, dhidden_d, dbias_d, dweight_d, cus, s);
+    else rc = run_grad<Bf16, 1, __bf16>(h, p, sv, g, kLog2e / tau, dhidden_d, dbias_d, dweight_d, cus, s);
+    if (rc) return rc;
     if (dhidden_d && rows > 0) {
-        const unsigned gr = gs_blocks(rows, 4, 8192);
-#define GSV_HG(O)                                                                                                           \
-    hipLaunchKernelGGL((k_hidden_grad<O>), dim3(gr), dim3(256), 0, s, g.part, sv.s.inv, sv.s.n, rows, h->dim, p.l.dimp, p.h_tr, \
-                       p.h_bc, p.slots, p.h_most, g.scale, (O *)dhidden_d)
-        if (h->type == GS_H_F32) GSV_HG(float);
-        else if (h->type == GS_H_F16) GSV_HG(_Float16);
-        else GSV_HG(__bf16);
+        const dim3 gr(gs_blocks((int64_t)rows * ((h->dim + 255) / 256), 4, 8192));
+#define GSV_HG(O)                                                                                                        \
+    hipLaunchKernelGGL((k_hidden_grad<O>), gr, dim3(256), 0, s, g.part, sv.c.inv, sv.c.n, g.parts, rows, h->dim, p.l.dimp, \
+                       g.scale, (O *)dhidden_d)
+        GSV_BY_VALUE(h->type, GSV_HG)
 #undef GSV_HG
         GS_CHECK_LAUNCH();
     }
     if (dbias_d) {
-        const int bc = p.small ? 64 : 128;
-#define GSV_BG(O)                                                                                                            \
-    hipLaunchKernelGGL((k_bias_grad<O>), dim3(gs_blocks(h->vocab, 256)), dim3(256), 0, s, g.sums, (int64_t)p.l.vocabp, sv.s.n, bc, \
-                       2, h->vocab, g.scale, (O *)dbias_d)
-        if (h->bias_type == GS_H_F32) GSV_BG(float);
-        else if (h->bias_type == GS_H_F16) GSV_BG(_Float16);
-        else GSV_BG(__bf16);
+#define GSV_BG(O)                                                                                                              \
+    hipLaunchKernelGGL((k_bias_grad<O>), dim3((h->vocab + 31) / 32), dim3(256), 0, s, g.sums, (int64_t)p.l.vocabp, sv.c.n,       \
+                       edge_of(p.l.cls), col_waves_of(p.l.cls), h->vocab, g.scale, (O *)dbias_d)
+        GSV_BY_VALUE(h->bias_type, GSV_BG)
 #undef GSV_BG
         GS_CHECK_LAUNCH();
     }
@@ -1349,26 +1460,26 @@ extern "C" int gs_term_weights_workspace(const gs_vocab_head *h, int32_t tokens,
     GS_REQUIRE(bytes && grad_bytes, "NULL size pointer");
     const Layout l = layout_of(h);
     gs_arena a{nullptr, 0, 0}, b{nullptr, 0, 0};
-    Saved s;
-    take_saved(a, l, h, true, &s);
+    Common c;
+    take_common(a, l, h, true, &c);
     const size_t n = (size_t)h->texts * h->vocab;
-    a.take<char>(n * (tokens ? 8 : 4));
+    a.take<float>(n * (tokens ? 2 : 1));
     b.take<float>(n);
     b.take<int>(n);
     b.take<int>((size_t)h->texts * (h->length + 1));
-    *bytes = a.used + 256, *grad_bytes = b.used + 256;
+    *bytes = a.used, *grad_bytes = b.used;
     return GS_OK;
 }
 
 extern "C" int gs_term_weights(const gs_vocab_head *h, const uint8_t *mask_d, float *weights_d, int32_t *tokens_d,
                                void *workspace_d, size_t workspace_bytes, void *stream) {
     if (int rc = check_head(h)) return rc;
-    int cus = 256;
+    int cus = 0;
     if (int rc = cu_count(&cus)) return rc;
     const Layout l = layout_of(h);
     gs_arena a{(char *)workspace_d, 0, workspace_bytes};
-    Saved sv;
-    take_saved(a, l, h, true, &sv);
+    Common c;
+    take_common(a, l, h, true, &c);
     const int64_t n = (int64_t)h->texts * h->vocab;
     const int64_t words = tokens_d ? 2 * n : n;
     float *best = a.take<float>(words);
@@ -1377,38 +1488,39 @@ extern "C" int gs_term_weights(const gs_vocab_head *h, const uint8_t *mask_d, fl
         return GS_ENOSPC;
     }
     if (n == 0) return GS_OK;
+    GS_REQUIRE(weights_d && workspace_d, "NULL weights or workspace");
     const hipStream_t s = gs_stream(stream);
-    hipLaunchKernelGGL(k_fill, dim3(gs_blocks(words, 256, 4096)), dim3(256), 0, s, best, words, 0.f);
-    GS_CHECK_LAUNCH();
+    if (int rc = prepare(h, l, Keep{mask_d, nullptr, 0, h->vocab, l.rows}, c, best, words, s)) return rc;
     if (l.rows > 0) {
-        // seg is read a whole tile at a time: -1 past the kept rows
-        hipLaunchKernelGGL(k_fill, dim3(gs_blocks(l.rows + kRowPad, 256, 1024)), dim3(256), 0, s, (float *)sv.seg,
-                           (int64_t)l.rows + kRowPad, __builtin_bit_cast(float, 0xFFFFFFFFu));
-        GS_CHECK_LAUNCH();
-        if (int rc = prepare(h, l, mask_d, sv, s)) return rc;
-        const Dims d{l.rows, h->vocab, l.dimp, sv.n, 1, 0, 0, 1, 0, 0};
-        const Operand hid = hidden_operand(l, sv), w = weight_operand(l, sv, h);
+        const Dims d{l.rows, h->vocab, l.dimp, c.n, 1, 0, 0};
+        const Operand hid = hidden_operand(l, c), w = weight_operand(l, c, h);
+        const EpiTextMax<true> et{c.bias, c.seg, best, h->vocab};
+        const EpiTextMax<false> ef{c.bias, c.seg, best, h->vocab};
         int rc = GS_OK;
-#define GSV_MAX(T, NP)                                                                                                    \
-    if (tokens_d) {                                                                                                       \
-        const EpiTextMax<true> e{sv.bias, sv.seg, best, h->vocab};                                                        \
-        rc = l.rows <= kSmallRows ? launch_product<Small<T, NP, false, false>>(hid, w, d, e, cus, s)                      \
-                                  : launch_product<Large<T, NP, false, false>>(hid, w, d, e, cus, s);                     \
-    } else {                                                                                                              \
-        const EpiTextMax<false> e{sv.bias, sv.seg, best, h->vocab};                                                       \
-        rc = l.rows <= kSmallRows ? launch_product<Small<T, NP, false, false>>(hid, w, d, e, cus, s)                      \
-                                  : launch_product<Large<T, NP, false, false>>(hid, w, d, e, cus, s);                     \
-    }
-        GSV_BY_TYPE(h->type, GSV_MAX)
-#undef GSV_MAX
+#define GSV_TILE(TL) rc = tokens_d ? launch_product<TL<GSV_T, false, false>>(hid, w, d, et, cus, s) \
+                                   : launch_product<TL<GSV_T, false, false>>(hid, w, d, ef, cus, s)
+        if (h->type == GS_H_F32) {
+#define GSV_T Bf16, 3
+            GSV_BY_CLASS(l.cls, GSV_TILE)
+#undef GSV_T
+        } else if (h->type == GS_H_F16) {
+#define GSV_T F16, 1
+            GSV_BY_CLASS(l.cls, GSV_TILE)
+#undef GSV_T
+        } else {
+#define GSV_T Bf16, 1
+            GSV_BY_CLASS(l.cls, GSV_TILE)
+#undef GSV_T
+        }
+#undef GSV_TILE
         if (rc) return rc;
     }
     const unsigned g = gs_blocks(n, 256, 8192);
     const int length = h->length > 0 ? h->length : 1;
     if (tokens_d)
-        hipLaunchKernelGGL(k_term_weights<true>, dim3(g), dim3(256), 0, s, best, n, h->vocab, sv.rows, length, weights_d, tokens_d);
+        hipLaunchKernelGGL(k_term_weights<true>, dim3(g), dim3(256), 0, s, best, n, h->vocab, c.rows, length, weights_d, tokens_d);
     else
-        hipLaunchKernelGGL(k_term_weights<false>, dim3(g), dim3(256), 0, s, best, n, h->vocab, sv.rows, length, weights_d, tokens_d);
+        hipLaunchKernelGGL(k_term_weights<false>, dim3(g), dim3(256), 0, s, best, n, h->vocab, c.rows, length, weights_d, tokens_d);
     GS_CHECK_LAUNCH();
     return GS_OK;
 }

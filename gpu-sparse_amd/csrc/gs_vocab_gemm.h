@@ -45,7 +45,7 @@ struct F16 {
     }
 };
 
-constexpr int kStep = 32;  // k values per stage: one 16x16x32 product deep
+constexpr int kStep = 64;  // k values per stage: two 16x16x32 products deep, and whole 128-byte lines of [x][k] rows
 
 // A 16-bit matrix.  [x][k]: row x starts at p + x * stride; [k][x]: row k does.  Plane i of an
 // fp32 matrix starts `plane` values further along each row.
@@ -61,14 +61,7 @@ struct Dims {
     int32_t r, c, k;
     const int32_t *n_d;
     int32_t dev_r, dev_c, dev_k;  // 1: the size is min(*n_d, the one given)
-    int32_t split;                // parts of k, each a tile of its own; 0: as many as fill `slots` workgroups,
-    int32_t slots, most;          //   at most `most` (parts_of)
 };
-
-// Parts of k for a product of tr x ceil(c / bc) tiles.  Device code: c is known there alone.
-__device__ __forceinline__ int parts_of(int c, int tr, int bc, int slots, int most) {
-    return max(1, min(most, slots / max(1, tr * ((c + bc - 1) / bc))));
-}
 
 // The plane pairs, smallest products first, so that they are summed before the sum is large: (2,0) (0,2) (1,1) (1,0)
 // (0,1) (0,0).
@@ -82,77 +75,74 @@ __device__ __forceinline__ int turn(int k) {
     return X >= 128 ? (k & 3) | ((k >> 1) & 4) : k & 3;
 }
 
-// Issues one stage's 1 KiB pieces of an operand that belong to this wave, straight to LDS.
-// [x][k]: a piece is 16 rows of 64 bytes, and slot s of row x holds 16-byte chunk s ^ (x >> 1 & 3), so that the
-// eight rows that one read cycle takes lie in different banks.  [k][x]: a piece is 1024 / (2 X) rows of X values,
-// chunks moved in pairs by the k row, so that the four k rows of a transposing read do.
-template <int X, bool KM, int NW>
-struct Loader {
-    static constexpr int pieces = X / 16 / NW;
-    int off[pieces];
-    __device__ __forceinline__ void init(const Operand &o, int wave, int lane) {
-#pragma unroll
-        for (int u = 0; u < pieces; u++) {
-            const int at = ((wave * pieces + u) << 6) + lane;  // 16-byte slot of the tile
-            if (KM) {
-                constexpr int per = X / 8;
-                const int k = at / per, s = at % per;
-                off[u] = (int)(k * o.stride * 2) + (s ^ (turn<X>(k) << 1)) * 16;
-            } else {
-                const int x = at >> 2, s = at & 3;
-                off[u] = (int)(x * o.stride * 2) + (s ^ ((x >> 1) & 3)) * 16;
-            }
-        }
-    }
-    __device__ __forceinline__ void issue(__amdgpu_buffer_rsrc_t r, lds_t lds, int soff, int wave) const {
-#if defined(__HIP_DEVICE_COMPILE__)  // the host pass does not know 16-byte pieces and would leave the kernel out
-#pragma unroll
-        for (int u = 0; u < pieces; u++)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)(lds + ((wave * pieces + u) << 10)),
-                                                     16, off[u], soff, 0, 0);
-#endif
-    }
-};
-
+// The first `values` values at p; reads past them give 0.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc64(const uint16_t *p, int64_t values) {
     const int64_t b = values <= 0 ? 0 : values * 2;
     return gs_rsrc(p, (uint32_t)(b > 0x7FFFFFF0ll ? 0x7FFFFFF0ll : b));
 }
 
-// The buffer of one stage: [x][k] tiles keep one for all k (the offset moves), [k][x] tiles move it.
+// Issues one stage's 1 KiB pieces of an operand that belong to this wave, straight to LDS.
+// [x][k]: a piece is eight rows of 128 bytes, and slot s of row x holds 16-byte chunk s ^ (x & 7), so that the eight rows
+// that one read cycle takes lie in different banks.  (Rows of 64 bytes asked the L2 for half lines: 20% slower.)  [k][x]:
+// a piece is 1024 / (2 X) rows of X values, chunks moved in pairs by the k row, so that the rows of a transposing read do.
+// The waves take pieces in turn, so that a wave's pieces differ by whole rows and share one offset per lane.
+template <int X, bool KM, int NW>
+struct Loader {
+    static constexpr int pieces = X / 8 / NW;
+    static constexpr int per = KM ? X / 8 : 8;       // 16-byte chunks of a row
+    static constexpr int step = 64 / per * NW;       // rows between a wave's pieces
+    static_assert(pieces == 1 || step % (KM ? 16 : 8) == 0, "chunks move alike in all of a wave's pieces");
+    __device__ __forceinline__ static int offset(const Operand &o, int wave, int lane) {
+        const int row = wave * (64 / per) + lane / per, s = lane % per;
+        return (int)(row * o.stride * 2) + (s ^ (KM ? turn<X>(row) << 1 : row & 7)) * 16;
+    }
+    // values: what may be read from p on; gap: bytes between a wave's pieces
+    __device__ __forceinline__ static void issue(const uint16_t *p, int64_t values, int gap, int off, lds_t lds, int wave) {
+#if defined(__HIP_DEVICE_COMPILE__)  // the host pass does not know 16-byte pieces and would leave the kernel out
+        const auto r = rsrc64(p, values);
+#pragma unroll
+        for (int u = 0; u < pieces; u++)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)(lds + ((wave + u * NW) << 10)), 16,
+                                                     off + u * gap, 0, 0, 0);
+#endif
+    }
+};
+
+// Where stage k of an operand's tile at x0 starts, and how much may be read from there.
 template <bool KM>
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t stage_rsrc(const Operand &o, int64_t x0, int64_t nx, int64_t k,
-                                                             int64_t nk, int plane) {
-    if (KM) return rsrc64(o.p + k * o.stride + plane * o.plane + x0, (nk - k - 1) * o.stride + o.width - plane * o.plane - x0);
-    return rsrc64(o.p + x0 * o.stride, (nx - x0 - 1) * o.stride + o.width);
+__device__ __forceinline__ const uint16_t *stage_at(const Operand &o, int64_t x0, int64_t nx, int64_t k, int64_t nk, int plane,
+                                                    int64_t *values) {
+    const int64_t row = KM ? k : x0, rows = KM ? nk : nx, in = plane * o.plane + (KM ? x0 : k);
+    *values = (rows - row - 1) * o.stride + o.width - in;
+    return o.p + row * o.stride + in;
 }
 
-// Fragments of 16 rows (columns) x 32 k values: lane l holds row l & 15, k = 8 (l >> 4) .. + 7.
+// Fragments of 16 rows (columns) x 32 k values, half h of a stage: lane l holds row l & 15, k = 32 h + 8 (l >> 4) .. + 7.
 template <int X, bool KM, int M>
 struct Frags {
-    int at[KM ? M : 1];
+    int at[KM ? M : 2];
     __device__ __forceinline__ void init(int x0, int lane) {  // x0: the wave's first row in the tile
+        const int i = lane & 15, q = lane >> 4;
         if (KM) {
-            const int i = lane & 15, q = lane >> 4;
             const int k = 8 * q + (i >> 2);
             const int g = turn<X>(k);
             const int base = k * (X * 2) + ((i >> 1) & 1) * 16 + (i & 1) * 8;
 #pragma unroll
             for (int m = 0; m < M; m++) at[m] = base + (((x0 >> 4) + m) ^ g) * 32;
         } else {
-            const int i = lane & 15, q = lane >> 4;
-            at[0] = (x0 + i) * 64 + (q ^ ((i >> 1) & 3)) * 16;
+            at[0] = (x0 + i) * 128 + (q ^ (i & 7)) * 16;
+            at[1] = at[0] ^ 64;
         }
     }
-    __device__ __forceinline__ s16x8 read(lds_t lds, int m) const {
+    __device__ __forceinline__ s16x8 read(lds_t lds, int m, int h) const {
         typedef __attribute__((address_space(3))) s16x4 *lp4;
         typedef __attribute__((address_space(3))) s16x8 *lp8;
         if (KM) {
-            const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp4)(lds + at[m]));
-            const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp4)(lds + at[m] + 4 * X * 2));
+            const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp4)(lds + at[m] + h * 64 * X));
+            const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp4)(lds + at[m] + h * 64 * X + 8 * X));
             return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
         }
-        return *(lp8)(lds + at[0] + m * 1024);
+        return *(lp8)(lds + at[h] + m * 2048);
     }
 };
 
@@ -162,18 +152,19 @@ __device__ __forceinline__ void wait_loads() {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 __device__ __forceinline__ void tile_barrier() {
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+    asm volatile("" ::: "memory");
 }
 
-template <class T, int NP, int BR_, int BC_, int WR_, int WC_, int NS_, bool RK, bool CK>
+// A workgroup's tile: BR x BC over WR x WC waves, NS stages in LDS, OCC waves per SIMD.
+template <class T, int NP, int BR_, int BC_, int WR_, int WC_, int NS_, int OCC, bool RK, bool CK>
 struct Tile {
     using type = T;
     static constexpr int BR = BR_, BC = BC_, WR = WR_, WC = WC_, NS = NS_, planes = NP;
-    static constexpr int waves = WR * WC, threads = 64 * waves;
+    static constexpr int waves = WR * WC, threads = 64 * waves, waves_per_simd = OCC;
     static constexpr int MR = BR / WR / 16, MC = BC / WC / 16;
-    static constexpr int stage_bytes = (BR + BC) * 64;
+    static constexpr int stage_bytes = (BR + BC) * kStep * 2;
     static constexpr int lds_bytes = NS * stage_bytes;
     static constexpr bool r_kmajor = RK, c_kmajor = CK;
 };
@@ -185,110 +176,258 @@ struct Place {
     int n_r, n_c;
 };
 
-// Persistent over tiles.  Workgroups of one XCD (blockIdx mod 8) take a contiguous run of tiles, eight tiles of
-// rows to each tile of columns, so that what runs at a time in an XCD shares operands in its L2.
+// A product's sizes as the device knows them.
+struct Shape {
+    int nr, nc, nk, tr, tc, steps;
+};
+template <class TL>
+__device__ __forceinline__ Shape shape_of(const Dims &d, int n_dev) {
+    Shape s;
+    s.nr = d.dev_r ? min(n_dev, d.r) : d.r;
+    s.nc = d.dev_c ? min(n_dev, d.c) : d.c;
+    s.nk = d.dev_k ? min(n_dev, d.k) : d.k;
+    s.tr = (s.nr + TL::BR - 1) / TL::BR;
+    s.tc = (s.nc + TL::BC - 1) / TL::BC;
+    s.steps = (s.nk + kStep - 1) / kStep;
+    return s;
+}
+
+// One product of a launch: tiles [0, tr * tc * parts) of it, each part a range of k.
 template <class TL, class Epi>
-__global__ __launch_bounds__(TL::threads, 2) void k_product(Operand R, Operand C, Dims d, Epi epi) {
+struct Side {
+    using tile = TL;
+    Operand R, C;
+    Dims d;
+    Epi epi;
+};
+
+struct Work {  // a tile: where it lies, which part of k, its first k step and how many
+    int r0, c0, part, k0, per;
+};
+// Tile t.  Eight tiles of rows go with each tile of columns, so that tiles in a row share operands.
+template <class TL>
+__device__ __forceinline__ Work work_of(const Shape &s, int parts, int t) {
+    const int area = s.tr * s.tc, part = t / area, in = t - part * area;
+    const int group = in / (8 * s.tc), left = in - group * 8 * s.tc;
+    const int tall = min(8, s.tr - group * 8);
+    const int k0 = (int)((int64_t)s.steps * part / parts);
+    return Work{(group * 8 + left % tall) * TL::BR, (left / tall) * TL::BC, part, k0,
+                (int)((int64_t)s.steps * (part + 1) / parts) - k0};
+}
+
+// The stages of a workgroup's tiles, issued one after the other whatever tile they belong to: while a tile's epilogue
+// runs, the next one's first stages are on their way.
+template <class SA, class SB>
+struct Stream {
+    using TA = typename SA::tile;
+    using TB = typename SB::tile;
+    using LR = Loader<TA::BR, TA::r_kmajor, TA::waves>;
+    using LC = Loader<TA::BC, TA::c_kmajor, TA::waves>;
+    static constexpr int loads = LR::pieces + LC::pieces;
+    Work w;
+    int r_off, c_off;     // the lane's
+    int r_gap, c_gap;
+    const uint16_t *r_p, *c_p;  // the next stage of either operand, what may be read from there, and the way to the one after
+    int64_t r_n, c_n, r_by, c_by;
+    int t, last, by, na;  // tiles t, t + by, ... below last; those below na are the first product's
+    int ik, seg, buf, left;
+
+    template <class TL>
+    __device__ __forceinline__ void offsets(const Operand &R, const Operand &C, int wave, int lane) {
+        using R_ = Loader<TL::BR, TL::r_kmajor, TL::waves>;
+        using C_ = Loader<TL::BC, TL::c_kmajor, TL::waves>;
+        r_off = R_::offset(R, wave, lane);
+        c_off = C_::offset(C, wave, lane);
+        r_gap = (int)(R_::step * R.stride * 2);
+        c_gap = (int)(C_::step * C.stride * 2);
+        r_by = TL::r_kmajor ? kStep * R.stride : kStep;
+        c_by = TL::c_kmajor ? kStep * C.stride : kStep;
+    }
+    // Moves to the first stage of plane pair seg
+    template <class TL>
+    __device__ __forceinline__ void start(const Operand &R, const Operand &C, const Shape &s) {
+        const int pr = TL::planes == 3 ? plane_r(seg) : 0, pc = TL::planes == 3 ? plane_c(seg) : 0;
+        r_p = stage_at<TL::r_kmajor>(R, w.r0, s.nr, w.k0 * kStep, s.nk, pr, &r_n);
+        c_p = stage_at<TL::c_kmajor>(C, w.c0, s.nc, w.k0 * kStep, s.nk, pc, &c_n);
+        ik = 0;
+    }
+    // Moves to tile t, or the next one with stages
+    __device__ __forceinline__ void seek(const SA &A, const SB &B, const Shape &a, const Shape &b, int parts, int wave, int lane) {
+        for (; t < last; t += by) {
+            w = t < na ? work_of<TA>(a, parts, t) : work_of<TB>(b, 1, t - na);
+            left = w.per * (TA::planes == 3 ? 6 : 1);
+            if (left == 0) continue;
+            seg = 0;
+            if (t < na) {
+                offsets<TA>(A.R, A.C, wave, lane);
+                start<TA>(A.R, A.C, a);
+            } else {
+                offsets<TB>(B.R, B.C, wave, lane);
+                start<TB>(B.R, B.C, b);
+            }
+            return;
+        }
+    }
+    __device__ __forceinline__ bool issue(lds_t lds, const SA &A, const SB &B, const Shape &a, const Shape &b, int parts, int wave,
+                                          int lane) {
+        if (t >= last) return false;
+        const lds_t to = lds + buf * TA::stage_bytes;
+        LR::issue(r_p, r_n, r_gap, r_off, to, wave);
+        LC::issue(c_p, c_n, c_gap, c_off, to + TA::BR * kStep * 2, wave);
+        buf = buf == TA::NS - 1 ? 0 : buf + 1;
+        if (--left == 0) {
+            t += by;
+            seek(A, B, a, b, parts, wave, lane);
+        } else if (TA::planes == 3 && ++ik == w.per) {
+            seg++;
+            if (t < na) start<TA>(A.R, A.C, a);
+            else start<TB>(B.R, B.C, b);
+        } else {
+            r_p += r_by, c_p += c_by;
+            r_n -= r_by, c_n -= c_by;
+        }
+        return true;
+    }
+};
+
+// Parts of k for the first of two products that share a launch: as many as make its tiles as long as the second's, or
+// fill `slots` workgroups, at most `most`.  Device code: the sizes are known there alone.
+__device__ __forceinline__ int parts_of(int steps, int tiles, int other_steps, int other_tiles, int slots, int most) {
+    const int even = (steps + other_steps / 2) / max(1, other_steps);
+    const int fill = other_tiles >= slots ? 1 : (slots - other_tiles) / max(1, tiles);
+    return max(1, min(most, max(even, fill)));
+}
+
+struct Pairing {
+    int piece;     // most columns of the second product
+    int slots;     // workgroups
+    int most;      // parts
+    int *parts_d;  // receives the parts; NULL: one, and there is no second product
+};
+
+// One or two products in a launch.  Persistent: workgroups of one XCD (blockIdx mod 8) take a contiguous run of tiles, so
+// that what runs at a time in an XCD shares operands in its L2.
+template <class SA, class SB>
+__global__ __launch_bounds__(SA::tile::threads, SA::tile::waves_per_simd) void k_product(SA A, SB B, Pairing pair) {
+    using TA = typename SA::tile;
+    using TB = typename SB::tile;
+    static_assert(TA::lds_bytes == TB::lds_bytes && TA::MR == TB::MR && TA::MC == TB::MC, "one tile shape per launch");
     extern __shared__ __align__(1024) char smem[];
     const lds_t lds = (lds_t)smem;
     const int lane = gs_lane(), wave = gs_uniform((int)threadIdx.x >> 6);
-    const int wr = wave / TL::WC, wc = wave % TL::WC;
-    const int n_dev = d.n_d ? gs_uniform(*d.n_d) : 0;
-    const int nr = d.dev_r ? min(n_dev, d.r) : d.r, nc = d.dev_c ? min(n_dev, d.c) : d.c;
-    const int nk = d.dev_k ? min(n_dev, d.k) : d.k;
-    const int tr = (nr + TL::BR - 1) / TL::BR, tc = (nc + TL::BC - 1) / TL::BC;
-    const int steps = (nk + kStep - 1) / kStep;
-    const int split = d.split ? d.split : parts_of(nc, tr, TL::BC, d.slots, d.most);
-    const int64_t tiles = (int64_t)tr * tc * split;
+    const int wr = wave / TA::WC, wc = wave % TA::WC;
+    const int n = A.d.n_d ? gs_uniform(*A.d.n_d) : 0;
+    const Shape a = shape_of<TA>(A.d, n), b = shape_of<TB>(B.d, n);
+    int parts = 1, nb = 0;
+    if (pair.parts_d) {
+        nb = b.tr * b.tc;
+        // from a whole piece's size, so that every piece has the same parts
+        parts = parts_of((pair.piece + kStep - 1) / kStep, a.tr * a.tc, b.steps, b.tr * ((pair.piece + TB::BC - 1) / TB::BC),
+                         pair.slots, pair.most);
+        if (blockIdx.x == 0 && threadIdx.x == 0) *pair.parts_d = parts;
+    }
+    const int na = a.tr * a.tc * parts, tiles = na + nb;
+    const int xcds = gridDim.x >= 8 ? 8 : 1, xcd = blockIdx.x % xcds;
 
-    Loader<TL::BR, TL::r_kmajor, TL::waves> lr;
-    Loader<TL::BC, TL::c_kmajor, TL::waves> lc;
-    lr.init(R, wave, lane);
-    lc.init(C, wave, lane);
-    Frags<TL::BR, TL::r_kmajor, TL::MR> fr;
-    Frags<TL::BC, TL::c_kmajor, TL::MC> fc;
-    fr.init(wr * TL::MR * 16, lane);
-    fc.init(wc * TL::MC * 16, lane);
-    constexpr int loads = decltype(lr)::pieces + decltype(lc)::pieces;
+    Stream<SA, SB> st;
+    st.t = (int)((int64_t)tiles * xcd / xcds) + blockIdx.x / xcds;
+    st.last = (int)((int64_t)tiles * (xcd + 1) / xcds);
+    st.by = (gridDim.x - xcd + xcds - 1) / xcds;
+    st.na = na;
+    st.buf = 0;
+    const int first = st.t, last = st.last, by = st.by;
+    st.seek(A, B, a, b, parts, wave, lane);
+    constexpr int loads = Stream<SA, SB>::loads, NS = TA::NS;
+    int ahead = 0;  // stages issued and not yet left behind
+#pragma unroll
+    for (int s = 0; s < NS - 1; s++) ahead += st.issue(lds, A, B, a, b, parts, wave, lane);
+    int buf = 0;
 
-    const int xcds = gridDim.x >= 8 ? 8 : 1;
-    const int xcd = blockIdx.x % xcds, slot = blockIdx.x / xcds;
-    const int slots = (gridDim.x - xcd + xcds - 1) / xcds;
-    const int64_t first = tiles * xcd / xcds, last = tiles * (xcd + 1) / xcds;
-    for (int64_t t = first + slot; t < last; t += slots) {
-        const int sp = (int)(t / ((int64_t)tr * tc));
-        const int in = (int)(t - (int64_t)sp * tr * tc);
-        const int group = in / (8 * tc), left = in - group * 8 * tc;
-        const int tall = min(8, tr - group * 8);
-        const int r0 = (group * 8 + left % tall) * TL::BR, c0 = (left / tall) * TL::BC;
-        const int k_lo = (int)((int64_t)steps * sp / split), k_hi = (int)((int64_t)steps * (sp + 1) / split);
-        const int per = k_hi - k_lo;
-        const int total = per * (TL::planes == 3 ? 6 : 1);
+    auto landed = [&]() {  // the oldest of the stages ahead is there, for every wave; and every wave is past the one before
+        if (NS > 2 && ahead == NS - 1) wait_loads<(NS > 2 ? NS - 2 : 0) * loads>();
+        else wait_loads<0>();
+        tile_barrier();
+    };
+    landed();
+    ahead += st.issue(lds, A, B, a, b, parts, wave, lane);
 
+    // A tile.  The fragments of a half stage are read while the products of the half before run.  Before a stage's second
+    // half the next stage has to have landed, and this one, which every wave holds by then, makes room for another.
+    auto run = [&](auto &side, const Work &w, const Shape &s) {
+        using TL = typename std::remove_reference_t<decltype(side)>::tile;
+        Frags<TL::BR, TL::r_kmajor, TL::MR> fr;
+        Frags<TL::BC, TL::c_kmajor, TL::MC> fc;
+        fr.init(wr * TL::MR * 16, lane);
+        fc.init(wc * TL::MC * 16, lane);
         f32x4 acc[TL::MR][TL::MC];
 #pragma unroll
         for (int i = 0; i < TL::MR; i++)
 #pragma unroll
             for (int j = 0; j < TL::MC; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-
-        const auto r_all = stage_rsrc<false>(R, r0, nr, 0, 0, 0);
-        const auto c_all = stage_rsrc<false>(C, c0, nc, 0, 0, 0);
-        int ik = 0, iseg = 0, ibuf = 0;  // the next stage to issue
-        auto issue = [&]() {
-            const int pr = TL::planes == 3 ? plane_r(iseg) : 0, pc = TL::planes == 3 ? plane_c(iseg) : 0;
-            const int k = (k_lo + ik) * kStep;
-            const lds_t to = lds + ibuf * TL::stage_bytes;
-            if (TL::r_kmajor) lr.issue(stage_rsrc<true>(R, r0, 0, k, nk, pr), to, 0, wave);
-            else lr.issue(r_all, to, (int)(pr * R.plane + k) * 2, wave);
-            if (TL::c_kmajor) lc.issue(stage_rsrc<true>(C, c0, 0, k, nk, pc), to + TL::BR * 64, 0, wave);
-            else lc.issue(c_all, to + TL::BR * 64, (int)(pc * C.plane + k) * 2, wave);
-            if (++ik == per) {
-                ik = 0;
-                iseg++;
-            }
-            ibuf = ibuf == TL::NS - 1 ? 0 : ibuf + 1;
+        s16x8 fa[2][TL::MR], fb[2][TL::MC];
+        auto read = [&](int h) {
+            const lds_t from = lds + buf * TL::stage_bytes;
+#pragma unroll
+            for (int j = 0; j < TL::MC; j++) fb[h][j] = fc.read(from + TL::BR * kStep * 2, j, h);
+#pragma unroll
+            for (int i = 0; i < TL::MR; i++) fa[h][i] = fr.read(from, i, h);
         };
-        tile_barrier();  // the last tile's reads are done
-        const int ahead = min(TL::NS - 1, total);
-        for (int s = 0; s < ahead; s++) issue();
-        int buf = 0;
-        for (int it = 0; it < total; it++) {
-            // stage `it` has landed once only the later ones issued so far are outstanding
-            if (it + TL::NS - 1 <= total) wait_loads<(TL::NS - 2) * loads>();
-            else wait_loads<0>();
-            tile_barrier();
-            if (it + TL::NS - 1 < total) issue();
-            const lds_t at = lds + buf * TL::stage_bytes;
-            s16x8 a[TL::MR], b[TL::MC];
-#pragma unroll
-            for (int j = 0; j < TL::MC; j++) b[j] = fc.read(at + TL::BR * 64, j);
-#pragma unroll
-            for (int i = 0; i < TL::MR; i++) a[i] = fr.read(at, i);
+        auto multiply = [&](int h) {
 #pragma unroll
             for (int i = 0; i < TL::MR; i++)
 #pragma unroll
-                for (int j = 0; j < TL::MC; j++) acc[i][j] = TL::type::mfma(a[i], b[j], acc[i][j]);
-            buf = buf == TL::NS - 1 ? 0 : buf + 1;
+                for (int j = 0; j < TL::MC; j++) acc[i][j] = TL::type::mfma(fa[h][i], fb[h][j], acc[i][j]);
+        };
+        const int total = w.per * (TL::planes == 3 ? 6 : 1);
+        if (total > 0) read(0);
+        for (int it = 0; it < total; it++) {
+            read(1);
+            multiply(0);
+            buf = buf == NS - 1 ? 0 : buf + 1;
+            ahead--;
+            landed();
+            read(0);  // the last one reads the next tile's fragments, or what is there; nothing uses them
+            ahead += st.issue(lds, A, B, a, b, parts, wave, lane);
+            multiply(1);
         }
-        const Place at{r0 + wr * TL::MR * 16, c0 + wc * TL::MC * 16, lane, sp, nr, nc};
-        epi.template run<TL>(acc, at);
+        side.epi.template run<TL>(acc, Place{w.r0 + wr * TL::MR * 16, w.c0 + wc * TL::MC * 16, lane, w.part, s.nr, s.nc});
+    };
+    for (int t = first; t < last; t += by) {
+        if (t < na) run(A, work_of<TA>(a, parts, t), a);
+        else if constexpr (!std::is_same_v<SA, SB>) run(B, work_of<TB>(b, 1, t - na), b);
     }
 }
 
-// Launches a product on at most two workgroups per CU.
-template <class TL, class Epi>
-int launch_product(const Operand &R, const Operand &C, const Dims &d, const Epi &epi, int cus, hipStream_t s) {
-    const int64_t tiles = (int64_t)((d.r + TL::BR - 1) / TL::BR) * ((d.c + TL::BC - 1) / TL::BC) *
-                          (d.split ? d.split : d.most);
-    if (tiles <= 0) return GS_OK;
+template <class TL>
+constexpr int slots_per_cu = TL::waves_per_simd * 4 / TL::waves;
+
+template <class SA, class SB>
+int launch_products(const SA &A, const SB &B, const Pairing &pair, int64_t grid, hipStream_t s) {
+    using TL = typename SA::tile;
+    const void *f = reinterpret_cast<const void *>(&k_product<SA, SB>);
     if (TL::lds_bytes > 65536)
-        GS_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(&k_product<TL, Epi>),
-                                         hipFuncAttributeMaxDynamicSharedMemorySize, TL::lds_bytes));
-    const int per_cu = TL::lds_bytes > 81920 ? 1 : 2;
-    const int64_t grid = tiles < (int64_t)per_cu * cus ? tiles : (int64_t)per_cu * cus;
-    hipLaunchKernelGGL((k_product<TL, Epi>), dim3((unsigned)grid), dim3(TL::threads), TL::lds_bytes, s, R, C, d, epi);
+        GS_CHECK_HIP(hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, TL::lds_bytes));
+    hipLaunchKernelGGL((k_product<SA, SB>), dim3((unsigned)grid), dim3(TL::threads), TL::lds_bytes, s, A, B, pair);
     GS_CHECK_LAUNCH();
     return GS_OK;
+}
+
+// Launches a product on as many workgroups as run at a time.
+template <class TL, class Epi>
+int launch_product(const Operand &R, const Operand &C, const Dims &d, const Epi &epi, int cus, hipStream_t s) {
+    const int64_t tiles = (int64_t)((d.r + TL::BR - 1) / TL::BR) * ((d.c + TL::BC - 1) / TL::BC);
+    const int64_t slots = (int64_t)slots_per_cu<TL> * cus;
+    if (tiles <= 0) return GS_OK;
+    const Side<TL, Epi> A{R, C, d, epi};
+    return launch_products(A, A, Pairing{0, 0, 1, nullptr}, tiles < slots ? tiles : slots, s);
+}
+
+// Two: the first in parts of its k, the second of columns that are the first's k, a piece of at most `piece` of them.
+template <class TA, class TB, class EA, class EB>
+int launch_pair(const Operand &Ra, const Operand &Ca, const Dims &da, const EA &ea, const Operand &Rb, const Operand &Cb,
+                const Dims &db, const EB &eb, int piece, int most, int *parts_d, int cus, hipStream_t s) {
+    const int slots = slots_per_cu<TA> * cus;
+    return launch_products(Side<TA, EA>{Ra, Ca, da, ea}, Side<TB, EB>{Rb, Cb, db, eb}, Pairing{piece, slots, most, parts_d}, slots, s);
 }
 
 }  // namespace gsv
