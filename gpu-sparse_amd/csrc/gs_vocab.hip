@@ -832,122 +832,259 @@ __global__ void k_term_weights(const void *best, int64_t n, int vocab, const int
     }
 }
 
-// Entries of one text sorted by token, terms ascending within a token: entry_v / entry_g[text * vocab ...], and the
-// first entry of each token (first[text][length + 1]).  One workgroup per text.  Each wave owns a run of terms, so a
-// count per (wave, token) places every entry without an atomic that decides an order; tokens go in passes of kTok.
-constexpr int kTok = 512, kSortWaves = 16;
-__global__ __launch_bounds__(1024) void k_sort_entries(const float *grad, const float *weights, const int *tokens, int vocab,
-                                                       int length, float *entry_g, int *entry_v, int *first) {
-    __shared__ int count[kSortWaves][kTok];
-    __shared__ int start[kTok];
-    __shared__ int wsum[16];
+// The gradient of the term weights has one entry per (text, term) with a positive weight: g' = g e^-w at the term's token.
+// dW adds g' H[token] over texts, dH g' W[term] over a token's terms; for dH a text's entries are sorted by token (terms
+// ascending within a token), stably and without an atomic that decides an order, so that every sum has one order.
+//
+// A wave owns a run of kRun terms.  k_entry_counts: entries per (run, token); k_entry_starts: where they go;
+// k_entry_place: there they go.  first[text][length + 1]: the first entry of each token.
+constexpr int kRun = 256, kTok = 1024;
+
+// For each entry of the lanes' tokens t (`on`): how many lanes before hold the same token, and how many do in all.
+__device__ __forceinline__ void same_token(int t, bool on, int bits, int &rank, int &all) {
+    uint64_t same = __ballot(on);
+    for (int b = 0; b < bits; b++) {
+        const bool one = (t >> b) & 1;
+        const uint64_t m = __ballot(on && one);
+        same &= one ? m : ~m;
+    }
+    rank = __popcll(same & gs_lanemask_lt());
+    all = __popcll(same);
+}
+
+// f(v, t, rank, all) for the run's entries whose token lies in [t0, t0 + kTok); v: the term, t: token - t0
+template <class F>
+__device__ __forceinline__ void each_entry(const int *tokens, int run, int vocab, int length, int t0, F &&f) {
+    const int lane = gs_lane(), most = min(kTok, length - t0);
+    const int bits = 32 - __clz(max(most - 1, 1));
+    int t[kRun / 64];
+#pragma unroll
+    for (int c = 0; c < kRun / 64; c++) {
+        const int v = run * kRun + c * 64 + lane;
+        t[c] = v < vocab ? tokens[v] - t0 : -1;
+    }
+#pragma unroll
+    for (int c = 0; c < kRun / 64; c++) {
+        const bool on = t[c] >= 0 && t[c] < most;
+        int rank, all;
+        same_token(t[c], on, bits, rank, all);
+        f(run * kRun + c * 64 + lane, t[c], on, rank, all);
+    }
+}
+
+__global__ __launch_bounds__(256) void k_entry_counts(const int *tokens, int vocab, int length, int runs, uint16_t *counts) {
+    __shared__ int count[4][kTok];
+    const int64_t b = blockIdx.y;
+    const int lane = gs_lane(), wave = threadIdx.x >> 6, run = blockIdx.x * 4 + wave;
+    if (run >= runs) return;
+    for (int t0 = 0; t0 < length; t0 += kTok) {
+        const int most = min(kTok, length - t0);
+        for (int t = lane; t < most; t += 64) count[wave][t] = 0;
+        gs_wave_sync();
+        each_entry(tokens + b * vocab, run, vocab, length, t0, [&](int, int t, bool on, int rank, int all) {
+            if (on && rank == 0) count[wave][t] += all;
+            gs_wave_sync();
+        });
+        uint16_t *to = counts + (b * runs + run) * length + t0;
+        for (int t = lane; t < most; t += 64) to[t] = (uint16_t)count[wave][t];
+        gs_wave_sync();
+    }
+}
+
+// starts[text][run][token]: the place of the run's first entry of the token.  One workgroup per text.
+__global__ __launch_bounds__(1024) void k_entry_starts(const uint16_t *counts, int length, int runs, int *starts, int *first) {
+    __shared__ int part[16];
     const int64_t b = blockIdx.x;
     const int tid = threadIdx.x, lane = gs_lane(), wave = tid >> 6;
-    const float *g = grad + b * vocab, *w = weights + b * vocab;
-    const int *tk = tokens + b * vocab;
-    const int run = (int)round_up((vocab + kSortWaves - 1) / kSortWaves, 64);
-    const int lo = min(vocab, wave * run), hi = min(vocab, lo + run);
     int base = 0;
-    for (int t0 = 0; t0 < length; t0 += kTok) {
-        for (int t = lane; t < kTok; t += 64) count[wave][t] = 0;
-        gs_wave_sync();
-        auto walk = [&](bool place) {
-            for (int v0 = lo; v0 < hi; v0 += 64) {
-                const int v = v0 + lane;
-                const int t = v < hi ? tk[v] - t0 : -1;
-                const bool on = t >= 0 && t < kTok && t0 + t < length;
-                uint64_t left = __ballot(on);
-                int rank = 0, all = 0;
-                while (left) {  // one turn per distinct token among the lanes
-                    const int lead = __ffsll((unsigned long long)left) - 1;
-                    const int tl = __builtin_amdgcn_readlane(t, lead);
-                    const uint64_t same = __ballot(on && t == tl);
-                    if (on && t == tl) {
-                        rank = __popcll(same & gs_lanemask_lt());
-                        all = __popcll(same);
-                    }
-                    left &= ~same;
-                }
-                if (on) {
-                    const int had = count[wave][t];
-                    if (place) {
-                        const int64_t at = b * vocab + start[t] + had + rank;
-                        entry_v[at] = v;
-                        entry_g[at] = g[v] * expf(-w[v]);  // d log(1 + x) / dx = 1 / (1 + x) = e^-w
-                    }
-                    gs_wave_sync();
-                    if (rank == all - 1) count[wave][t] = had + all;
-                }
-                gs_wave_sync();
-            }
-        };
-        walk(false);
-        __syncthreads();
-        // each token's total, its start, and where each wave's part of it begins
+    for (int t0 = 0; t0 < length; t0 += 1024) {
+        const int t = t0 + tid;
+        const uint16_t *from = counts + b * runs * length + t;
+        int *to = starts + b * runs * length + t;
         int c = 0;
-        if (tid < kTok)
-            for (int wv = 0; wv < kSortWaves; wv++) {
-                const int x = count[wv][tid];
-                count[wv][tid] = c;
-                c += x;
-            }
+        if (t < length) {
+#pragma unroll 8
+            for (int r = 0; r < runs; r++) c += from[(int64_t)r * length];
+        }
         const int inc = (int)gs_wave_incl_scan((uint32_t)c);
-        if (lane == 63) wsum[wave] = inc;
+        if (lane == 63) part[wave] = inc;
         __syncthreads();
-        int before = base;
-        for (int i = 0; i < wave; i++) before += wsum[i];
-        if (tid < kTok) start[tid] = before + inc - c;
-        if (tid < kTok && t0 + tid < length) first[b * (length + 1) + t0 + tid] = before + inc - c;
-        int total = 0;
-        for (int i = 0; i < 16; i++) total += wsum[i];
-        __syncthreads();
-        walk(true);
-        base += total;
+        int at = base + inc - c;
+        for (int w = 0; w < 16; w++) {
+            if (w < wave) at += part[w];
+            base += part[w];
+        }
+        if (t < length) {
+            first[b * (length + 1) + t] = at;
+#pragma unroll 8
+            for (int r = 0; r < runs; r++) {
+                to[(int64_t)r * length] = at;
+                at += from[(int64_t)r * length];
+            }
+        }
         __syncthreads();
     }
     if (tid == 0) first[b * (length + 1) + length] = base;
 }
 
-// out[row] = sum over the row's entries of entry_g * W[entry_v]: one workgroup per token, the waves take entries in
-// turn and are added in order.
-template <int HT>
-__global__ __launch_bounds__(256) void k_entries_hidden(const void *weight, int64_t wr, int64_t wd, int wvec, const float *entry_g,
-                                                        const int *entry_v, const int *first, int vocab, int length, int dim,
-                                                        typename HVal<HT>::t *out) {
-    using T = typename HVal<HT>::t;
-    __shared__ f32x4 red[3][64];
-    const int lane = gs_lane(), wave = threadIdx.x >> 6;
-    const int64_t row = blockIdx.x, b = row / length, t = row % length;
-    const int lo = first[b * (length + 1) + t], hi = first[b * (length + 1) + t + 1];
-    const float *g = entry_g + b * vocab;
-    const int *ev = entry_v + b * vocab;
-    const bool vec = (dim & 3) == 0;
-    for (int d0 = 0; d0 < dim; d0 += 256) {
-        const int d = d0 + lane * 4;
-        f32x4 s = f32x4{0.f, 0.f, 0.f, 0.f};
-        if (d < dim) {
-#pragma unroll 4
-            for (int e = lo + wave; e < hi; e += 4) {
-                const float x = g[e];
-                s += x * row4((const T *)weight + (int64_t)ev[e] * wr, wd, d, dim, wvec);
+struct Entry {
+    int v, t;
+    float g;
+};
+
+__global__ __launch_bounds__(256) void k_entry_place(const float *grad, const float *weights, const int *tokens, int vocab,
+                                                     int length, int runs, const int *starts, Entry *entries) {
+    __shared__ int next[4][kTok];
+    const int64_t b = blockIdx.y;
+    const int lane = gs_lane(), wave = threadIdx.x >> 6, run = blockIdx.x * 4 + wave;
+    if (run >= runs) return;
+    for (int t0 = 0; t0 < length; t0 += kTok) {
+        const int most = min(kTok, length - t0);
+        const int *from = starts + (b * runs + run) * length + t0;
+        for (int t = lane; t < most; t += 64) next[wave][t] = from[t];
+        gs_wave_sync();
+        each_entry(tokens + b * vocab, run, vocab, length, t0, [&](int v, int t, bool on, int rank, int all) {
+            const int at = on ? next[wave][t] : 0;
+            gs_wave_sync();
+            if (on) {
+                // d log(1 + x) / dx = 1 / (1 + x) = e^-w
+                entries[b * vocab + at + rank] = Entry{v, t0 + t, grad[b * vocab + v] * expf(-weights[b * vocab + v])};
+                if (rank == 0) next[wave][t] = at + all;
             }
-        }
-        if (wave) red[wave - 1][lane] = s;
-        __syncthreads();
-        if (wave == 0 && d < dim) {
-            for (int w = 0; w < 3; w++) s += red[w][lane];
-            T *to = out + row * dim + d;
-            if (vec) store4(to, s);
-            else
-                for (int e = 0; e < 4; e++)
-                    if (d + e < dim) to[e] = (T)s[e];
-        }
-        __syncthreads();
+            gs_wave_sync();
+        });
     }
 }
 
-// dW[v] = sum over texts of g' H[text, token], db[v] = sum of g': a workgroup per 16 terms, a wave per 4 of them.
+// U rows of up to 256 NC values in a wave's registers, all on their way at once: lane l holds values 256 c + 4 l .. + 3.
+// Aligned rows (`vec`) are read through a buffer that ends with the row, so that no lane branches.
+template <int U, int NC, class T>
+__device__ __forceinline__ void rows_load(f32x4 (&x)[U][NC], const T *const (&row)[U], int64_t ds, int d0, int dim, bool vec) {
+    const int lane = gs_lane();
+    if (vec) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const auto r = gs_rsrc(row[u], (uint32_t)(dim * sizeof(T)));
+#pragma unroll
+            for (int c = 0; c < NC; c++) {
+                const int off = (d0 + c * 256 + lane * 4) * (int)sizeof(T);
+                Four<T> v;
+                if constexpr (sizeof(T) == 4) v = __builtin_bit_cast(Four<T>, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0));
+                else v = __builtin_bit_cast(Four<T>, __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 0));
+                x[u][c] = f32x4{(float)v.v[0], (float)v.v[1], (float)v.v[2], (float)v.v[3]};
+            }
+        }
+    } else {
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int c = 0; c < NC; c++) x[u][c] = row4(row[u], ds, d0 + c * 256 + lane * 4, dim, false);
+    }
+}
+template <int NC, class T>
+__device__ __forceinline__ void row_store(T *row, const f32x4 (&x)[NC], int d0, int dim) {
+    const bool vec = (dim & 3) == 0;
+#pragma unroll
+    for (int c = 0; c < NC; c++) {
+        const int d = d0 + c * 256 + gs_lane() * 4;
+        if (vec && d < dim) store4(row + d, x[c]);
+        else
+            for (int e = 0; e < 4; e++)
+                if (d + e < dim) row[d + e] = (T)x[c][e];
+    }
+}
+
+// dH by chunks of a text's entries, one wave each, whatever tokens they belong to: a token whose entries all lie in the
+// chunk is written; a share of one goes to part[chunk][1] where its entries begin in the chunk, else to part[chunk][0].
+template <int HT, int NC>
+__global__ __launch_bounds__(256) void k_entries_hidden(const void *weight, int64_t wr, int64_t wd, int wvec, const Entry *entries,
+                                                        const int *first, int vocab, int length, int dim, int chunk, int chunks,
+                                                        float *part, int dimp, typename HVal<HT>::t *out) {
+    using T = typename HVal<HT>::t;
+    const int64_t b = blockIdx.y;
+    const int c = blockIdx.x * 4 + (threadIdx.x >> 6), lane = gs_lane();
+    const int total = first[b * (length + 1) + length];
+    const int lo = c * chunk, hi = min(lo + chunk, total);
+    if (c >= chunks || lo >= hi) return;
+    const Entry *es = entries + b * vocab;
+    const int before = lo > 0 ? es[lo - 1].t : -1, after = hi < total ? es[hi].t : -1;
+    constexpr int U = 4;
+    for (int d0 = 0; d0 < dim; d0 += NC * 256) {
+        f32x4 sum[NC];
+#pragma unroll
+        for (int k = 0; k < NC; k++) sum[k] = f32x4{0.f, 0.f, 0.f, 0.f};
+        int cur = -1;
+        auto flush = [&](bool ends) {
+            const bool begins = cur != before;
+            if (begins && ends) row_store<NC>(out + (b * length + cur) * dim, sum, d0, dim);
+            else row_store<NC>(part + ((b * chunks + c) * 2 + (begins ? 1 : 0)) * dimp, sum, d0, dimp);
+        };
+        for (int e0 = lo; e0 < hi; e0 += 64) {
+            const int n = min(64, hi - e0);
+            const Entry mine = es[min(e0 + lane, hi - 1)];
+            for (int u0 = 0; u0 < n; u0 += U) {
+                f32x4 x[U][NC];
+                const T *row[U];
+                float g[U];
+                int t[U];
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    const int l = min(u0 + u, n - 1);
+                    const int v = __builtin_amdgcn_readlane(mine.v, l);
+                    t[u] = __builtin_amdgcn_readlane(mine.t, l);
+                    g[u] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, mine.g), l));
+                    row[u] = (const T *)weight + v * wr;
+                }
+                rows_load<U, NC, T>(x, row, wd, d0, dim, wvec);
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    if (u0 + u >= n) break;
+                    if (t[u] != cur) {
+                        if (cur >= 0) flush(true);
+                        cur = t[u];
+#pragma unroll
+                        for (int k = 0; k < NC; k++) sum[k] = f32x4{0.f, 0.f, 0.f, 0.f};
+                    }
+#pragma unroll
+                    for (int k = 0; k < NC; k++) sum[k] += g[u] * x[u][k];
+                }
+            }
+        }
+        flush(cur != after);
+    }
+}
+
+// What k_entries_hidden left open: zeros for tokens without entries, sums of the shares of those in several chunks.
 template <int HT>
+__global__ __launch_bounds__(256) void k_entries_join(const int *first, int64_t rows, int length, int dim, int chunk, int chunks,
+                                                      const float *part, int dimp, typename HVal<HT>::t *out) {
+    const int lane = gs_lane();
+    const bool vec = (dim & 3) == 0;
+    for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < rows; r += (int64_t)gridDim.x * 4) {
+        const int64_t b = r / length, t = r % length;
+        const int lo = first[b * (length + 1) + t], hi = first[b * (length + 1) + t + 1];
+        const int c0 = lo / chunk, c1 = (hi - 1) / chunk;
+        if (hi > lo && c0 == c1) continue;
+        for (int d = lane * 4; d < dim; d += 256) {
+            f32x4 x = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (hi > lo) {
+                const float *p = part + (b * chunks + c0) * 2 * dimp + d;
+                x = *reinterpret_cast<const f32x4 *>(p + dimp);
+#pragma unroll 4
+                for (int c = c0 + 1; c <= c1; c++) x += *reinterpret_cast<const f32x4 *>(p + (int64_t)(c - c0) * 2 * dimp);
+            }
+            auto *to = out + r * dim + d;
+            if (vec) store4(to, x);
+            else
+                for (int e = 0; e < 4; e++)
+                    if (d + e < dim) to[e] = (typename HVal<HT>::t)x[e];
+        }
+    }
+}
+
+// dW[v] = sum over texts of g' H[text, token], db[v] = sum of g', texts in order: a workgroup per 16 terms, a wave per 4 of
+// them, four rows of hidden states on their way at a time.
+template <int HT, int NC>
 __global__ __launch_bounds__(256) void k_entries_weight(Source h, const float *grad, const float *weights, const int *tokens,
                                                         int texts, int vocab, typename HVal<HT>::t *dw, void *db, int db_type) {
     using T = typename HVal<HT>::t;
@@ -955,14 +1092,14 @@ __global__ __launch_bounds__(256) void k_entries_weight(Source h, const float *g
     __shared__ int st[64][17];
     const int lane = gs_lane(), wave = threadIdx.x >> 6, tid = threadIdx.x;
     const int v0 = blockIdx.x * 16;
-    const int dim = h.dim;
-    const bool vec = (dim & 3) == 0;
-    for (int d0 = 0; d0 < dim; d0 += 256) {
-        const int d = d0 + lane * 4;
-        f32x4 s[4];
+    constexpr int U = 4;
+    for (int d0 = 0; d0 < h.dim; d0 += NC * 256) {
+        f32x4 sum[4][NC];
         float bs[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int u = 0; u < 4; u++) s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int u = 0; u < 4; u++)
+#pragma unroll
+            for (int c = 0; c < NC; c++) sum[u][c] = f32x4{0.f, 0.f, 0.f, 0.f};
         for (int b0 = 0; b0 < texts; b0 += 64) {
             __syncthreads();
             for (int x = tid; x < 64 * 16; x += 256) {
@@ -977,17 +1114,33 @@ __global__ __launch_bounds__(256) void k_entries_weight(Source h, const float *g
             __syncthreads();
 #pragma unroll
             for (int u = 0; u < 4; u++) {
-                const int v = wave * 4 + u;
-                const int t = st[lane][v];
-                const float g = sg[lane][v];
+                const int t = st[lane][wave * 4 + u];
+                const float g = sg[lane][wave * 4 + u];
                 uint64_t left = __ballot(t >= 0);
                 while (left) {
-                    const int l = __ffsll((unsigned long long)left) - 1;
-                    left &= left - 1;
-                    const int tl = __builtin_amdgcn_readlane(t, l);
-                    const float gl = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, g), l));
-                    bs[u] += gl;
-                    if (d < dim) s[u] += gl * row4((const T *)h.p + (int64_t)(b0 + l) * h.s0 + (int64_t)tl * h.s1, h.sd, d, dim, h.vec);
+                    f32x4 x[U][NC];
+                    const T *row[U];
+                    float gl[U];
+                    bool live[U];
+                    int l = 0;
+#pragma unroll
+                    for (int k = 0; k < U; k++) {  // past the last entry: its row again, not used
+                        const bool on = left != 0;
+                        l = on ? __ffsll((unsigned long long)left) - 1 : l;
+                        left &= left - 1;
+                        const int tl = __builtin_amdgcn_readlane(t, l);
+                        gl[k] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, g), l));
+                        live[k] = on;
+                        row[k] = (const T *)h.p + (int64_t)(b0 + l) * h.s0 + (int64_t)tl * h.s1;
+                    }
+                    rows_load<U, NC, T>(x, row, h.sd, d0, h.dim, h.vec);
+#pragma unroll
+                    for (int k = 0; k < U; k++) {
+                        if (!live[k]) break;
+                        bs[u] += gl[k];
+#pragma unroll
+                        for (int c = 0; c < NC; c++) sum[u][c] += gl[k] * x[k][c];
+                    }
                 }
             }
         }
@@ -995,13 +1148,7 @@ __global__ __launch_bounds__(256) void k_entries_weight(Source h, const float *g
         for (int u = 0; u < 4; u++) {
             const int v = v0 + wave * 4 + u;
             if (v >= vocab) continue;
-            if (dw && d < dim) {
-                T *to = dw + (int64_t)v * dim + d;
-                if (vec) store4(to, s[u]);
-                else
-                    for (int e = 0; e < 4; e++)
-                        if (d + e < dim) to[e] = (T)s[u][e];
-            }
+            if (dw) row_store<NC>(dw + (int64_t)v * h.dim, sum[u], d0, h.dim);
             if (db && d0 == 0 && lane == 0) {
                 if (db_type == GS_H_F32) ((float *)db)[v] = bs[u];
                 else if (db_type == GS_H_F16) ((_Float16 *)db)[v] = (_Float16)bs[u];
@@ -1455,6 +1602,77 @@ extern "C" int gs_vocab_loss_grad(const gs_vocab_head *h, const gs_vocab_targets
 
 // ---------------------------------------------------------------- term weights
 
+namespace gsv {
+
+struct EntryPlan {
+    int runs, chunk, chunks, dimp;
+    Entry *entries;
+    int *first, *starts;
+    uint16_t *counts;
+    float *part;
+};
+// Chunks of 64 entries fill the GPU on small batches; larger ones take fewer open ends (two rows of fp32 a chunk).
+void take_entries(gs_arena &a, const gs_vocab_head *h, EntryPlan *p) {
+    const size_t n = (size_t)h->texts * h->vocab, rows = (size_t)h->texts * h->length;
+    p->runs = (h->vocab + kRun - 1) / kRun;
+    p->chunk = n <= (size_t)4 << 20 ? 64 : 256;
+    p->chunks = (h->vocab + p->chunk - 1) / p->chunk;
+    p->dimp = (int)round_up(h->dim, 4);
+    p->entries = a.take<Entry>(n);
+    p->first = a.take<int>(rows + h->texts);
+    p->starts = a.take<int>(rows * p->runs);
+    p->counts = a.take<uint16_t>(rows * p->runs);
+    p->part = a.take<float>((size_t)h->texts * p->chunks * 2 * p->dimp);
+}
+
+// f(NC) for the registers a row of `dim` values takes, 256 a piece
+#define GSV_BY_CHUNKS(dim, CALL)              \
+    switch (((dim) + 255) / 256) {            \
+        case 1: CALL(1); break;               \
+        case 2: CALL(2); break;               \
+        case 3: CALL(3); break;               \
+        default: CALL(4); break;              \
+    }
+
+template <int HT>
+int run_entries(const gs_vocab_head *h, const float *grad_d, const float *weights_d, const int32_t *tokens_d, void *dhidden_d,
+                void *dweight_d, void *dbias_d, const EntryPlan &p, hipStream_t s) {
+    using T = typename HVal<HT>::t;
+    const int64_t rows = (int64_t)h->texts * h->length;
+    const Source ws = weight_source(h), hs = hidden_source(h);
+    if (dhidden_d && rows > 0) {
+        const dim3 g((p.runs + 3) / 4, h->texts);
+        hipLaunchKernelGGL(k_entry_counts, g, dim3(256), 0, s, tokens_d, h->vocab, h->length, p.runs, p.counts);
+        GS_CHECK_LAUNCH();
+        hipLaunchKernelGGL(k_entry_starts, dim3(h->texts), dim3(1024), 0, s, p.counts, h->length, p.runs, p.starts, p.first);
+        GS_CHECK_LAUNCH();
+        hipLaunchKernelGGL(k_entry_place, g, dim3(256), 0, s, grad_d, weights_d, tokens_d, h->vocab, h->length, p.runs, p.starts,
+                           p.entries);
+        GS_CHECK_LAUNCH();
+#define GSV_EH(NC)                                                                                                             \
+    hipLaunchKernelGGL((k_entries_hidden<HT, NC>), dim3((p.chunks + 3) / 4, h->texts), dim3(256), 0, s, h->weight_d,            \
+                       h->weight_row_stride, h->weight_dim_stride, ws.vec, p.entries, p.first, h->vocab, h->length, h->dim,     \
+                       p.chunk, p.chunks, p.part, p.dimp, (T *)dhidden_d)
+        GSV_BY_CHUNKS(h->dim, GSV_EH)
+#undef GSV_EH
+        GS_CHECK_LAUNCH();
+        hipLaunchKernelGGL((k_entries_join<HT>), dim3(gs_blocks(rows, 4, 8192)), dim3(256), 0, s, p.first, rows, h->length, h->dim,
+                           p.chunk, p.chunks, p.part, p.dimp, (T *)dhidden_d);
+        GS_CHECK_LAUNCH();
+    }
+    if (dweight_d || dbias_d) {
+#define GSV_EW(NC)                                                                                                          \
+    hipLaunchKernelGGL((k_entries_weight<HT, NC>), dim3((h->vocab + 15) / 16), dim3(256), 0, s, hs, grad_d, weights_d, tokens_d, \
+                       h->texts, h->vocab, (T *)dweight_d, dbias_d, h->bias_type)
+        GSV_BY_CHUNKS(h->dim, GSV_EW)
+#undef GSV_EW
+        GS_CHECK_LAUNCH();
+    }
+    return GS_OK;
+}
+
+}  // namespace gsv
+
 extern "C" int gs_term_weights_workspace(const gs_vocab_head *h, int32_t tokens, size_t *bytes, size_t *grad_bytes) {
     if (int rc = check_head(h)) return rc;
     GS_REQUIRE(bytes && grad_bytes, "NULL size pointer");
@@ -1462,11 +1680,9 @@ extern "C" int gs_term_weights_workspace(const gs_vocab_head *h, int32_t tokens,
     gs_arena a{nullptr, 0, 0}, b{nullptr, 0, 0};
     Common c;
     take_common(a, l, h, true, &c);
-    const size_t n = (size_t)h->texts * h->vocab;
-    a.take<float>(n * (tokens ? 2 : 1));
-    b.take<float>(n);
-    b.take<int>(n);
-    b.take<int>((size_t)h->texts * (h->length + 1));
+    a.take<float>((size_t)h->texts * h->vocab * (tokens ? 2 : 1));
+    EntryPlan p;
+    take_entries(b, h, &p);
     *bytes = a.used, *grad_bytes = b.used;
     return GS_OK;
 }
@@ -1529,41 +1745,16 @@ extern "C" int gs_term_weights_grad(const gs_vocab_head *h, const float *grad_d,
                                     void *dhidden_d, void *dweight_d, void *dbias_d, void *workspace_d, size_t workspace_bytes,
                                     void *stream) {
     if (int rc = check_head(h)) return rc;
+    GS_REQUIRE(h->texts <= 65535, "texts=%d exceed 65535", h->texts);
     gs_arena a{(char *)workspace_d, 0, workspace_bytes};
-    const size_t n = (size_t)h->texts * h->vocab;
-    float *entry_g = a.take<float>(n);
-    int *entry_v = a.take<int>(n);
-    int *first = a.take<int>((size_t)h->texts * (h->length + 1));
+    EntryPlan p;
+    take_entries(a, h, &p);
     if (!a.ok()) {
         gs_set_error("term_weights_grad workspace too small: need %zu bytes, got %zu", a.used, workspace_bytes);
         return GS_ENOSPC;
     }
     const hipStream_t s = gs_stream(stream);
-    const int rows = h->texts * h->length;
-    const Source ws = weight_source(h), hs = hidden_source(h);
-    if (dhidden_d && rows > 0) {
-        hipLaunchKernelGGL(k_sort_entries, dim3(h->texts), dim3(1024), 0, s, grad_d, weights_d, tokens_d, h->vocab, h->length,
-                           entry_g, entry_v, first);
-        GS_CHECK_LAUNCH();
-#define GSV_EH(HT)                                                                                                         \
-    hipLaunchKernelGGL((k_entries_hidden<HT>), dim3(rows), dim3(256), 0, s, h->weight_d, h->weight_row_stride,              \
-                       h->weight_dim_stride, ws.vec, entry_g, entry_v, first, h->vocab, h->length, h->dim,                  \
-                       (typename HVal<HT>::t *)dhidden_d)
-        if (h->type == GS_H_F32) GSV_EH(GS_H_F32);
-        else if (h->type == GS_H_F16) GSV_EH(GS_H_F16);
-        else GSV_EH(GS_H_BF16);
-#undef GSV_EH
-        GS_CHECK_LAUNCH();
-    }
-    if (dweight_d || dbias_d) {
-#define GSV_EW(HT)                                                                                                         \
-    hipLaunchKernelGGL((k_entries_weight<HT>), dim3((h->vocab + 15) / 16), dim3(256), 0, s, hs, grad_d, weights_d, tokens_d, \
-                       h->texts, h->vocab, (typename HVal<HT>::t *)dweight_d, dbias_d, h->bias_type)
-        if (h->type == GS_H_F32) GSV_EW(GS_H_F32);
-        else if (h->type == GS_H_F16) GSV_EW(GS_H_F16);
-        else GSV_EW(GS_H_BF16);
-#undef GSV_EW
-        GS_CHECK_LAUNCH();
-    }
-    return GS_OK;
+    if (h->type == GS_H_F32) return run_entries<GS_H_F32>(h, grad_d, weights_d, tokens_d, dhidden_d, dweight_d, dbias_d, p, s);
+    if (h->type == GS_H_F16) return run_entries<GS_H_F16>(h, grad_d, weights_d, tokens_d, dhidden_d, dweight_d, dbias_d, p, s);
+    return run_entries<GS_H_BF16>(h, grad_d, weights_d, tokens_d, dhidden_d, dweight_d, dbias_d, p, s);
 }
