@@ -150,8 +150,8 @@ struct Keep {
 };
 
 // rows[i]: the i-th kept row, ascending; inv[row]: its place or -1; *n: how many.  For texts of `length` rows, seg[i]
-// is the row's text, -1 for the rest of the last tile.  One workgroup of 1024, 16 rows per thread and turn.
-__device__ __forceinline__ void kept_rows(const Keep &keep, int length, int *rows, int *inv, int *seg, int *n) {
+// is the row's text, -1 for the rest of the last tile, and text_first[b] the first place of a text's rows.  One workgroup of 1024, 16 rows per thread and turn.
+__device__ __forceinline__ void kept_rows(const Keep &keep, int length, int *rows, int *inv, int *seg, int *text_first, int *n) {
     __shared__ int part[16];
     const int tid = threadIdx.x, lane = gs_lane(), wave = tid >> 6;
     int base = 0;
@@ -172,6 +172,7 @@ __device__ __forceinline__ void kept_rows(const Keep &keep, int length, int *row
             const bool k = (m >> e) & 1;
             const int row = (int)(r0 + e);
             if (inv) inv[row] = k ? o : -1;
+            if (seg && row % length == 0) text_first[row / length] = o;
             if (k) {
                 rows[o] = row;
                 if (seg) seg[o] = row / length;
@@ -180,6 +181,7 @@ __device__ __forceinline__ void kept_rows(const Keep &keep, int length, int *row
         }
         __syncthreads();
     }
+    if (seg && tid == 0) text_first[keep.total / length] = base;
     if (seg)
         for (int i = base + tid; i < round_up(base, kRowPad); i += 1024) seg[i] = -1;
     if (tid == 0) *n = base;
@@ -187,10 +189,10 @@ __device__ __forceinline__ void kept_rows(const Keep &keep, int length, int *row
 
 // First launch of a call.  Workgroup 0 lists the kept rows; the others write the bias in fp32 (0 without one, -inf for
 // the rows that pad the vocabulary: they drop out of every softmax and maximum) and clear what is added to later.
-__global__ __launch_bounds__(1024) void k_setup(Keep keep, int length, int *rows, int *inv, int *seg, int *n, const void *bias,
+__global__ __launch_bounds__(1024) void k_setup(Keep keep, int length, int *rows, int *inv, int *seg, int *text_first, int *n, const void *bias,
                                                 int bias_type, int vocab, int padded, float *bias_o, float *zero, int64_t zeros) {
     if (blockIdx.x == 0) {
-        kept_rows(keep, length, rows, inv, seg, n);
+        kept_rows(keep, length, rows, inv, seg, text_first, n);
         return;
     }
     const int64_t by = (int64_t)(gridDim.x - 1) * 1024, at = (int64_t)(blockIdx.x - 1) * 1024 + threadIdx.x;
@@ -350,8 +352,8 @@ __global__ __launch_bounds__(256) void k_target_logits(Source h, const void *wei
 // The target shares of the kept rows, ascending by id within a row.
 struct Entries {
     const int *ids;         // [kept row][top]
-    const float *share;     // NULL: 1
-    const uint16_t *first;  // [vocabulary / kRowPad + 1][kept row] (top > 1)
+    const float *share;
+    const uint16_t *first;  // [vocabulary / kRowPad + 1][kept row]
     int64_t ld;
     int top;
     // f(mine, share) for each entry of the lanes' tokens n among the wave's terms [wv, wv + 16 MR): in the lane that
@@ -362,17 +364,14 @@ struct Entries {
         int k = 0, end = 0;
         if (on) {
             base = (int64_t)n * top;
-            end = 1;
-            if (top > 1) {
-                const int64_t t = (int64_t)(wv / kRowPad) * ld + n;
-                k = first[t];
-                end = first[t + ld];
-            }
+            const int64_t t = (int64_t)(wv / kRowPad) * ld + n;
+            k = first[t];
+            end = first[t + ld];
         }
         while (__any(k < end)) {
             const int lv = k < end ? ids[base + k] - wv : -1;
             if (__any(lv >= 0 && lv < MR * 16)) {
-                const float s = k < end ? (share ? share[base + k] : 1.f) : 0.f;
+                const float s = k < end ? share[base + k] : 0.f;
                 f(lv >= 0 && lv < MR * 16 && ((lv >> 2) & 3) == q ? (lv >> 4) * 4 + (lv & 3) : -1, s);
             }
             k++;
@@ -390,12 +389,14 @@ struct EpiSums {
     float *dots;
     int64_t ld;
     Entries entries;
+    static constexpr int sides = 1;
+    __device__ __forceinline__ SideArray side(int, int r0, int, const Shape &) const { return {bias + r0, 256}; }
     template <class TL>
     __device__ __forceinline__ void run(f32x4 (&acc)[TL::MR][TL::MC], const Place &at) const {
         const int q = at.lane >> 4;
 #pragma unroll
         for (int i = 0; i < TL::MR; i++) {
-            const f32x4 b = *reinterpret_cast<const f32x4 *>(bias + at.row0 + 16 * i + 4 * q);
+            const f32x4 b = at.side4(0, at.r_in + 16 * i + 4 * q);
 #pragma unroll
             for (int j = 0; j < TL::MC; j++) acc[i][j] += b;
         }
@@ -440,7 +441,7 @@ struct EpiSums {
 
 // Gradients of a tile's logits: (softmax - target shares) times the row's factor, rounded to 16 bits once (three
 // planes for fp32), token-major, and their sums over each wave's tokens for the bias.
-template <class S>
+template <class S, bool SHARES>
 struct EpiLogitGrad {
     const float *bias;
     float scale;
@@ -452,6 +453,13 @@ struct EpiLogitGrad {
     int64_t ld, plane;
     float *col_sums;       // NULL: not wanted; [wave's block of tokens][padded vocabulary]
     int64_t sums_ld;
+    static constexpr int sides = 4;
+    __device__ __forceinline__ SideArray side(int a, int r0, int c0, const Shape &s) const {
+        if (a == 0) return {bias + v0 + r0, 256};
+        if (a == 1) return {lse2 + c0, s.nc - c0};
+        if (a == 2) return {factor + c0, s.nc - c0};
+        return {entries.ids + c0, SHARES ? 0 : s.nc - c0};  // one target per row
+    }
     template <class TL>
     __device__ __forceinline__ void run(f32x4 (&acc)[TL::MR][TL::MC], const Place &at) const {
         const int q = at.lane >> 4;
@@ -459,7 +467,7 @@ struct EpiLogitGrad {
 #pragma unroll
         for (int i = 0; i < TL::MR; i++) {
             sums[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-            const f32x4 b = *reinterpret_cast<const f32x4 *>(bias + v0 + at.row0 + 16 * i + 4 * q);
+            const f32x4 b = at.side4(0, at.r_in + 16 * i + 4 * q);
 #pragma unroll
             for (int j = 0; j < TL::MC; j++) acc[i][j] += b;
         }
@@ -468,17 +476,25 @@ struct EpiLogitGrad {
         for (int j = 0; j < TL::MC; j++) {
             const int n = at.col0 + 16 * j + (at.lane & 15);
             const bool on = n < at.n_c;
-            const float l = on ? lse2[n] : 0.f, f = on ? factor[n] : 0.f;
+            const int in = at.c_in + 16 * j + (at.lane & 15);
+            const float l = at.side(1, in), f = at.side(2, in);
 #pragma unroll
             for (int i = 0; i < TL::MR; i++)
 #pragma unroll
                 for (int e = 0; e < 4; e++) acc[i][j][e] = __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], scale, -l));
-            entries.each<TL::MR>(n, on, wv, q, [&](int mine, float share) {
+            const auto off = [&](int mine, float share) {
 #pragma unroll
                 for (int i = 0; i < TL::MR; i++)
 #pragma unroll
                     for (int e = 0; e < 4; e++) acc[i][j][e] -= mine == i * 4 + e ? share : 0.f;
-            });
+            };
+            if constexpr (SHARES) {
+                entries.each<TL::MR>(n, on, wv, q, off);
+            } else {
+                const int lv = on ? __float_as_int(at.side(3, in)) - wv : -1;
+                const bool here = lv >= 0 && lv < TL::MR * 16;
+                if (__any(here)) off(here && ((lv >> 2) & 3) == q ? (lv >> 4) * 4 + (lv & 3) : -1, 1.f);
+            }
 #pragma unroll
             for (int i = 0; i < TL::MR; i++) {
                 acc[i][j] *= f;
@@ -505,6 +521,8 @@ struct EpiWeightGrad {
     O *out;
     const float *scale;
     int dim, vec;
+    static constexpr int sides = 0;
+    __device__ __forceinline__ SideArray side(int, int, int, const Shape &) const { return {nullptr, 0}; }
     template <class TL>
     __device__ __forceinline__ void run(f32x4 (&acc)[TL::MR][TL::MC], const Place &at) const {
         const float s = *scale;
@@ -531,6 +549,8 @@ struct EpiWeightGrad {
 struct EpiHiddenPart {
     float *part;
     int dimp, add;
+    static constexpr int sides = 0;
+    __device__ __forceinline__ SideArray side(int, int, int, const Shape &) const { return {nullptr, 0}; }
     template <class TL>
     __device__ __forceinline__ void run(f32x4 (&acc)[TL::MR][TL::MC], const Place &at) const {
         const int q = at.lane >> 4;
@@ -551,80 +571,79 @@ struct EpiHiddenPart {
     }
 };
 
-// Largest logit of each text and term: rows are kept tokens (ascending by text), columns terms.  best[text][term]
-// takes the maximum of the positive ones' bits; with tokens, of (bits, ~kept row), so that the lowest token wins a
-// tie.  Maxima do not depend on the order of the atomics.  The bias is added to a maximum (rounding keeps order).
+// Largest logit of each text and term: rows are kept tokens (ascending by text), columns terms.  A wave's rows are a
+// block w of tokens; for each text b in it the largest logits go to slot w + b (along the blocks and texts one of the
+// two grows with each pair, so slots are distinct, and those of a text lie one after the other), with TOK also the
+// lowest kept row that has it.  k_term_weights takes a text's slots together.  The bias is added to the maximum
+// (rounding keeps order).
 template <bool TOK>
 struct EpiTextMax {
     const float *bias;
-    const int *seg;   // text of each kept row, padded with -1 to a whole tile
-    void *best;
+    const int *seg;   // text of each kept row, -1 for the rest of the last tile
+    float *best;      // [slot][vocab]
+    int *where;
     int vocab;
+    static constexpr int sides = 2;
+    __device__ __forceinline__ SideArray side(int a, int r0, int c0, const Shape &) const {
+        return a == 0 ? SideArray{bias + c0, 256} : SideArray{seg + r0, 256};
+    }
 
-    // Takes rows row .. row + 3's values into the lane's maximum (and where it is; the first of equal ones)
+    // Takes rows row .. row + 3's values into the lane's maximum, and the first row that has it
     __device__ __forceinline__ static void take(f32x4 x, int row, float &top, int &tok) {
         if (TOK) {
-            float t = top;
-            int k = tok;
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                // a NaN is taken, and not given up for what follows
-                const bool up = !(x[e] <= t) && t == t;
-                t = up ? x[e] : t;
-                k = up ? row + e : k;
-            }
-            top = t, tok = k;
+            const float m = maximum(maximum(x[0], x[1], x[2]), x[3], x[3]);
+            int r = x[2] == m ? row + 2 : row + 3;
+            r = x[1] == m ? row + 1 : r;
+            r = x[0] == m ? row : r;
+            tok = m > top ? r : tok;
+            top = maximum(top, m, m);
         } else {
             top = maximum(maximum(top, x[0], x[1]), x[2], x[3]);
         }
     }
     template <int MC>
-    __device__ __forceinline__ void flush(int text, float (&top)[MC], int (&tok)[MC], const float (&b)[MC], const Place &at) const {
+    __device__ __forceinline__ void flush(int64_t slot, float (&top)[MC], int (&tok)[MC], const float (&b)[MC], const Place &at) const {
         static_assert(MC <= 4, "a lane group writes one column block");
         const int q = at.lane >> 4;
-        int mine = 0, row = 0;
+        float mine = 0.f;
+        int row = 0;
 #pragma unroll
         for (int j = 0; j < MC; j++) {
-            // as integers positive values order as they should, NaN above them, and the others are below 0
-            const float l = top[j] + b[j];
-            int x = l != l ? 0x7FC00000 : __float_as_int(l), r = tok[j];
+            float x = top[j];
+            int r = tok[j];
 #pragma unroll
             for (int d = 16; d <= 32; d <<= 1) {
-                const int xo = __shfl_xor(x, d, GS_WAVE);
+                const float xo = __shfl_xor(x, d, GS_WAVE);
                 if (TOK) {
                     const int ro = __shfl_xor(r, d, GS_WAVE);
                     r = xo > x || (xo == x && ro < r) ? ro : r;
                 }
-                x = max(x, xo);
+                x = maximum(x, xo, xo);
             }
-            if (j == q) mine = x, row = r;
+            if (j == q) mine = x + b[j], row = r;
         }
-        const int v = at.col0 + 16 * q + (at.lane & 15);
-        if (q < MC && v < vocab && mine > 0) {
-            const int64_t o = (int64_t)text * vocab + v;
-            if (TOK)
-                atomicMax((unsigned long long *)best + o,
-                          (unsigned long long)(uint32_t)mine << 32 | (0xFFFFFFFFu - (uint32_t)row));
-            else
-                atomicMax((uint32_t *)best + o, (uint32_t)mine);
+        const int v = at.col0 + at.lane;
+        if (q < MC && v < vocab) {
+            best[slot * vocab + v] = mine;
+            if (TOK) where[slot * vocab + v] = row;
         }
     }
     template <class TL>
     __device__ __forceinline__ void run(f32x4 (&acc)[TL::MR][TL::MC], const Place &at) const {
         const int q = at.lane >> 4;
         if (at.row0 >= at.n_r) return;
+        const int64_t block = at.row0 / (TL::MR * 16);
         float b[TL::MC], top[TL::MC];
         int tok[TL::MC];
 #pragma unroll
-        for (int j = 0; j < TL::MC; j++) b[j] = bias[at.col0 + 16 * j + (at.lane & 15)], top[j] = -INFINITY, tok[j] = 0x7FFFFFFF;
-        int4 s[TL::MR];
-#pragma unroll
-        for (int i = 0; i < TL::MR; i++) s[i] = *reinterpret_cast<const int4 *>(seg + at.row0 + 16 * i + 4 * q);
-        int cur = __builtin_amdgcn_readlane(s[0].x, 0);
+        for (int j = 0; j < TL::MC; j++) b[j] = at.side(0, at.c_in + 16 * j + (at.lane & 15)), top[j] = -INFINITY, tok[j] = 0x7FFFFFFF;
+        int cur = gs_uniform(__float_as_int(at.side(1, at.r_in)));
 #pragma unroll
         for (int i = 0; i < TL::MR; i++) {
             const int row = at.row0 + 16 * i + 4 * q;
-            const int lo = __builtin_amdgcn_readlane(s[i].x, 0), hi = __builtin_amdgcn_readlane(s[i].w, 48);
+            const f32x4 sf = at.side4(1, at.r_in + 16 * i + 4 * q);
+            const int sv[4] = {__float_as_int(sf[0]), __float_as_int(sf[1]), __float_as_int(sf[2]), __float_as_int(sf[3])};
+            const int lo = __builtin_amdgcn_readlane(sv[0], 0), hi = __builtin_amdgcn_readlane(sv[3], 48);
             if (lo == cur && hi == cur) {  // all of one text
 #pragma unroll
                 for (int j = 0; j < TL::MC; j++) take(acc[i][j], row, top[j], tok[j]);
@@ -633,12 +652,11 @@ struct EpiTextMax {
             int now = lo;
             while (now >= 0) {  // rows past the last kept one are -1, and come last
                 if (now != cur) {
-                    flush<TL::MC>(cur, top, tok, b, at);
+                    flush<TL::MC>(block + cur, top, tok, b, at);
                     cur = now;
 #pragma unroll
                     for (int j = 0; j < TL::MC; j++) top[j] = -INFINITY, tok[j] = 0x7FFFFFFF;
                 }
-                const int sv[4] = {s[i].x, s[i].y, s[i].z, s[i].w};
                 int next = 0x7FFFFFFF;
 #pragma unroll
                 for (int e = 0; e < 4; e++)
@@ -656,7 +674,7 @@ struct EpiTextMax {
                 now = next == 0x7FFFFFFF ? -1 : next;
             }
         }
-        flush<TL::MC>(cur, top, tok, b, at);
+        flush<TL::MC>(block + cur, top, tok, b, at);
     }
 };
 
@@ -818,17 +836,34 @@ __global__ __launch_bounds__(256) void k_bias_grad(const float *sums, int64_t ld
 
 // ---------------------------------------------------------------- term weights' small kernels
 
+// A text's weights from its slots: log(1 + relu(maximum)), and the lowest token that has it (-1 where the weight is 0).
 template <bool TOK>
-__global__ void k_term_weights(const void *best, int64_t n, int vocab, const int *rows, int length, float *weights,
-                               int *tokens) {
-    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
-        if (TOK) {
-            const unsigned long long k = ((const unsigned long long *)best)[i];
-            weights[i] = log1pf(__uint_as_float((uint32_t)(k >> 32)));
-            tokens[i] = k ? rows[0xFFFFFFFFu - (uint32_t)k] % length : -1;
-        } else {
-            weights[i] = log1pf(__uint_as_float(((const uint32_t *)best)[i]));
+__global__ __launch_bounds__(256) void k_term_weights(const float *best, const int *where, const int *text_first, int block, int vocab,
+                                                      const int *rows, int length, float *weights, int *tokens) {
+    const int64_t b = blockIdx.y;
+    const int f0 = text_first[b], f1 = text_first[b + 1];
+    const int w0 = f0 / block, w1 = (f1 - 1) / block;
+    for (int v = blockIdx.x * 256 + threadIdx.x; v < vocab; v += gridDim.x * 256) {
+        float x = 0.f;
+        int row = -1;
+        if (f1 > f0) {
+#pragma unroll 4
+            for (int w = w0; w <= w1; w++) {
+                const int64_t at = (w + b) * vocab + v;
+                const float y = best[at];
+                if (TOK && y > x) row = where[at];
+                x = maximum(x, y, y);
+            }
         }
+        weights[b * vocab + v] = log1pf(x);
+        if (TOK) tokens[b * vocab + v] = row >= 0 ? rows[row] % length : -1;
+    }
+}
+
+__global__ void k_no_tokens(int64_t n, float *weights, int *tokens) {
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
+        weights[i] = 0.f;
+        if (tokens) tokens[i] = -1;
     }
 }
 
@@ -1250,7 +1285,7 @@ Layout layout_of(const gs_vocab_head *h) {
 
 // What every call makes first.
 struct Common {
-    int *n, *rows, *inv, *seg;
+    int *n, *rows, *inv, *seg, *text_first;
     float *bias;
     uint16_t *hidden, *weight;
 };
@@ -1260,6 +1295,7 @@ void take_common(gs_arena &a, const Layout &l, const gs_vocab_head *h, bool text
     s->rows = a.take<int>(l.rows);
     s->inv = texts ? nullptr : a.take<int>(l.rows);
     s->seg = texts ? a.take<int>(l.rows + kRowPad) : nullptr;
+    s->text_first = texts ? a.take<int>(h->texts + 1) : nullptr;
     s->bias = a.take<float>(l.vocabp);
     s->hidden = a.take<uint16_t>((size_t)l.rows * l.planes * l.dimp);
     s->weight = l.w_direct ? nullptr : a.take<uint16_t>((size_t)h->vocab * l.planes * l.dimp);
@@ -1285,7 +1321,7 @@ Operand weight_operand(const Layout &l, const Common &s, const gs_vocab_head *h)
 // Kept rows, bias, cleared memory, then hidden states and (where needed) vocabulary rows in the product's form.
 int prepare(const gs_vocab_head *h, const Layout &l, const Keep &keep, const Common &c, float *zero, int64_t zeros, hipStream_t s) {
     hipLaunchKernelGGL(k_setup, dim3(1 + gs_blocks(l.vocabp + zeros / 4, 1024, 1024)), dim3(1024), 0, s, keep,
-                       h->length > 0 ? h->length : 1, c.rows, c.inv, c.seg, c.n, h->bias_d, h->bias_type, h->vocab, l.vocabp,
+                       h->length > 0 ? h->length : 1, c.rows, c.inv, c.seg, c.text_first, c.n, h->bias_d, h->bias_type, h->vocab, l.vocabp,
                        c.bias, zero, zeros);
     GS_CHECK_LAUNCH();
     const int w_rows = l.w_direct ? 0 : h->vocab;
@@ -1435,17 +1471,20 @@ int run_grad(const gs_vocab_head *h, const LossPlan &p, const LossSaved &s, cons
         if (nv <= 0) break;
         Operand wp = w;
         wp.p += (int64_t)v0 * w.stride;
-        const EpiLogitGrad<S> e{s.c.bias, scale, s.lse2, g.factor, entries_of(p, s), v0, g.dl, dl.stride, p.piece,
-                                want_db ? g.sums : nullptr, p.l.vocabp};
         const EpiHiddenPart eh{g.part, p.l.dimp, c > 0};
         const EpiWeightGrad<O> ew{(O *)dw_d + (int64_t)v0 * h->dim, g.scale, h->dim, h->dim % 4 == 0};
         const Dims de{nv, p.l.rows, p.l.dimp, s.c.n, 0, 1, 0};
         const Dims dh{want_dh ? h->dim : 0, p.l.rows, nv, s.c.n, 0, 1, 0};
         const Dims dw{dw_d ? h->dim : 0, nv, p.l.rows, s.c.n, 0, 0, 1};
         int rc = GS_OK;
-#define GSV_GRAD(TL) rc = launch_product<TL<T, NP, false, false>>(wp, hid, de, e, cus, st)
+#define GSV_EPI(SHARES) \
+    EpiLogitGrad<S, SHARES> { s.c.bias, scale, s.lse2, g.factor, entries_of(p, s), v0, g.dl, dl.stride, p.piece, want_db ? g.sums : nullptr, p.l.vocabp }
+#define GSV_GRAD(TL)                                                                              \
+    rc = s.share ? launch_product<TL<T, NP, false, false>>(wp, hid, de, GSV_EPI(true), cus, st)   \
+                 : launch_product<TL<T, NP, false, false>>(wp, hid, de, GSV_EPI(false), cus, st)
         GSV_BY_CLASS(p.l.cls, GSV_GRAD)
 #undef GSV_GRAD
+#undef GSV_EPI
         if (rc) return rc;
         if (!want_dh && !dw_d) continue;
 #define GSV_PAIR(TL)                                                                                                  \
@@ -1604,6 +1643,12 @@ extern "C" int gs_vocab_loss_grad(const gs_vocab_head *h, const gs_vocab_targets
 
 namespace gsv {
 
+// Slots of the maxima: a block of a wave's rows and a text each make one more.
+size_t text_slots(const gs_vocab_head *h, const Layout &l) {
+    const int block = edge_of(l.cls) / row_waves_of(l.cls);
+    return (size_t)(l.rows + block - 1) / block + h->texts;
+}
+
 struct EntryPlan {
     int runs, chunk, chunks, dimp;
     Entry *entries;
@@ -1680,7 +1725,9 @@ extern "C" int gs_term_weights_workspace(const gs_vocab_head *h, int32_t tokens,
     gs_arena a{nullptr, 0, 0}, b{nullptr, 0, 0};
     Common c;
     take_common(a, l, h, true, &c);
-    a.take<float>((size_t)h->texts * h->vocab * (tokens ? 2 : 1));
+    const size_t slots = text_slots(h, l);
+    a.take<float>(slots * h->vocab);
+    if (tokens) a.take<int>(slots * h->vocab);
     EntryPlan p;
     take_entries(b, h, &p);
     *bytes = a.used, *grad_bytes = b.used;
@@ -1696,22 +1743,29 @@ extern "C" int gs_term_weights(const gs_vocab_head *h, const uint8_t *mask_d, fl
     gs_arena a{(char *)workspace_d, 0, workspace_bytes};
     Common c;
     take_common(a, l, h, true, &c);
-    const int64_t n = (int64_t)h->texts * h->vocab;
-    const int64_t words = tokens_d ? 2 * n : n;
-    float *best = a.take<float>(words);
+    const size_t slots = text_slots(h, l);
+    float *best = a.take<float>(slots * h->vocab);
+    int *where = tokens_d ? a.take<int>(slots * h->vocab) : nullptr;
     if (!a.ok()) {
         gs_set_error("term_weights workspace too small: need %zu bytes, got %zu", a.used, workspace_bytes);
         return GS_ENOSPC;
     }
-    if (n == 0) return GS_OK;
+    if (h->texts == 0) return GS_OK;
     GS_REQUIRE(weights_d && workspace_d, "NULL weights or workspace");
+    GS_REQUIRE(h->texts <= 65535, "texts=%d exceed 65535", h->texts);
     const hipStream_t s = gs_stream(stream);
-    if (int rc = prepare(h, l, Keep{mask_d, nullptr, 0, h->vocab, l.rows}, c, best, words, s)) return rc;
-    if (l.rows > 0) {
+    if (l.rows == 0) {  // texts without tokens
+        const int64_t n = (int64_t)h->texts * h->vocab;
+        hipLaunchKernelGGL(k_no_tokens, dim3(gs_blocks(n, 256, 8192)), dim3(256), 0, s, n, weights_d, tokens_d);
+        GS_CHECK_LAUNCH();
+        return GS_OK;
+    }
+    if (int rc = prepare(h, l, Keep{mask_d, nullptr, 0, h->vocab, l.rows}, c, nullptr, 0, s)) return rc;
+    {
         const Dims d{l.rows, h->vocab, l.dimp, c.n, 1, 0, 0};
         const Operand hid = hidden_operand(l, c), w = weight_operand(l, c, h);
-        const EpiTextMax<true> et{c.bias, c.seg, best, h->vocab};
-        const EpiTextMax<false> ef{c.bias, c.seg, best, h->vocab};
+        const EpiTextMax<true> et{c.bias, c.seg, best, where, h->vocab};
+        const EpiTextMax<false> ef{c.bias, c.seg, best, where, h->vocab};
         int rc = GS_OK;
 #define GSV_TILE(TL) rc = tokens_d ? launch_product<TL<GSV_T, false, false>>(hid, w, d, et, cus, s) \
                                    : launch_product<TL<GSV_T, false, false>>(hid, w, d, ef, cus, s)
@@ -1731,12 +1785,14 @@ extern "C" int gs_term_weights(const gs_vocab_head *h, const uint8_t *mask_d, fl
 #undef GSV_TILE
         if (rc) return rc;
     }
-    const unsigned g = gs_blocks(n, 256, 8192);
-    const int length = h->length > 0 ? h->length : 1;
+    const dim3 g(gs_blocks(h->vocab, 256, 1024), h->texts);
+    const int block = edge_of(l.cls) / row_waves_of(l.cls);
     if (tokens_d)
-        hipLaunchKernelGGL(k_term_weights<true>, dim3(g), dim3(256), 0, s, best, n, h->vocab, c.rows, length, weights_d, tokens_d);
+        hipLaunchKernelGGL(k_term_weights<true>, g, dim3(256), 0, s, best, where, c.text_first, block, h->vocab, c.rows, h->length,
+                           weights_d, tokens_d);
     else
-        hipLaunchKernelGGL(k_term_weights<false>, dim3(g), dim3(256), 0, s, best, n, h->vocab, c.rows, length, weights_d, tokens_d);
+        hipLaunchKernelGGL(k_term_weights<false>, g, dim3(256), 0, s, best, where, c.text_first, block, h->vocab, c.rows, h->length,
+                           weights_d, tokens_d);
     GS_CHECK_LAUNCH();
     return GS_OK;
 }

@@ -45,6 +45,7 @@ struct F16 {
     }
 };
 
+constexpr int kSides = 4;
 constexpr int kStep = 64;  // k values per stage: two 16x16x32 products deep, and whole 128-byte lines of [x][k] rows
 
 // A 16-bit matrix.  [x][k]: row x starts at p + x * stride; [k][x]: row k does.  Plane i of an
@@ -75,12 +76,6 @@ __device__ __forceinline__ int turn(int k) {
     return X >= 128 ? (k & 3) | ((k >> 1) & 4) : k & 3;
 }
 
-// The first `values` values at p; reads past them give 0.
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc64(const uint16_t *p, int64_t values) {
-    const int64_t b = values <= 0 ? 0 : values * 2;
-    return gs_rsrc(p, (uint32_t)(b > 0x7FFFFFF0ll ? 0x7FFFFFF0ll : b));
-}
-
 // Issues one stage's 1 KiB pieces of an operand that belong to this wave, straight to LDS.
 // [x][k]: a piece is eight rows of 128 bytes, and slot s of row x holds 16-byte chunk s ^ (x & 7), so that the eight rows
 // that one read cycle takes lie in different banks.  (Rows of 64 bytes asked the L2 for half lines: 20% slower.)  [k][x]:
@@ -96,26 +91,57 @@ struct Loader {
         const int row = wave * (64 / per) + lane / per, s = lane % per;
         return (int)(row * o.stride * 2) + (s ^ (KM ? turn<X>(row) << 1 : row & 7)) * 16;
     }
-    // values: what may be read from p on; gap: bytes between a wave's pieces
-    __device__ __forceinline__ static void issue(const uint16_t *p, int64_t values, int gap, int off, lds_t lds, int wave) {
+    // gap: bytes between a wave's pieces
+    __device__ __forceinline__ static void issue(__amdgpu_buffer_rsrc_t r, int gap, int off, int soff, lds_t lds, int wave) {
 #if defined(__HIP_DEVICE_COMPILE__)  // the host pass does not know 16-byte pieces and would leave the kernel out
-        const auto r = rsrc64(p, values);
 #pragma unroll
         for (int u = 0; u < pieces; u++)
             __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)(lds + ((wave + u * NW) << 10)), 16,
-                                                     off + u * gap, 0, 0, 0);
+                                                     off + u * gap, soff, 0, 0);
 #endif
     }
 };
 
-// Where stage k of an operand's tile at x0 starts, and how much may be read from there.
-template <bool KM>
-__device__ __forceinline__ const uint16_t *stage_at(const Operand &o, int64_t x0, int64_t nx, int64_t k, int64_t nk, int plane,
-                                                    int64_t *values) {
-    const int64_t row = KM ? k : x0, rows = KM ? nk : nx, in = plane * o.plane + (KM ? x0 : k);
-    *values = (rows - row - 1) * o.stride + o.width - in;
-    return o.p + row * o.stride + in;
-}
+// The next stage of an operand's tile: a buffer that ends with the rows that exist, and an offset into its rows.  The
+// buffer of a [x][k] tile stays and the offset moves along its rows (never past them, so the rows that exist are those
+// whose own offset lies in the buffer); that of a [k][x] tile moves by the stage's rows.
+template <int X, bool KM>
+struct Cursor {
+    const char *p;
+    int bytes, soff, rows;
+    __device__ __forceinline__ void start(const Operand &o, int x0, int nx, int k, int nk, int plane) {
+        const int64_t in = plane * o.plane;
+        if (KM) {
+            p = reinterpret_cast<const char *>(o.p + k * o.stride + in + x0);
+            rows = nk - k;
+            bytes = (int)(o.width - in - x0) * 2;
+            soff = 0;
+        } else {
+            p = reinterpret_cast<const char *>(o.p + x0 * o.stride);
+            bytes = (int)((min(nx - x0, X) - 1) * o.stride + o.width) * 2;
+            soff = (int)(in + k) * 2;
+            rows = 0;
+        }
+        uniform();
+    }
+    // one value per wave, which the compiler does not see through the stream's loop
+    __device__ __forceinline__ void uniform() {
+        p = reinterpret_cast<const char *>(gs_uniform64(reinterpret_cast<int64_t>(p)));
+        bytes = gs_uniform(bytes), soff = gs_uniform(soff), rows = gs_uniform(rows);
+    }
+    __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const Operand &o) const {
+        return gs_rsrc(p, (uint32_t)(KM ? (min(rows, kStep) - 1) * (int)(o.stride * 2) + bytes : bytes));
+    }
+    __device__ __forceinline__ void next(const Operand &o) {
+        if (KM) {
+            p += o.stride * (2 * kStep);
+            rows -= kStep;
+        } else {
+            soff += 2 * kStep;
+        }
+        uniform();
+    }
+};
 
 // Fragments of 16 rows (columns) x 32 k values, half h of a stage: lane l holds row l & 15, k = 32 h + 8 (l >> 4) .. + 7.
 template <int X, bool KM, int M>
@@ -165,8 +191,16 @@ struct Tile {
     static constexpr int waves = WR * WC, threads = 64 * waves, waves_per_simd = OCC;
     static constexpr int MR = BR / WR / 16, MC = BC / WC / 16;
     static constexpr int stage_bytes = (BR + BC) * kStep * 2;
-    static constexpr int lds_bytes = NS * stage_bytes;
+    static constexpr int side_bytes = kSides * 1024;
+    static constexpr int lds_bytes = NS * stage_bytes + 2 * side_bytes;
     static constexpr bool r_kmajor = RK, c_kmajor = CK;
+};
+
+// What an epilogue reads per row or column of a tile (a bias, a row's softmax sum) comes to LDS with the tile's first
+// stage: up to kSides arrays of 32-bit values, twice (a tile's epilogue runs while the next tile's arrive).
+struct SideArray {
+    const void *p;  // of the tile's first row or column
+    int count;      // values from there on that exist; the others read 0
 };
 
 // Where a wave's 16x16 blocks lie: block (i, j) has rows row0 + 16 i + 4 (lane >> 4) + 0..3 and column
@@ -174,6 +208,15 @@ struct Tile {
 struct Place {
     int row0, col0, lane, split;
     int n_r, n_c;
+    int r_in, c_in;  // row0 and col0 within the tile
+    lds_t sides;
+    // side array a's values at in .. in + 3 (of the tile), or the one at in
+    __device__ __forceinline__ f32x4 side4(int a, int in) const {
+        return *(__attribute__((address_space(3))) f32x4 *)(sides + a * 1024 + in * 4);
+    }
+    __device__ __forceinline__ float side(int a, int in) const {
+        return *(__attribute__((address_space(3))) float *)(sides + a * 1024 + in * 4);
+    }
 };
 
 // A product's sizes as the device knows them.
@@ -196,6 +239,7 @@ __device__ __forceinline__ Shape shape_of(const Dims &d, int n_dev) {
 template <class TL, class Epi>
 struct Side {
     using tile = TL;
+    using epilogue = Epi;
     Operand R, C;
     Dims d;
     Epi epi;
@@ -210,9 +254,9 @@ __device__ __forceinline__ Work work_of(const Shape &s, int parts, int t) {
     const int area = s.tr * s.tc, part = t / area, in = t - part * area;
     const int group = in / (8 * s.tc), left = in - group * 8 * s.tc;
     const int tall = min(8, s.tr - group * 8);
-    const int k0 = (int)((int64_t)s.steps * part / parts);
-    return Work{(group * 8 + left % tall) * TL::BR, (left / tall) * TL::BC, part, k0,
-                (int)((int64_t)s.steps * (part + 1) / parts) - k0};
+    const int k0 = s.steps * part / parts;  // at most 2^22 steps and 64 parts
+    return Work{gs_uniform((group * 8 + left % tall) * TL::BR), gs_uniform((left / tall) * TL::BC), gs_uniform(part), gs_uniform(k0),
+                gs_uniform(s.steps * (part + 1) / parts - k0)};
 }
 
 // The stages of a workgroup's tiles, issued one after the other whatever tile they belong to: while a tile's epilogue
@@ -221,70 +265,91 @@ template <class SA, class SB>
 struct Stream {
     using TA = typename SA::tile;
     using TB = typename SB::tile;
-    using LR = Loader<TA::BR, TA::r_kmajor, TA::waves>;
-    using LC = Loader<TA::BC, TA::c_kmajor, TA::waves>;
-    static constexpr int loads = LR::pieces + LC::pieces;
+    static constexpr bool pair = !std::is_same_v<SA, SB>;
+    static constexpr int loads = Loader<TA::BR, TA::r_kmajor, TA::waves>::pieces + Loader<TA::BC, TA::c_kmajor, TA::waves>::pieces;
     Work w;
     int r_off, c_off;     // the lane's
-    int r_gap, c_gap;
-    const uint16_t *r_p, *c_p;  // the next stage of either operand, what may be read from there, and the way to the one after
-    int64_t r_n, c_n, r_by, c_by;
+    Cursor<TA::BR, TA::r_kmajor> ra;
+    Cursor<TA::BC, TA::c_kmajor> ca;
+    Cursor<TB::BR, TB::r_kmajor> rb;
+    Cursor<TB::BC, TB::c_kmajor> cb;
     int t, last, by, na;  // tiles t, t + by, ... below last; those below na are the first product's
     int ik, seg, buf, left;
+    bool fresh;           // the next stage is its tile's first
+    int parity;           // of the tile, for its side arrays
 
-    template <class TL>
-    __device__ __forceinline__ void offsets(const Operand &R, const Operand &C, int wave, int lane) {
-        using R_ = Loader<TL::BR, TL::r_kmajor, TL::waves>;
-        using C_ = Loader<TL::BC, TL::c_kmajor, TL::waves>;
-        r_off = R_::offset(R, wave, lane);
-        c_off = C_::offset(C, wave, lane);
-        r_gap = (int)(R_::step * R.stride * 2);
-        c_gap = (int)(C_::step * C.stride * 2);
-        r_by = TL::r_kmajor ? kStep * R.stride : kStep;
-        c_by = TL::c_kmajor ? kStep * C.stride : kStep;
+    __device__ __forceinline__ bool in_a() const { return !pair || t < na; }
+    template <class S>
+    __device__ __forceinline__ void sides(const S &side, const Shape &s, lds_t lds, int wave, int lane) const {
+#if defined(__HIP_DEVICE_COMPILE__)
+#pragma unroll
+        for (int a = 0; a < S::epilogue::sides; a++) {
+            if (wave != a % TA::waves) continue;
+            const SideArray x = side.epi.side(a, w.r0, w.c0, s);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                gs_rsrc(x.p, (uint32_t)max(x.count, 0) * 4u),
+                (__attribute__((address_space(3))) void *)(lds + TA::NS * TA::stage_bytes + parity * TA::side_bytes + a * 1024), 16,
+                lane * 16, 0, 0, 0);
+        }
+#endif
     }
-    // Moves to the first stage of plane pair seg
-    template <class TL>
-    __device__ __forceinline__ void start(const Operand &R, const Operand &C, const Shape &s) {
-        const int pr = TL::planes == 3 ? plane_r(seg) : 0, pc = TL::planes == 3 ? plane_c(seg) : 0;
-        r_p = stage_at<TL::r_kmajor>(R, w.r0, s.nr, w.k0 * kStep, s.nk, pr, &r_n);
-        c_p = stage_at<TL::c_kmajor>(C, w.c0, s.nc, w.k0 * kStep, s.nk, pc, &c_n);
-        ik = 0;
+    template <class S, class CR, class CC>
+    __device__ __forceinline__ void seek_in(const S &side, const Shape &s, int parts, int at, CR &r, CC &c, int wave, int lane) {
+        using TL = typename S::tile;
+        w = work_of<TL>(s, parts, at);
+        left = w.per * (TL::planes == 3 ? 6 : 1);
+        seg = ik = 0;
+        r_off = Loader<TL::BR, TL::r_kmajor, TL::waves>::offset(side.R, wave, lane);
+        c_off = Loader<TL::BC, TL::c_kmajor, TL::waves>::offset(side.C, wave, lane);
+        planes(side, s, r, c);
+    }
+    // To the first stage of plane pair seg
+    template <class S, class CR, class CC>
+    __device__ __forceinline__ void planes(const S &side, const Shape &s, CR &r, CC &c) {
+        constexpr bool three = S::tile::planes == 3;
+        r.start(side.R, w.r0, s.nr, w.k0 * kStep, s.nk, three ? plane_r(seg) : 0);
+        c.start(side.C, w.c0, s.nc, w.k0 * kStep, s.nk, three ? plane_c(seg) : 0);
     }
     // Moves to tile t, or the next one with stages
     __device__ __forceinline__ void seek(const SA &A, const SB &B, const Shape &a, const Shape &b, int parts, int wave, int lane) {
         for (; t < last; t += by) {
-            w = t < na ? work_of<TA>(a, parts, t) : work_of<TB>(b, 1, t - na);
-            left = w.per * (TA::planes == 3 ? 6 : 1);
+            if (in_a()) seek_in(A, a, parts, t, ra, ca, wave, lane);
+            else seek_in(B, b, 1, t - na, rb, cb, wave, lane);
             if (left == 0) continue;
-            seg = 0;
-            if (t < na) {
-                offsets<TA>(A.R, A.C, wave, lane);
-                start<TA>(A.R, A.C, a);
-            } else {
-                offsets<TB>(B.R, B.C, wave, lane);
-                start<TB>(B.R, B.C, b);
-            }
+            fresh = true;
+            parity ^= 1;
             return;
+        }
+    }
+    template <class S, class CR, class CC>
+    __device__ __forceinline__ void issue_in(const S &side, const Shape &s, CR &r, CC &c, lds_t lds, int wave, int lane) {
+        using TL = typename S::tile;
+        const lds_t to = lds + buf * TL::stage_bytes;
+        if (S::epilogue::sides > 0 && fresh) sides(side, s, lds, wave, lane);
+        using LR = Loader<TL::BR, TL::r_kmajor, TL::waves>;
+        using LC = Loader<TL::BC, TL::c_kmajor, TL::waves>;
+        LR::issue(r.buffer(side.R), LR::step * (int)side.R.stride * 2, r_off, r.soff, to, wave);
+        LC::issue(c.buffer(side.C), LC::step * (int)side.C.stride * 2, c_off, c.soff, to + TL::BR * kStep * 2, wave);
+        fresh = false;
+        if (TL::planes == 3 && ++ik == w.per) {
+            ik = 0;
+            seg++;
+            if (left > 1) planes(side, s, r, c);
+        } else {
+            r.next(side.R);
+            c.next(side.C);
         }
     }
     __device__ __forceinline__ bool issue(lds_t lds, const SA &A, const SB &B, const Shape &a, const Shape &b, int parts, int wave,
                                           int lane) {
         if (t >= last) return false;
-        const lds_t to = lds + buf * TA::stage_bytes;
-        LR::issue(r_p, r_n, r_gap, r_off, to, wave);
-        LC::issue(c_p, c_n, c_gap, c_off, to + TA::BR * kStep * 2, wave);
+        if (in_a()) issue_in(A, a, ra, ca, lds, wave, lane);
+        else issue_in(B, b, rb, cb, lds, wave, lane);
         buf = buf == TA::NS - 1 ? 0 : buf + 1;
-        if (--left == 0) {
-            t += by;
+        left = gs_uniform(left - 1);
+        if (left == 0) {
+            t = gs_uniform(t + by);
             seek(A, B, a, b, parts, wave, lane);
-        } else if (TA::planes == 3 && ++ik == w.per) {
-            seg++;
-            if (t < na) start<TA>(A.R, A.C, a);
-            else start<TB>(B.R, B.C, b);
-        } else {
-            r_p += r_by, c_p += c_by;
-            r_n -= r_by, c_n -= c_by;
         }
         return true;
     }
@@ -335,6 +400,7 @@ __global__ __launch_bounds__(SA::tile::threads, SA::tile::waves_per_simd) void k
     st.by = (gridDim.x - xcd + xcds - 1) / xcds;
     st.na = na;
     st.buf = 0;
+    st.parity = 1;
     const int first = st.t, last = st.last, by = st.by;
     st.seek(A, B, a, b, parts, wave, lane);
     constexpr int loads = Stream<SA, SB>::loads, NS = TA::NS;
@@ -350,6 +416,7 @@ __global__ __launch_bounds__(SA::tile::threads, SA::tile::waves_per_simd) void k
     };
     landed();
     ahead += st.issue(lds, A, B, a, b, parts, wave, lane);
+    int parity = 0;
 
     // A tile.  The fragments of a half stage are read while the products of the half before run.  Before a stage's second
     // half the next stage has to have landed, and this one, which every wave holds by then, makes room for another.
@@ -390,11 +457,18 @@ __global__ __launch_bounds__(SA::tile::threads, SA::tile::waves_per_simd) void k
             ahead += st.issue(lds, A, B, a, b, parts, wave, lane);
             multiply(1);
         }
-        side.epi.template run<TL>(acc, Place{w.r0 + wr * TL::MR * 16, w.c0 + wc * TL::MC * 16, lane, w.part, s.nr, s.nc});
+        side.epi.template run<TL>(acc, Place{w.r0 + wr * TL::MR * 16, w.c0 + wc * TL::MC * 16, lane, w.part, s.nr, s.nc,
+                                             wr * TL::MR * 16, wc * TL::MC * 16,
+                                             lds + NS * TL::stage_bytes + parity * TL::side_bytes});
+        if (total > 0) parity ^= 1;  // as the stream, which knows tiles with stages alone
     };
     for (int t = first; t < last; t += by) {
-        if (t < na) run(A, work_of<TA>(a, parts, t), a);
-        else if constexpr (!std::is_same_v<SA, SB>) run(B, work_of<TB>(b, 1, t - na), b);
+        if constexpr (!std::is_same_v<SA, SB>) {
+            if (t < na) run(A, work_of<TA>(a, parts, t), a);
+            else run(B, work_of<TB>(b, 1, t - na), b);
+        } else {
+            run(A, work_of<TA>(a, 1, t), a);
+        }
     }
 }
 
