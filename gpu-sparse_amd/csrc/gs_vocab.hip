@@ -103,6 +103,22 @@ __device__ __forceinline__ float wave_max(float v) {
     for (int d = 32; d >= 1; d >>= 1) v = fmaxf(v, __shfl_xor(v, d, GS_WAVE));
     return v;
 }
+// The values of lanes l and l ^ D (D 16 or 32), the lower lane's first: the same two in both lanes.
+template <class T>
+struct Two {
+    T a, b;
+};
+template <int D, class T>
+__device__ __forceinline__ Two<T> across(T x) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, x);
+    if constexpr (D == 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+        return {__builtin_bit_cast(T, (uint32_t)r[0]), __builtin_bit_cast(T, (uint32_t)r[1])};
+    } else {
+        const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+        return {__builtin_bit_cast(T, (uint32_t)r[0]), __builtin_bit_cast(T, (uint32_t)r[1])};
+    }
+}
 // the larger one, NaN if either is
 __device__ __forceinline__ float maximum(float a, float b, float c) {
     return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c);
@@ -123,61 +139,57 @@ struct Keep {
     int64_t ignore;
     int vocab;
     int total;
-    // bit e: row r0 + e is kept
-    __device__ __forceinline__ uint32_t sixteen(int64_t r0) const {
-        if (r0 >= total) return 0;
-        const uint32_t in = r0 + 16 > total ? (1u << (total - r0)) - 1u : 0xFFFFu;
-        uint32_t m = 0;
+    __device__ __forceinline__ bool row(int64_t r) const {
         if (targets) {
-#pragma unroll
-            for (int e = 0; e < 16; e++) {
-                const int64_t t = targets[min(r0 + e, (int64_t)total - 1)];
-                m |= (t >= 0 && t < vocab && t != ignore ? 1u : 0u) << e;
-            }
-        } else if (!mask) {
-            m = 0xFFFF;
-        } else if ((reinterpret_cast<uintptr_t>(mask) & 15) == 0 && r0 + 16 <= total) {
-            const uint4 w = *reinterpret_cast<const uint4 *>(mask + r0);
-            const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-            for (int e = 0; e < 16; e++) m |= (((ws[e >> 2] >> (8 * (e & 3))) & 255u) ? 1u : 0u) << e;
-        } else {
-#pragma unroll
-            for (int e = 0; e < 16; e++) m |= (mask[min(r0 + e, (int64_t)total - 1)] ? 1u : 0u) << e;
+            const int64_t t = targets[min(r, (int64_t)total - 1)];
+            return r < total && t >= 0 && t < vocab && t != ignore;
         }
-        return m & in;
+        return r < total && (!mask || mask[min(r, (int64_t)total - 1)] != 0);
     }
 };
 
 // rows[i]: the i-th kept row, ascending; inv[row]: its place or -1; *n: how many.  For texts of `length` rows, seg[i]
-// is the row's text, -1 for the rest of the last tile, and text_first[b] the first place of a text's rows.  One workgroup of 1024, 16 rows per thread and turn.
+// is the row's text, -1 for the rest of the last tile, and text_first[b] the first place of a text's rows.  One workgroup of
+// 1024; a wave takes 1024 rows a turn, 64 at a time.
 __device__ __forceinline__ void kept_rows(const Keep &keep, int length, int *rows, int *inv, int *seg, int *text_first, int *n) {
     __shared__ int part[16];
     const int tid = threadIdx.x, lane = gs_lane(), wave = tid >> 6;
+    const double by_length = 1.0 / length;
     int base = 0;
     for (int64_t at = 0; at < keep.total; at += 16384) {
-        const int64_t r0 = at + tid * 16;
-        const uint32_t m = keep.sixteen(r0);
-        const uint32_t c = __popc(m);
-        const uint32_t inc = gs_wave_incl_scan(c);
-        if (lane == 63) part[wave] = (int)inc;
+        const int64_t r0 = at + wave * 1024;
+        uint64_t kept[16];
+        int c = 0;
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+            kept[e] = __ballot(keep.row(r0 + e * 64 + lane));
+            c += __popcll(kept[e]);
+        }
+        if (lane == 0) part[wave] = c;
         __syncthreads();
-        int before = base;
+        int o = base;
         for (int w = 0; w < 16; w++) {
-            if (w < wave) before += part[w];
+            if (w < wave) o += part[w];
             base += part[w];
         }
-        int o = before + (int)(inc - c);
-        for (int e = 0; e < 16 && r0 + e < keep.total; e++) {
-            const bool k = (m >> e) & 1;
-            const int row = (int)(r0 + e);
-            if (inv) inv[row] = k ? o : -1;
-            if (seg && row % length == 0) text_first[row / length] = o;
-            if (k) {
-                rows[o] = row;
-                if (seg) seg[o] = row / length;
-                o++;
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+            const int64_t r = r0 + e * 64 + lane;
+            const bool k = (kept[e] >> lane) & 1;
+            const int i = o + __popcll(kept[e] & gs_lanemask_lt());
+            if (r < keep.total) {
+                const int row = (int)r;
+                if (inv) inv[row] = k ? i : -1;
+                if (seg) {
+                    int text = (int)(row * by_length);  // at most one off
+                    text += (text + 1) * length <= row ? 1 : 0;
+                    text -= text * length > row ? 1 : 0;
+                    if (row == text * length) text_first[text] = i;
+                    if (k) seg[i] = text;
+                }
+                if (k) rows[i] = row;
             }
+            o += __popcll(kept[e]);
         }
         __syncthreads();
     }
@@ -423,14 +435,14 @@ struct EpiSums {
                         for (int e = 0; e < 4; e++) x = mine == i * 4 + e ? acc[i][j][e] : x;
                     if (share != 0.f) dot = fmaf(share, x, dot);
                 });
-#pragma unroll
-            for (int d = 16; d <= 32; d <<= 1) {
-                const float mo = __shfl_xor(mc, d, GS_WAVE), so = __shfl_xor(s, d, GS_WAVE);
-                const float mn = fmaxf(mc, mo), by = mn == -INFINITY ? 0.f : mn;
-                s = s * __builtin_amdgcn_exp2f(mc - by) + so * __builtin_amdgcn_exp2f(mo - by);
-                mc = mn;
-                if (SHARES) dot += __shfl_xor(dot, d, GS_WAVE);
-            }
+            const auto join = [&](Two<float> m2, Two<float> s2, Two<float> d2) {
+                mc = fmaxf(m2.a, m2.b);
+                const float by = mc == -INFINITY ? 0.f : mc;
+                s = s2.a * __builtin_amdgcn_exp2f(m2.a - by) + s2.b * __builtin_amdgcn_exp2f(m2.b - by);
+                if (SHARES) dot = d2.a + d2.b;
+            };
+            join(across<16>(mc), across<16>(s), SHARES ? across<16>(dot) : Two<float>{0.f, 0.f});
+            join(across<32>(mc), across<32>(s), SHARES ? across<32>(dot) : Two<float>{0.f, 0.f});
             if (q == 0 && n < at.n_c) {
                 part[block * ld + n] = make_float2(mc, s);
                 if (SHARES) dots[block * ld + n] = dot;
@@ -611,15 +623,12 @@ struct EpiTextMax {
         for (int j = 0; j < MC; j++) {
             float x = top[j];
             int r = tok[j];
-#pragma unroll
-            for (int d = 16; d <= 32; d <<= 1) {
-                const float xo = __shfl_xor(x, d, GS_WAVE);
-                if (TOK) {
-                    const int ro = __shfl_xor(r, d, GS_WAVE);
-                    r = xo > x || (xo == x && ro < r) ? ro : r;
-                }
-                x = maximum(x, xo, xo);
-            }
+            const auto join = [&](Two<float> x2, Two<int> r2) {
+                if (TOK) r = x2.b > x2.a || (x2.b == x2.a && r2.b < r2.a) ? r2.b : r2.a;
+                x = maximum(x2.a, x2.b, x2.b);
+            };
+            join(across<16>(x), TOK ? across<16>(r) : Two<int>{0, 0});
+            join(across<32>(x), TOK ? across<32>(r) : Two<int>{0, 0});
             if (j == q) mine = x + b[j], row = r;
         }
         const int v = at.col0 + at.lane;
@@ -668,9 +677,8 @@ struct EpiTextMax {
                     for (int e = 0; e < 4; e++) x[e] = sv[e] == now ? acc[i][j][e] : -INFINITY;
                     take(x, row, top[j], tok[j]);
                 }
-                next = min(next, __shfl_xor(next, 16, GS_WAVE));
-                next = min(next, __shfl_xor(next, 32, GS_WAVE));
-                next = gs_uniform(next);
+                next = min(min(__builtin_amdgcn_readlane(next, 0), __builtin_amdgcn_readlane(next, 16)),
+                           min(__builtin_amdgcn_readlane(next, 32), __builtin_amdgcn_readlane(next, 48)));
                 now = next == 0x7FFFFFFF ? -1 : next;
             }
         }
@@ -680,13 +688,16 @@ struct EpiTextMax {
 
 // ---------------------------------------------------------------- losses' small kernels
 
-// log2 of each kept row's softmax sum, and its loss.  Sixteen rows per 256 threads.
+// log2 of each kept row's softmax sum, and its loss.  X rows per 256 threads: 16 read the sums by 128-byte lines, 4 leave
+// few rows enough threads (45 rows of 954 sums: 25 -> 8 us).
+template <int X>
 __global__ __launch_bounds__(256) void k_row_loss(const float2 *part, const float *dots, int64_t ld, int blocks,
                                                   const int *rows, const int *n_d, const float *target, const float *ent, float tau, float *lse2_o,
                                                   float *loss_o, float *loss_rows) {
-    __shared__ float sm[16][17], ss[16][17], sd[16][17];
-    const int n = *n_d, x = threadIdx.x & 15, y = threadIdx.x >> 4;
-    for (int64_t i0 = (int64_t)blockIdx.x * 16; i0 < n; i0 += (int64_t)gridDim.x * 16) {
+    constexpr int Y = 256 / X;
+    __shared__ float sm[Y][X + 1], ss[Y][X + 1], sd[Y][X + 1];
+    const int n = *n_d, x = threadIdx.x % X, y = threadIdx.x / X;
+    for (int64_t i0 = (int64_t)blockIdx.x * X; i0 < n; i0 += (int64_t)gridDim.x * X) {
         const int64_t i = i0 + x;
         float m = -INFINITY, s = 0.f, dot = 0.f;
         auto add = [&](float mo, float so) {
@@ -696,7 +707,7 @@ __global__ __launch_bounds__(256) void k_row_loss(const float2 *part, const floa
         };
         if (i < n) {
 #pragma unroll 4
-            for (int b = y; b < blocks; b += 16) {
+            for (int b = y; b < blocks; b += Y) {
                 const float2 p = part[b * ld + i];
                 if (dots) dot += dots[b * ld + i];
                 add(p.x, p.y);
@@ -704,11 +715,15 @@ __global__ __launch_bounds__(256) void k_row_loss(const float2 *part, const floa
         }
         sm[y][x] = m, ss[y][x] = s, sd[y][x] = dot;
         __syncthreads();
-        if (y == 0 && i < n) {
-            for (int b = 1; b < 16; b++) {
-                add(sm[b][x], ss[b][x]);
-                dot += sd[b][x];
+        for (int by = Y / 2; by > 0; by >>= 1) {  // joined in a tree
+            if (y < by) {
+                add(sm[y + by][x], ss[y + by][x]);
+                dot += sd[y + by][x];
+                sm[y][x] = m, ss[y][x] = s, sd[y][x] = dot;
             }
+            __syncthreads();
+        }
+        if (y == 0 && i < n) {
             const float l2 = m + log2f(s);
             const int row = rows[i];
             const float loss = tau * tau * ((ent ? ent[row] : 0.f) + (l2 * kLn2 - (target ? target[i] : dot) / tau));
@@ -798,7 +813,7 @@ __global__ __launch_bounds__(256) void k_hidden_grad(const float *part, const in
         const int i = r < total ? inv[r] : -1;
         f32x4 x = f32x4{0.f, 0.f, 0.f, 0.f};
         if (i >= 0 && d < dimp) {
-#pragma unroll 4
+#pragma unroll 8
             for (int p = by == 4 ? 0 : wave; p < parts; p += by == 4 ? 1 : 4)
                 x += *reinterpret_cast<const f32x4 *>(part + ((int64_t)p * n + i) * dimp + d);
         }
@@ -843,20 +858,51 @@ __global__ __launch_bounds__(256) void k_term_weights(const float *best, const i
     const int64_t b = blockIdx.y;
     const int f0 = text_first[b], f1 = text_first[b + 1];
     const int w0 = f0 / block, w1 = (f1 - 1) / block;
-    for (int v = blockIdx.x * 256 + threadIdx.x; v < vocab; v += gridDim.x * 256) {
-        float x = 0.f;
-        int row = -1;
+    // rows of any length: values of 4 bytes are aligned, groups of four need not be
+    typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
+    typedef int i4u __attribute__((ext_vector_type(4), aligned(4)));
+    for (int v = (blockIdx.x * 256 + threadIdx.x) * 4; v < vocab; v += gridDim.x * 1024) {
+        const bool four = v + 3 < vocab;
+        f32x4 x = f32x4{0.f, 0.f, 0.f, 0.f};
+        i4u row = {-1, -1, -1, -1};
         if (f1 > f0) {
-#pragma unroll 4
             for (int w = w0; w <= w1; w++) {
                 const int64_t at = (w + b) * vocab + v;
-                const float y = best[at];
-                if (TOK && y > x) row = where[at];
-                x = maximum(x, y, y);
+                f32x4 y = f32x4{0.f, 0.f, 0.f, 0.f};
+                i4u wh = row;
+                if (four) {
+                    y = *reinterpret_cast<const f4u *>(best + at);
+                    if (TOK) wh = *reinterpret_cast<const i4u *>(where + at);
+                } else {
+                    for (int e = 0; v + e < vocab; e++) {
+                        y[e] = best[at + e];
+                        if (TOK) wh[e] = where[at + e];
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    if (TOK) row[e] = y[e] > x[e] ? wh[e] : row[e];
+                    x[e] = maximum(x[e], y[e], y[e]);
+                }
             }
         }
-        weights[b * vocab + v] = log1pf(x);
-        if (TOK) tokens[b * vocab + v] = row >= 0 ? rows[row] % length : -1;
+        f4u out;
+        i4u tok;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            out[e] = log1pf(x[e]);
+            if (TOK) tok[e] = row[e] >= 0 ? rows[row[e]] % length : -1;
+        }
+        const int64_t to = b * vocab + v;
+        if (four) {
+            *reinterpret_cast<f4u *>(weights + to) = out;
+            if (TOK) *reinterpret_cast<i4u *>(tokens + to) = tok;
+        } else {
+            for (int e = 0; v + e < vocab; e++) {
+                weights[to + e] = out[e];
+                if (TOK) tokens[to + e] = tok[e];
+            }
+        }
     }
 }
 
@@ -1195,36 +1241,40 @@ __global__ __launch_bounds__(256) void k_entries_weight(Source h, const float *g
 
 // ---------------------------------------------------------------- host
 
-// Tiles.  Two operands' tiles cross LDS once per wave that shares them, so the larger the wave's share the better the
-// matrix units are fed; but a tile needs work for every CU.
-//   Large  256 x 256, eight waves of 128 x 64, one workgroup per CU
-//   Mid    128 x 128, four waves of 64 x 64, two workgroups per CU: up to kMidRows rows
-//   Small  64 x 64, four waves of 32 x 32, four stages: up to kSmallRows rows, where reading the vocabulary is what
-//          takes the time
-template <class T, int NP, bool RK, bool CK>
-using Large = Tile<T, NP, 256, 256, 2, 4, 2, 2, RK, CK>;
-template <class T, int NP, bool RK, bool CK>  // k-major operands: waves of 64 x 128, dW 880 -> 915 TFLOP/s
-using LargeK = Tile<T, NP, 256, 256, 4, 2, 2, 2, RK, CK>;
-template <class T, int NP, bool RK, bool CK>
-using Mid = Tile<T, NP, 128, 128, 2, 2, 2, 2, RK, CK>;
+// Tiles.  A tile's operands cross LDS once per wave that shares them, so larger ones feed the matrix units better; but a
+// tile needs work for every CU, and few rows leave the vocabulary's bytes as what takes the time.  30522 terms of 768
+// bf16 values, microseconds of the product alone:
+//   rows    64 x 64   256 x 128   256 x 256
+//     45       11.4        13.0        18.5
+//    128       13.5        13.5        18.7
+//    200       22.9        14.8        19.2
+//    320       27.3        23.5        20.3
+//   1250       90.5        57.2        53.7
+// k-major operands (dH, dW) do better with waves of 64 x 128 than of 128 x 64 (dW 880 -> 915 TFLOP/s).
 template <class T, int NP, bool RK, bool CK>
 using Small = Tile<T, NP, 64, 64, 2, 2, 4, 2, RK, CK>;
+template <class T, int NP, bool RK, bool CK>
+using Wide = Tile<T, NP, 256, 128, 4, 2, 3, 2, RK, CK>;
+template <class T, int NP, bool RK, bool CK>  // tokens as rows
+using Flat = Tile<T, NP, 128, 256, 2, 4, 3, 2, RK, CK>;
+template <class T, int NP, bool RK, bool CK>
+using Large = Tile<T, NP, 256, 256, 2, 4, 2, 2, RK, CK>;
+template <class T, int NP, bool RK, bool CK>
+using LargeK = Tile<T, NP, 256, 256, 4, 2, 2, 2, RK, CK>;
 
-constexpr int kSmallRows = 64, kMidRows = 1024;
+constexpr int kSmallRows = 64, kWideRows = 256;
 
-enum TileClass { kSmall, kMid, kLarge };
-TileClass class_of(int64_t rows) { return rows <= kSmallRows ? kSmall : rows <= kMidRows ? kMid : kLarge; }
-int edge_of(TileClass c) { return c == kSmall ? 64 : c == kMid ? 128 : 256; }
-int row_waves_of(TileClass) { return 2; }
-int col_waves_of(TileClass c) { return c == kLarge ? 4 : 2; }
+enum TileClass { kSmall, kWide, kLarge };
+TileClass class_of(int64_t rows) { return rows <= kSmallRows ? kSmall : rows <= kWideRows ? kWide : kLarge; }
+// tokens of a tile
+int token_edge(TileClass c) { return c == kSmall ? 64 : c == kWide ? 128 : 256; }
+// terms of a tile of the losses, terms of a wave of it, and waves along its tokens
+int term_edge(TileClass c) { return c == kSmall ? 64 : 256; }
+int term_block(TileClass c) { return c == kSmall ? 32 : c == kWide ? 64 : 128; }
+int token_waves(TileClass c) { return c == kLarge ? 4 : 2; }
+// tokens of a wave where they are the rows
+int token_block(TileClass c) { return token_edge(c) / 2; }
 
-// CALL(tile template) for a class
-#define GSV_BY_CLASS(cls, CALL)   \
-    switch (cls) {                \
-        case kSmall: CALL(Small); break; \
-        case kMid: CALL(Mid); break;     \
-        default: CALL(Large); break;     \
-    }
 // CALL(operand type, planes) for a head's type
 #define GSV_BY_TYPE(type, CALL)              \
     switch (type) {                          \
@@ -1344,7 +1394,7 @@ struct LossPlan {
     Layout l;
     int top;
     int piece, pieces;   // terms per piece (a multiple of kRowPad)
-    int block, blocks;   // terms per softmax-sum block, and blocks
+    int blocks;          // blocks of softmax sums
     int most;            // parts of dH
     int64_t part_rows;   // rows of all of dH's parts
     int64_t sum_rows;    // rows of the bias's sums
@@ -1354,25 +1404,23 @@ LossPlan loss_plan(const gs_vocab_head *h, const gs_vocab_targets *t, int cus) {
     LossPlan p;
     p.l = layout_of(h);
     p.top = t->teacher_ids_d ? t->top : 1;
-    const int edge = edge_of(p.l.cls);
     const int64_t per = (int64_t)(p.l.rows > 0 ? p.l.rows : 1) * p.l.planes * 2;
     int64_t most = (int64_t)kPieceBytes / per / kRowPad * kRowPad;
     if (most < kRowPad) most = kRowPad;
     p.pieces = (int)((p.l.vocabp + most - 1) / most);
     p.piece = (int)round_up((p.l.vocabp + p.pieces - 1) / p.pieces, kRowPad);
     p.pieces = (p.l.vocabp + p.piece - 1) / p.piece;
-    p.block = edge / row_waves_of(p.l.cls);
-    p.blocks = (h->vocab + edge - 1) / edge * row_waves_of(p.l.cls);
+    p.blocks = (h->vocab + term_edge(p.l.cls) - 1) / term_edge(p.l.cls) * (term_edge(p.l.cls) / term_block(p.l.cls));
     p.most = p.piece / kStep / 8 < 64 ? p.piece / kStep / 8 : 64;
     if (p.most < 1) p.most = 1;
     // parts_of: parts that even out hold at most a piece's terms and the rows, parts that fill at most a tile's rows for
     // each workgroup that runs at a time
-    const int tr = (h->dim + edge - 1) / edge;
-    const int64_t even = (int64_t)p.piece + p.l.rows, fill = (int64_t)2 * cus * edge / tr + p.l.rows;
+    const int tr = (h->dim + term_edge(p.l.cls) - 1) / term_edge(p.l.cls);
+    const int64_t even = (int64_t)p.piece + p.l.rows, fill = (int64_t)2 * cus * token_edge(p.l.cls) / tr + p.l.rows;
     const int64_t by_most = (int64_t)p.most * p.l.rows;
     p.part_rows = even > fill ? even : fill;
     if (p.part_rows > by_most) p.part_rows = by_most;
-    p.sum_rows = (int64_t)(p.l.rows + edge - 1) / edge * col_waves_of(p.l.cls);
+    p.sum_rows = (int64_t)(p.l.rows + token_edge(p.l.cls) - 1) / token_edge(p.l.cls) * token_waves(p.l.cls);
     return p;
 }
 
@@ -1456,7 +1504,11 @@ int run_sums(const gs_vocab_head *h, const LossPlan &p, const LossSaved &s, cons
                          w, hid, d, EpiSums<true>{s.c.bias, scale, x.part, x.dots, p.l.rows, entries_of(p, s)}, cus, st)  \
                    : launch_product<TL<T, NP, false, false>>(                                                            \
                          w, hid, d, EpiSums<false>{s.c.bias, scale, x.part, x.dots, p.l.rows, entries_of(p, s)}, cus, st)
-    GSV_BY_CLASS(p.l.cls, GSV_SUMS)
+    switch (p.l.cls) {
+        case kSmall: GSV_SUMS(Small);
+        case kWide: GSV_SUMS(Wide);
+        default: GSV_SUMS(Large);
+    }
 #undef GSV_SUMS
 }
 
@@ -1475,25 +1527,33 @@ int run_grad(const gs_vocab_head *h, const LossPlan &p, const LossSaved &s, cons
         const EpiWeightGrad<O> ew{(O *)dw_d + (int64_t)v0 * h->dim, g.scale, h->dim, h->dim % 4 == 0};
         const Dims de{nv, p.l.rows, p.l.dimp, s.c.n, 0, 1, 0};
         const Dims dh{want_dh ? h->dim : 0, p.l.rows, nv, s.c.n, 0, 1, 0};
-        const Dims dw{dw_d ? h->dim : 0, nv, p.l.rows, s.c.n, 0, 0, 1};
+        const Dims dw{dw_d ? h->dim : 0, nv, p.l.rows, s.c.n, 0, 0, 1}, none{0, 0, 0, s.c.n, 0, 0, 0};
         int rc = GS_OK;
 #define GSV_EPI(SHARES) \
     EpiLogitGrad<S, SHARES> { s.c.bias, scale, s.lse2, g.factor, entries_of(p, s), v0, g.dl, dl.stride, p.piece, want_db ? g.sums : nullptr, p.l.vocabp }
 #define GSV_GRAD(TL)                                                                              \
     rc = s.share ? launch_product<TL<T, NP, false, false>>(wp, hid, de, GSV_EPI(true), cus, st)   \
                  : launch_product<TL<T, NP, false, false>>(wp, hid, de, GSV_EPI(false), cus, st)
-        GSV_BY_CLASS(p.l.cls, GSV_GRAD)
+        switch (p.l.cls) {
+            case kSmall: GSV_GRAD(Small); break;
+            case kWide: GSV_GRAD(Wide); break;
+            default: GSV_GRAD(Large); break;
+        }
 #undef GSV_GRAD
 #undef GSV_EPI
         if (rc) return rc;
         if (!want_dh && !dw_d) continue;
-#define GSV_PAIR(TL)                                                                                                  \
-    rc = launch_pair<TL<T, NP, true, false>, TL<T, NP, true, true>>(wp, dl, dh, eh, hid, dl, dw, ew, p.piece, p.most,  \
+#define GSV_PAIR(TL, DW)                                                                                              \
+    rc = launch_pair<TL<T, NP, true, false>, TL<T, NP, true, true>>(wp, dl, dh, eh, hid, dl, DW, ew, p.piece, p.most, \
                                                                     g.parts, cus, st)
         switch (p.l.cls) {
-            case kSmall: GSV_PAIR(Small); break;
-            case kMid: GSV_PAIR(Mid); break;
-            default: GSV_PAIR(LargeK); break;
+            case kSmall:
+                // few rows: dW is its output's bytes, which larger tiles write faster
+                GSV_PAIR(Small, none);
+                if (!rc) rc = launch_product<Wide<T, NP, true, true>>(hid, dl, dw, ew, cus, st);
+                break;
+            case kWide: GSV_PAIR(Wide, dw); break;
+            default: GSV_PAIR(LargeK, dw); break;
         }
 #undef GSV_PAIR
         if (rc) return rc;
@@ -1576,8 +1636,12 @@ extern "C" int gs_vocab_loss(const gs_vocab_head *h, const gs_vocab_targets *t, 
         GSV_BY_TYPE(h->type, GSV_SUMS)
 #undef GSV_SUMS
         if (rc) return rc;
-        hipLaunchKernelGGL(k_row_loss, dim3(gs_blocks(rows, 16, 4096)), dim3(256), 0, s, x.part, x.dots, (int64_t)rows, p.blocks,
-                           sv.c.rows, sv.c.n, x.target, x.ent, tau, sv.lse2, sv.loss, reduction == GS_REDUCE_NONE ? loss_d : nullptr);
+#define GSV_RL(X)                                                                                                          \
+    hipLaunchKernelGGL(k_row_loss<X>, dim3(gs_blocks(rows, X, 4096)), dim3(256), 0, s, x.part, x.dots, (int64_t)rows, p.blocks, \
+                       sv.c.rows, sv.c.n, x.target, x.ent, tau, sv.lse2, sv.loss, reduction == GS_REDUCE_NONE ? loss_d : nullptr)
+        if (rows <= 1024) GSV_RL(4);
+        else GSV_RL(16);
+#undef GSV_RL
         GS_CHECK_LAUNCH();
     }
     if (reduction != GS_REDUCE_NONE) {
@@ -1631,7 +1695,7 @@ extern "C" int gs_vocab_loss_grad(const gs_vocab_head *h, const gs_vocab_targets
     if (dbias_d) {
 #define GSV_BG(O)                                                                                                              \
     hipLaunchKernelGGL((k_bias_grad<O>), dim3((h->vocab + 31) / 32), dim3(256), 0, s, g.sums, (int64_t)p.l.vocabp, sv.c.n,       \
-                       edge_of(p.l.cls), col_waves_of(p.l.cls), h->vocab, g.scale, (O *)dbias_d)
+                       token_edge(p.l.cls), token_waves(p.l.cls), h->vocab, g.scale, (O *)dbias_d)
         GSV_BY_VALUE(h->bias_type, GSV_BG)
 #undef GSV_BG
         GS_CHECK_LAUNCH();
@@ -1645,7 +1709,7 @@ namespace gsv {
 
 // Slots of the maxima: a block of a wave's rows and a text each make one more.
 size_t text_slots(const gs_vocab_head *h, const Layout &l) {
-    const int block = edge_of(l.cls) / row_waves_of(l.cls);
+    const int block = token_block(l.cls);
     return (size_t)(l.rows + block - 1) / block + h->texts;
 }
 
@@ -1767,26 +1831,22 @@ extern "C" int gs_term_weights(const gs_vocab_head *h, const uint8_t *mask_d, fl
         const EpiTextMax<true> et{c.bias, c.seg, best, where, h->vocab};
         const EpiTextMax<false> ef{c.bias, c.seg, best, where, h->vocab};
         int rc = GS_OK;
-#define GSV_TILE(TL) rc = tokens_d ? launch_product<TL<GSV_T, false, false>>(hid, w, d, et, cus, s) \
-                                   : launch_product<TL<GSV_T, false, false>>(hid, w, d, ef, cus, s)
-        if (h->type == GS_H_F32) {
-#define GSV_T Bf16, 3
-            GSV_BY_CLASS(l.cls, GSV_TILE)
-#undef GSV_T
-        } else if (h->type == GS_H_F16) {
-#define GSV_T F16, 1
-            GSV_BY_CLASS(l.cls, GSV_TILE)
-#undef GSV_T
-        } else {
-#define GSV_T Bf16, 1
-            GSV_BY_CLASS(l.cls, GSV_TILE)
-#undef GSV_T
-        }
+#define GSV_TILE(TL, T, NP)                                                                  \
+    rc = tokens_d ? launch_product<TL<T, NP, false, false>>(hid, w, d, et, cus, s)             \
+                  : launch_product<TL<T, NP, false, false>>(hid, w, d, ef, cus, s)
+#define GSV_TILES(T, NP)                                 \
+    switch (l.cls) {                                     \
+        case kSmall: GSV_TILE(Small, T, NP); break;      \
+        case kWide: GSV_TILE(Flat, T, NP); break;        \
+        default: GSV_TILE(Large, T, NP); break;          \
+    }
+        GSV_BY_TYPE(h->type, GSV_TILES)
+#undef GSV_TILES
 #undef GSV_TILE
         if (rc) return rc;
     }
-    const dim3 g(gs_blocks(h->vocab, 256, 1024), h->texts);
-    const int block = edge_of(l.cls) / row_waves_of(l.cls);
+    const dim3 g(gs_blocks(h->vocab, 1024, 1024), h->texts);
+    const int block = token_block(l.cls);
     if (tokens_d)
         hipLaunchKernelGGL(k_term_weights<true>, g, dim3(256), 0, s, best, where, c.text_first, block, h->vocab, c.rows, h->length,
                            weights_d, tokens_d);

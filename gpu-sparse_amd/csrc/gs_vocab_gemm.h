@@ -358,7 +358,7 @@ struct Stream {
 // Parts of k for the first of two products that share a launch: as many as make its tiles as long as the second's, or
 // fill `slots` workgroups, at most `most`.  Device code: the sizes are known there alone.
 __device__ __forceinline__ int parts_of(int steps, int tiles, int other_steps, int other_tiles, int slots, int most) {
-    const int even = (steps + other_steps / 2) / max(1, other_steps);
+    const int even = other_tiles > 0 ? (steps + other_steps / 2) / max(1, other_steps) : 1;
     const int fill = other_tiles >= slots ? 1 : (slots - other_tiles) / max(1, tiles);
     return max(1, min(most, max(even, fill)));
 }

@@ -92,6 +92,7 @@ class _TermWeights(torch.autograd.Function):
         if track:
             ctx.save_for_backward(hidden, weight, bias, weights, tokens)
             ctx.grad_bytes = grad_need.value
+            ctx.set_materialize_grads(False)
         if tokens is None:
             return weights, None
         ctx.mark_non_differentiable(tokens)
@@ -100,6 +101,8 @@ class _TermWeights(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad, _):
+        if grad is None:
+            return None, None, None, None, None
         hidden, weight, bias, weights, tokens = ctx.saved_tensors
         dev = hidden.device
         dh, dw, db = _grads(ctx, hidden, weight, bias)
