@@ -12,7 +12,7 @@ namespace gsv {
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 constexpr int kRowPad = 256;           // rows of the vocabulary are padded to this (bias -inf beyond the last)
 constexpr int kMaxTop = 1024;          // teacher logits per row
-constexpr size_t kPieceBytes = 512u << 20;  // logit gradients held at a time
+constexpr size_t kPieceBytes = 1u << 30;  // logit gradients held at a time
 
 __host__ __device__ inline int64_t round_up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
 
@@ -240,18 +240,6 @@ __device__ __forceinline__ void pack_row(const Source &s, int row, int dimp, uin
     for (int d = lane * 4; d < dimp; d += 256) store_planes4<S, NP>(dst, dimp, d, row4(src, s.sd, d, s.dim, s.vec));
 }
 
-// Rows of the kept hidden states and, where the product cannot read it in place (w_rows > 0), of the vocabulary as
-// contiguous 16-bit ones (fp32: three planes), zero to a multiple of kStep values.  One wave per row.
-template <int HT, int NP>
-__global__ __launch_bounds__(256) void k_pack(Source h, const int *rows, const int *n_d, uint16_t *h_out, Source w, int w_rows,
-                                              uint16_t *w_out, int dimp) {
-    const int n = *n_d, lane = gs_lane();
-    for (int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); i < (int64_t)n + w_rows; i += (int64_t)gridDim.x * 4) {
-        if (i < n) pack_row<HT, NP>(h, rows[i], dimp, h_out + i * (int64_t)NP * dimp, lane);
-        else pack_row<HT, NP>(w, (int)(i - n), dimp, w_out + (i - n) * (int64_t)NP * dimp, lane);
-    }
-}
-
 // ---------------------------------------------------------------- targets
 
 // A teacher's row: q = softmax(logits / tau) over its ids inside the vocabulary, sorted by id (equal ids stay apart,
@@ -313,13 +301,18 @@ __global__ __launch_bounds__(256) void k_teacher(const int64_t *ids, const void 
     }
 }
 
-// A teacher's entries by kept row, and first[t][i]: the first of kept row i's with an id of at least t * kRowPad, t up to
-// tiles.  One wave per row.
-__global__ __launch_bounds__(256) void k_entries(const int *ids, const float *share, int top, const int *rows, const int *n_d,
-                                                 int tiles, int64_t ld, int *ids_o, float *share_o, uint16_t *first) {
-    const int n = *n_d, lane = gs_lane();
-    for (int i = blockIdx.x * 4 + (threadIdx.x >> 6); i < n; i += gridDim.x * 4) {
-        const int64_t from = (int64_t)rows[i] * top, to = (int64_t)i * top;
+// A teacher's entries of kept row i (source row `row`), and first[t][i]: the first of them with an id of at least
+// t * kRowPad, t up to tiles.  One wave.
+struct TeacherRows {
+    const int *ids;  // NULL: no teacher
+    const float *share;
+    int top, tiles;
+    int64_t ld;
+    int *ids_o;
+    float *share_o;
+    uint16_t *first;
+    __device__ __forceinline__ void take(int64_t i, int row, int lane) const {
+        const int64_t from = (int64_t)row * top, to = i * top;
         for (int k = lane; k <= top; k += 64) {
             // entry k is the first of the tiles past its predecessor's, up to its own
             const int id = k < top ? ids[from + k] : 0x7FFFFFFF;
@@ -333,22 +326,21 @@ __global__ __launch_bounds__(256) void k_entries(const int *ids, const float *sh
             for (; t <= t1; t++) first[t * ld + i] = (uint16_t)k;
         }
     }
-}
+};
 
-// Each kept row's target id, and its logit from the unpacked values in fp32.  One wave per row.
-template <int HT>
-__global__ __launch_bounds__(256) void k_target_logits(Source h, const void *weight, int64_t wr, int64_t wd, int wvec,
-                                                       const float *bias, const int64_t *targets, const int *rows,
-                                                       const int *n_d, int *ids, float *out) {
-    using T = typename HVal<HT>::t;
-    const int n = *n_d, lane = gs_lane();
-    for (int i = blockIdx.x * 4 + (threadIdx.x >> 6); i < n; i += gridDim.x * 4) {
-        const int row = rows[i], id = (int)targets[row];
-        const T *src = (const T *)h.p + (int64_t)(row / h.length) * h.s0 + (int64_t)(row % h.length) * h.s1;
-        const T *w = (const T *)weight + id * wr;
+// Kept row i's target id, and its logit from the unpacked values in fp32.  One wave.
+struct TargetRows {
+    const int64_t *targets;  // NULL: none
+    const float *bias;
+    int *ids;
+    float *out;
+    template <class T>
+    __device__ __forceinline__ void take(int64_t i, int row, int lane, const Source &h, const T *src, const Source &w) const {
+        const int id = (int)targets[row];
+        const T *wrow = (const T *)w.p + id * w.s1;
         float a = 0.f;
         for (int d = lane * 4; d < h.dim; d += 256) {
-            const f32x4 x = row4(src, h.sd, d, h.dim, h.vec), y = row4(w, wd, d, h.dim, wvec);
+            const f32x4 x = row4(src, h.sd, d, h.dim, h.vec), y = row4(wrow, w.sd, d, h.dim, w.vec);
             a = fmaf(x[0], y[0], fmaf(x[1], y[1], fmaf(x[2], y[2], fmaf(x[3], y[3], a))));
         }
         a = wave_sum(a);
@@ -357,7 +349,43 @@ __global__ __launch_bounds__(256) void k_target_logits(Source h, const void *wei
             ids[i] = id;
         }
     }
+};
+
+// Second launch of a call, a wave per row: the kept hidden states and, where the product cannot read it in place
+// (w_rows > 0), the vocabulary as contiguous 16-bit rows (fp32: three planes), zero to a multiple of kStep values; and the
+// kept rows' targets.
+template <int HT, int NP>
+__global__ __launch_bounds__(256) void k_pack(Source h, const int *rows, const int *n_d, uint16_t *h_out, Source w, int w_rows,
+                                              uint16_t *w_out, int dimp, TargetRows targets, TeacherRows teacher) {
+    using T = typename HVal<HT>::t;
+    const int n = *n_d, lane = gs_lane();
+    const int64_t items = (int64_t)n + w_rows + (targets.targets || teacher.ids ? n : 0);
+    for (int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); i < items; i += (int64_t)gridDim.x * 4) {
+        if (i < n) {
+            pack_row<HT, NP>(h, rows[i], dimp, h_out + i * (int64_t)NP * dimp, lane);
+        } else if (i < (int64_t)n + w_rows) {
+            pack_row<HT, NP>(w, (int)(i - n), dimp, w_out + (i - n) * (int64_t)NP * dimp, lane);
+        } else {
+            const int64_t k = i - n - w_rows;
+            const int row = rows[k];
+            if (teacher.ids) teacher.take(k, row, lane);
+            else targets.take(k, row, lane, h, (const T *)h.p + (int64_t)(row / h.length) * h.s0 + (int64_t)(row % h.length) * h.s1, w);
+        }
+    }
 }
+
+// One upstream value for all rows is kept out of the rounding of the logit gradients, so that their largest parts, p - 1
+// at a target, are rounded next to 1, where they almost lie; what is summed over them is multiplied with value().  Values
+// of their own (one per row) go into the gradients.  fp16's range asks for a power of two `up` as well: |p - share| <= 1, so
+// the gradients' largest magnitude is put at 2^11 to 2^12.
+struct Upstream {
+    const float *grad;
+    const int *n;
+    int mean;
+    float by;            // temperature / up
+    const float *scale;  // per-row values: 1 / up, made by k_row_factor
+    __device__ __forceinline__ float value() const { return scale ? *scale : *grad * (mean ? by / (float)max(*n, 1) : by); }
+};
 
 // ---------------------------------------------------------------- epilogues
 
@@ -391,6 +419,19 @@ struct Entries {
     }
 };
 
+// Adds the bias of a tile's rows (side array 0) where its sums did not start with it.
+template <class TL, class Epi>
+__device__ __forceinline__ void add_row_bias(f32x4 (&acc)[TL::MR][TL::MC], const Place &at) {
+    if constexpr (!starts_with_rows<TL, Epi>) {
+#pragma unroll
+        for (int i = 0; i < TL::MR; i++) {
+            const f32x4 b = at.side4(0, at.r_in + 16 * i + 4 * (at.lane >> 4));
+#pragma unroll
+            for (int j = 0; j < TL::MC; j++) acc[i][j] += b;
+        }
+    }
+}
+
 // Softmax sums of a tile: per token the largest scaled logit and the sum of 2^(scaled logit - it), over each wave's
 // terms: part[block of terms][token]; with SHARES also the sum of share * logit: dots[block of terms][token].
 template <bool SHARES>
@@ -402,16 +443,12 @@ struct EpiSums {
     int64_t ld;
     Entries entries;
     static constexpr int sides = 1;
+    static constexpr bool row_bias = true;
     __device__ __forceinline__ SideArray side(int, int r0, int, const Shape &) const { return {bias + r0, 256}; }
     template <class TL>
     __device__ __forceinline__ void run(f32x4 (&acc)[TL::MR][TL::MC], const Place &at) const {
         const int q = at.lane >> 4;
-#pragma unroll
-        for (int i = 0; i < TL::MR; i++) {
-            const f32x4 b = at.side4(0, at.r_in + 16 * i + 4 * q);
-#pragma unroll
-            for (int j = 0; j < TL::MC; j++) acc[i][j] += b;
-        }
+        add_row_bias<TL, EpiSums>(acc, at);
         const int64_t block = at.row0 / (TL::MR * 16);
 #pragma unroll
         for (int j = 0; j < TL::MC; j++) {
@@ -458,7 +495,8 @@ struct EpiLogitGrad {
     const float *bias;
     float scale;
     const float *lse2;     // log2 of the softmax sum, per kept row
-    const float *factor;   // per kept row
+    const float *factor;   // per kept row; NULL: `up` for all
+    float up, up_log2;     // a power of two
     Entries entries;
     int v0;                // first term of this piece
     uint16_t *out;
@@ -466,10 +504,11 @@ struct EpiLogitGrad {
     float *col_sums;       // NULL: not wanted; [wave's block of tokens][padded vocabulary]
     int64_t sums_ld;
     static constexpr int sides = 4;
+    static constexpr bool row_bias = true;
     __device__ __forceinline__ SideArray side(int a, int r0, int c0, const Shape &s) const {
         if (a == 0) return {bias + v0 + r0, 256};
         if (a == 1) return {lse2 + c0, s.nc - c0};
-        if (a == 2) return {factor + c0, s.nc - c0};
+        if (a == 2) return {factor + c0, factor ? s.nc - c0 : 0};
         return {entries.ids + c0, SHARES ? 0 : s.nc - c0};  // one target per row
     }
     template <class TL>
@@ -477,19 +516,15 @@ struct EpiLogitGrad {
         const int q = at.lane >> 4;
         f32x4 sums[TL::MR];
 #pragma unroll
-        for (int i = 0; i < TL::MR; i++) {
-            sums[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-            const f32x4 b = at.side4(0, at.r_in + 16 * i + 4 * q);
-#pragma unroll
-            for (int j = 0; j < TL::MC; j++) acc[i][j] += b;
-        }
+        for (int i = 0; i < TL::MR; i++) sums[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        add_row_bias<TL, EpiLogitGrad>(acc, at);
         const int wv = v0 + at.row0;  // the wave's first term
 #pragma unroll
         for (int j = 0; j < TL::MC; j++) {
             const int n = at.col0 + 16 * j + (at.lane & 15);
             const bool on = n < at.n_c;
             const int in = at.c_in + 16 * j + (at.lane & 15);
-            const float l = at.side(1, in), f = at.side(2, in);
+            const float l = at.side(1, in) - up_log2;  // 2^(x - l) comes out times up
 #pragma unroll
             for (int i = 0; i < TL::MR; i++)
 #pragma unroll
@@ -498,7 +533,7 @@ struct EpiLogitGrad {
 #pragma unroll
                 for (int i = 0; i < TL::MR; i++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) acc[i][j][e] -= mine == i * 4 + e ? share : 0.f;
+                    for (int e = 0; e < 4; e++) acc[i][j][e] -= mine == i * 4 + e ? share * up : 0.f;
             };
             if constexpr (SHARES) {
                 entries.each<TL::MR>(n, on, wv, q, off);
@@ -507,9 +542,13 @@ struct EpiLogitGrad {
                 const bool here = lv >= 0 && lv < TL::MR * 16;
                 if (__any(here)) off(here && ((lv >> 2) & 3) == q ? (lv >> 4) * 4 + (lv & 3) : -1, 1.f);
             }
+            if (factor) {
+                const float f = at.side(2, in);
+#pragma unroll
+                for (int i = 0; i < TL::MR; i++) acc[i][j] *= f;
+            }
 #pragma unroll
             for (int i = 0; i < TL::MR; i++) {
-                acc[i][j] *= f;
                 sums[i] += on ? acc[i][j] : f32x4{0.f, 0.f, 0.f, 0.f};
                 if (on) store_planes4<S, TL::planes>(out + n * ld, plane, at.row0 + 16 * i + 4 * q, acc[i][j]);
             }
@@ -531,13 +570,14 @@ struct EpiLogitGrad {
 template <class O>
 struct EpiWeightGrad {
     O *out;
-    const float *scale;
+    Upstream up;
     int dim, vec;
     static constexpr int sides = 0;
+    static constexpr bool row_bias = false;
     __device__ __forceinline__ SideArray side(int, int, int, const Shape &) const { return {nullptr, 0}; }
     template <class TL>
     __device__ __forceinline__ void run(f32x4 (&acc)[TL::MR][TL::MC], const Place &at) const {
-        const float s = *scale;
+        const float s = up.value();
         const int q = at.lane >> 4;
 #pragma unroll
         for (int j = 0; j < TL::MC; j++) {
@@ -562,6 +602,7 @@ struct EpiHiddenPart {
     float *part;
     int dimp, add;
     static constexpr int sides = 0;
+    static constexpr bool row_bias = false;
     __device__ __forceinline__ SideArray side(int, int, int, const Shape &) const { return {nullptr, 0}; }
     template <class TL>
     __device__ __forceinline__ void run(f32x4 (&acc)[TL::MR][TL::MC], const Place &at) const {
@@ -596,6 +637,7 @@ struct EpiTextMax {
     int *where;
     int vocab;
     static constexpr int sides = 2;
+    static constexpr bool row_bias = false;
     __device__ __forceinline__ SideArray side(int a, int r0, int c0, const Shape &) const {
         return a == 0 ? SideArray{bias + c0, 256} : SideArray{seg + r0, 256};
     }
@@ -751,21 +793,10 @@ __global__ __launch_bounds__(1024) void k_loss_sum(const float *loss, const int 
     }
 }
 
-// What a kept row's logit gradient is multiplied with before it is rounded to 16 bits, and what the sums over such
-// gradients are: scale[0].  With one upstream value for all rows that value is kept out of the rounding, so that the
-// largest parts, p - 1 at a target, are rounded next to 1, where they almost lie.  Values of their own (one per row)
-// go into the gradients.  fp16's range asks for a power of two as well: |p - share| <= 1, so the gradients' largest
-// magnitude is put at 2^11 to 2^12.
-__global__ __launch_bounds__(1024) void k_row_factor(const float *grad, int per_row, const int *rows, const int *n_d, int mean,
-                                                     float tau, int f16, float *factor, float *scale) {
+__global__ __launch_bounds__(1024) void k_row_factor(const float *grad, const int *rows, const int *n_d, float tau, int f16,
+                                                     float *factor, float *scale) {
     __shared__ float part[16];
     const int n = *n_d;
-    if (!per_row) {
-        const float up = f16 ? 2048.f : 1.f;
-        for (int i = threadIdx.x; i < n; i += 1024) factor[i] = up;
-        if (threadIdx.x == 0) scale[0] = grad[0] * (mean ? tau / (float)max(n, 1) : tau) / up;
-        return;
-    }
     float most = 0.f;
     for (int i = threadIdx.x; i < n; i += 1024) {
         const float f = grad[rows[i]] * tau;
@@ -784,16 +815,51 @@ __global__ __launch_bounds__(1024) void k_row_factor(const float *grad, int per_
             for (int i = threadIdx.x; i < n; i += 1024) factor[i] *= up;
         }
     }
-    if (threadIdx.x == 0) scale[0] = 1.f / up;
+    if (threadIdx.x == 0) *scale = 1.f / up;
 }
 
-// dH of every source row from its parts (0 for rows that are not kept)
-template <class O>
-__global__ __launch_bounds__(256) void k_hidden_grad(const float *part, const int *inv, const int *n_d, const int *parts_d,
-                                                     int total, int dim, int dimp, const float *scale, O *out) {
-    __shared__ f32x4 red[3][64];
-    const int n = *n_d, parts = *parts_d, lane = gs_lane(), wave = threadIdx.x >> 6;
-    const float s = *scale;
+// The bias's gradient: the tiles' column sums added up in order.  `blocks` of them.
+struct BiasSums {
+    const float *sums;  // NULL: not wanted
+    int64_t ld;
+    int edge, waves;    // tokens of a tile, sums of one
+    int vocab, type;
+    void *out;
+};
+
+// Last launch of a gradient.  dH of every source row from its parts (0 for rows that are not kept): with few rows, and so
+// many parts, a workgroup of W = 16 waves takes 256 values of a row, the waves take parts in turn and are added in order; else
+// (W = 4) a wave does.  Then workgroups of 32 terms of the bias.
+template <class O, int W>
+__global__ __launch_bounds__(64 * W) void k_finish_grad(const float *part, const int *inv, const int *n_d, const int *parts_d,
+                                                        int total, int dim, int dimp, Upstream up, O *out, int hidden_blocks,
+                                                        BiasSums bias) {
+    __shared__ f32x4 red[W][64];
+    const int n = *n_d, lane = gs_lane(), wave = threadIdx.x >> 6;
+    const float s = up.value();
+    if ((int)blockIdx.x >= hidden_blocks) {
+        constexpr int Y = 2 * W;
+        float *const sum = reinterpret_cast<float *>(red);  // [Y][32]
+        const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
+        const int v = ((int)blockIdx.x - hidden_blocks) * 32 + x;
+        const int blocks = (n + bias.edge - 1) / bias.edge * bias.waves;
+        float t = 0.f;
+        if (v < bias.vocab) {
+#pragma unroll 4
+            for (int b = y; b < blocks; b += Y) t += bias.sums[b * bias.ld + v];
+        }
+        sum[y * 32 + x] = t;
+        __syncthreads();
+        if (y == 0 && v < bias.vocab) {
+            for (int i = 1; i < Y; i++) t += sum[i * 32 + x];
+            t *= s;
+            if (bias.type == GS_H_F32) ((float *)bias.out)[v] = t;
+            else if (bias.type == GS_H_F16) ((_Float16 *)bias.out)[v] = (_Float16)t;
+            else ((__bf16 *)bias.out)[v] = (__bf16)t;
+        }
+        return;
+    }
+    const int parts = *parts_d;
     const bool vec = (dim & 3) == 0;
     const int chunks = (dim + 255) / 256;
     const auto put = [&](int64_t r, int d, f32x4 x) {
@@ -804,48 +870,30 @@ __global__ __launch_bounds__(256) void k_hidden_grad(const float *part, const in
             for (int e = 0; e < 4; e++)
                 if (d + e < dim) to[e] = (O)x[e];
     };
-    // few parts: a wave per (row, 256 values); many: a workgroup, whose waves take parts in turn and are added in order
-    const int by = parts > 8 ? 1 : 4;
-    for (int64_t w0 = (int64_t)blockIdx.x * by; w0 < (int64_t)total * chunks; w0 += (int64_t)gridDim.x * by) {
-        const int64_t w = by == 4 ? w0 + wave : w0;
+    constexpr bool share = W > 4;  // a workgroup per item
+    constexpr int by = share ? 1 : W, step = share ? W : 1;
+    for (int64_t w0 = (int64_t)blockIdx.x * by; w0 < (int64_t)total * chunks; w0 += (int64_t)hidden_blocks * by) {
+        const int64_t w = share ? w0 : w0 + wave;
         const int64_t r = w / chunks;
         const int d = (int)(w - r * chunks) * 256 + lane * 4;
         const int i = r < total ? inv[r] : -1;
         f32x4 x = f32x4{0.f, 0.f, 0.f, 0.f};
         if (i >= 0 && d < dimp) {
 #pragma unroll 8
-            for (int p = by == 4 ? 0 : wave; p < parts; p += by == 4 ? 1 : 4)
+            for (int p = share ? wave : 0; p < parts; p += step)
                 x += *reinterpret_cast<const f32x4 *>(part + ((int64_t)p * n + i) * dimp + d);
         }
-        if (by == 4) {
+        if (!share) {
             if (r < total && d < dim) put(r, d, x);
             continue;
         }
-        if (wave) red[wave - 1][lane] = x;
+        red[wave][lane] = x;
         __syncthreads();
-        if (wave == 0 && d < dim) put(r, d, x + red[0][lane] + red[1][lane] + red[2][lane]);
+        if (wave == 0 && d < dim) {
+            for (int k = 1; k < W; k++) x += red[k][lane];
+            put(r, d, x);
+        }
         __syncthreads();
-    }
-}
-
-// db: the tiles' column sums added up in order
-template <class O>
-__global__ __launch_bounds__(256) void k_bias_grad(const float *sums, int64_t ld, const int *n_d, int bc, int per_tile, int vocab,
-                                                   const float *scale, O *out) {
-    __shared__ float red[8][33];
-    const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
-    const int v = blockIdx.x * 32 + x;
-    const int blocks = (*n_d + bc - 1) / bc * per_tile;
-    float s = 0.f;
-    if (v < vocab) {
-#pragma unroll 4
-        for (int b = y; b < blocks; b += 8) s += sums[b * ld + v];
-    }
-    red[y][x] = s;
-    __syncthreads();
-    if (y == 0 && v < vocab) {
-        for (int i = 1; i < 8; i++) s += red[i][x];
-        out[v] = (O)(s * *scale);
     }
 }
 
@@ -1368,18 +1416,20 @@ Operand weight_operand(const Layout &l, const Common &s, const gs_vocab_head *h)
     return Operand{s.weight, (int64_t)l.planes * l.dimp, l.dimp, (int64_t)l.planes * l.dimp};
 }
 
-// Kept rows, bias, cleared memory, then hidden states and (where needed) vocabulary rows in the product's form.
-int prepare(const gs_vocab_head *h, const Layout &l, const Keep &keep, const Common &c, float *zero, int64_t zeros, hipStream_t s) {
+// Kept rows, bias, cleared memory; then hidden states, (where needed) vocabulary rows and targets in the product's form.
+int prepare(const gs_vocab_head *h, const Layout &l, const Keep &keep, const Common &c, float *zero, int64_t zeros,
+            const TargetRows &targets, const TeacherRows &teacher, hipStream_t s) {
     hipLaunchKernelGGL(k_setup, dim3(1 + gs_blocks(l.vocabp + zeros / 4, 1024, 1024)), dim3(1024), 0, s, keep,
-                       h->length > 0 ? h->length : 1, c.rows, c.inv, c.seg, c.text_first, c.n, h->bias_d, h->bias_type, h->vocab, l.vocabp,
-                       c.bias, zero, zeros);
+                       h->length > 0 ? h->length : 1, c.rows, c.inv, c.seg, c.text_first, c.n, h->bias_d, h->bias_type, h->vocab,
+                       l.vocabp, c.bias, zero, zeros);
     GS_CHECK_LAUNCH();
     const int w_rows = l.w_direct ? 0 : h->vocab;
     if (l.rows + w_rows == 0) return GS_OK;
-    const dim3 g(gs_blocks((int64_t)l.rows + w_rows, 4, 8192));
+    const dim3 g(gs_blocks((targets.targets || teacher.ids ? 2 : 1) * (int64_t)l.rows + w_rows, 4, 8192));
     const Source hs = hidden_source(h), ws = weight_source(h);
-#define GSV_PACK(HT, NP) \
-    hipLaunchKernelGGL((k_pack<HT, NP>), g, dim3(256), 0, s, hs, c.rows, c.n, c.hidden, ws, w_rows, c.weight, l.dimp)
+#define GSV_PACK(HT, NP)                                                                                                     \
+    hipLaunchKernelGGL((k_pack<HT, NP>), g, dim3(256), 0, s, hs, c.rows, c.n, c.hidden, ws, w_rows, c.weight, l.dimp, targets, \
+                       teacher)
     if (h->type == GS_H_F32) GSV_PACK(GS_H_F32, 3);
     else if (h->type == GS_H_F16) GSV_PACK(GS_H_F16, 1);
     else GSV_PACK(GS_H_BF16, 1);
@@ -1411,7 +1461,7 @@ LossPlan loss_plan(const gs_vocab_head *h, const gs_vocab_targets *t, int cus) {
     p.piece = (int)round_up((p.l.vocabp + p.pieces - 1) / p.pieces, kRowPad);
     p.pieces = (p.l.vocabp + p.piece - 1) / p.piece;
     p.blocks = (h->vocab + term_edge(p.l.cls) - 1) / term_edge(p.l.cls) * (term_edge(p.l.cls) / term_block(p.l.cls));
-    p.most = p.piece / kStep / 8 < 64 ? p.piece / kStep / 8 : 64;
+    p.most = p.piece / kStep / 3 < 128 ? p.piece / kStep / 3 : 128;
     if (p.most < 1) p.most = 1;
     // parts_of: parts that even out hold at most a piece's terms and the rows, parts that fill at most a tile's rows for
     // each workgroup that runs at a time
@@ -1513,8 +1563,8 @@ int run_sums(const gs_vocab_head *h, const LossPlan &p, const LossSaved &s, cons
 }
 
 template <class T, int NP, class O>
-int run_grad(const gs_vocab_head *h, const LossPlan &p, const LossSaved &s, const GradScratch &g, float scale, bool want_dh,
-             bool want_db, void *dw_d, int cus, hipStream_t st) {
+int run_grad(const gs_vocab_head *h, const LossPlan &p, const LossSaved &s, const GradScratch &g, float scale, const Upstream &up,
+             float power, bool want_dh, bool want_db, void *dw_d, int cus, hipStream_t st) {
     using S = typename T::store_t;
     const Operand w = weight_operand(p.l, s.c, h), hid = hidden_operand(p.l, s.c);
     const Operand dl{g.dl, (int64_t)NP * p.piece, p.piece, (int64_t)NP * p.piece};
@@ -1524,13 +1574,13 @@ int run_grad(const gs_vocab_head *h, const LossPlan &p, const LossSaved &s, cons
         Operand wp = w;
         wp.p += (int64_t)v0 * w.stride;
         const EpiHiddenPart eh{g.part, p.l.dimp, c > 0};
-        const EpiWeightGrad<O> ew{(O *)dw_d + (int64_t)v0 * h->dim, g.scale, h->dim, h->dim % 4 == 0};
+        const EpiWeightGrad<O> ew{(O *)dw_d + (int64_t)v0 * h->dim, up, h->dim, h->dim % 4 == 0};
         const Dims de{nv, p.l.rows, p.l.dimp, s.c.n, 0, 1, 0};
         const Dims dh{want_dh ? h->dim : 0, p.l.rows, nv, s.c.n, 0, 1, 0};
         const Dims dw{dw_d ? h->dim : 0, nv, p.l.rows, s.c.n, 0, 0, 1}, none{0, 0, 0, s.c.n, 0, 0, 0};
         int rc = GS_OK;
 #define GSV_EPI(SHARES) \
-    EpiLogitGrad<S, SHARES> { s.c.bias, scale, s.lse2, g.factor, entries_of(p, s), v0, g.dl, dl.stride, p.piece, want_db ? g.sums : nullptr, p.l.vocabp }
+    EpiLogitGrad<S, SHARES> { s.c.bias, scale, s.lse2, up.scale ? g.factor : nullptr, power, power == 2048.f ? 11.f : 0.f, entries_of(p, s), v0, g.dl, dl.stride, p.piece, want_db ? g.sums : nullptr, p.l.vocabp }
 #define GSV_GRAD(TL)                                                                              \
     rc = s.share ? launch_product<TL<T, NP, false, false>>(wp, hid, de, GSV_EPI(true), cus, st)   \
                  : launch_product<TL<T, NP, false, false>>(wp, hid, de, GSV_EPI(false), cus, st)
@@ -1589,7 +1639,7 @@ extern "C" int gs_vocab_loss(const gs_vocab_head *h, const gs_vocab_targets *t, 
     if (int rc = check_head(h)) return rc;
     if (int rc = check_targets(h, t)) return rc;
     GS_REQUIRE(reduction >= GS_REDUCE_NONE && reduction <= GS_REDUCE_SUM, "unknown reduction %d", reduction);
-    GS_REQUIRE(saved_d && scratch_d && loss_d, "NULL loss or workspace");
+    GS_REQUIRE(saved_d && (loss_d || (reduction == GS_REDUCE_NONE && (int64_t)h->texts * h->length == 0)), "NULL loss or workspace");
     int cus = 0;
     if (int rc = cu_count(&cus)) return rc;
     const LossPlan p = loss_plan(h, t, cus);
@@ -1598,6 +1648,7 @@ extern "C" int gs_vocab_loss(const gs_vocab_head *h, const gs_vocab_targets *t, 
     gs_arena a{(char *)saved_d, 0, saved_bytes}, b{(char *)scratch_d, 0, scratch_bytes};
     take_loss_saved(a, p, h, t, &sv);
     take_loss_scratch(b, p, t, &x);
+    GS_REQUIRE(scratch_d || b.used == 0, "NULL workspace");
     if (!a.ok() || !b.ok()) {
         gs_set_error("vocab_loss workspace too small: need %zu + %zu bytes, got %zu + %zu", a.used, b.used, saved_bytes,
                      scratch_bytes);
@@ -1614,23 +1665,10 @@ extern "C" int gs_vocab_loss(const gs_vocab_head *h, const gs_vocab_targets *t, 
         GS_CHECK_LAUNCH();
     }
     const Keep keep{x.keep, teacher ? nullptr : t->targets_d, t->ignore_index, h->vocab, rows};
-    if (int rc = prepare(h, p.l, keep, sv.c, loss_d, reduction == GS_REDUCE_NONE ? rows : 0, s)) return rc;
+    const TargetRows targets{teacher ? nullptr : t->targets_d, sv.c.bias, sv.ids, x.target};
+    const TeacherRows entries{teacher ? x.ids : nullptr, x.share, p.top, p.l.vocabp / kRowPad, rows, sv.ids, sv.share, sv.first};
+    if (int rc = prepare(h, p.l, keep, sv.c, loss_d, reduction == GS_REDUCE_NONE ? rows : 0, targets, entries, s)) return rc;
     if (rows > 0) {
-        const dim3 g(gs_blocks(rows, 4, 4096));
-        if (teacher) {
-            hipLaunchKernelGGL(k_entries, g, dim3(256), 0, s, x.ids, x.share, p.top, sv.c.rows, sv.c.n, p.l.vocabp / kRowPad,
-                               (int64_t)rows, sv.ids, sv.share, sv.first);
-        } else {
-            const Source hs = hidden_source(h), ws = weight_source(h);
-#define GSV_TL(HT)                                                                                                         \
-    hipLaunchKernelGGL((k_target_logits<HT>), g, dim3(256), 0, s, hs, h->weight_d, h->weight_row_stride, h->weight_dim_stride, \
-                       ws.vec, sv.c.bias, t->targets_d, sv.c.rows, sv.c.n, sv.ids, x.target)
-            if (h->type == GS_H_F32) GSV_TL(GS_H_F32);
-            else if (h->type == GS_H_F16) GSV_TL(GS_H_F16);
-            else GSV_TL(GS_H_BF16);
-#undef GSV_TL
-        }
-        GS_CHECK_LAUNCH();
         int rc = GS_OK;
 #define GSV_SUMS(T, NP) rc = run_sums<T, NP>(h, p, sv, x, kLog2e / tau, cus, s)
         GSV_BY_TYPE(h->type, GSV_SUMS)
@@ -1657,7 +1695,7 @@ extern "C" int gs_vocab_loss_grad(const gs_vocab_head *h, const gs_vocab_targets
     if (int rc = check_head(h)) return rc;
     if (int rc = check_targets(h, t)) return rc;
     GS_REQUIRE(reduction >= GS_REDUCE_NONE && reduction <= GS_REDUCE_SUM, "unknown reduction %d", reduction);
-    GS_REQUIRE(saved_d && scratch_d && grad_d, "NULL gradient or workspace");
+    GS_REQUIRE(saved_d && scratch_d && (grad_d || (reduction == GS_REDUCE_NONE && (int64_t)h->texts * h->length == 0)), "NULL gradient or workspace");
     int cus = 0;
     if (int rc = cu_count(&cus)) return rc;
     const LossPlan p = loss_plan(h, t, cus);
@@ -1674,32 +1712,37 @@ extern "C" int gs_vocab_loss_grad(const gs_vocab_head *h, const gs_vocab_targets
     const hipStream_t s = gs_stream(stream);
     const int rows = p.l.rows;
     const float tau = tau_of(t);
-    hipLaunchKernelGGL(k_row_factor, dim3(1), dim3(1024), 0, s, grad_d, reduction == GS_REDUCE_NONE, sv.c.rows, sv.c.n,
-                       reduction == GS_REDUCE_MEAN, tau, h->type == GS_H_F16, g.factor, g.scale);
-    GS_CHECK_LAUNCH();
+    const bool per_row = reduction == GS_REDUCE_NONE, f16 = h->type == GS_H_F16;
+    if (per_row) {
+        hipLaunchKernelGGL(k_row_factor, dim3(1), dim3(1024), 0, s, grad_d, sv.c.rows, sv.c.n, tau, f16, g.factor, g.scale);
+        GS_CHECK_LAUNCH();
+    }
+    const float power = f16 && !per_row ? 2048.f : 1.f;
+    const Upstream up{grad_d, sv.c.n, reduction == GS_REDUCE_MEAN, tau / power, per_row ? g.scale : nullptr};
     int rc = GS_OK;
     // without a kept row no launch has a tile but dW's, which writes its zeros
-    if (h->type == GS_H_F32) rc = run_grad<Bf16, 3, float>(h, p, sv, g, kLog2e / tau, dhidden_d, dbias_d, dweight_d, cus, s);
-    else if (h->type == GS_H_F16) rc = run_grad<F16, 1, _Float16>(h, p, sv, g, kLog2e / tau, dhidden_d, dbias_d, dweight_d, cus, s);
-    else rc = run_grad<Bf16, 1, __bf16>(h, p, sv, g, kLog2e / tau, dhidden_d, dbias_d, dweight_d, cus, s);
+#define GSV_RUN(T, NP, O) rc = run_grad<T, NP, O>(h, p, sv, g, kLog2e / tau, up, power, dhidden_d, dbias_d, dweight_d, cus, s)
+    if (h->type == GS_H_F32) GSV_RUN(Bf16, 3, float);
+    else if (f16) GSV_RUN(F16, 1, _Float16);
+    else GSV_RUN(Bf16, 1, __bf16);
+#undef GSV_RUN
     if (rc) return rc;
-    if (dhidden_d && rows > 0) {
-        const dim3 gr(gs_blocks((int64_t)rows * ((h->dim + 255) / 256), 4, 8192));
-#define GSV_HG(O)                                                                                                        \
-    hipLaunchKernelGGL((k_hidden_grad<O>), gr, dim3(256), 0, s, g.part, sv.c.inv, sv.c.n, g.parts, rows, h->dim, p.l.dimp, \
-                       g.scale, (O *)dhidden_d)
-        GSV_BY_VALUE(h->type, GSV_HG)
-#undef GSV_HG
-        GS_CHECK_LAUNCH();
-    }
-    if (dbias_d) {
-#define GSV_BG(O)                                                                                                              \
-    hipLaunchKernelGGL((k_bias_grad<O>), dim3((h->vocab + 31) / 32), dim3(256), 0, s, g.sums, (int64_t)p.l.vocabp, sv.c.n,       \
-                       token_edge(p.l.cls), token_waves(p.l.cls), h->vocab, g.scale, (O *)dbias_d)
-        GSV_BY_VALUE(h->bias_type, GSV_BG)
-#undef GSV_BG
-        GS_CHECK_LAUNCH();
-    }
+    const int64_t items = dhidden_d ? (int64_t)rows * ((h->dim + 255) / 256) : 0;
+    const bool few = items <= 1024;
+    const int hidden_blocks = items ? (int)gs_blocks(items, few ? 1 : 4, 8192) : 0;
+    const int bias_blocks = dbias_d ? (h->vocab + 31) / 32 : 0;
+    if (hidden_blocks + bias_blocks == 0) return GS_OK;
+    const BiasSums bias{g.sums, p.l.vocabp, token_edge(p.l.cls), token_waves(p.l.cls), h->vocab, h->bias_type, dbias_d};
+#define GSV_FG(O, W)                                                                                                       \
+    hipLaunchKernelGGL((k_finish_grad<O, W>), dim3(hidden_blocks + bias_blocks), dim3(64 * W), 0, s, g.part, sv.c.inv, sv.c.n, \
+                       g.parts, rows, h->dim, p.l.dimp, up, (O *)dhidden_d, hidden_blocks, bias)
+#define GSV_FINISH(O)               \
+    if (few) GSV_FG(O, 16);         \
+    else GSV_FG(O, 4)
+    GSV_BY_VALUE(h->type, GSV_FINISH)
+#undef GSV_FINISH
+#undef GSV_FG
+    GS_CHECK_LAUNCH();
     return GS_OK;
 }
 
@@ -1824,7 +1867,7 @@ extern "C" int gs_term_weights(const gs_vocab_head *h, const uint8_t *mask_d, fl
         GS_CHECK_LAUNCH();
         return GS_OK;
     }
-    if (int rc = prepare(h, l, Keep{mask_d, nullptr, 0, h->vocab, l.rows}, c, nullptr, 0, s)) return rc;
+    if (int rc = prepare(h, l, Keep{mask_d, nullptr, 0, h->vocab, l.rows}, c, nullptr, 0, TargetRows{}, TeacherRows{}, s)) return rc;
     {
         const Dims d{l.rows, h->vocab, l.dimp, c.n, 1, 0, 0};
         const Operand hid = hidden_operand(l, c), w = weight_operand(l, c, h);

@@ -45,7 +45,6 @@ struct F16 {
     }
 };
 
-constexpr int kSides = 4;
 constexpr int kStep = 64;  // k values per stage: two 16x16x32 products deep, and whole 128-byte lines of [x][k] rows
 
 // A 16-bit matrix.  [x][k]: row x starts at p + x * stride; [k][x]: row k does.  Plane i of an
@@ -191,13 +190,13 @@ struct Tile {
     static constexpr int waves = WR * WC, threads = 64 * waves, waves_per_simd = OCC;
     static constexpr int MR = BR / WR / 16, MC = BC / WC / 16;
     static constexpr int stage_bytes = (BR + BC) * kStep * 2;
-    static constexpr int side_bytes = kSides * 1024;
-    static constexpr int lds_bytes = NS * stage_bytes + 2 * side_bytes;
+    static constexpr int edge = BR > BC ? BR : BC;
     static constexpr bool r_kmajor = RK, c_kmajor = CK;
 };
 
 // What an epilogue reads per row or column of a tile (a bias, a row's softmax sum) comes to LDS with the tile's first
-// stage: up to kSides arrays of 32-bit values, twice (a tile's epilogue runs while the next tile's arrive).
+// stage: arrays of TL::edge 32-bit values.  A tile's epilogue runs when NS more stages have been issued, which belong to
+// NS more tiles where each has a single one: NS + 1 sets of arrays.
 struct SideArray {
     const void *p;  // of the tile's first row or column
     int count;      // values from there on that exist; the others read 0
@@ -210,12 +209,13 @@ struct Place {
     int n_r, n_c;
     int r_in, c_in;  // row0 and col0 within the tile
     lds_t sides;
+    int edge;
     // side array a's values at in .. in + 3 (of the tile), or the one at in
     __device__ __forceinline__ f32x4 side4(int a, int in) const {
-        return *(__attribute__((address_space(3))) f32x4 *)(sides + a * 1024 + in * 4);
+        return *(__attribute__((address_space(3))) f32x4 *)(sides + (a * edge + in) * 4);
     }
     __device__ __forceinline__ float side(int a, int in) const {
-        return *(__attribute__((address_space(3))) float *)(sides + a * 1024 + in * 4);
+        return *(__attribute__((address_space(3))) float *)(sides + (a * edge + in) * 4);
     }
 };
 
@@ -235,11 +235,18 @@ __device__ __forceinline__ Shape shape_of(const Dims &d, int n_dev) {
     return s;
 }
 
+// Whether a tile's sums start with the epilogue's side array 0, one value per row (a bias), instead of 0.  Not with fp32
+// operands, whose small products are summed first.
+template <class TL, class Epi>
+constexpr bool starts_with_rows = std::remove_cv_t<std::remove_reference_t<Epi>>::row_bias && TL::planes == 1;
+
 // One product of a launch: tiles [0, tr * tc * parts) of it, each part a range of k.
 template <class TL, class Epi>
 struct Side {
     using tile = TL;
     using epilogue = Epi;
+    static constexpr int set_bytes = Epi::sides * TL::edge * 4;  // of side arrays
+    static constexpr int lds_bytes = TL::NS * TL::stage_bytes + (TL::NS + 1) * set_bytes;
     Operand R, C;
     Dims d;
     Epi epi;
@@ -254,10 +261,20 @@ __device__ __forceinline__ Work work_of(const Shape &s, int parts, int t) {
     const int area = s.tr * s.tc, part = t / area, in = t - part * area;
     const int group = in / (8 * s.tc), left = in - group * 8 * s.tc;
     const int tall = min(8, s.tr - group * 8);
-    const int k0 = s.steps * part / parts;  // at most 2^22 steps and 64 parts
+    const int k0 = s.steps * part / parts;  // at most 2^22 steps and 128 parts
     return Work{gs_uniform((group * 8 + left % tall) * TL::BR), gs_uniform((left / tall) * TL::BC), gs_uniform(part), gs_uniform(k0),
                 gs_uniform(s.steps * (part + 1) / parts - k0)};
 }
+
+// What an XCD (blockIdx mod 8) takes of a launch: a contiguous run of either product's tiles, so that what runs at a time in
+// an XCD shares operands in its L2, and as much of the long tiles as of the short ones as every other.
+struct Share {
+    int a0, na, b0, nb;
+    __device__ __forceinline__ Share(int ta, int tb, int xcd, int xcds) {
+        a0 = (int)((int64_t)ta * xcd / xcds), na = (int)((int64_t)ta * (xcd + 1) / xcds) - a0;
+        b0 = (int)((int64_t)tb * xcd / xcds), nb = (int)((int64_t)tb * (xcd + 1) / xcds) - b0;
+    }
+};
 
 // The stages of a workgroup's tiles, issued one after the other whatever tile they belong to: while a tile's epilogue
 // runs, the next one's first stages are on their way.
@@ -273,22 +290,23 @@ struct Stream {
     Cursor<TA::BC, TA::c_kmajor> ca;
     Cursor<TB::BR, TB::r_kmajor> rb;
     Cursor<TB::BC, TB::c_kmajor> cb;
-    int t, last, by, na;  // tiles t, t + by, ... below last; those below na are the first product's
+    Share share;
+    int t, by;            // the workgroup's tiles: t, t + by, ... of its XCD's share
     int ik, seg, buf, left;
     bool fresh;           // the next stage is its tile's first
-    int parity;           // of the tile, for its side arrays
+    int set;              // of the tile's side arrays
 
-    __device__ __forceinline__ bool in_a() const { return !pair || t < na; }
+    __device__ __forceinline__ bool in_a() const { return !pair || t < share.na; }
     template <class S>
     __device__ __forceinline__ void sides(const S &side, const Shape &s, lds_t lds, int wave, int lane) const {
 #if defined(__HIP_DEVICE_COMPILE__)
 #pragma unroll
         for (int a = 0; a < S::epilogue::sides; a++) {
-            if (wave != a % TA::waves) continue;
+            if (wave != a % TA::waves || lane * 4 >= TA::edge) continue;
             const SideArray x = side.epi.side(a, w.r0, w.c0, s);
             __builtin_amdgcn_raw_ptr_buffer_load_lds(
                 gs_rsrc(x.p, (uint32_t)max(x.count, 0) * 4u),
-                (__attribute__((address_space(3))) void *)(lds + TA::NS * TA::stage_bytes + parity * TA::side_bytes + a * 1024), 16,
+                (__attribute__((address_space(3))) void *)(lds + TA::NS * TA::stage_bytes + set * S::set_bytes + a * TA::edge * 4), 16,
                 lane * 16, 0, 0, 0);
         }
 #endif
@@ -312,12 +330,12 @@ struct Stream {
     }
     // Moves to tile t, or the next one with stages
     __device__ __forceinline__ void seek(const SA &A, const SB &B, const Shape &a, const Shape &b, int parts, int wave, int lane) {
-        for (; t < last; t += by) {
-            if (in_a()) seek_in(A, a, parts, t, ra, ca, wave, lane);
-            else seek_in(B, b, 1, t - na, rb, cb, wave, lane);
+        for (; t < share.na + share.nb; t += by) {
+            if (in_a()) seek_in(A, a, parts, share.a0 + t, ra, ca, wave, lane);
+            else seek_in(B, b, 1, share.b0 + t - share.na, rb, cb, wave, lane);
             if (left == 0) continue;
             fresh = true;
-            parity ^= 1;
+            set = set == TA::NS ? 0 : set + 1;
             return;
         }
     }
@@ -342,7 +360,7 @@ struct Stream {
     }
     __device__ __forceinline__ bool issue(lds_t lds, const SA &A, const SB &B, const Shape &a, const Shape &b, int parts, int wave,
                                           int lane) {
-        if (t >= last) return false;
+        if (t >= share.na + share.nb) return false;
         if (in_a()) issue_in(A, a, ra, ca, lds, wave, lane);
         else issue_in(B, b, rb, cb, lds, wave, lane);
         buf = buf == TA::NS - 1 ? 0 : buf + 1;
@@ -370,13 +388,12 @@ struct Pairing {
     int *parts_d;  // receives the parts; NULL: one, and there is no second product
 };
 
-// One or two products in a launch.  Persistent: workgroups of one XCD (blockIdx mod 8) take a contiguous run of tiles, so
-// that what runs at a time in an XCD shares operands in its L2.
+// One or two products in a launch, persistent over their tiles.
 template <class SA, class SB>
 __global__ __launch_bounds__(SA::tile::threads, SA::tile::waves_per_simd) void k_product(SA A, SB B, Pairing pair) {
     using TA = typename SA::tile;
     using TB = typename SB::tile;
-    static_assert(TA::lds_bytes == TB::lds_bytes && TA::MR == TB::MR && TA::MC == TB::MC, "one tile shape per launch");
+    static_assert(SA::lds_bytes == SB::lds_bytes && SA::lds_bytes <= 163840 && TA::MR == TB::MR && TA::MC == TB::MC, "one tile shape per launch");
     extern __shared__ __align__(1024) char smem[];
     const lds_t lds = (lds_t)smem;
     const int lane = gs_lane(), wave = gs_uniform((int)threadIdx.x >> 6);
@@ -391,17 +408,15 @@ __global__ __launch_bounds__(SA::tile::threads, SA::tile::waves_per_simd) void k
                          pair.slots, pair.most);
         if (blockIdx.x == 0 && threadIdx.x == 0) *pair.parts_d = parts;
     }
-    const int na = a.tr * a.tc * parts, tiles = na + nb;
     const int xcds = gridDim.x >= 8 ? 8 : 1, xcd = blockIdx.x % xcds;
+    const Share share(a.tr * a.tc * parts, nb, xcd, xcds);
 
-    Stream<SA, SB> st;
-    st.t = (int)((int64_t)tiles * xcd / xcds) + blockIdx.x / xcds;
-    st.last = (int)((int64_t)tiles * (xcd + 1) / xcds);
+    Stream<SA, SB> st{.share = share};
+    st.t = blockIdx.x / xcds;
     st.by = (gridDim.x - xcd + xcds - 1) / xcds;
-    st.na = na;
     st.buf = 0;
-    st.parity = 1;
-    const int first = st.t, last = st.last, by = st.by;
+    st.set = TA::NS;
+    const int first = st.t, by = st.by;
     st.seek(A, B, a, b, parts, wave, lane);
     constexpr int loads = Stream<SA, SB>::loads, NS = TA::NS;
     int ahead = 0;  // stages issued and not yet left behind
@@ -416,7 +431,7 @@ __global__ __launch_bounds__(SA::tile::threads, SA::tile::waves_per_simd) void k
     };
     landed();
     ahead += st.issue(lds, A, B, a, b, parts, wave, lane);
-    int parity = 0;
+    int set = 0;
 
     // A tile.  The fragments of a half stage are read while the products of the half before run.  Before a stage's second
     // half the next stage has to have landed, and this one, which every wave holds by then, makes room for another.
@@ -426,11 +441,16 @@ __global__ __launch_bounds__(SA::tile::threads, SA::tile::waves_per_simd) void k
         Frags<TL::BC, TL::c_kmajor, TL::MC> fc;
         fr.init(wr * TL::MR * 16, lane);
         fc.init(wc * TL::MC * 16, lane);
+        const Place at{w.r0 + wr * TL::MR * 16, w.c0 + wc * TL::MC * 16, lane, w.part, s.nr, s.nc, wr * TL::MR * 16,
+                       wc * TL::MC * 16, lds + NS * TL::stage_bytes + set * std::remove_reference_t<decltype(side)>::set_bytes, TL::edge};
         f32x4 acc[TL::MR][TL::MC];
 #pragma unroll
-        for (int i = 0; i < TL::MR; i++)
+        for (int i = 0; i < TL::MR; i++) {
+            const f32x4 x = starts_with_rows<TL, decltype(side.epi)> ? at.side4(0, at.r_in + 16 * i + 4 * (lane >> 4))
+                                                                     : f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int j = 0; j < TL::MC; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int j = 0; j < TL::MC; j++) acc[i][j] = x;
+        }
         s16x8 fa[2][TL::MR], fb[2][TL::MC];
         auto read = [&](int h) {
             const lds_t from = lds + buf * TL::stage_bytes;
@@ -457,17 +477,15 @@ __global__ __launch_bounds__(SA::tile::threads, SA::tile::waves_per_simd) void k
             ahead += st.issue(lds, A, B, a, b, parts, wave, lane);
             multiply(1);
         }
-        side.epi.template run<TL>(acc, Place{w.r0 + wr * TL::MR * 16, w.c0 + wc * TL::MC * 16, lane, w.part, s.nr, s.nc,
-                                             wr * TL::MR * 16, wc * TL::MC * 16,
-                                             lds + NS * TL::stage_bytes + parity * TL::side_bytes});
-        if (total > 0) parity ^= 1;  // as the stream, which knows tiles with stages alone
+        side.epi.template run<TL>(acc, at);
+        if (total > 0) set = set == NS ? 0 : set + 1;  // as the stream, which knows tiles with stages alone
     };
-    for (int t = first; t < last; t += by) {
+    for (int t = first; t < share.na + share.nb; t += by) {
         if constexpr (!std::is_same_v<SA, SB>) {
-            if (t < na) run(A, work_of<TA>(a, parts, t), a);
-            else run(B, work_of<TB>(b, 1, t - na), b);
+            if (t < share.na) run(A, work_of<TA>(a, parts, share.a0 + t), a);
+            else run(B, work_of<TB>(b, 1, share.b0 + t - share.na), b);
         } else {
-            run(A, work_of<TA>(a, 1, t), a);
+            run(A, work_of<TA>(a, 1, share.a0 + t), a);
         }
     }
 }
@@ -479,9 +497,9 @@ template <class SA, class SB>
 int launch_products(const SA &A, const SB &B, const Pairing &pair, int64_t grid, hipStream_t s) {
     using TL = typename SA::tile;
     const void *f = reinterpret_cast<const void *>(&k_product<SA, SB>);
-    if (TL::lds_bytes > 65536)
-        GS_CHECK_HIP(hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, TL::lds_bytes));
-    hipLaunchKernelGGL((k_product<SA, SB>), dim3((unsigned)grid), dim3(TL::threads), TL::lds_bytes, s, A, B, pair);
+    if (SA::lds_bytes > 65536)
+        GS_CHECK_HIP(hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, SA::lds_bytes));
+    hipLaunchKernelGGL((k_product<SA, SB>), dim3((unsigned)grid), dim3(TL::threads), SA::lds_bytes, s, A, B, pair);
     GS_CHECK_LAUNCH();
     return GS_OK;
 }

@@ -184,7 +184,7 @@ class _VocabLoss(torch.autograd.Function):
 def _loss(hidden, weight, bias, ids, logits, ignore_index, temperature, reduction):
     lead = hidden.shape[:-1]
     bias = None if bias is None else bias.contiguous()
-    flat = hidden.reshape(1, -1, hidden.shape[-1]) if hidden.numel() else hidden.new_empty((1, lead.numel(), hidden.shape[-1]))
+    flat = hidden.reshape(1, lead.numel(), hidden.shape[-1])
     out = _VocabLoss.apply(flat, weight, bias, ids, logits, ignore_index, temperature, REDUCTIONS[reduction])
     return out.reshape(lead) if reduction == "none" else out
 
@@ -242,5 +242,5 @@ def distill_loss(hidden, weight, teacher_ids, teacher_logits, bias=None, *, temp
         raise ValueError(f"temperature must be positive and finite, got {temperature}")
     ids = _ids(teacher_ids, teacher_logits.shape, "teacher_ids", dev)
     _same_device(dev, teacher_logits=teacher_logits)
-    logits = teacher_logits.detach().reshape(-1, top).contiguous()
-    return _loss(hidden, weight, bias, ids.reshape(-1, top), logits, 0, float(temperature), reduction)
+    logits = teacher_logits.detach().reshape(ids.numel() // top, top).contiguous()
+    return _loss(hidden, weight, bias, ids.reshape(ids.numel() // top, top), logits, 0, float(temperature), reduction)
