@@ -19,6 +19,8 @@ the current stream of the tensors' device; results are deterministic.
 """
 from __future__ import annotations
 
+from contextlib import nullcontext
+
 import torch
 from torch.autograd.function import once_differentiable
 
@@ -63,6 +65,11 @@ def _head(hidden, weight, bias) -> _lib.GsVocabHead:
                             hidden.shape[1], hidden.shape[2], weight.shape[0])
 
 
+def _on(dev):
+    """The tensors' device as the current one; entering it costs more than asking whether it is."""
+    return nullcontext() if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+
 def _bytes(n: int, dev) -> torch.Tensor:
     return torch.empty(int(n), dtype=torch.uint8, device=dev)
 
@@ -83,7 +90,7 @@ class _TermWeights(torch.autograd.Function):
         tokens = torch.empty((texts, vocab), dtype=torch.int32, device=dev) if want_tokens or track else None
         L, head = _lib.lib(), _head(hidden, weight, bias)
         need, grad_need = C.c_size_t(), C.c_size_t()
-        with torch.cuda.device(dev):
+        with _on(dev):
             _lib.check(L.gs_term_weights_workspace(C.byref(head), tokens is not None, C.byref(need), C.byref(grad_need)),
                        "gs_term_weights_workspace")
             ws = _bytes(need.value, dev)
@@ -108,7 +115,7 @@ class _TermWeights(torch.autograd.Function):
         dh, dw, db = _grads(ctx, hidden, weight, bias)
         L, head = _lib.lib(), _head(hidden, weight, bias)
         grad = grad.to(torch.float32).contiguous()
-        with torch.cuda.device(dev):
+        with _on(dev):
             ws = _bytes(ctx.grad_bytes, dev)
             _lib.check(L.gs_term_weights_grad(C.byref(head), grad.data_ptr(), weights.data_ptr(), tokens.data_ptr(),
                                               _lib.ptr(dh), _lib.ptr(dw), _lib.ptr(db), ws.data_ptr(), ws.numel(),
@@ -154,7 +161,7 @@ class _VocabLoss(torch.autograd.Function):
         loss = torch.empty((rows,) if reduction == _lib.GS_REDUCE_NONE else (), dtype=torch.float32, device=dev)
         L = _lib.lib()
         need = [C.c_size_t() for _ in range(3)]
-        with torch.cuda.device(dev):
+        with _on(dev):
             _lib.check(L.gs_vocab_loss_workspace(C.byref(head), C.byref(targets), *map(C.byref, need)),
                        "gs_vocab_loss_workspace")
             saved, ws = _bytes(need[0].value, dev), _bytes(need[1].value, dev)
@@ -173,7 +180,7 @@ class _VocabLoss(torch.autograd.Function):
         dh, dw, db = _grads(ctx, hidden, weight, bias)
         L, head = _lib.lib(), _head(hidden, weight, bias)
         grad = grad.to(torch.float32).contiguous()
-        with torch.cuda.device(dev):
+        with _on(dev):
             ws = _bytes(ctx.grad_bytes, dev)
             _lib.check(L.gs_vocab_loss_grad(C.byref(head), C.byref(ctx.targets), ctx.reduction, grad.data_ptr(),
                                             saved.data_ptr(), saved.numel(), _lib.ptr(dh), _lib.ptr(dw), _lib.ptr(db),
