@@ -302,28 +302,34 @@ __global__ __launch_bounds__(256) void k_teacher(const int64_t *ids, const void 
 }
 
 // A teacher's entries of kept row i (source row `row`), and first[t][i]: the first of them with an id of at least
-// t * kRowPad, t up to tiles.  One wave.
+// t * width, t up to tiles.  One wave.
 struct TeacherRows {
     const int *ids;  // NULL: no teacher
     const float *share;
-    int top, tiles;
+    int top, tiles, width;
     int64_t ld;
     int *ids_o;
     float *share_o;
     uint16_t *first;
-    __device__ __forceinline__ void take(int64_t i, int row, int lane) const {
+    __device__ __forceinline__ void take(int64_t i, int row, int lane, int *lds) const {  // lds: room for a row
         const int64_t from = (int64_t)row * top, to = i * top;
-        for (int k = lane; k <= top; k += 64) {
-            // entry k is the first of the tiles past its predecessor's, up to its own
-            const int id = k < top ? ids[from + k] : 0x7FFFFFFF;
-            const int prev = k > 0 ? ids[from + k - 1] : -1;
-            if (k < top) {
-                ids_o[to + k] = id;
-                share_o[to + k] = share[from + k];
+        gs_wave_sync();
+        for (int k = lane; k < top; k += 64) {
+            const int id = ids[from + k];
+            lds[k] = id;
+            ids_o[to + k] = id;
+            share_o[to + k] = share[from + k];
+        }
+        gs_wave_sync();
+        for (int t = lane; t <= tiles; t += 64) {
+            const int v = t * width;
+            int lo = 0, hi = top;
+            while (lo < hi) {
+                const int mid = (lo + hi) >> 1;
+                if (lds[mid] < v) lo = mid + 1;
+                else hi = mid;
             }
-            const int t1 = id == 0x7FFFFFFF ? tiles : id / kRowPad;
-            int t = prev < 0 ? 0 : prev == 0x7FFFFFFF ? tiles + 1 : prev / kRowPad + 1;
-            for (; t <= t1; t++) first[t * ld + i] = (uint16_t)k;
+            first[t * ld + i] = (uint16_t)lo;
         }
     }
 };
@@ -358,6 +364,7 @@ template <int HT, int NP>
 __global__ __launch_bounds__(256) void k_pack(Source h, const int *rows, const int *n_d, uint16_t *h_out, Source w, int w_rows,
                                               uint16_t *w_out, int dimp, TargetRows targets, TeacherRows teacher) {
     using T = typename HVal<HT>::t;
+    __shared__ int ids_s[4][kMaxTop];
     const int n = *n_d, lane = gs_lane();
     const int64_t items = (int64_t)n + w_rows + (targets.targets || teacher.ids ? n : 0);
     for (int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); i < items; i += (int64_t)gridDim.x * 4) {
@@ -368,7 +375,7 @@ __global__ __launch_bounds__(256) void k_pack(Source h, const int *rows, const i
         } else {
             const int64_t k = i - n - w_rows;
             const int row = rows[k];
-            if (teacher.ids) teacher.take(k, row, lane);
+            if (teacher.ids) teacher.take(k, row, lane, ids_s[threadIdx.x >> 6]);
             else targets.take(k, row, lane, h, (const T *)h.p + (int64_t)(row / h.length) * h.s0 + (int64_t)(row % h.length) * h.s1, w);
         }
     }
@@ -393,31 +400,66 @@ struct Upstream {
 struct Entries {
     const int *ids;         // [kept row][top]
     const float *share;
-    const uint16_t *first;  // [vocabulary / kRowPad + 1][kept row]
+    const uint16_t *first;  // [block of terms + 1][kept row]: a block is what a wave of the losses' tiles holds
     int64_t ld;
     int top;
-    // f(mine, share) for each entry of the lanes' tokens n among the wave's terms [wv, wv + 16 MR): in the lane that
-    // holds the entry's term in register `mine` = 4 i + e; other lanes get -1.
-    template <int MR, class F>
-    __device__ __forceinline__ void each(int n, bool on, int wv, int q, F &&f) const {
-        int64_t base = 0;
-        int k = 0, end = 0;
-        if (on) {
-            base = (int64_t)n * top;
-            const int64_t t = (int64_t)(wv / kRowPad) * ld + n;
-            k = first[t];
-            end = first[t + ld];
+};
+
+// A wave's part of them: lane l holds those of token n0 + l (of the wave's 16 MC) in the wave's block of terms.  The first
+// four come with two waits for memory, before the tile's exponents are worked out (one after the other, column block by
+// column block, they took as long as a third of the product).
+template <int MR, int MC>
+struct Held {
+    static constexpr int M = 4;
+    const int *ids;
+    const float *share;
+    int wv, count;
+    int id[M];
+    float part[M];
+    __device__ __forceinline__ Held(const Entries &s, int n0, int n_c, int wv_, int lane) : wv(wv_) {
+        const int n = n0 + lane;
+        const bool on = lane < 16 * MC && n < n_c;
+        const int64_t t = (int64_t)(wv / (16 * MR)) * s.ld + n;
+        const int k = on ? s.first[t] : 0;
+        count = on ? s.first[t + s.ld] - k : 0;
+        ids = s.ids + (int64_t)n * s.top + k;
+        share = s.share + (int64_t)n * s.top + k;
+#pragma unroll
+        for (int m = 0; m < M; m++) {
+            id[m] = m < count ? ids[m] : 0;
+            part[m] = m < count ? share[m] : 0.f;
         }
-        while (__any(k < end)) {
-            const int lv = k < end ? ids[base + k] - wv : -1;
-            if (__any(lv >= 0 && lv < MR * 16)) {
-                const float s = k < end ? share[base + k] : 0.f;
-                f(lv >= 0 && lv < MR * 16 && ((lv >> 2) & 3) == q ? (lv >> 4) * 4 + (lv & 3) : -1, s);
-            }
-            k++;
+    }
+    // f(mine, share) for each entry of column block j's tokens: in the lane that holds the entry's term in register
+    // `mine` = 4 i + e; other lanes get -1.
+    template <class F>
+    __device__ __forceinline__ void each(int j, int lane, F &&f) const {
+        const int from = 16 * j + (lane & 15), q = lane >> 4;
+        const uint64_t block = 0xFFFFull << (16 * j);
+        const auto one = [&](int m, int x, float s) {
+            if (!(__ballot(m < count) & block)) return false;
+            const int lv = __shfl(m < count ? x - wv : -1, from, GS_WAVE);
+            const float sh = __shfl(s, from, GS_WAVE);
+            f(lv >= 0 && ((lv >> 2) & 3) == q ? (lv >> 4) * 4 + (lv & 3) : -1, sh);
+            return true;
+        };
+#pragma unroll
+        for (int m = 0; m < M; m++)
+            if (!one(m, id[m], part[m])) return;
+        for (int m = M; one(m, m < count ? ids[m] : 0, m < count ? share[m] : 0.f); m++) {
         }
     }
 };
+
+struct NoneHeld {
+    template <class F>
+    __device__ __forceinline__ void each(int, int, F &&) const {}
+};
+template <class TL, bool SHARES>
+__device__ __forceinline__ auto held_of(const Entries &s, const Place &at, int wv) {
+    if constexpr (SHARES) return Held<TL::MR, TL::MC>(s, at.col0, at.n_c, wv, at.lane);
+    else return NoneHeld{};
+}
 
 // Adds the bias of a tile's rows (side array 0) where its sums did not start with it.
 template <class TL, class Epi>
@@ -448,6 +490,7 @@ struct EpiSums {
     template <class TL>
     __device__ __forceinline__ void run(f32x4 (&acc)[TL::MR][TL::MC], const Place &at) const {
         const int q = at.lane >> 4;
+        const auto held = held_of<TL, SHARES>(entries, at, at.row0);
         add_row_bias<TL, EpiSums>(acc, at);
         const int64_t block = at.row0 / (TL::MR * 16);
 #pragma unroll
@@ -464,7 +507,7 @@ struct EpiSums {
                 for (int e = 0; e < 4; e++) s += __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], scale, -sub));
             float dot = 0.f;
             if (SHARES)
-                entries.each<TL::MR>(n, n < at.n_c, at.row0, q, [&](int mine, float share) {
+                held.each(j, at.lane, [&](int mine, float share) {
                     float x = 0.f;
 #pragma unroll
                     for (int i = 0; i < TL::MR; i++)
@@ -519,6 +562,7 @@ struct EpiLogitGrad {
         for (int i = 0; i < TL::MR; i++) sums[i] = f32x4{0.f, 0.f, 0.f, 0.f};
         add_row_bias<TL, EpiLogitGrad>(acc, at);
         const int wv = v0 + at.row0;  // the wave's first term
+        const auto held = held_of<TL, SHARES>(entries, at, wv);
 #pragma unroll
         for (int j = 0; j < TL::MC; j++) {
             const int n = at.col0 + 16 * j + (at.lane & 15);
@@ -536,7 +580,7 @@ struct EpiLogitGrad {
                     for (int e = 0; e < 4; e++) acc[i][j][e] -= mine == i * 4 + e ? share * up : 0.f;
             };
             if constexpr (SHARES) {
-                entries.each<TL::MR>(n, on, wv, q, off);
+                held.each(j, at.lane, off);
             } else {
                 const int lv = on ? __float_as_int(at.side(3, in)) - wv : -1;
                 const bool here = lv >= 0 && lv < TL::MR * 16;
@@ -1599,7 +1643,7 @@ void take_loss_saved(gs_arena &a, const LossPlan &p, const gs_vocab_head *h, con
     s->loss = a.take<float>(p.l.rows);
     s->ids = a.take<int>((size_t)p.l.rows * p.top);
     s->share = teacher ? a.take<float>((size_t)p.l.rows * p.top) : nullptr;
-    s->first = teacher ? a.take<uint16_t>((size_t)(p.l.vocabp / kRowPad + 1) * p.l.rows) : nullptr;
+    s->first = teacher ? a.take<uint16_t>((size_t)(p.l.vocabp / term_block(p.l.cls) + 1) * p.l.rows) : nullptr;
 }
 
 struct LossScratch {
@@ -1776,7 +1820,7 @@ extern "C" int gs_vocab_loss(const gs_vocab_head *h, const gs_vocab_targets *t, 
     }
     const Keep keep{x.keep, teacher ? nullptr : t->targets_d, t->ignore_index, h->vocab, rows};
     const TargetRows targets{teacher ? nullptr : t->targets_d, sv.c.bias, sv.ids, x.target};
-    const TeacherRows entries{teacher ? x.ids : nullptr, x.share, p.top, p.l.vocabp / kRowPad, rows, sv.ids, sv.share, sv.first};
+    const TeacherRows entries{teacher ? x.ids : nullptr, x.share, p.top, p.l.vocabp / term_block(p.l.cls), term_block(p.l.cls), rows, sv.ids, sv.share, sv.first};
     if (int rc = prepare(h, p.l, keep, sv.c, loss_d, reduction == GS_REDUCE_NONE ? rows : 0, targets, entries, s)) return rc;
     if (rows > 0) {
         int rc = GS_OK;
