@@ -547,3 +547,21 @@ def test_refusals(device):
             call()
     with pytest.raises(RuntimeError, match="GPU"):
         gs.term_weights(h.cpu(), w.cpu())
+
+
+# ---------------------------------------------------------------- together
+
+
+def test_train_and_search_example(device):
+    """The three operators as they are used together: losses fall, and the searched index finds what it should."""
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "gpu-sparse_amd", "examples",
+                        "train_and_search.py")
+    spec = importlib.util.spec_from_file_location("train_and_search", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    got = example.run(steps=30, n_docs=600, vocab=1500, dim=64, length=40, batch=48)
+    assert all(math.isfinite(x) for x in got["last"])
+    assert got["last"][0] < got["first"][0] and got["last"][3] < got["first"][3]
+    assert got["after"] > 0.8 and got["after"] >= got["before"]
