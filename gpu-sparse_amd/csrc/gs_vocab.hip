@@ -93,6 +93,32 @@ __device__ __forceinline__ void store_planes4(uint16_t *row, int64_t plane, int 
     }
 }
 
+// 32 columns of 16 rows in blocks: lane l holds those at 4 (l >> 4) of column blocks a and b of row l & 15.  Lanes of two
+// rows of lanes swap halves, so that a lane writes eight columns, those of column block (l >> 4) & 1 from 8 (l >> 5) on, and
+// the wave whole lines.
+template <class T, int NP>
+__device__ __forceinline__ void store_blocks(uint16_t *to, int64_t plane, f32x4 a, f32x4 b) {
+    uint16_t x[NP][8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        const float v = e < 4 ? a[e & 3] : b[e & 3];
+        if constexpr (NP == 1) {
+            x[0][e] = bits16<T>(v);
+        } else {
+            uint16_t s[3];
+            split3(v, s);
+            x[0][e] = s[0], x[1][e] = s[1], x[2][e] = s[2];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < NP; i++) {
+        const auto two = [&](int e) { return (uint32_t)x[i][e] | (uint32_t)x[i][e + 1] << 16; };
+        const auto u = __builtin_amdgcn_permlane16_swap(two(0), two(4), false, false);
+        const auto v = __builtin_amdgcn_permlane16_swap(two(2), two(6), false, false);
+        *reinterpret_cast<uint4 *>(to + i * plane) = make_uint4(u[0], v[0], u[1], v[1]);
+    }
+}
+
 __device__ __forceinline__ float wave_sum(float v) {
 #pragma unroll
     for (int d = 32; d >= 1; d >>= 1) v += __shfl_xor(v, d, GS_WAVE);
@@ -532,7 +558,8 @@ struct EpiSums {
 };
 
 // Gradients of a tile's logits: (softmax - target shares) times the row's factor, rounded to 16 bits once (three
-// planes for fp32), token-major, and their sums over each wave's tokens for the bias.
+// planes for fp32), in blocks, and their sums over each wave's tokens for the bias.  The rows of a block past the last
+// kept row are zeros: dW sums over them.
 template <class S, bool SHARES>
 struct EpiLogitGrad {
     const float *bias;
@@ -543,7 +570,7 @@ struct EpiLogitGrad {
     Entries entries;
     int v0;                // first term of this piece
     uint16_t *out;
-    int64_t ld, plane;
+    int64_t ld, plane;     // of the blocks, as an Operand's
     float *col_sums;       // NULL: not wanted; [wave's block of tokens][padded vocabulary]
     int64_t sums_ld;
     static constexpr int sides = 4;
@@ -563,6 +590,9 @@ struct EpiLogitGrad {
         add_row_bias<TL, EpiLogitGrad>(acc, at);
         const int wv = v0 + at.row0;  // the wave's first term
         const auto held = held_of<TL, SHARES>(entries, at, wv);
+        const bool written = at.col0 / kBlock * kBlock < at.n_c;
+        uint16_t *to = out + at.col0 / kBlock * ld + (int64_t)(at.row0 / kBlock) * kBlockValues +
+                       in_block(at.col0 % kBlock + (at.lane & 15), at.row0 % kBlock + 16 * (q & 1) + 8 * (q >> 1));
 #pragma unroll
         for (int j = 0; j < TL::MC; j++) {
             const int n = at.col0 + 16 * j + (at.lane & 15);
@@ -593,8 +623,13 @@ struct EpiLogitGrad {
             }
 #pragma unroll
             for (int i = 0; i < TL::MR; i++) {
-                sums[i] += on ? acc[i][j] : f32x4{0.f, 0.f, 0.f, 0.f};
-                if (on) store_planes4<S, TL::planes>(out + n * ld, plane, at.row0 + 16 * i + 4 * q, acc[i][j]);
+                acc[i][j] = on ? acc[i][j] : f32x4{0.f, 0.f, 0.f, 0.f};
+                sums[i] += acc[i][j];
+            }
+            if (written) {
+#pragma unroll
+                for (int i = 0; i < TL::MR; i += 2)
+                    store_blocks<S, TL::planes>(to + in_block(16 * j, 16 * (i & 3)) + (i >> 2) * kBlockValues, plane, acc[i][j], acc[i + 1][j]);
             }
         }
         if (col_sums) {
@@ -1021,11 +1056,11 @@ __global__ __launch_bounds__(256, 2) void k_few_rows(Source h, const uint8_t *ma
                      ? (int)((text * h.s0 + (row - text * length) * h.s1) * 2) + ((lane % 8) ^ (row & 7)) * 16
                      : 0x7FFFFFF0;
     }
-    const auto hr = gs_rsrc(h.p, (uint32_t)(((texts - 1) * h.s0 + (length - 1) * h.s1 + h.dim) * 2));
-    using LW = Loader<64, false, 4>;
-    Cursor<64, false> w;
+    [[maybe_unused]] const auto hr = gs_rsrc(h.p, (uint32_t)(((texts - 1) * h.s0 + (length - 1) * h.s1 + h.dim) * 2));
+    using LW = Loader<64, false, false, 4>;
+    Cursor<64, false, false> w;
     w.start(W, c0, vocab, 0, 0, 0);
-    const int w_off = LW::offset(W, wave, lane), w_gap = LW::step * (int)W.stride * 2;
+    [[maybe_unused]] const int w_off = LW::offset(W, wave, lane), w_gap = LW::gap(W);
     const int total = h.dim / kStep;
     auto issue = [&](int st) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -1042,8 +1077,8 @@ __global__ __launch_bounds__(256, 2) void k_few_rows(Source h, const uint8_t *ma
     if (bias && v < vocab)
         b = bias_type == GS_H_F32 ? ((const float *)bias)[v]
                                   : bias_type == GS_H_F16 ? (float)((const _Float16 *)bias)[v] : (float)((const __bf16 *)bias)[v];
-    Frags<64, false, 4> fr;
-    Frags<64, false, 1> fc;
+    Frags<64, false, false, 4> fr;
+    Frags<64, false, false, 1> fc;
     fr.init(0, lane);
     fc.init(wave * 16, lane);
     f32x4 acc[4];
@@ -1453,16 +1488,16 @@ __global__ __launch_bounds__(256) void k_entry_sums(Source h, Source w, const fl
 //    320       27.3        23.5        20.3
 //   1250       90.5        57.2        53.7
 // k-major operands (dH, dW) do better with waves of 64 x 128 than of 128 x 64 (dW 880 -> 915 TFLOP/s).
-template <class T, int NP, bool RK, bool CK>
-using Small = Tile<T, NP, 64, 64, 2, 2, 4, 2, RK, CK>;
-template <class T, int NP, bool RK, bool CK>
-using Wide = Tile<T, NP, 256, 128, 4, 2, 3, 2, RK, CK>;
-template <class T, int NP, bool RK, bool CK>  // tokens as rows
-using Flat = Tile<T, NP, 128, 256, 2, 4, 3, 2, RK, CK>;
-template <class T, int NP, bool RK, bool CK>
-using Large = Tile<T, NP, 256, 256, 2, 4, 2, 2, RK, CK>;
-template <class T, int NP, bool RK, bool CK>
-using LargeK = Tile<T, NP, 256, 256, 4, 2, 2, 2, RK, CK>;
+template <class T, int NP, bool RK, bool CK, bool CB = false>
+using Small = Tile<T, NP, 64, 64, 2, 2, 4, 2, RK, CK, CB>;
+template <class T, int NP, bool RK, bool CK, bool CB = false>
+using Wide = Tile<T, NP, 256, 128, 4, 2, 3, 2, RK, CK, CB>;
+template <class T, int NP, bool RK, bool CK, bool CB = false>  // tokens as rows
+using Flat = Tile<T, NP, 128, 256, 2, 4, 3, 2, RK, CK, CB>;
+template <class T, int NP, bool RK, bool CK, bool CB = false>
+using Large = Tile<T, NP, 256, 256, 2, 4, 2, 2, RK, CK, CB>;
+template <class T, int NP, bool RK, bool CK, bool CB = false>
+using LargeK = Tile<T, NP, 256, 256, 4, 2, 2, 2, RK, CK, CB>;
 
 constexpr int kSmallRows = 64, kWideRows = 256;
 
@@ -1677,7 +1712,7 @@ void take_grad_scratch(gs_arena &a, const LossPlan &p, GradScratch *s) {
     s->parts = a.take<int>(64);
     s->sums = a.take<float>((size_t)p.sum_rows * p.l.vocabp);
     s->part = a.take<float>((size_t)p.part_rows * p.l.dimp);
-    s->dl = a.take<uint16_t>((size_t)p.l.rows * p.l.planes * p.piece);
+    s->dl = a.take<uint16_t>((size_t)round_up(p.l.rows, kBlock) * p.l.planes * p.piece);
 }
 
 int check_targets(const gs_vocab_head *h, const gs_vocab_targets *t) {
@@ -1721,7 +1756,8 @@ int run_grad(const gs_vocab_head *h, const LossPlan &p, const LossSaved &s, cons
              float power, bool want_dh, bool want_db, void *dw_d, int cus, hipStream_t st) {
     using S = typename T::store_t;
     const Operand w = weight_operand(p.l, s.c, h), hid = hidden_operand(p.l, s.c);
-    const Operand dl{g.dl, (int64_t)NP * p.piece, p.piece, (int64_t)NP * p.piece};
+    const int64_t row = (int64_t)p.piece * kBlock;  // values of a row of blocks
+    const Operand dl{g.dl, NP * row, row, NP * row};
     for (int c = 0; c < p.pieces; c++) {
         const int v0 = c * p.piece, nv = min(p.piece, h->vocab - v0);
         if (nv <= 0) break;
@@ -1734,7 +1770,7 @@ int run_grad(const gs_vocab_head *h, const LossPlan &p, const LossSaved &s, cons
         const Dims dw{dw_d ? h->dim : 0, nv, p.l.rows, s.c.n, 0, 0, 1}, none{0, 0, 0, s.c.n, 0, 0, 0};
         int rc = GS_OK;
 #define GSV_EPI(SHARES) \
-    EpiLogitGrad<S, SHARES> { s.c.bias, scale, s.lse2, up.scale ? g.factor : nullptr, power, power == 2048.f ? 11.f : 0.f, entries_of(p, s), v0, g.dl, dl.stride, p.piece, want_db ? g.sums : nullptr, p.l.vocabp }
+    EpiLogitGrad<S, SHARES> { s.c.bias, scale, s.lse2, up.scale ? g.factor : nullptr, power, power == 2048.f ? 11.f : 0.f, entries_of(p, s), v0, g.dl, dl.stride, dl.plane, want_db ? g.sums : nullptr, p.l.vocabp }
 #define GSV_GRAD(TL)                                                                              \
     rc = s.share ? launch_product<TL<T, NP, false, false>>(wp, hid, de, GSV_EPI(true), cus, st)   \
                  : launch_product<TL<T, NP, false, false>>(wp, hid, de, GSV_EPI(false), cus, st)
@@ -1748,13 +1784,13 @@ int run_grad(const gs_vocab_head *h, const LossPlan &p, const LossSaved &s, cons
         if (rc) return rc;
         if (!want_dh && !dw_d) continue;
 #define GSV_PAIR(TL, DW)                                                                                              \
-    rc = launch_pair<TL<T, NP, true, false>, TL<T, NP, true, true>>(wp, dl, dh, eh, hid, dl, DW, ew, p.piece, p.most, \
+    rc = launch_pair<TL<T, NP, true, false, true>, TL<T, NP, true, true, true>>(wp, dl, dh, eh, hid, dl, DW, ew, p.piece, p.most, \
                                                                     g.parts, cus, st)
         switch (p.l.cls) {
             case kSmall:
                 // few rows: dW is its output's bytes, which larger tiles write faster
                 GSV_PAIR(Small, none);
-                if (!rc) rc = launch_product<Wide<T, NP, true, true>>(hid, dl, dw, ew, cus, st);
+                if (!rc) rc = launch_product<Wide<T, NP, true, true, true>>(hid, dl, dw, ew, cus, st);
                 break;
             case kWide: GSV_PAIR(Wide, dw); break;
             default: GSV_PAIR(LargeK, dw); break;

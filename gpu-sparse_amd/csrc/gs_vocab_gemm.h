@@ -49,12 +49,22 @@ constexpr int kStep = 64;  // k values per stage: two 16x16x32 products deep, an
 
 // A 16-bit matrix.  [x][k]: row x starts at p + x * stride; [k][x]: row k does.  Plane i of an
 // fp32 matrix starts `plane` values further along each row.
+//
+// In blocks: 64 x 64 values are 8 KiB on end, 64 rows of them `stride` values from the next 64; planes follow one another
+// along these rows of blocks.  A block holds eight rows at a time, of these the first eight values of each row, then the
+// second eight, ...  (The logit gradients, [token][term]: the wave that makes them writes whole lines, either product that
+// reads them, along terms or along tokens, copies whole blocks to LDS, and a stage lies in a few pages.)
 struct Operand {
     const uint16_t *p;
     int64_t stride;
     int64_t plane;
-    int64_t width;  // values of a row that may be read (all planes)
+    int64_t width;  // values of a row (of blocks) that may be read (all planes)
 };
+constexpr int kBlock = 64, kBlockValues = kBlock * kBlock;
+// Where in a block value v of row x is
+__host__ __device__ __forceinline__ constexpr int in_block(int x, int v) {
+    return (x >> 3) * 512 + (v >> 3) * 64 + (x & 7) * 8 + (v & 7);
+}
 
 // Sizes of a product.  Those that depend on the number of kept rows are read from n_d.
 struct Dims {
@@ -80,15 +90,23 @@ __device__ __forceinline__ int turn(int k) {
 // that one read cycle takes lie in different banks.  (Rows of 64 bytes asked the L2 for half lines: 20% slower.)  [k][x]:
 // a piece is 1024 / (2 X) rows of X values, chunks moved in pairs by the k row, so that the rows of a transposing read do.
 // The waves take pieces in turn, so that a wave's pieces differ by whole rows and share one offset per lane.
-template <int X, bool KM, int NW>
+// In blocks: a piece is eight rows of a block as they lie, the rows' odd chunks with their halves of four rows swapped, so
+// that a transposing read's four rows of two chunks differ in their banks.
+template <int X, bool KM, bool BL, int NW>
 struct Loader {
     static constexpr int pieces = X / 8 / NW;
     static constexpr int per = KM ? X / 8 : 8;       // 16-byte chunks of a row
     static constexpr int step = 64 / per * NW;       // rows between a wave's pieces
-    static_assert(pieces == 1 || step % (KM ? 16 : 8) == 0, "chunks move alike in all of a wave's pieces");
+    static_assert(BL || pieces == 1 || step % (KM ? 16 : 8) == 0, "chunks move alike in all of a wave's pieces");
+    static_assert(!BL || NW == 8 || X == kBlock, "a wave's pieces are a block apart, or in one block");
     __device__ __forceinline__ static int offset(const Operand &o, int wave, int lane) {
+        if (BL) return wave * 1024 + (lane >> 3) * 128 + ((lane & 7) ^ ((lane >> 1) & 4)) * 16;
         const int row = wave * (64 / per) + lane / per, s = lane % per;
         return (int)(row * o.stride * 2) + (s ^ (KM ? turn<X>(row) << 1 : row & 7)) * 16;
+    }
+    __device__ __forceinline__ static int gap(const Operand &o) {
+        if (BL) return NW < 8 ? NW * 1024 : KM ? kBlockValues * 2 : (int)o.stride * 2;
+        return step * (int)o.stride * 2;
     }
     // gap: bytes between a wave's pieces
     __device__ __forceinline__ static void issue(__amdgpu_buffer_rsrc_t r, int gap, int off, int soff, lds_t lds, int wave) {
@@ -104,13 +122,22 @@ struct Loader {
 // The next stage of an operand's tile: a buffer that ends with the rows that exist, and an offset into its rows.  The
 // buffer of a [x][k] tile stays and the offset moves along its rows (never past them, so the rows that exist are those
 // whose own offset lies in the buffer); that of a [k][x] tile moves by the stage's rows.
-template <int X, bool KM>
+template <int X, bool KM, bool BL>
 struct Cursor {
     const char *p;
     int bytes, soff, rows;
     __device__ __forceinline__ void start(const Operand &o, int x0, int nx, int k, int nk, int plane) {
         const int64_t in = plane * o.plane;
-        if (KM) {
+        rows = 0;
+        if (BL && KM) {
+            p = reinterpret_cast<const char *>(o.p + k / kBlock * o.stride + in + (int64_t)x0 * kBlock);
+            bytes = (int)(o.width - in - (int64_t)x0 * kBlock) * 2;
+            soff = 0;
+        } else if (BL) {
+            p = reinterpret_cast<const char *>(o.p + x0 / kBlock * o.stride);
+            bytes = (int)((min(nx - x0, X) - 1) / kBlock * o.stride + o.width) * 2;
+            soff = (int)(in + (int64_t)k * kBlock) * 2;
+        } else if (KM) {
             p = reinterpret_cast<const char *>(o.p + k * o.stride + in + x0);
             rows = nk - k;
             bytes = (int)(o.width - in - x0) * 2;
@@ -119,7 +146,6 @@ struct Cursor {
             p = reinterpret_cast<const char *>(o.p + x0 * o.stride);
             bytes = (int)((min(nx - x0, X) - 1) * o.stride + o.width) * 2;
             soff = (int)(in + k) * 2;
-            rows = 0;
         }
         uniform();
     }
@@ -129,10 +155,13 @@ struct Cursor {
         bytes = gs_uniform(bytes), soff = gs_uniform(soff), rows = gs_uniform(rows);
     }
     __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const Operand &o) const {
-        return gs_rsrc(p, (uint32_t)(KM ? (min(rows, kStep) - 1) * (int)(o.stride * 2) + bytes : bytes));
+        return gs_rsrc(p, (uint32_t)(KM && !BL ? (min(rows, kStep) - 1) * (int)(o.stride * 2) + bytes : bytes));
     }
     __device__ __forceinline__ void next(const Operand &o) {
-        if (KM) {
+        if (BL) {
+            if (KM) p += o.stride * 2;
+            else soff += kBlockValues * 2;
+        } else if (KM) {
             p += o.stride * (2 * kStep);
             rows -= kStep;
         } else {
@@ -143,12 +172,19 @@ struct Cursor {
 };
 
 // Fragments of 16 rows (columns) x 32 k values, half h of a stage: lane l holds row l & 15, k = 32 h + 8 (l >> 4) .. + 7.
-template <int X, bool KM, int M>
+template <int X, bool KM, bool BL, int M>
 struct Frags {
-    int at[KM ? M : 2];
+    int at[KM && !BL ? M : 2];
     __device__ __forceinline__ void init(int x0, int lane) {  // x0: the wave's first row in the tile
         const int i = lane & 15, q = lane >> 4;
-        if (KM) {
+        if (BL && KM) {
+            const int odd = (i >> 1) & 1;
+            at[0] = (x0 >> 6) * 8192 + q * 1024 + ((x0 >> 3) & 7) * 128 + odd * 128 + ((i >> 2) ^ (odd << 2)) * 16 + (i & 1) * 8;
+            at[1] = at[0] ^ 64;  // four rows on
+        } else if (BL) {
+            at[0] = ((x0 + i) >> 3) * 1024 + q * 128 + ((i & 7) ^ ((q & 1) << 2)) * 16;
+            at[1] = at[0] + 512;
+        } else if (KM) {
             const int k = 8 * q + (i >> 2);
             const int g = turn<X>(k);
             const int base = k * (X * 2) + ((i >> 1) & 1) * 16 + (i & 1) * 8;
@@ -163,8 +199,10 @@ struct Frags {
         typedef __attribute__((address_space(3))) s16x4 *lp4;
         typedef __attribute__((address_space(3))) s16x8 *lp8;
         if (KM) {
-            const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp4)(lds + at[m] + h * 64 * X));
-            const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp4)(lds + at[m] + h * 64 * X + 8 * X));
+            const int a_at = BL ? at[0] + (m >> 2) * 8192 + (m & 3) * 256 + h * 4096 : at[BL ? 0 : m] + h * 64 * X;
+            const int b_at = BL ? at[1] + (m >> 2) * 8192 + (m & 3) * 256 + h * 4096 : a_at + 8 * X;
+            const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp4)(lds + a_at));
+            const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp4)(lds + b_at));
             return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
         }
         return *(lp8)(lds + at[h] + m * 2048);
@@ -182,8 +220,9 @@ __device__ __forceinline__ void tile_barrier() {
     asm volatile("" ::: "memory");
 }
 
-// A workgroup's tile: BR x BC over WR x WC waves, NS stages in LDS, OCC waves per SIMD.
-template <class T, int NP, int BR_, int BC_, int WR_, int WC_, int NS_, int OCC, bool RK, bool CK>
+// A workgroup's tile: BR x BC over WR x WC waves, NS stages in LDS, OCC waves per SIMD.  RK, CK: R, C lie k-major; CB: C
+// lies in blocks.
+template <class T, int NP, int BR_, int BC_, int WR_, int WC_, int NS_, int OCC, bool RK, bool CK, bool CB = false>
 struct Tile {
     using type = T;
     static constexpr int BR = BR_, BC = BC_, WR = WR_, WC = WC_, NS = NS_, planes = NP;
@@ -191,7 +230,7 @@ struct Tile {
     static constexpr int MR = BR / WR / 16, MC = BC / WC / 16;
     static constexpr int stage_bytes = (BR + BC) * kStep * 2;
     static constexpr int edge = BR > BC ? BR : BC;
-    static constexpr bool r_kmajor = RK, c_kmajor = CK;
+    static constexpr bool r_kmajor = RK, c_kmajor = CK, c_blocks = CB;
 };
 
 // What an epilogue reads per row or column of a tile (a bias, a row's softmax sum) comes to LDS with the tile's first
@@ -283,13 +322,14 @@ struct Stream {
     using TA = typename SA::tile;
     using TB = typename SB::tile;
     static constexpr bool pair = !std::is_same_v<SA, SB>;
-    static constexpr int loads = Loader<TA::BR, TA::r_kmajor, TA::waves>::pieces + Loader<TA::BC, TA::c_kmajor, TA::waves>::pieces;
+    static constexpr int loads = Loader<TA::BR, TA::r_kmajor, false, TA::waves>::pieces +
+                                 Loader<TA::BC, TA::c_kmajor, TA::c_blocks, TA::waves>::pieces;
     Work w;
     int r_off, c_off;     // the lane's
-    Cursor<TA::BR, TA::r_kmajor> ra;
-    Cursor<TA::BC, TA::c_kmajor> ca;
-    Cursor<TB::BR, TB::r_kmajor> rb;
-    Cursor<TB::BC, TB::c_kmajor> cb;
+    Cursor<TA::BR, TA::r_kmajor, false> ra;
+    Cursor<TA::BC, TA::c_kmajor, TA::c_blocks> ca;
+    Cursor<TB::BR, TB::r_kmajor, false> rb;
+    Cursor<TB::BC, TB::c_kmajor, TB::c_blocks> cb;
     Share share;
     int t, by;            // the workgroup's tiles: t, t + by, ... of its XCD's share
     int ik, seg, buf, left;
@@ -317,8 +357,8 @@ struct Stream {
         w = work_of<TL>(s, parts, at);
         left = w.per * (TL::planes == 3 ? 6 : 1);
         seg = ik = 0;
-        r_off = Loader<TL::BR, TL::r_kmajor, TL::waves>::offset(side.R, wave, lane);
-        c_off = Loader<TL::BC, TL::c_kmajor, TL::waves>::offset(side.C, wave, lane);
+        r_off = Loader<TL::BR, TL::r_kmajor, false, TL::waves>::offset(side.R, wave, lane);
+        c_off = Loader<TL::BC, TL::c_kmajor, TL::c_blocks, TL::waves>::offset(side.C, wave, lane);
         planes(side, s, r, c);
     }
     // To the first stage of plane pair seg
@@ -344,10 +384,10 @@ struct Stream {
         using TL = typename S::tile;
         const lds_t to = lds + buf * TL::stage_bytes;
         if (S::epilogue::sides > 0 && fresh) sides(side, s, lds, wave, lane);
-        using LR = Loader<TL::BR, TL::r_kmajor, TL::waves>;
-        using LC = Loader<TL::BC, TL::c_kmajor, TL::waves>;
-        LR::issue(r.buffer(side.R), LR::step * (int)side.R.stride * 2, r_off, r.soff, to, wave);
-        LC::issue(c.buffer(side.C), LC::step * (int)side.C.stride * 2, c_off, c.soff, to + TL::BR * kStep * 2, wave);
+        using LR = Loader<TL::BR, TL::r_kmajor, false, TL::waves>;
+        using LC = Loader<TL::BC, TL::c_kmajor, TL::c_blocks, TL::waves>;
+        LR::issue(r.buffer(side.R), LR::gap(side.R), r_off, r.soff, to, wave);
+        LC::issue(c.buffer(side.C), LC::gap(side.C), c_off, c.soff, to + TL::BR * kStep * 2, wave);
         fresh = false;
         if (TL::planes == 3 && ++ik == w.per) {
             ik = 0;
@@ -437,8 +477,8 @@ __global__ __launch_bounds__(SA::tile::threads, SA::tile::waves_per_simd) void k
     // half the next stage has to have landed, and this one, which every wave holds by then, makes room for another.
     auto run = [&](auto &side, const Work &w, const Shape &s) {
         using TL = typename std::remove_reference_t<decltype(side)>::tile;
-        Frags<TL::BR, TL::r_kmajor, TL::MR> fr;
-        Frags<TL::BC, TL::c_kmajor, TL::MC> fc;
+        Frags<TL::BR, TL::r_kmajor, false, TL::MR> fr;
+        Frags<TL::BC, TL::c_kmajor, TL::c_blocks, TL::MC> fc;
         fr.init(wr * TL::MR * 16, lane);
         fc.init(wc * TL::MC * 16, lane);
         const Place at{w.r0 + wr * TL::MR * 16, w.c0 + wc * TL::MC * 16, lane, w.part, s.nr, s.nc, wr * TL::MR * 16,
