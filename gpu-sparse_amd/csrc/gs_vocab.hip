@@ -432,8 +432,8 @@ struct Entries {
 };
 
 // A wave's part of them: lane l holds those of token n0 + l (of the wave's 16 MC) in the wave's block of terms.  The first
-// four come with two waits for memory, before the tile's exponents are worked out (one after the other, column block by
-// column block, they took as long as a third of the product).
+// four are asked for before the tile's last stage (one after the other, column block by column block, they took as long as a
+// third of the product).
 template <int MR, int MC>
 struct Held {
     static constexpr int M = 4;
@@ -514,9 +514,12 @@ struct EpiSums {
     static constexpr bool row_bias = true;
     __device__ __forceinline__ SideArray side(int, int r0, int, const Shape &) const { return {bias + r0, 256}; }
     template <class TL>
-    __device__ __forceinline__ void run(f32x4 (&acc)[TL::MR][TL::MC], const Place &at) const {
+    __device__ __forceinline__ auto before(const Place &at) const {
+        return held_of<TL, SHARES>(entries, at, at.row0);
+    }
+    template <class TL, class H>
+    __device__ __forceinline__ void run(f32x4 (&acc)[TL::MR][TL::MC], const Place &at, const H &held) const {
         const int q = at.lane >> 4;
-        const auto held = held_of<TL, SHARES>(entries, at, at.row0);
         add_row_bias<TL, EpiSums>(acc, at);
         const int64_t block = at.row0 / (TL::MR * 16);
 #pragma unroll
@@ -536,10 +539,12 @@ struct EpiSums {
                 held.each(j, at.lane, [&](int mine, float share) {
                     float x = 0.f;
 #pragma unroll
-                    for (int i = 0; i < TL::MR; i++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++) x = mine == i * 4 + e ? acc[i][j][e] : x;
-                    if (share != 0.f) dot = fmaf(share, x, dot);
+                    for (int i = 0; i < TL::MR; i++) {
+                        const f32x4 &y = acc[i][j];
+                        const float a = mine & 1 ? y[1] : y[0], b = mine & 1 ? y[3] : y[2];
+                        x = mine >> 2 == i ? (mine & 2 ? b : a) : x;
+                    }
+                    if (share != 0.f) dot = fmaf(share, x, dot);  // x is 0 in the lanes without the entry
                 });
             const auto join = [&](Two<float> m2, Two<float> s2, Two<float> d2) {
                 mc = fmaxf(m2.a, m2.b);
@@ -582,14 +587,17 @@ struct EpiLogitGrad {
         return {entries.ids + c0, SHARES ? 0 : s.nc - c0};  // one target per row
     }
     template <class TL>
-    __device__ __forceinline__ void run(f32x4 (&acc)[TL::MR][TL::MC], const Place &at) const {
+    __device__ __forceinline__ auto before(const Place &at) const {
+        return held_of<TL, SHARES>(entries, at, v0 + at.row0);
+    }
+    template <class TL, class H>
+    __device__ __forceinline__ void run(f32x4 (&acc)[TL::MR][TL::MC], const Place &at, const H &held) const {
         const int q = at.lane >> 4;
         f32x4 sums[TL::MR];
 #pragma unroll
         for (int i = 0; i < TL::MR; i++) sums[i] = f32x4{0.f, 0.f, 0.f, 0.f};
         add_row_bias<TL, EpiLogitGrad>(acc, at);
         const int wv = v0 + at.row0;  // the wave's first term
-        const auto held = held_of<TL, SHARES>(entries, at, wv);
         const bool written = at.col0 / kBlock * kBlock < at.n_c;
         uint16_t *to = out + at.col0 / kBlock * ld + (int64_t)(at.row0 / kBlock) * kBlockValues +
                        in_block(at.col0 % kBlock + (at.lane & 15), at.row0 % kBlock + 16 * (q & 1) + 8 * (q >> 1));
@@ -604,10 +612,15 @@ struct EpiLogitGrad {
 #pragma unroll
                 for (int e = 0; e < 4; e++) acc[i][j][e] = __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], scale, -l));
             const auto off = [&](int mine, float share) {
+                float by[4];
 #pragma unroll
-                for (int i = 0; i < TL::MR; i++)
+                for (int e = 0; e < 4; e++) by[e] = (mine & 3) == e ? share * up : 0.f;
 #pragma unroll
-                    for (int e = 0; e < 4; e++) acc[i][j][e] -= mine == i * 4 + e ? share * up : 0.f;
+                for (int i = 0; i < TL::MR; i++) {
+                    const float here = mine >> 2 == i ? -1.f : 0.f;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) acc[i][j][e] = fmaf(here, by[e], acc[i][j][e]);
+                }
             };
             if constexpr (SHARES) {
                 held.each(j, at.lane, off);
@@ -655,7 +668,11 @@ struct EpiWeightGrad {
     static constexpr bool row_bias = false;
     __device__ __forceinline__ SideArray side(int, int, int, const Shape &) const { return {nullptr, 0}; }
     template <class TL>
-    __device__ __forceinline__ void run(f32x4 (&acc)[TL::MR][TL::MC], const Place &at) const {
+    __device__ __forceinline__ NoneHeld before(const Place &) const {
+        return {};
+    }
+    template <class TL>
+    __device__ __forceinline__ void run(f32x4 (&acc)[TL::MR][TL::MC], const Place &at, const NoneHeld &) const {
         const float s = up.value();
         const int q = at.lane >> 4;
 #pragma unroll
@@ -684,7 +701,11 @@ struct EpiHiddenPart {
     static constexpr bool row_bias = false;
     __device__ __forceinline__ SideArray side(int, int, int, const Shape &) const { return {nullptr, 0}; }
     template <class TL>
-    __device__ __forceinline__ void run(f32x4 (&acc)[TL::MR][TL::MC], const Place &at) const {
+    __device__ __forceinline__ NoneHeld before(const Place &) const {
+        return {};
+    }
+    template <class TL>
+    __device__ __forceinline__ void run(f32x4 (&acc)[TL::MR][TL::MC], const Place &at, const NoneHeld &) const {
         const int q = at.lane >> 4;
 #pragma unroll
         for (int j = 0; j < TL::MC; j++) {
@@ -759,7 +780,11 @@ struct EpiTextMax {
         }
     }
     template <class TL>
-    __device__ __forceinline__ void run(f32x4 (&acc)[TL::MR][TL::MC], const Place &at) const {
+    __device__ __forceinline__ NoneHeld before(const Place &) const {
+        return {};
+    }
+    template <class TL>
+    __device__ __forceinline__ void run(f32x4 (&acc)[TL::MR][TL::MC], const Place &at, const NoneHeld &) const {
         const int q = at.lane >> 4;
         if (at.row0 >= at.n_r) return;
         const int64_t block = at.row0 / (TL::MR * 16);

@@ -507,7 +507,7 @@ __global__ __launch_bounds__(SA::tile::threads, SA::tile::waves_per_simd) void k
         };
         const int total = w.per * (TL::planes == 3 ? 6 : 1);
         if (total > 0) read(0);
-        for (int it = 0; it < total; it++) {
+        auto stage = [&]() {
             read(1);
             multiply(0);
             buf = buf == NS - 1 ? 0 : buf + 1;
@@ -516,8 +516,11 @@ __global__ __launch_bounds__(SA::tile::threads, SA::tile::waves_per_simd) void k
             read(0);  // the last one reads the next tile's fragments, or what is there; nothing uses them
             ahead += st.issue(lds, A, B, a, b, parts, wave, lane);
             multiply(1);
-        }
-        side.epi.template run<TL>(acc, at);
+        };
+        for (int it = 0; it < total - 1; it++) stage();
+        const auto held = side.epi.template before<TL>(at);  // on their way during the last stage
+        if (total > 0) stage();
+        side.epi.template run<TL>(acc, at, held);
         if (total > 0) set = set == NS ? 0 : set + 1;  // as the stream, which knows tiles with stages alone
     };
     for (int t = first; t < share.na + share.nb; t += by) {
