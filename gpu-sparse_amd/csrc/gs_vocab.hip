@@ -226,7 +226,8 @@ __device__ __forceinline__ void kept_rows(const Keep &keep, int length, int *row
 }
 
 // First launch of a call.  Workgroup 0 lists the kept rows; the others write the bias in fp32 (0 without one, -inf for
-// the rows that pad the vocabulary: they drop out of every softmax and maximum) and clear what is added to later.
+// the rows that pad the vocabulary: they drop out of every softmax and maximum) and clear what is added to later.  One
+// workgroup's walk is what takes the time: 5 us of 45 rows, 14 of 16384.
 __global__ __launch_bounds__(1024) void k_setup(Keep keep, int length, int *rows, int *inv, int *seg, int *text_first, int *n, const void *bias,
                                                 int bias_type, int vocab, int padded, float *bias_o, float *zero, int64_t zeros) {
     if (blockIdx.x == 0) {
@@ -269,7 +270,8 @@ __device__ __forceinline__ void pack_row(const Source &s, int row, int dimp, uin
 // ---------------------------------------------------------------- targets
 
 // A teacher's row: q = softmax(logits / tau) over its ids inside the vocabulary, sorted by id (equal ids stay apart,
-// in their order), ids beyond them INT_MAX; sum of q log q.  One workgroup per row; LDS holds the row.
+// in their order), ids beyond them INT_MAX; sum of q log q.  One workgroup per row; LDS holds the row, where each id counts
+// those before it: 8192 rows of 64, 13 us.
 __global__ __launch_bounds__(256) void k_teacher(const int64_t *ids, const void *logits, int type, int top, int vocab,
                                                  float inv_tau, int *ids_o, float *q_o, float *ent_o, uint8_t *keep) {
     __shared__ int sid[kMaxTop];
@@ -385,7 +387,7 @@ struct TargetRows {
 
 // Second launch of a call, a wave per row: the kept hidden states and, where the product cannot read it in place
 // (w_rows > 0), the vocabulary as contiguous 16-bit rows (fp32: three planes), zero to a multiple of kStep values; and the
-// kept rows' targets.
+// kept rows' targets.  Bytes: 77 rows and 30522 terms of 384 fp32 values, 119 MB in 22 us (5.4 TB/s).
 template <int HT, int NP>
 __global__ __launch_bounds__(256) void k_pack(Source h, const int *rows, const int *n_d, uint16_t *h_out, Source w, int w_rows,
                                               uint16_t *w_out, int dimp, TargetRows targets, TeacherRows teacher) {
@@ -501,7 +503,9 @@ __device__ __forceinline__ void add_row_bias(f32x4 (&acc)[TL::MR][TL::MC], const
 }
 
 // Softmax sums of a tile: per token the largest scaled logit and the sum of 2^(scaled logit - it), over each wave's
-// terms: part[block of terms][token]; with SHARES also the sum of share * logit: dots[block of terms][token].
+// terms: part[block of terms][token]; with SHARES also the sum of share * logit: dots[block of terms][token].  An exponent
+// takes four times an addition's cycles, and two waves' epilogues share a SIMD: a fifth of a tile's time at 768 values.
+// 8192 rows, 128003 terms, 1024 values: 1.65 ms (1300 TFLOP/s); 5734 rows, 30522, 768, with entries: 302 us (890).
 template <bool SHARES>
 struct EpiSums {
     const float *bias;
@@ -564,7 +568,9 @@ struct EpiSums {
 
 // Gradients of a tile's logits: (softmax - target shares) times the row's factor, rounded to 16 bits once (three
 // planes for fp32), in blocks, and their sums over each wave's tokens for the bias.  The rows of a block past the last
-// kept row are zeros: dW sums over them.
+// kept row are zeros: dW sums over them.  The products are made a second time rather than kept: 8192 rows of 128003
+// logits are 2 GB to write and to read, 0.8 ms, against 1.6 for the product, but in 16 bits they would lose what the losses need.
+// 1.79 ms there, in two pieces (1200 TFLOP/s, 2.1 GB written).
 template <class S, bool SHARES>
 struct EpiLogitGrad {
     const float *bias;
@@ -658,7 +664,8 @@ struct EpiLogitGrad {
     }
 };
 
-// dW: rows are dim, columns terms; out[term][dim] times *scale
+// dW: rows are dim, columns terms; out[term][dim] times *scale.  It and dH, one launch: 8192 rows, 128003 terms, 1024 values
+// 4.0 ms (1070 TFLOP/s); 2458 rows, 30522, 768 233 us (990).  What bounds them: loads that two stages do not hide.
 template <class O>
 struct EpiWeightGrad {
     O *out;
@@ -728,7 +735,8 @@ struct EpiHiddenPart {
 // block w of tokens; for each text b in it the largest logits go to slot w + b (along the blocks and texts one of the
 // two grows with each pair, so slots are distinct, and those of a text lie one after the other), with TOK also the
 // lowest kept row that has it.  k_term_weights takes a text's slots together.  The bias is added to the maximum
-// (rounding keeps order).
+// (rounding keeps order).  The product bounds it: 10240 rows, 30522 terms, 768 values, 370 us (1300 TFLOP/s); texts of 20 tokens,
+// whose maxima are joined across lanes and written seven times a wave: 1280 rows 69 us (870).
 template <bool TOK>
 struct EpiTextMax {
     const float *bias;
@@ -933,7 +941,7 @@ struct BiasSums {
 
 // Last launch of a gradient.  dH of every source row from its parts (0 for rows that are not kept): with few rows, and so
 // many parts, a workgroup of W = 16 waves takes 256 values of a row, the waves take parts in turn and are added in order; else
-// (W = 4) a wave does.  Then workgroups of 32 terms of the bias.
+// (W = 4) a wave does.  Then workgroups of 32 terms of the bias.  Bytes: 8192 rows of 1024 values, 54 us.
 template <class O, int W>
 __global__ __launch_bounds__(64 * W) void k_finish_grad(const float *part, const int *inv, const int *n_d, const int *parts_d,
                                                         int total, int dim, int dimp, Upstream up, O *out, int hidden_blocks,
@@ -1004,6 +1012,7 @@ __global__ __launch_bounds__(64 * W) void k_finish_grad(const float *part, const
 // ---------------------------------------------------------------- term weights' small kernels
 
 // A text's weights from its slots: log(1 + relu(maximum)), and the lowest token that has it (-1 where the weight is 0).
+// 64 texts of 160 tokens, 30522 terms: 25 MB in 9 us.
 template <bool TOK>
 __global__ __launch_bounds__(256) void k_term_weights(const float *best, const int *where, const int *text_first, int block, int vocab,
                                                       const int *rows, int length, float *weights, int *tokens) {
@@ -1060,8 +1069,8 @@ __global__ __launch_bounds__(256) void k_term_weights(const float *best, const i
 
 // Term weights of at most 64 rows in one launch, for latency: a workgroup takes 64 terms and all rows where they lie (16-bit,
 // 16-byte aligned; rows that the mask leaves out are read as zeros and not looked at), so that there is nothing to list,
-// pack or join.  What bounds it is the vocabulary's bytes: 30522 terms of 768 values, 24 rows, 13 us (3.6 TB/s) against 27
-// in four launches.
+// pack or join.  What bounds it is the vocabulary's bytes: 30522 terms of 768 values, 24 rows, 11 us (4.4 TB/s)
+// against 27 in four launches.
 template <class T, bool TOK>
 __global__ __launch_bounds__(256, 2) void k_few_rows(Source h, const uint8_t *mask, Operand W, const void *bias, int bias_type,
                                                      int texts, int length, int vocab, float *weights, int *tokens) {
@@ -1485,7 +1494,8 @@ __device__ __forceinline__ void entries_weight(int block, const Source &h, const
     }
 }
 
-// Both in one launch: workgroups [0, weight_blocks) take terms, the others chunks of the texts' entries.
+// Both in one launch: workgroups [0, weight_blocks) take terms, the others chunks of the texts' entries.  Either gathers a row
+// of 16-bit values per entry, mostly from the L2: 0.24 M entries of 384 values 48 us, a write of 23 MB among it.
 template <int HT, int NC>
 __global__ __launch_bounds__(256) void k_entry_sums(Source h, Source w, const float *grad, const float *weights, const int *tokens,
                                                     const Entry *entries, const int *first, int texts, int vocab, int chunk,

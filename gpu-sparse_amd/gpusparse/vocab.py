@@ -13,9 +13,9 @@ product with what follows it, without the ``[tokens, vocab]`` logits in memory:
 All three work with autograd (first derivatives).  Tensors are float32, float16 or
 bfloat16, hidden states and weight of one type; sums and softmaxes are in 32 bits, and
 gradients of 16-bit tensors are rounded to their type.  Hidden states and weight may
-have any strides and sizes; a weight whose rows are 16-byte aligned and a multiple of 32
-values wide is read where it is, others are laid out once per call.  Work is queued on
-the current stream of the tensors' device; results are deterministic.
+have any strides and sizes; a 16-bit weight whose rows are 16-byte aligned and a multiple
+of 64 values wide is read where it is, others are laid out once per call.  Work is queued
+on the current stream of the tensors' device; results are deterministic.
 """
 from __future__ import annotations
 
