@@ -19,6 +19,8 @@
 // the rounding of an fp32 product.
 #pragma once
 
+#include <atomic>
+
 #include "gs_common.h"
 
 namespace gsv {
@@ -540,8 +542,16 @@ template <class SA, class SB>
 int launch_products(const SA &A, const SB &B, const Pairing &pair, int64_t grid, hipStream_t s) {
     using TL = typename SA::tile;
     const void *f = reinterpret_cast<const void *>(&k_product<SA, SB>);
-    if (SA::lds_bytes > 65536)
-        GS_CHECK_HIP(hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, SA::lds_bytes));
+    if (SA::lds_bytes > 65536) {  // once per device
+        static std::atomic<uint64_t> set{0};
+        int dev = 0;
+        GS_CHECK_HIP(hipGetDevice(&dev));
+        const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+        if (!(set.load(std::memory_order_relaxed) & bit)) {
+            GS_CHECK_HIP(hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, SA::lds_bytes));
+            set.fetch_or(bit, std::memory_order_relaxed);
+        }
+    }
     hipLaunchKernelGGL((k_product<SA, SB>), dim3((unsigned)grid), dim3(TL::threads), SA::lds_bytes, s, A, B, pair);
     GS_CHECK_LAUNCH();
     return GS_OK;

@@ -57,17 +57,23 @@ def _same_device(dev, **tensors):
 
 
 def _head(hidden, weight, bias) -> _lib.GsVocabHead:
-    """The C struct of hidden [texts, length, dim], weight [vocab, dim] and a contiguous bias."""
-    s = hidden.stride()
+    """The C struct of hidden [texts, length, dim] or [rows, dim], weight [vocab, dim] and a contiguous bias."""
+    s, n = hidden.stride(), hidden.shape
+    if len(n) == 2:
+        s, n = (0, *s), (1, *n)
     return _lib.GsVocabHead(hidden.data_ptr(), s[0], s[1], s[2], weight.data_ptr(), weight.stride(0), weight.stride(1),
                             _lib.ptr(bias), _lib.HTYPE_OF_DTYPE[hidden.dtype],
-                            _lib.GS_H_F32 if bias is None else _lib.HTYPE_OF_DTYPE[bias.dtype], hidden.shape[0],
-                            hidden.shape[1], hidden.shape[2], weight.shape[0])
+                            _lib.GS_H_F32 if bias is None else _lib.HTYPE_OF_DTYPE[bias.dtype], n[0], n[1], n[2],
+                            weight.shape[0])
 
 
 def _on(dev):
     """The tensors' device as the current one; entering it costs more than asking whether it is."""
     return nullcontext() if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+
+def _upstream(grad: torch.Tensor) -> torch.Tensor:
+    return grad if grad.dtype == torch.float32 and grad.is_contiguous() else grad.to(torch.float32).contiguous()
 
 
 def _bytes(n: int, dev) -> torch.Tensor:
@@ -114,7 +120,7 @@ class _TermWeights(torch.autograd.Function):
         dev = hidden.device
         dh, dw, db = _grads(ctx, hidden, weight, bias)
         L, head = _lib.lib(), _head(hidden, weight, bias)
-        grad = grad.to(torch.float32).contiguous()
+        grad = _upstream(grad)
         with _on(dev):
             ws = _bytes(ctx.grad_bytes, dev)
             _lib.check(L.gs_term_weights_grad(C.byref(head), grad.data_ptr(), weights.data_ptr(), tokens.data_ptr(),
@@ -151,7 +157,7 @@ class _VocabLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, bias, ids, logits, ignore_index, temperature, reduction):
         dev = hidden.device
-        rows = hidden.shape[1]
+        rows = hidden.shape[0]
         head = _head(hidden, weight, bias)
         if logits is None:
             targets = _lib.GsVocabTargets(_lib.ptr(ids), ignore_index, None, None, _lib.GS_H_F32, 0, 1.0)
@@ -160,16 +166,16 @@ class _VocabLoss(torch.autograd.Function):
                                           logits.shape[1], temperature)
         loss = torch.empty((rows,) if reduction == _lib.GS_REDUCE_NONE else (), dtype=torch.float32, device=dev)
         L = _lib.lib()
-        need = [C.c_size_t() for _ in range(3)]
+        need, scratch, grad_need = C.c_size_t(), C.c_size_t(), C.c_size_t()
         with _on(dev):
-            _lib.check(L.gs_vocab_loss_workspace(C.byref(head), C.byref(targets), *map(C.byref, need)),
-                       "gs_vocab_loss_workspace")
-            saved, ws = _bytes(need[0].value, dev), _bytes(need[1].value, dev)
+            _lib.check(L.gs_vocab_loss_workspace(C.byref(head), C.byref(targets), C.byref(need), C.byref(scratch),
+                                                 C.byref(grad_need)), "gs_vocab_loss_workspace")
+            saved, ws = _bytes(need.value, dev), _bytes(scratch.value, dev)
             _lib.check(L.gs_vocab_loss(C.byref(head), C.byref(targets), reduction, loss.data_ptr(), saved.data_ptr(),
                                        saved.numel(), ws.data_ptr(), ws.numel(), _lib.stream_ptr(dev)), "gs_vocab_loss")
         if any(ctx.needs_input_grad[:3]):
             ctx.save_for_backward(hidden, weight, bias, ids, logits, saved)
-            ctx.targets, ctx.reduction, ctx.grad_bytes = targets, reduction, need[2].value
+            ctx.targets, ctx.reduction, ctx.grad_bytes = targets, reduction, grad_need.value
         return loss
 
     @staticmethod
@@ -179,7 +185,7 @@ class _VocabLoss(torch.autograd.Function):
         dev = hidden.device
         dh, dw, db = _grads(ctx, hidden, weight, bias)
         L, head = _lib.lib(), _head(hidden, weight, bias)
-        grad = grad.to(torch.float32).contiguous()
+        grad = _upstream(grad)
         with _on(dev):
             ws = _bytes(ctx.grad_bytes, dev)
             _lib.check(L.gs_vocab_loss_grad(C.byref(head), C.byref(ctx.targets), ctx.reduction, grad.data_ptr(),
@@ -191,9 +197,9 @@ class _VocabLoss(torch.autograd.Function):
 def _loss(hidden, weight, bias, ids, logits, ignore_index, temperature, reduction):
     lead = hidden.shape[:-1]
     bias = None if bias is None else bias.contiguous()
-    flat = hidden.reshape(1, lead.numel(), hidden.shape[-1])
-    out = _VocabLoss.apply(flat, weight, bias, ids, logits, ignore_index, temperature, REDUCTIONS[reduction])
-    return out.reshape(lead) if reduction == "none" else out
+    rows = hidden if len(lead) == 1 else hidden.reshape(lead.numel(), hidden.shape[-1])  # a view is one more gradient
+    out = _VocabLoss.apply(rows, weight, bias, ids, logits, ignore_index, temperature, REDUCTIONS[reduction])
+    return out.reshape(lead) if reduction == "none" and len(lead) != 1 else out
 
 
 def _check_rows(hidden, reduction):
