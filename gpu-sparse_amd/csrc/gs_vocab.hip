@@ -145,6 +145,18 @@ __device__ __forceinline__ Two<T> across(T x) {
         return {__builtin_bit_cast(T, (uint32_t)r[0]), __builtin_bit_cast(T, (uint32_t)r[1])};
     }
 }
+// The same of two values at once: a's in the lanes where bit log2(D) of the lane is 0, b's in the others.
+template <int D, class T>
+__device__ __forceinline__ Two<T> across(T a, T b) {
+    const uint32_t x = __builtin_bit_cast(uint32_t, a), y = __builtin_bit_cast(uint32_t, b);
+    if constexpr (D == 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(x, y, false, false);
+        return {__builtin_bit_cast(T, (uint32_t)r[0]), __builtin_bit_cast(T, (uint32_t)r[1])};
+    } else {
+        const auto r = __builtin_amdgcn_permlane32_swap(x, y, false, false);
+        return {__builtin_bit_cast(T, (uint32_t)r[0]), __builtin_bit_cast(T, (uint32_t)r[1])};
+    }
+}
 // the larger one, NaN if either is
 __device__ __forceinline__ float maximum(float a, float b, float c) {
     return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c);
@@ -736,7 +748,7 @@ struct EpiHiddenPart {
 // two grows with each pair, so slots are distinct, and those of a text lie one after the other), with TOK also the
 // lowest kept row that has it.  k_term_weights takes a text's slots together.  The bias is added to the maximum
 // (rounding keeps order).  The product bounds it: 10240 rows, 30522 terms, 768 values, 370 us (1300 TFLOP/s); texts of 20 tokens,
-// whose maxima are joined across lanes and written seven times a wave: 1280 rows 69 us (870).
+// whose maxima are joined across lanes and written seven times a wave: 1280 rows 70 us (850).
 template <bool TOK>
 struct EpiTextMax {
     const float *bias;
@@ -763,28 +775,26 @@ struct EpiTextMax {
             top = maximum(maximum(top, x[0], x[1]), x[2], x[3]);
         }
     }
+    // The column blocks' maxima over the four rows of lanes, each block's in a row of lanes of its own.
     template <int MC>
-    __device__ __forceinline__ void flush(int64_t slot, float (&top)[MC], int (&tok)[MC], const float (&b)[MC], const Place &at) const {
-        static_assert(MC <= 4, "a lane group writes one column block");
-        const int q = at.lane >> 4;
-        float mine = 0.f;
-        int row = 0;
+    __device__ __forceinline__ void flush(int64_t slot, float (&top)[MC], int (&tok)[MC], float b, const Place &at) const {
+        static_assert(MC == 2 || MC == 4, "a row of lanes writes one column block");
+        const auto join = [&](Two<float> x2, Two<int> r2, float &x, int &r) {
+            if (TOK) r = x2.b > x2.a || (x2.b == x2.a && r2.b < r2.a) ? r2.b : r2.a;
+            x = maximum(x2.a, x2.b, x2.b);
+        };
+        float x[MC / 2];
+        int r[MC / 2];
 #pragma unroll
-        for (int j = 0; j < MC; j++) {
-            float x = top[j];
-            int r = tok[j];
-            const auto join = [&](Two<float> x2, Two<int> r2) {
-                if (TOK) r = x2.b > x2.a || (x2.b == x2.a && r2.b < r2.a) ? r2.b : r2.a;
-                x = maximum(x2.a, x2.b, x2.b);
-            };
-            join(across<16>(x), TOK ? across<16>(r) : Two<int>{0, 0});
-            join(across<32>(x), TOK ? across<32>(r) : Two<int>{0, 0});
-            if (j == q) mine = x + b[j], row = r;
-        }
+        for (int j = 0; j < MC; j += 2)
+            join(across<16>(top[j], top[j + 1]), TOK ? across<16>(tok[j], tok[j + 1]) : Two<int>{0, 0}, x[j / 2], r[j / 2]);
+        float best_x;
+        int best_r = 0;
+        join(across<32>(x[0], x[MC / 2 - 1]), TOK ? across<32>(r[0], r[MC / 2 - 1]) : Two<int>{0, 0}, best_x, best_r);
         const int v = at.col0 + at.lane;
-        if (q < MC && v < vocab) {
-            best[slot * vocab + v] = mine;
-            if (TOK) where[slot * vocab + v] = row;
+        if (at.lane < 16 * MC && v < vocab) {
+            best[slot * vocab + v] = best_x + b;
+            if (TOK) where[slot * vocab + v] = best_r;
         }
     }
     template <class TL>
@@ -796,10 +806,11 @@ struct EpiTextMax {
         const int q = at.lane >> 4;
         if (at.row0 >= at.n_r) return;
         const int64_t block = at.row0 / (TL::MR * 16);
-        float b[TL::MC], top[TL::MC];
+        const float b = at.side(0, at.c_in + (at.lane & (16 * TL::MC - 1)));  // of the column that the lane writes
+        float top[TL::MC];
         int tok[TL::MC];
 #pragma unroll
-        for (int j = 0; j < TL::MC; j++) b[j] = at.side(0, at.c_in + 16 * j + (at.lane & 15)), top[j] = -INFINITY, tok[j] = 0x7FFFFFFF;
+        for (int j = 0; j < TL::MC; j++) top[j] = -INFINITY, tok[j] = 0x7FFFFFFF;
         int cur = gs_uniform(__float_as_int(at.side(1, at.r_in)));
 #pragma unroll
         for (int i = 0; i < TL::MR; i++) {
