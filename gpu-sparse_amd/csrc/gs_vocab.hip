@@ -1165,7 +1165,9 @@ __global__ __launch_bounds__(256, 2) void k_few_rows(Source h, const uint8_t *ma
         };
         join(across<16>(x), TOK ? across<16>(r) : Two<int>{0, 0});
         join(across<32>(x), TOK ? across<32>(r) : Two<int>{0, 0});
-        x = maximum(x + b, 0.f, 0.f);
+        // the bias of a text without a kept row is not looked at either: it may be infinite or NaN
+        const bool any = (kept >> lo) & (~0ull >> (64 - length));
+        x = any ? maximum(x + b, 0.f, 0.f) : 0.f;
         if (q == 0 && v < vocab) {
             weights[(int64_t)text * vocab + v] = log1pf(x);
             if (TOK) tokens[(int64_t)text * vocab + v] = x > 0.f ? r - lo : -1;

@@ -219,6 +219,19 @@ def test_infinite_bias(device, dtype):
     assert abs(float(loss) + float(ref.mean())) <= float(logit_error(h, w[keep], b[keep]).max()) * 2 + 512 * U * 10
 
 
+@pytest.mark.parametrize("length", [7, 40])
+def test_the_bias_of_an_empty_text_is_not_looked_at(device, length):
+    """In one launch (21 rows) and in several (120): a text without a kept token has weights 0 whatever the bias holds."""
+    h, w, b = (x.detach() for x in inputs(device, (3, length, 64), 300, BF16, 14))
+    b = b.clone()
+    b[3::5], b[4::5] = float("inf"), float("nan")
+    mask = torch.ones((3, length), dtype=torch.bool, device=device)
+    mask[1] = False
+    weights, tokens = gs.term_weights(h, w, b, mask=mask, return_tokens=True)
+    assert not bool(weights[1].any()) and bool((tokens[1] == -1).all())
+    assert bool(torch.isinf(weights[::2, 3::5]).all()) and bool(torch.isnan(weights[::2, 4::5]).all())
+
+
 def test_sizes_of_nothing(device):
     w = torch.randn((50, 64), device=device)
     for shape in ((0, 5, 64), (3, 0, 64), (0, 0, 64)):
