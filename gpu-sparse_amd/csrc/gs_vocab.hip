@@ -1599,6 +1599,12 @@ int check_head(const gs_vocab_head *h) {
     return GS_OK;
 }
 
+// What a call that launches reads of a head
+int check_data(const gs_vocab_head *h) {
+    GS_REQUIRE(h->weight_d && (h->hidden_d || (int64_t)h->texts * h->length == 0), "NULL hidden states or weight");
+    return GS_OK;
+}
+
 struct Layout {
     int rows, dimp, planes, vocabp;
     bool w_direct;
@@ -1892,6 +1898,7 @@ extern "C" int gs_vocab_loss(const gs_vocab_head *h, const gs_vocab_targets *t, 
                      scratch_bytes);
         return GS_ENOSPC;
     }
+    if (int rc = check_data(h)) return rc;
     const hipStream_t s = gs_stream(stream);
     const int rows = p.l.rows;
     const float tau = tau_of(t);
@@ -1947,6 +1954,7 @@ extern "C" int gs_vocab_loss_grad(const gs_vocab_head *h, const gs_vocab_targets
                      scratch_bytes);
         return GS_ENOSPC;
     }
+    if (int rc = check_data(h)) return rc;
     const hipStream_t s = gs_stream(stream);
     const int rows = p.l.rows;
     const float tau = tau_of(t);
@@ -2101,6 +2109,7 @@ extern "C" int gs_term_weights(const gs_vocab_head *h, const uint8_t *mask_d, fl
         return GS_ENOSPC;
     }
     if (h->texts == 0) return GS_OK;
+    if (int rc = check_data(h)) return rc;
     GS_REQUIRE(weights_d && workspace_d, "NULL weights or workspace");
     GS_REQUIRE(h->texts <= 65535, "texts=%d exceed 65535", h->texts);
     const hipStream_t s = gs_stream(stream);
@@ -2173,6 +2182,9 @@ extern "C" int gs_term_weights_grad(const gs_vocab_head *h, const float *grad_d,
         gs_set_error("term_weights_grad workspace too small: need %zu bytes, got %zu", a.used, workspace_bytes);
         return GS_ENOSPC;
     }
+    if (int rc = check_data(h)) return rc;
+    GS_REQUIRE((grad_d && weights_d && tokens_d) || h->texts == 0, "NULL gradient, weights or tokens");
+    GS_REQUIRE(workspace_d || a.used == 0, "NULL workspace");
     const hipStream_t s = gs_stream(stream);
     if (h->type == GS_H_F32) return run_entries<GS_H_F32>(h, grad_d, weights_d, tokens_d, dhidden_d, dweight_d, dbias_d, p, s);
     if (h->type == GS_H_F16) return run_entries<GS_H_F16>(h, grad_d, weights_d, tokens_d, dhidden_d, dweight_d, dbias_d, p, s);

@@ -61,3 +61,16 @@ def test_term_weights_workspace_is_checked():
     assert a.value > 0 and b.value > 0
     rc = L.gs_term_weights_grad(C.byref(head()), 8, 8, 8, 8, 8, 8, 8, b.value - 1, None)
     assert rc == _lib.GS_ENOSPC and b"too small" in L.gs_last_error()
+
+
+@pytest.mark.parametrize("over,given,match", [
+    (dict(weight_d=8), 8, "NULL hidden states or weight"), (dict(hidden_d=8), 8, "NULL hidden states or weight"),
+    (dict(hidden_d=8, weight_d=8), None, "NULL gradient, weights or tokens"),
+])
+def test_missing_tensors_are_refused(over, given, match):
+    L = _lib.lib()
+    a, b = C.c_size_t(), C.c_size_t()
+    h = C.byref(head(**over))
+    assert L.gs_term_weights_workspace(h, 1, C.byref(a), C.byref(b)) == _lib.GS_OK
+    with pytest.raises(ValueError, match=match):
+        _lib.check(L.gs_term_weights_grad(h, given, given, given, None, None, None, 8, b.value, None), "gs_term_weights_grad")
