@@ -45,7 +45,9 @@ def _check_head(hidden, weight, bias, dims: str) -> torch.device:
         raise ValueError(f"hidden must be {dims} with dim {weight.shape[1]}, got {tuple(hidden.shape)}")
     if bias is not None and tuple(bias.shape) != (weight.shape[0],):
         raise ValueError(f"bias must be [{weight.shape[0]}], got {tuple(bias.shape)}")
-    dev = _lib.require_gpu(hidden.device)
+    dev = hidden.device
+    if dev.type != "cuda":
+        dev = _lib.require_gpu(dev)
     _same_device(dev, weight=weight, bias=bias)
     return dev
 
@@ -86,28 +88,34 @@ def _grads(ctx, hidden, weight, bias):
             for t, need in zip((hidden, weight, bias), ctx.needs_input_grad[:3])]
 
 
+def _differentiable(*inputs) -> bool:
+    """Whether a gradient may be asked for; a call without one leaves autograd out (5 us of a query's 21)."""
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in inputs)
+
+
+def _weights(hidden, weight, bias, mask, want_tokens: bool):
+    """Weights, tokens or None, and the bytes that a gradient's workspace takes."""
+    dev = hidden.device
+    texts, vocab = hidden.shape[0], weight.shape[0]
+    weights = torch.empty((texts, vocab), dtype=torch.float32, device=dev)
+    tokens = torch.empty((texts, vocab), dtype=torch.int32, device=dev) if want_tokens else None
+    L, head = _lib.lib(), _head(hidden, weight, bias)
+    need, grad_need = C.c_size_t(), C.c_size_t()
+    with _on(dev):
+        _lib.check(L.gs_term_weights_workspace(C.byref(head), want_tokens, C.byref(need), C.byref(grad_need)),
+                   "gs_term_weights_workspace")
+        ws = _bytes(need.value, dev)
+        _lib.check(L.gs_term_weights(C.byref(head), _lib.ptr(mask), weights.data_ptr(), _lib.ptr(tokens), ws.data_ptr(),
+                                     need.value, _lib.stream_ptr(dev)), "gs_term_weights")
+    return weights, tokens, grad_need.value
+
+
 class _TermWeights(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, hidden, weight, bias, mask, want_tokens):
-        dev = hidden.device
-        texts, vocab = hidden.shape[0], weight.shape[0]
-        track = any(ctx.needs_input_grad[:3])
-        weights = torch.empty((texts, vocab), dtype=torch.float32, device=dev)
-        tokens = torch.empty((texts, vocab), dtype=torch.int32, device=dev) if want_tokens or track else None
-        L, head = _lib.lib(), _head(hidden, weight, bias)
-        need, grad_need = C.c_size_t(), C.c_size_t()
-        with _on(dev):
-            _lib.check(L.gs_term_weights_workspace(C.byref(head), tokens is not None, C.byref(need), C.byref(grad_need)),
-                       "gs_term_weights_workspace")
-            ws = _bytes(need.value, dev)
-            _lib.check(L.gs_term_weights(C.byref(head), _lib.ptr(mask), weights.data_ptr(), _lib.ptr(tokens), ws.data_ptr(),
-                                         ws.numel(), _lib.stream_ptr(dev)), "gs_term_weights")
-        if track:
-            ctx.save_for_backward(hidden, weight, bias, weights, tokens)
-            ctx.grad_bytes = grad_need.value
-            ctx.set_materialize_grads(False)
-        if tokens is None:
-            return weights, None
+    def forward(ctx, hidden, weight, bias, mask):
+        weights, tokens, ctx.grad_bytes = _weights(hidden, weight, bias, mask, True)
+        ctx.save_for_backward(hidden, weight, bias, weights, tokens)
+        ctx.set_materialize_grads(False)
         ctx.mark_non_differentiable(tokens)
         return weights, tokens
 
@@ -115,7 +123,7 @@ class _TermWeights(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, grad, _):
         if grad is None:
-            return None, None, None, None, None
+            return None, None, None, None
         hidden, weight, bias, weights, tokens = ctx.saved_tensors
         dev = hidden.device
         dh, dw, db = _grads(ctx, hidden, weight, bias)
@@ -126,7 +134,7 @@ class _TermWeights(torch.autograd.Function):
             _lib.check(L.gs_term_weights_grad(C.byref(head), grad.data_ptr(), weights.data_ptr(), tokens.data_ptr(),
                                               _lib.ptr(dh), _lib.ptr(dw), _lib.ptr(db), ws.data_ptr(), ws.numel(),
                                               _lib.stream_ptr(dev)), "gs_term_weights_grad")
-        return dh, dw, db, None, None
+        return dh, dw, db, None
 
 
 def term_weights(hidden, weight, bias=None, *, mask=None, return_tokens: bool = False):
@@ -149,33 +157,42 @@ def term_weights(hidden, weight, bias=None, *, mask=None, return_tokens: bool = 
             mask = mask != 0
         mask = mask.contiguous()
     bias = None if bias is None else bias.contiguous()
-    weights, tokens = _TermWeights.apply(hidden, weight, bias, mask, bool(return_tokens))
+    if _differentiable(hidden, weight, bias):
+        weights, tokens = _TermWeights.apply(hidden, weight, bias, mask)
+    else:
+        weights, tokens, _ = _weights(hidden, weight, bias, mask, bool(return_tokens))
     return (weights, tokens) if return_tokens else weights
+
+
+def _losses(hidden, weight, bias, ids, logits, ignore_index, temperature, reduction):
+    """The loss, what a gradient reads of the call (targets struct, saved bytes) and the bytes its workspace takes."""
+    dev = hidden.device
+    head = _head(hidden, weight, bias)
+    if logits is None:
+        targets = _lib.GsVocabTargets(_lib.ptr(ids), ignore_index, None, None, _lib.GS_H_F32, 0, 1.0)
+    else:
+        targets = _lib.GsVocabTargets(None, 0, _lib.ptr(ids), logits.data_ptr(), _lib.HTYPE_OF_DTYPE[logits.dtype],
+                                      logits.shape[1], temperature)
+    shape = (hidden.shape[0],) if reduction == _lib.GS_REDUCE_NONE else ()
+    loss = torch.empty(shape, dtype=torch.float32, device=dev)
+    L = _lib.lib()
+    need, scratch, grad_need = C.c_size_t(), C.c_size_t(), C.c_size_t()
+    with _on(dev):
+        _lib.check(L.gs_vocab_loss_workspace(C.byref(head), C.byref(targets), C.byref(need), C.byref(scratch),
+                                             C.byref(grad_need)), "gs_vocab_loss_workspace")
+        saved, ws = _bytes(need.value, dev), _bytes(scratch.value, dev)
+        _lib.check(L.gs_vocab_loss(C.byref(head), C.byref(targets), reduction, loss.data_ptr(), saved.data_ptr(),
+                                   need.value, ws.data_ptr(), scratch.value, _lib.stream_ptr(dev)), "gs_vocab_loss")
+    return loss, targets, saved, grad_need.value
 
 
 class _VocabLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, bias, ids, logits, ignore_index, temperature, reduction):
-        dev = hidden.device
-        rows = hidden.shape[0]
-        head = _head(hidden, weight, bias)
-        if logits is None:
-            targets = _lib.GsVocabTargets(_lib.ptr(ids), ignore_index, None, None, _lib.GS_H_F32, 0, 1.0)
-        else:
-            targets = _lib.GsVocabTargets(None, 0, _lib.ptr(ids), logits.data_ptr(), _lib.HTYPE_OF_DTYPE[logits.dtype],
-                                          logits.shape[1], temperature)
-        loss = torch.empty((rows,) if reduction == _lib.GS_REDUCE_NONE else (), dtype=torch.float32, device=dev)
-        L = _lib.lib()
-        need, scratch, grad_need = C.c_size_t(), C.c_size_t(), C.c_size_t()
-        with _on(dev):
-            _lib.check(L.gs_vocab_loss_workspace(C.byref(head), C.byref(targets), C.byref(need), C.byref(scratch),
-                                                 C.byref(grad_need)), "gs_vocab_loss_workspace")
-            saved, ws = _bytes(need.value, dev), _bytes(scratch.value, dev)
-            _lib.check(L.gs_vocab_loss(C.byref(head), C.byref(targets), reduction, loss.data_ptr(), saved.data_ptr(),
-                                       saved.numel(), ws.data_ptr(), ws.numel(), _lib.stream_ptr(dev)), "gs_vocab_loss")
-        if any(ctx.needs_input_grad[:3]):
-            ctx.save_for_backward(hidden, weight, bias, ids, logits, saved)
-            ctx.targets, ctx.reduction, ctx.grad_bytes = targets, reduction, grad_need.value
+        loss, ctx.targets, saved, ctx.grad_bytes = _losses(hidden, weight, bias, ids, logits, ignore_index, temperature,
+                                                           reduction)
+        ctx.save_for_backward(hidden, weight, bias, ids, logits, saved)
+        ctx.reduction = reduction
         return loss
 
     @staticmethod
@@ -198,7 +215,8 @@ def _loss(hidden, weight, bias, ids, logits, ignore_index, temperature, reductio
     lead = hidden.shape[:-1]
     bias = None if bias is None else bias.contiguous()
     rows = hidden if len(lead) == 1 else hidden.reshape(lead.numel(), hidden.shape[-1])  # a view is one more gradient
-    out = _VocabLoss.apply(rows, weight, bias, ids, logits, ignore_index, temperature, REDUCTIONS[reduction])
+    args = (rows, weight, bias, ids, logits, ignore_index, temperature, REDUCTIONS[reduction])
+    out = _VocabLoss.apply(*args) if _differentiable(hidden, weight, bias) else _losses(*args)[0]
     return out.reshape(lead) if reduction == "none" and len(lead) != 1 else out
 
 
