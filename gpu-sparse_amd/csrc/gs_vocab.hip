@@ -1241,38 +1241,49 @@ __global__ __launch_bounds__(256) void k_entry_counts(const int *tokens, int voc
     }
 }
 
-// starts[text][run][token]: the place of the run's first entry of the token.  One workgroup per text.
+// starts[text][run][token]: the place of the run's first entry of the token.  One workgroup per text; T tokens at a time, the
+// runs in 1024 / T slices, so that short texts have the loads of all threads on their way (64 tokens, 120 runs: 9.3 -> 7.1 us).
 __global__ __launch_bounds__(1024) void k_entry_starts(const uint16_t *counts, int length, int runs, int *starts, int *first) {
-    __shared__ int part[16];
+    __shared__ int sums[1024], part[16];
     const int64_t b = blockIdx.x;
     const int tid = threadIdx.x, lane = gs_lane(), wave = tid >> 6;
+    const int T = length <= 64 ? 64 : length <= 128 ? 128 : length <= 256 ? 256 : length <= 512 ? 512 : 1024;
+    const int slices = 1024 / T, waves = T / 64, g = tid / T;
+    const int r0 = runs * g / slices, r1 = runs * (g + 1) / slices;
     int base = 0;
-    for (int t0 = 0; t0 < length; t0 += 1024) {
-        const int t = t0 + tid;
+    for (int t0 = 0; t0 < length; t0 += T) {
+        const int t = t0 + tid % T;
         const uint16_t *from = counts + b * runs * length + t;
         int *to = starts + b * runs * length + t;
         int c = 0;
         if (t < length) {
 #pragma unroll 8
-            for (int r = 0; r < runs; r++) c += from[(int64_t)r * length];
+            for (int r = r0; r < r1; r++) c += from[(int64_t)r * length];
         }
-        const int inc = (int)gs_wave_incl_scan((uint32_t)c);
+        sums[tid] = c;
+        __syncthreads();
+        int before = 0, all = 0;  // of the token: in the slices before this one, in all
+        for (int k = 0; k < slices; k++) {
+            const int x = sums[k * T + tid % T];
+            before += k < g ? x : 0;
+            all += x;
+        }
+        const int inc = (int)gs_wave_incl_scan((uint32_t)all);
         if (lane == 63) part[wave] = inc;
         __syncthreads();
-        int at = base + inc - c;
-        for (int w = 0; w < 16; w++) {
-            if (w < wave) at += part[w];
+        int at = base + inc - all + before;
+        for (int w = 0; w < waves; w++) {
+            if (w < wave % waves) at += part[w];
             base += part[w];
         }
         if (t < length) {
-            first[b * (length + 1) + t] = at;
+            if (g == 0) first[b * (length + 1) + t] = at;
 #pragma unroll 8
-            for (int r = 0; r < runs; r++) {
+            for (int r = r0; r < r1; r++) {
                 to[(int64_t)r * length] = at;
                 at += from[(int64_t)r * length];
             }
         }
-        __syncthreads();
     }
     if (tid == 0) first[b * (length + 1) + length] = base;
 }
