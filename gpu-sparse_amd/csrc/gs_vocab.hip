@@ -1242,7 +1242,8 @@ __global__ __launch_bounds__(256) void k_entry_counts(const int *tokens, int voc
 }
 
 // starts[text][run][token]: the place of the run's first entry of the token.  One workgroup per text; T tokens at a time, the
-// runs in 1024 / T slices, so that short texts have the loads of all threads on their way (120 runs, 64 tokens 9.7 -> 5.9 us, 256 tokens 10.2 -> 9.6).
+// runs in 1024 / T slices, so that short texts have the loads of all threads on their way (120 runs, 64
+// tokens: 9.7 -> 5.9 us, 256 tokens: 10.2 -> 9.6).
 __global__ __launch_bounds__(1024) void k_entry_starts(const uint16_t *counts, int length, int runs, int *starts, int *first) {
     __shared__ int sums[1024], part[16];
     const int64_t b = blockIdx.x;
