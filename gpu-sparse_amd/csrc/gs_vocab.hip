@@ -1665,6 +1665,12 @@ void take_common(gs_arena &a, const Layout &l, const gs_vocab_head *h, bool text
     s->text_first = texts ? a.take<int>(h->texts + 1) : nullptr;
     s->bias = a.take<float>(l.vocabp);
     s->hidden = a.take<uint16_t>((size_t)l.rows * l.planes * l.dimp);
+}
+
+// The last of a buffer: whether there is a copy moves nothing else.  A loss and its gradient may be given the weight at
+// different places (autograd's hooks on saved tensors bring it back where they like); a gradient that can read it where it
+// is does, whether or not the loss copied it.
+void take_weight(gs_arena &a, const Layout &l, const gs_vocab_head *h, Common *s) {
     s->weight = l.w_direct ? nullptr : a.take<uint16_t>((size_t)h->vocab * l.planes * l.dimp);
 }
 
@@ -1759,6 +1765,7 @@ void take_loss_saved(gs_arena &a, const LossPlan &p, const gs_vocab_head *h, con
     s->ids = a.take<int>((size_t)p.l.rows * p.top);
     s->share = teacher ? a.take<float>((size_t)p.l.rows * p.top) : nullptr;
     s->first = teacher ? a.take<uint16_t>((size_t)(p.l.vocabp / term_block(p.l.cls) + 1) * p.l.rows) : nullptr;
+    take_weight(a, p.l, h, &s->c);
 }
 
 struct LossScratch {
@@ -2112,6 +2119,7 @@ extern "C" int gs_term_weights_workspace(const gs_vocab_head *h, int32_t tokens,
     const size_t slots = text_slots(h, l);
     a.take<float>(slots * h->vocab);
     if (tokens) a.take<int>(slots * h->vocab);
+    take_weight(a, l, h, &c);
     EntryPlan p;
     take_entries(b, h, &p);
     *bytes = a.used, *grad_bytes = b.used;
@@ -2130,6 +2138,7 @@ extern "C" int gs_term_weights(const gs_vocab_head *h, const uint8_t *mask_d, fl
     const size_t slots = text_slots(h, l);
     float *best = a.take<float>(slots * h->vocab);
     int *where = tokens_d ? a.take<int>(slots * h->vocab) : nullptr;
+    take_weight(a, l, h, &c);
     if (!a.ok()) {
         gs_set_error("term_weights workspace too small: need %zu bytes, got %zu", a.used, workspace_bytes);
         return GS_ENOSPC;

@@ -29,6 +29,7 @@ from . import _lib
 C = _lib.C
 REDUCTIONS = {"none": _lib.GS_REDUCE_NONE, "mean": _lib.GS_REDUCE_MEAN, "sum": _lib.GS_REDUCE_SUM}
 MAX_TOP = 1024  # most teacher logits per row
+SAVED_ALIGN = 256  # of what a loss saves for its gradient
 
 
 def _check_head(hidden, weight, bias, dims: str) -> torch.device:
@@ -88,6 +89,21 @@ def _grads(ctx, hidden, weight, bias):
             for t, need in zip((hidden, weight, bias), ctx.needs_input_grad[:3])]
 
 
+def _kinds(*tensors):
+    return [None if t is None else (t.shape, t.dtype, t.device) for t in tensors]
+
+
+def _unpack(ctx):
+    """The saved tensors.  Hooks on them (offloading, packing) may bring them back at other addresses and in other strides,
+    which what reads them has to bear, but not as tensors of another kind, whose memory the kernels would misread."""
+    saved = ctx.saved_tensors
+    for t, kind in zip(saved, ctx.kinds):
+        if t is not None and (t.shape, t.dtype, t.device) != kind:
+            raise RuntimeError(f"a saved tensor came back as {t.dtype} {tuple(t.shape)} on {t.device}, not as "
+                               f"{kind[1]} {tuple(kind[0])} on {kind[2]}")
+    return saved
+
+
 def _differentiable(*inputs) -> bool:
     """Whether a gradient may be asked for; a call without one leaves autograd out (5 us of a query's 21)."""
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in inputs)
@@ -115,6 +131,7 @@ class _TermWeights(torch.autograd.Function):
     def forward(ctx, hidden, weight, bias, mask):
         weights, tokens, ctx.grad_bytes = _weights(hidden, weight, bias, mask, True)
         ctx.save_for_backward(hidden, weight, bias, weights, tokens)
+        ctx.kinds = _kinds(hidden, weight, bias, weights, tokens)
         ctx.set_materialize_grads(False)
         ctx.mark_non_differentiable(tokens)
         return weights, tokens
@@ -124,7 +141,8 @@ class _TermWeights(torch.autograd.Function):
     def backward(ctx, grad, _):
         if grad is None:
             return None, None, None, None
-        hidden, weight, bias, weights, tokens = ctx.saved_tensors
+        hidden, weight, bias, weights, tokens = _unpack(ctx)
+        weights, tokens = weights.contiguous(), tokens.contiguous()
         dev = hidden.device
         dh, dw, db = _grads(ctx, hidden, weight, bias)
         L, head = _lib.lib(), _head(hidden, weight, bias)
@@ -186,20 +204,40 @@ def _losses(hidden, weight, bias, ids, logits, ignore_index, temperature, reduct
     return loss, targets, saved, grad_need.value
 
 
+def _place(weight):
+    return weight.stride(), weight.data_ptr() % SAVED_ALIGN
+
+
+def _as_loss_read_it(hidden, weight, bias, targets, saved_bytes):
+    """The weight as a gradient can read it: where it is, or from the copy among the saved bytes; where the loss made no copy
+    and the weight came back in another layout, a contiguous one, as it was then."""
+    need, other = C.c_size_t(), C.c_size_t()
+    with _on(hidden.device):
+        _lib.check(_lib.lib().gs_vocab_loss_workspace(C.byref(_head(hidden, weight, bias)), C.byref(targets), C.byref(need),
+                                                      C.byref(other), C.byref(other)), "gs_vocab_loss_workspace")
+    return weight if need.value <= saved_bytes else weight.clone(memory_format=torch.contiguous_format)
+
+
 class _VocabLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, bias, ids, logits, ignore_index, temperature, reduction):
         loss, ctx.targets, saved, ctx.grad_bytes = _losses(hidden, weight, bias, ids, logits, ignore_index, temperature,
                                                            reduction)
         ctx.save_for_backward(hidden, weight, bias, ids, logits, saved)
+        ctx.kinds = _kinds(hidden, weight, bias, ids, logits, saved)
+        ctx.weight_at = _place(weight)
         ctx.reduction = reduction
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        hidden, weight, bias, _, _, saved = ctx.saved_tensors
+        hidden, weight, bias, _, _, saved = _unpack(ctx)
         dev = hidden.device
+        if saved.data_ptr() % SAVED_ALIGN or not saved.is_contiguous():
+            saved = saved.clone(memory_format=torch.contiguous_format)
+        if _place(weight) != ctx.weight_at:
+            weight = _as_loss_read_it(hidden, weight, bias, ctx.targets, saved.numel())
         dh, dw, db = _grads(ctx, hidden, weight, bias)
         L, head = _lib.lib(), _head(hidden, weight, bias)
         grad = _upstream(grad)

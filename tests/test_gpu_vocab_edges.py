@@ -1,0 +1,83 @@
+"""The vocabulary head's operators at the edges: values that are not finite, tensors that autograd hands back elsewhere, and
+calls under other kinds of differentiation.  References are in float64; bounds as in test_gpu_vocab.py."""
+import math
+
+import pytest
+import torch
+
+import gpusparse as gs
+from test_gpu_vocab import BF16, F16, F32, TINY, U, UT, assert_within, inputs, logit_error, logits64, mask_of
+
+pytestmark = pytest.mark.gpu
+
+INF, NAN = float("inf"), float("nan")
+
+
+# ---------------------------------------------------------------- tensors that autograd hands back
+
+
+def _aligned(t):
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _off_by_one(t):
+    """The same values, contiguous, one value past a 16-byte boundary."""
+    store = torch.empty(t.numel() + 1, dtype=t.dtype, device=t.device)
+    out = store[1:].view(t.shape)
+    out.copy_(t)
+    return out
+
+
+def _last_dim_first(t):
+    return t.transpose(0, -1).contiguous().transpose(0, -1)
+
+
+PLACES = {"aligned": _aligned, "off by one": _off_by_one, "last dimension first": _last_dim_first}
+
+
+def _head_calls(device, vocab):
+    g = torch.Generator().manual_seed(72)
+    t = torch.randint(0, vocab, (70,), generator=g).to(device)
+    ids = torch.randint(0, vocab, (70, 9), generator=g).to(device)
+    z = torch.randn((70, 9), generator=g).to(device)
+    return {"vocab_loss": lambda h, w, b: gs.vocab_loss(h, w, t, b), "distill_loss": lambda h, w, b: gs.distill_loss(h, w, ids, z, b),
+            "term_weights": lambda h, w, b: gs.term_weights(h.view(7, 10, -1), w, b).sum()}
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("back", list(PLACES))
+@pytest.mark.parametrize("there", list(PLACES))
+def test_saved_tensors_may_come_back_elsewhere(device, dtype, there, back):
+    """Hooks on saved tensors (offloading, packing) hand a call's tensors back at other addresses and in other strides: the
+    weight that forward laid out may then be one that can be read in place, and the other way round."""
+    h, w, b = (x.detach() for x in inputs(device, (70, 128), 900, dtype, 71))
+    for name, call in _head_calls(device, 900).items():
+        args = [x.requires_grad_() for x in (h.clone(), PLACES[there](w), b.clone())]
+        want = torch.autograd.grad(call(*args), args)
+        with torch.autograd.graph.saved_tensors_hooks(lambda x: x, PLACES[back]):
+            loss = call(*args)
+        for got, ref in zip(torch.autograd.grad(loss, args), want):
+            assert torch.equal(got, ref), name
+
+
+def test_saved_tensors_on_the_host_and_back(device):
+    h, w, b = (x.detach() for x in inputs(device, (70, 128), 900, BF16, 71))
+    for name, call in _head_calls(device, 900).items():
+        args = [x.requires_grad_() for x in (h.clone(), _last_dim_first(w), b.clone())]
+        want = torch.autograd.grad(call(*args), args)
+        with torch.autograd.graph.save_on_cpu(pin_memory=True):
+            loss = call(*args)
+        for got, ref in zip(torch.autograd.grad(loss, args), want):
+            assert torch.equal(got, ref), name
+
+
+@pytest.mark.parametrize("back,match", [(lambda t: t.cpu(), "on cpu, not"), (lambda t: t.double() if t.is_floating_point() else t, "float64"),
+                                        (lambda t: t[:1], r"\(1,")])
+def test_saved_tensors_of_another_kind_are_refused(device, back, match):
+    h, w, b = (x.detach() for x in inputs(device, (70, 128), 900, BF16, 71))
+    for call in _head_calls(device, 900).values():
+        args = [x.requires_grad_() for x in (h.clone(), w.clone(), b.clone())]
+        with torch.autograd.graph.saved_tensors_hooks(lambda x: x, lambda t: back(t) if t.dim() < 3 else t):
+            loss = call(*args)
+        with pytest.raises(RuntimeError, match=match):
+            torch.autograd.grad(loss, args)
