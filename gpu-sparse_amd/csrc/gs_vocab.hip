@@ -1332,14 +1332,16 @@ __global__ __launch_bounds__(256) void k_entry_place(const float *grad, const fl
 }
 
 // U rows of up to 256 NC values in a wave's registers, all on their way at once: lane l holds values 256 c + 4 l .. + 3.
-// Aligned rows (`vec`) are read through a buffer that ends with the row, so that no lane branches.
+// Aligned rows (`vec`) are read through a buffer that ends with the row, so that no lane branches: with the word that holds its
+// last value, since one that the buffer ends in reads 0 (the rows are 8-byte aligned, so the word is the row's own memory or
+// what pads it).
 template <int U, int NC, class T>
 __device__ __forceinline__ void rows_load(f32x4 (&x)[U][NC], const T *const (&row)[U], int64_t ds, int d0, int dim, bool vec) {
     const int lane = gs_lane();
     if (vec) {
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            const auto r = gs_rsrc(row[u], (uint32_t)(dim * sizeof(T)));
+            const auto r = gs_rsrc(row[u], (uint32_t)round_up(dim * sizeof(T), 4));
 #pragma unroll
             for (int c = 0; c < NC; c++) {
                 const int off = (d0 + c * 256 + lane * 4) * (int)sizeof(T);

@@ -81,3 +81,26 @@ def test_saved_tensors_of_another_kind_are_refused(device, back, match):
             loss = call(*args)
         with pytest.raises(RuntimeError, match=match):
             torch.autograd.grad(loss, args)
+
+
+# ---------------------------------------------------------------- more layouts and sizes
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("dim", [65, 66, 67])
+def test_gradients_of_aligned_rows_of_odd_width(device, dtype, dim):
+    """Rows of 65 to 67 values, 72 apart: aligned, and the last values share a word with what is not theirs."""
+    texts, length, vocab = 5, 30, 260
+    plain_h, plain_w, b = (x.detach() for x in inputs(device, (texts, length, dim), vocab, dtype, 95))
+    h = torch.full((texts, length, 72), NAN, dtype=dtype, device=device)[..., :dim]
+    w = torch.full((vocab, 72), NAN, dtype=dtype, device=device)[:, :dim]
+    h.copy_(plain_h), w.copy_(plain_w)
+    mask = mask_of("holes", texts, length, device)
+    t = torch.where(mask, torch.randint(0, vocab, (texts, length), generator=torch.Generator().manual_seed(96)).to(device), -100)
+    results = []
+    for x, y in ((h, w), (plain_h, plain_w)):
+        x, y = x.detach().requires_grad_(), y.detach().requires_grad_()
+        weights, loss = gs.term_weights(x, y, b, mask=mask), gs.vocab_loss(x, y, t, b)
+        results.append([weights.detach(), loss.detach(), *torch.autograd.grad(weights.sum(), [x, y]), *torch.autograd.grad(loss, [x, y])])
+    for got, want in zip(*results):
+        assert bool(torch.isfinite(want).all()) and torch.equal(got, want)
