@@ -746,7 +746,7 @@ struct EpiHiddenPart {
 // Largest logit of each text and term: rows are kept tokens (ascending by text), columns terms.  A wave's rows are a
 // block w of tokens; for each text b in it the largest logits go to slot w + b (along the blocks and texts one of the
 // two grows with each pair, so slots are distinct, and those of a text lie one after the other), with TOK also the
-// lowest kept row that has it.  k_term_weights takes a text's slots together.  The bias is added to the maximum
+// lowest kept row that has it (any number where that is a NaN or -inf).  k_term_weights takes a text's slots together.  The bias is added to the maximum
 // (rounding keeps order).  The product bounds it: 10240 rows, 30522 terms, 768 values, 370 us (1300 TFLOP/s); texts of 20 tokens,
 // whose maxima are joined across lanes and written seven times a wave: 1280 rows 70 us (850).
 template <bool TOK>
@@ -1022,11 +1022,29 @@ __global__ __launch_bounds__(64 * W) void k_finish_grad(const float *part, const
 
 // ---------------------------------------------------------------- term weights' small kernels
 
-// A text's weights from its slots: log(1 + relu(maximum)), and the lowest token that has it (-1 where the weight is 0).
-// 64 texts of 160 tokens, 30522 terms: 25 MB in 9 us.
-template <bool TOK>
+// The lowest kept row i in [f0, f1) whose logit of term v is NaN; f0 if the sum has one in another order only.  Comparisons
+// lose a NaN, and to keep it in the tiles' epilogue takes registers that they do not have (step of 32 x 256: 357 -> 569 us),
+// so the logits are made again where a maximum turned out to be NaN.
+template <int HT>
+__device__ __forceinline__ int nan_row(const Source &h, const Source &w, float bias, const int *rows, int f0, int f1, int v) {
+    using T = typename HVal<HT>::t;
+    if (bias != bias) return f0;
+    const T *y = (const T *)w.p + (int64_t)v * w.s1;
+    for (int i = f0; i < f1; i++) {
+        const T *x = (const T *)h.p + (int64_t)(rows[i] / h.length) * h.s0 + (int64_t)(rows[i] % h.length) * h.s1;
+        float a = 0.f;
+        for (int d = 0; d < h.dim && a == a; d++) a = fmaf((float)x[d * h.sd], (float)y[d * w.sd], a);
+        if (a + bias != a + bias) return i;
+    }
+    return f0;
+}
+
+// A text's weights from its slots: log(1 + relu(maximum)), and the lowest token that has it (-1 where the weight is 0).  HT:
+// the hidden states' type, for the tokens of NaNs.  64 texts of 160 tokens, 30522 terms: 25 MB in 9 us.
+template <bool TOK, int HT>
 __global__ __launch_bounds__(256) void k_term_weights(const float *best, const int *where, const int *text_first, int block, int vocab,
-                                                      const int *rows, int length, float *weights, int *tokens) {
+                                                      const int *rows, int length, float *weights, int *tokens, Source h, Source w,
+                                                      const float *bias) {
     const int64_t b = blockIdx.y;
     const int f0 = text_first[b], f1 = text_first[b + 1];
     const int w0 = f0 / block, w1 = (f1 - 1) / block;
@@ -1063,6 +1081,7 @@ __global__ __launch_bounds__(256) void k_term_weights(const float *best, const i
 #pragma unroll
         for (int e = 0; e < 4; e++) {
             out[e] = log1pf(x[e]);
+            if (TOK && x[e] != x[e]) row[e] = nan_row<HT>(h, w, bias[v + e], rows, f0, f1, v + e);
             if (TOK) tok[e] = row[e] >= 0 ? rows[row[e]] % length : -1;
         }
         const int64_t to = b * vocab + v;
@@ -1165,12 +1184,27 @@ __global__ __launch_bounds__(256, 2) void k_few_rows(Source h, const uint8_t *ma
         };
         join(across<16>(x), TOK ? across<16>(r) : Two<int>{0, 0});
         join(across<32>(x), TOK ? across<32>(r) : Two<int>{0, 0});
+        if (TOK && __any(!(x + b > -INFINITY))) {  // no comparison found a NaN's row, see nan_row: the least of these keys does
+            int key = 0x7FFFFFFF;
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int row = 16 * i + 4 * q + e;
+                    const float l = acc[i][e] + b;
+                    if (row >= lo && row < hi && ((kept >> row) & 1)) key = min(key, l != l ? row : row + 64);
+                }
+            const auto least = [&](Two<int> k) { key = min(k.a, k.b); };
+            least(across<16>(key));
+            least(across<32>(key));
+            r = x + b > -INFINITY ? r : key & 63;
+        }
         // the bias of a text without a kept row is not looked at either: it may be infinite or NaN
         const bool any = (kept >> lo) & (~0ull >> (64 - length));
         x = any ? maximum(x + b, 0.f, 0.f) : 0.f;
         if (q == 0 && v < vocab) {
             weights[(int64_t)text * vocab + v] = log1pf(x);
-            if (TOK) tokens[(int64_t)text * vocab + v] = x > 0.f ? r - lo : -1;
+            if (TOK) tokens[(int64_t)text * vocab + v] = x > 0.f || x != x ? r - lo : -1;
         }
     }
 }
@@ -2197,12 +2231,15 @@ extern "C" int gs_term_weights(const gs_vocab_head *h, const uint8_t *mask_d, fl
     }
     const dim3 g(gs_blocks(h->vocab, 1024, 1024), h->texts);
     const int block = token_block(l.cls);
-    if (tokens_d)
-        hipLaunchKernelGGL(k_term_weights<true>, g, dim3(256), 0, s, best, where, c.text_first, block, h->vocab, c.rows, h->length,
-                           weights_d, tokens_d);
-    else
-        hipLaunchKernelGGL(k_term_weights<false>, g, dim3(256), 0, s, best, where, c.text_first, block, h->vocab, c.rows, h->length,
-                           weights_d, tokens_d);
+    const Source hs = hidden_source(h), ws = weight_source(h);
+#define GSV_TW(TOK, HT)                                                                                                        \
+    hipLaunchKernelGGL((k_term_weights<TOK, HT>), g, dim3(256), 0, s, best, where, c.text_first, block, h->vocab, c.rows, h->length, \
+                       weights_d, tokens_d, hs, ws, c.bias)
+    if (!tokens_d) GSV_TW(false, GS_H_F32);
+    else if (h->type == GS_H_F32) GSV_TW(true, GS_H_F32);
+    else if (h->type == GS_H_F16) GSV_TW(true, GS_H_F16);
+    else GSV_TW(true, GS_H_BF16);
+#undef GSV_TW
     GS_CHECK_LAUNCH();
     return GS_OK;
 }

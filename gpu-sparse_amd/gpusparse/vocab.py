@@ -163,7 +163,8 @@ def term_weights(hidden, weight, bias=None, *, mask=None, return_tokens: bool = 
     mask: [texts, length], nonzero for the tokens that count (None: all do); the hidden
     states of the others are never read, and a text without any has weights 0.
     return_tokens: also the int32 [texts, vocab] lowest token that reaches the maximum
-    (-1 where the weight is 0), through which the gradient flows."""
+    (compared before the bias is added; -1 where the weight is 0), through which the gradient
+    flows.  A NaN is the maximum of its text: the weight is NaN, and the gradient where it flows."""
     if not isinstance(hidden, torch.Tensor) or hidden.dim() != 3:
         raise ValueError("hidden must be [texts, length, dim]")
     dev = _check_head(hidden, weight, bias, "[texts, length, dim]")

@@ -424,7 +424,9 @@ typedef struct gs_vocab_head {
 
 /* Term weights: weights_d fp32 [texts][vocab] = log(1 + relu(max over the text's kept tokens of l)); 0 for a text
  * without one.  mask_d uint8 [texts][length], 0: the token is left out (its hidden state is never read); NULL: all are
- * kept.  tokens_d int32 [texts][vocab] (or NULL): the lowest token whose l is the maximum, -1 where the weight is 0. */
+ * kept.  tokens_d int32 [texts][vocab] (or NULL): the lowest token whose l is the maximum (compared before the
+ * bias is added and rounded), -1 where the weight is 0.  A NaN among a text's l is their maximum: the weight is NaN, the
+ * token the lowest with one. */
 int gs_term_weights_workspace(const gs_vocab_head *head, int32_t tokens, size_t *bytes, size_t *grad_bytes);
 int gs_term_weights(const gs_vocab_head *head, const uint8_t *mask_d, float *weights_d, int32_t *tokens_d,
                     void *workspace_d, size_t workspace_bytes, void *stream);

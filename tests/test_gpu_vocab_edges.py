@@ -104,3 +104,57 @@ def test_gradients_of_aligned_rows_of_odd_width(device, dtype, dim):
         results.append([weights.detach(), loss.detach(), *torch.autograd.grad(weights.sum(), [x, y]), *torch.autograd.grad(loss, [x, y])])
     for got, want in zip(*results):
         assert bool(torch.isfinite(want).all()) and torch.equal(got, want)
+
+
+# ---------------------------------------------------------------- values that are not finite
+
+
+NAN_PLACES = [
+    # texts, length, dim, vocab, tokens of text 1 with a NaN
+    (2, 12, 64, 300, (5,)),              # one launch
+    (3, 21, 128, 130, (0, 20)),
+    (2, 30, 70, 300, (4, 17)),           # 64 rows at most, packed
+    (3, 50, 64, 300, (7,)),              # up to 256 rows
+    (3, 130, 64, 517, (129,)),
+    (3, 400, 64, 300, (310, 399)),       # several blocks of rows, the NaN in a later one
+    (40, 9, 64, 300, (8, 3)),            # several texts per block
+]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("texts,length,dim,vocab,at", NAN_PLACES)
+def test_a_nan_is_the_maximum_and_takes_the_gradient(device, dtype, texts, length, dim, vocab, at):
+    """The weight is NaN, its token the lowest with a NaN, and the gradient that flows there is NaN: no step is taken on it."""
+    h, w, b = inputs(device, (texts, length, dim), vocab, dtype, 81)
+    h = h.detach().clone()
+    h[1, list(at), 3] = NAN
+    h.requires_grad_()
+    weights, tokens = gs.term_weights(h, w, b, return_tokens=True)
+    assert bool(torch.isnan(weights[1]).all()) and int(torch.isnan(weights).sum()) == vocab
+    assert bool((tokens[1] == min(at)).all())
+    dh, dw, db = torch.autograd.grad(weights, [h, w, b], torch.ones_like(weights))
+    assert bool(torch.isnan(dh[1, min(at)]).all()) and int(torch.isnan(dh).sum()) == dim
+    assert bool(torch.isnan(dw).all()) and bool(torch.isnan(db).all())
+    mask = torch.ones((texts, length), dtype=torch.bool, device=device)
+    mask[1, list(at)] = False                                # left out: nothing of it is seen
+    weights = gs.term_weights(h, w, b, mask=mask)
+    assert not any(bool(torch.isnan(x).any()) for x in (weights, *torch.autograd.grad(weights.sum(), [h, w, b])))
+
+
+@pytest.mark.parametrize("texts,length,dim", [(2, 12, 64), (2, 30, 70), (3, 50, 64), (3, 400, 64)])
+def test_a_nan_of_the_bias_has_a_token(device, texts, length, dim):
+    """Logits of -inf with a bias of inf are NaN: the lowest kept token has them; with a finite bias the weight is 0."""
+    h, w, b = (x.detach() for x in inputs(device, (texts, length, dim), 200, BF16, 82))
+    h, w, b = h.clone(), w.abs() + 0.1, b.clone()
+    h[1, :, 2] = -INF
+    b[::3] = INF
+    b.requires_grad_()
+    mask = torch.ones((texts, length), dtype=torch.bool, device=device)
+    mask[1, 0] = False
+    weights, tokens = gs.term_weights(h, w, b, mask=mask, return_tokens=True)
+    assert bool(torch.isnan(weights[1, ::3]).all()) and bool((tokens[1, ::3] == 1).all())
+    off = torch.ones(200, dtype=torch.bool, device=device)
+    off[::3] = False
+    assert not bool(weights[1, off].any()) and bool((tokens[1, off] == -1).all())
+    db, = torch.autograd.grad(weights.sum(), [b])
+    assert bool(torch.isnan(db[::3]).all()) and not bool(torch.isnan(db[off]).any())
