@@ -431,7 +431,11 @@ struct Upstream {
     int mean;
     float by;            // temperature / up
     const float *scale;  // per-row values: 1 / up, made by k_row_factor
-    __device__ __forceinline__ float value() const { return scale ? *scale : *grad * (mean ? by / (float)max(*n, 1) : by); }
+    // 0 where no row counts: sums of nothing stay 0 under an infinite value
+    __device__ __forceinline__ float value() const {
+        const int rows = *n;
+        return rows == 0 ? 0.f : scale ? *scale : *grad * (mean ? by / (float)rows : by);
+    }
 };
 
 // ---------------------------------------------------------------- epilogues
@@ -985,8 +989,8 @@ __global__ __launch_bounds__(64 * W) void k_finish_grad(const float *part, const
     const int parts = *parts_d;
     const bool vec = (dim & 3) == 0;
     const int chunks = (dim + 255) / 256;
-    const auto put = [&](int64_t r, int d, f32x4 x) {
-        x *= s;
+    const auto put = [&](int64_t r, int i, int d, f32x4 x) {
+        x *= i < 0 ? 0.f : s;  // an infinite value leaves rows that are not kept 0
         O *to = out + r * dim + d;
         if (vec) store4(to, x);
         else
@@ -1007,14 +1011,14 @@ __global__ __launch_bounds__(64 * W) void k_finish_grad(const float *part, const
                 x += *reinterpret_cast<const f32x4 *>(part + ((int64_t)p * n + i) * dimp + d);
         }
         if (!share) {
-            if (r < total && d < dim) put(r, d, x);
+            if (r < total && d < dim) put(r, i, d, x);
             continue;
         }
         red[wave][lane] = x;
         __syncthreads();
         if (wave == 0 && d < dim) {
             for (int k = 1; k < W; k++) x += red[k][lane];
-            put(r, d, x);
+            put(r, i, d, x);
         }
         __syncthreads();
     }

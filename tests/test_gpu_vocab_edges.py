@@ -158,3 +158,21 @@ def test_a_nan_of_the_bias_has_a_token(device, texts, length, dim):
     assert not bool(weights[1, off].any()) and bool((tokens[1, off] == -1).all())
     db, = torch.autograd.grad(weights.sum(), [b])
     assert bool(torch.isnan(db[::3]).all()) and not bool(torch.isnan(db[off]).any())
+
+
+@pytest.mark.parametrize("up", [INF, NAN])
+@pytest.mark.parametrize("rows,dtype", [(20, F16), (90, F32), (300, BF16), (5000, BF16)])
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_rows_left_out_stay_out_of_an_infinite_gradient(device, reduction, rows, dtype, up):
+    """A scaled loss that overflows: rows left out have gradient 0 still, and so has everything where no row counts."""
+    h, w, b = inputs(device, (rows, 64), 300, dtype, 85)
+    t = torch.randint(0, 300, (rows,), generator=torch.Generator().manual_seed(86))
+    t[::3] = -100
+    for targets in (t, torch.full_like(t, -100)):
+        keep = (targets >= 0).to(device)
+        loss = gs.vocab_loss(h, w, targets.to(device), b, reduction=reduction)
+        dh, dw, db = torch.autograd.grad(loss, [h, w, b], torch.full_like(loss, up))
+        assert not bool(dh[~keep].any())
+        assert not bool(torch.isfinite(dh[keep]).any())
+        if not bool(keep.any()):
+            assert not bool(dw.any()) and not bool(db.any())
