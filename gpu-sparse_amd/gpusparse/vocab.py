@@ -10,7 +10,7 @@ product with what follows it, without the ``[tokens, vocab]`` logits in memory:
 - :func:`vocab_loss`: softmax cross entropy over the vocabulary;
 - :func:`distill_loss`: distillation from a teacher's top logits.
 
-All three work with autograd (first derivatives).  Tensors are float32, float16 or
+All three work with autograd (first derivatives, in reverse mode).  Tensors are float32, float16 or
 bfloat16, hidden states and weight of one type; sums and softmaxes are in 32 bits, and
 gradients of 16-bit tensors are rounded to their type.  Hidden states and weight may
 have any strides and sizes; a 16-bit weight whose rows are 16-byte aligned and a multiple
@@ -22,6 +22,7 @@ from __future__ import annotations
 from contextlib import nullcontext
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -105,8 +106,12 @@ def _unpack(ctx):
 
 
 def _differentiable(*inputs) -> bool:
-    """Whether a gradient may be asked for; a call without one leaves autograd out (5 us of a query's 21)."""
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in inputs)
+    """Whether a call has to go through autograd: a gradient may be asked for, tensors may carry tangents or belong to a
+    functional transform (both of which autograd refuses here), or a trace records it.  One that need not leaves autograd
+    out (5 us of a query's 21)."""
+    return ((torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in inputs))
+            or forward_ad._current_level >= 0 or torch._C._are_functorch_transforms_active()
+            or torch._C._get_tracing_state() is not None)
 
 
 def _weights(hidden, weight, bias, mask, want_tokens: bool):

@@ -176,3 +176,27 @@ def test_rows_left_out_stay_out_of_an_infinite_gradient(device, reduction, rows,
         assert not bool(torch.isfinite(dh[keep]).any())
         if not bool(keep.any()):
             assert not bool(dw.any()) and not bool(db.any())
+
+
+# ---------------------------------------------------------------- other kinds of differentiation
+
+
+def test_forward_mode_is_refused(device):
+    """There is no forward-mode derivative: a dual tensor is refused, not answered without its tangent."""
+    h, w, b = (x.detach() for x in inputs(device, (70, 64), 300, BF16, 75))
+    t = torch.zeros(70, dtype=torch.int64, device=device)
+    with torch.autograd.forward_ad.dual_level():
+        for call in (lambda w: gs.vocab_loss(h, w, t, b), lambda w: gs.term_weights(h.view(7, 10, 64), w, b)):
+            assert bool(torch.isfinite(call(w)).all())
+            with pytest.raises(NotImplementedError, match="jvp"):
+                call(torch.autograd.forward_ad.make_dual(w, torch.ones_like(w)))
+            with torch.no_grad(), pytest.raises(NotImplementedError, match="jvp"):
+                call(torch.autograd.forward_ad.make_dual(w, torch.ones_like(w)))
+    with pytest.raises(RuntimeError, match="functorch transforms"):
+        torch.func.jvp(lambda w: gs.term_weights(h.view(7, 10, 64), w, b), (w,), (torch.ones_like(w),))
+
+
+def test_a_trace_records_the_call(device):
+    h, w, b = (x.detach() for x in inputs(device, (4, 10, 64), 300, BF16, 76))
+    traced = torch.jit.trace(lambda h: gs.term_weights(h, w, b), h, check_trace=False)
+    assert torch.equal(traced(-h), gs.term_weights(-h, w, b))
