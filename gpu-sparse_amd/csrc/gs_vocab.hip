@@ -63,13 +63,15 @@ __device__ __forceinline__ uint16_t bits16(float x) {
     return __builtin_bit_cast(uint16_t, (T)x);
 }
 
-// x as bf16 planes, each the nearest to what is left.  A value that is not finite is its first plane alone.
+// x as bf16 planes, each the nearest to what is left.  A value that is not finite is its first plane alone; one beyond the
+// largest bf16 value (0x7F7F) takes that for its first, not the infinity that is nearer.
 __device__ __forceinline__ void split3(float x, uint16_t (&p)[3]) {
-    const __bf16 a = (__bf16)x;
+    const bool fin = fabsf(x) < INFINITY;
+    const float most = __uint_as_float(0x7F7F0000u);
+    const __bf16 a = (__bf16)(fin ? fminf(fmaxf(x, -most), most) : x);
     const float r = x - (float)a;
     const __bf16 b = (__bf16)r;
     const __bf16 c = (__bf16)(r - (float)b);
-    const bool fin = fabsf(x) < 3.3e38f;
     p[0] = __builtin_bit_cast(uint16_t, a);
     p[1] = fin ? __builtin_bit_cast(uint16_t, b) : 0;
     p[2] = fin ? __builtin_bit_cast(uint16_t, c) : 0;

@@ -200,3 +200,23 @@ def test_a_trace_records_the_call(device):
     h, w, b = (x.detach() for x in inputs(device, (4, 10, 64), 300, BF16, 76))
     traced = torch.jit.trace(lambda h: gs.term_weights(h, w, b), h, check_trace=False)
     assert torch.equal(traced(-h), gs.term_weights(-h, w, b))
+
+
+@pytest.mark.parametrize("x", [torch.finfo(F32).max, -torch.finfo(F32).max, 3.3e38, -3.395e38])
+def test_the_largest_fp32_values_are_finite(device, x):
+    """fp32 values beyond the largest bf16 value, among the hidden states and in the vocabulary: products with smaller
+    values are finite."""
+    h, w, b = (v.detach().clone() for v in inputs(device, (3, 40, 64), 300, F32, 91))
+    h *= 0.125
+    w *= 2.0 ** -20
+    h[1, 2, 3] = x
+    w[6, 3] = x
+    keep = torch.ones((3, 300), dtype=torch.bool, device=device)
+    keep[1, 6] = False                                       # x times x is infinite
+    top = logits64(h, w, b).amax(1).clamp(min=0)
+    want, got = torch.log1p(top), gs.term_weights(h, w, b)
+    bound = logit_error(h, w, b).amax(1) / (1 + top) * 1.01 + 8 * U * (1 + want)
+    assert bool(torch.isfinite(got[keep]).all())
+    # the text and the term of the largest value: its logits' error is of their own size; elsewhere as everywhere
+    assert_within(got[keep], want[keep], bound[keep], "weights")
+    assert float(want[0, 6]) > 80 and float(want[1].max()) > 60
