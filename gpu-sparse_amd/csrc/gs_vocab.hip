@@ -63,8 +63,10 @@ __device__ __forceinline__ uint16_t bits16(float x) {
     return __builtin_bit_cast(uint16_t, (T)x);
 }
 
-// x as bf16 planes, each the nearest to what is left.  A value that is not finite is its first plane alone; one beyond the
-// largest bf16 value (0x7F7F) takes that for its first, not the infinity that is nearer.
+// x as bf16 planes, each the nearest to what is left.  A value beyond the largest bf16 value (0x7F7F) takes that for its first,
+// not the infinity that is nearer.  An infinity is (+-1, 0, +-inf): a third plane meets first planes alone, which are 0 where
+// their value is and else have its sign, so that the pair makes the infinity (or NaN) of an fp32 product, and the other
+// pairs finite values that it swallows; as a first plane it would meet 0 and either sign in the other planes.
 __device__ __forceinline__ void split3(float x, uint16_t (&p)[3]) {
     const bool fin = fabsf(x) < INFINITY;
     const float most = __uint_as_float(0x7F7F0000u);
@@ -72,9 +74,10 @@ __device__ __forceinline__ void split3(float x, uint16_t (&p)[3]) {
     const float r = x - (float)a;
     const __bf16 b = (__bf16)r;
     const __bf16 c = (__bf16)(r - (float)b);
-    p[0] = __builtin_bit_cast(uint16_t, a);
+    const bool nan = x != x;
+    p[0] = fin || nan ? __builtin_bit_cast(uint16_t, a) : (__float_as_uint(x) >> 16 & 0x8000) | 0x3F80;
     p[1] = fin ? __builtin_bit_cast(uint16_t, b) : 0;
-    p[2] = fin ? __builtin_bit_cast(uint16_t, c) : 0;
+    p[2] = fin ? __builtin_bit_cast(uint16_t, c) : nan ? 0 : __float_as_uint(x) >> 16;
 }
 
 template <class T, int NP>

@@ -16,7 +16,7 @@
 // fp32 operands come as three bf16 planes each (x = p0 + p1 + p2, each the bf16 nearest to
 // what is left, 2^-27 of x at most lost) and the product runs over the six plane pairs whose
 // product is at least 2^-18 of the largest: what is left out is below 2^-25 of |x||y|, less than
-// the rounding of an fp32 product.
+// the rounding of an fp32 product.  (Infinities: split3.)
 #pragma once
 
 #include <atomic>

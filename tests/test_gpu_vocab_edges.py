@@ -220,3 +220,49 @@ def test_the_largest_fp32_values_are_finite(device, x):
     # the text and the term of the largest value: its logits' error is of their own size; elsewhere as everywhere
     assert_within(got[keep], want[keep], bound[keep], "weights")
     assert float(want[0, 6]) > 80 and float(want[1].max()) > 60
+
+
+def _same(got, want, bound, what):
+    """NaN and infinities where the reference has them, the others within the bound."""
+    assert bool((torch.isnan(got) == torch.isnan(want)).all()), f"{what}: NaN"
+    infinite = torch.isinf(want)
+    assert bool((got.double()[infinite] == want[infinite]).all()), f"{what}: infinities"
+    fin = torch.isfinite(want)
+    assert_within(got[fin], want[fin], bound[fin], what)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("texts,length,dim", [(2, 12, 64), (3, 40, 100), (3, 300, 64)])
+def test_infinite_hidden_states_and_vocabulary(device, dtype, texts, length, dim):
+    """An infinity times a value is an infinity of the product's sign, NaN only times 0 or beside one of the other sign."""
+    vocab = 400
+    h, w, b = (x.detach() for x in inputs(device, (texts, length, dim), vocab, dtype, 87))
+    h, w = h.clone(), w.clone()
+    h[0, 3, 5], h[1, 7, 9], h[1, 7, 11] = INF, -INF, INF
+    w[17, 2], w[29, 4], w[31, 5] = INF, -INF, 0.0            # 31 times the infinity at [0, 3, 5] is NaN
+    x = logits64(h, w, b)
+    want = torch.log1p(x.amax(dim=1).clamp(min=0))           # NaN as amax has it
+    fine = torch.where(torch.isfinite(h), h, 0), torch.where(torch.isfinite(w), w, 0)
+    bound = logit_error(*fine, b).amax(dim=1) + 8 * U * (1 + torch.where(torch.isfinite(want), want, 0))
+    got, tokens = gs.term_weights(h, w, b, return_tokens=True)
+    _same(got, want, bound, "weights")
+    # rows of a loss: finite logits, and infinite ones of the lower sign, have a finite loss
+    t = torch.randint(0, 16, (texts, length), generator=torch.Generator().manual_seed(88)).to(device)
+    logp = x.log_softmax(-1)
+    ref = -logp.gather(-1, t[..., None])[..., 0]
+    big = torch.where(torch.isfinite(x), x, 0).abs().amax(-1) + math.log(vocab) + 1
+    err = 2 * logit_error(*fine, b).amax(-1) + 256 * U * big
+    hg, wg = h.clone().requires_grad_(), w.clone().requires_grad_()
+    loss = gs.vocab_loss(hg, wg, t, b, reduction="none")
+    _same(loss.detach(), ref, err + U * big, "loss")
+    # the gradients of the rows with a finite loss: dW of every finite row of the vocabulary
+    ok = torch.isfinite(ref)
+    assert 0 < int(ok.sum()) < ok.numel()
+    dw, = torch.autograd.grad(gs.vocab_loss(h, wg, torch.where(ok, t, -100), b, reduction="sum"), [wg])
+    hid = h[ok].double()
+    p = x[ok].softmax(-1)
+    dl = p.scatter_add(-1, t[ok][:, None], -torch.ones_like(p))
+    mag = p.scatter_add(-1, t[ok][:, None], torch.ones_like(p))
+    each = mag * (UT[dtype] * 1.01 + 2 * logit_error(*fine, b).amax() + 256 * U * big.max())
+    terms = 6 * (texts * length + 16) * U
+    assert_within(dw, dl.t() @ hid, each.t() @ hid.abs() + terms * mag.t() @ hid.abs() + UT[dtype] * 1.01 * (dl.t() @ hid).abs() + TINY[dtype], "dw")
