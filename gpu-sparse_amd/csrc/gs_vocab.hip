@@ -925,29 +925,46 @@ __global__ __launch_bounds__(1024) void k_loss_sum(const float *loss, const int 
     }
 }
 
-__global__ __launch_bounds__(1024) void k_row_factor(const float *grad, const int *rows, const int *n_d, float tau, int f16,
-                                                     float *factor, float *scale) {
-    __shared__ float part[16];
+// Upstream values of their own for the kept rows, times the temperature.  fp16: one power of two for all of them (`scale`
+// undoes it), and where they spread by more than 2^4 one for each row's own (`own`), with which the logit gradients are made
+// a second time, for dH: of n_own[0] rows, while dH of the first ones is of n_own[1] (4099 rows of 768, 30522 terms: 885 us,
+// spread 1090).  Next to 2^11 even the mean probability of 2^20 terms stays among fp16's normal numbers,
+// next to 2^-4 of that too, but rows of smaller values would lose theirs (dW and db, sums over rows, lose nothing next to the
+// largest's).  undo[i] gives dH's row back.
+struct RowFactors {
+    float *factor, *scale;
+    float *own, *undo;  // fp16 alone
+    int *n_own;
+};
+__global__ __launch_bounds__(1024) void k_row_factor(const float *grad, const int *rows, const int *n_d, float tau, RowFactors o) {
+    __shared__ float part[2][16];
     const int n = *n_d;
-    float most = 0.f;
+    float most = 0.f, least = INFINITY;
     for (int i = threadIdx.x; i < n; i += 1024) {
-        const float f = grad[rows[i]] * tau;
-        factor[i] = f;
-        most = fmaxf(most, fabsf(f));
+        const float f = grad[rows[i]] * tau, a = fabsf(f);
+        o.factor[i] = f;
+        most = fmaxf(most, a);
+        if (a > 0.f) least = fminf(least, a);
     }
     float up = 1.f;
-    if (f16) {
-        most = wave_max(most);
-        if (gs_lane() == 0) part[threadIdx.x >> 6] = most;
+    if (o.own) {
+        most = wave_max(most), least = -wave_max(-least);
+        if (gs_lane() == 0) part[0][threadIdx.x >> 6] = most, part[1][threadIdx.x >> 6] = least;
         __syncthreads();
-        most = part[0];
-        for (int w = 1; w < 16; w++) most = fmaxf(most, part[w]);
-        if (most > 0.f && most < 3e38f) {
-            up = ldexpf(1.f, max(-120, min(120, 11 - ilogbf(most))));
-            for (int i = threadIdx.x; i < n; i += 1024) factor[i] *= up;
+        most = part[0][0], least = part[1][0];
+        for (int w = 1; w < 16; w++) most = fmaxf(most, part[0][w]), least = fminf(least, part[1][w]);
+        const bool in_range = most > 0.f && most < 3e38f, spread = in_range && least < most * 0.0625f;
+        if (in_range) up = ldexpf(1.f, max(-120, min(120, 11 - ilogbf(most))));
+        for (int i = threadIdx.x; i < n; i += 1024) {
+            const float f = o.factor[i];
+            const int e = fabsf(f) > 0.f && fabsf(f) < INFINITY ? ilogbf(f) : 11;  // 0 and NaN as they are
+            o.own[i] = ldexpf(f, 11 - e);
+            o.undo[i] = spread ? ldexpf(1.f, e - 11) : 1.f / up;
+            o.factor[i] = f * up;
         }
+        if (threadIdx.x == 0) o.n_own[0] = spread ? n : 0, o.n_own[1] = spread ? 0 : n;
     }
-    if (threadIdx.x == 0) *scale = 1.f / up;
+    if (threadIdx.x == 0) *o.scale = 1.f / up;
 }
 
 // The bias's gradient: the tiles' column sums added up in order.  `blocks` of them.
@@ -961,11 +978,11 @@ struct BiasSums {
 
 // Last launch of a gradient.  dH of every source row from its parts (0 for rows that are not kept): with few rows, and so
 // many parts, a workgroup of W = 16 waves takes 256 values of a row, the waves take parts in turn and are added in order; else
-// (W = 4) a wave does.  Then workgroups of 32 terms of the bias.  Bytes: 8192 rows of 1024 values, 54 us.
+// (W = 4) a wave does.  undo: a row's own scale, NULL: the upstream value's.  Then workgroups of 32 terms of the bias.  Bytes: 8192 rows of 1024 values, 54 us.
 template <class O, int W>
 __global__ __launch_bounds__(64 * W) void k_finish_grad(const float *part, const int *inv, const int *n_d, const int *parts_d,
-                                                        int total, int dim, int dimp, Upstream up, O *out, int hidden_blocks,
-                                                        BiasSums bias) {
+                                                        int total, int dim, int dimp, Upstream up, const float *undo, O *out,
+                                                        int hidden_blocks, BiasSums bias) {
     __shared__ f32x4 red[W][64];
     const int n = *n_d, lane = gs_lane(), wave = threadIdx.x >> 6;
     const float s = up.value();
@@ -995,7 +1012,7 @@ __global__ __launch_bounds__(64 * W) void k_finish_grad(const float *part, const
     const bool vec = (dim & 3) == 0;
     const int chunks = (dim + 255) / 256;
     const auto put = [&](int64_t r, int i, int d, f32x4 x) {
-        x *= i < 0 ? 0.f : s;  // an infinite value leaves rows that are not kept 0
+        x *= i < 0 ? 0.f : undo ? undo[i] : s;  // an infinite value leaves rows that are not kept 0
         O *to = out + r * dim + d;
         if (vec) store4(to, x);
         else
@@ -1768,11 +1785,13 @@ struct LossPlan {
     int most;            // parts of dH
     int64_t part_rows;   // rows of all of dH's parts
     int64_t sum_rows;    // rows of the bias's sums
+    bool f16;
 };
 
 LossPlan loss_plan(const gs_vocab_head *h, const gs_vocab_targets *t, int cus) {
     LossPlan p;
     p.l = layout_of(h);
+    p.f16 = h->type == GS_H_F16;
     p.top = t->teacher_ids_d ? t->top : 1;
     const int64_t per = (int64_t)(p.l.rows > 0 ? p.l.rows : 1) * p.l.planes * 2;
     int64_t most = (int64_t)kPieceBytes / per / kRowPad * kRowPad;
@@ -1834,14 +1853,18 @@ void take_loss_scratch(gs_arena &a, const LossPlan &p, const gs_vocab_targets *t
 }
 
 struct GradScratch {
-    float *factor, *scale, *sums, *part;
+    RowFactors rows;
+    float *sums, *part;
     int *parts;
     uint16_t *dl;
 };
 void take_grad_scratch(gs_arena &a, const LossPlan &p, GradScratch *s) {
-    s->factor = a.take<float>(p.l.rows);
-    s->scale = a.take<float>(64);
+    s->rows.factor = a.take<float>(p.l.rows);
+    s->rows.scale = a.take<float>(64);
+    s->rows.own = p.f16 ? a.take<float>(p.l.rows) : nullptr;
+    s->rows.undo = p.f16 ? a.take<float>(p.l.rows) : nullptr;
     s->parts = a.take<int>(64);
+    s->rows.n_own = s->parts + 1;
     s->sums = a.take<float>((size_t)p.sum_rows * p.l.vocabp);
     s->part = a.take<float>((size_t)p.part_rows * p.l.dimp);
     s->dl = a.take<uint16_t>((size_t)round_up(p.l.rows, kBlock) * p.l.planes * p.piece);
@@ -1885,7 +1908,7 @@ int run_sums(const gs_vocab_head *h, const LossPlan &p, const LossSaved &s, cons
 
 template <class T, int NP, class O>
 int run_grad(const gs_vocab_head *h, const LossPlan &p, const LossSaved &s, const GradScratch &g, float scale, const Upstream &up,
-             float power, bool want_dh, bool want_db, void *dw_d, int cus, hipStream_t st) {
+             const float *factor, const int *n, const int *n_dh, float power, bool want_dh, bool want_db, void *dw_d, int cus, hipStream_t st) {
     using S = typename T::store_t;
     const Operand w = weight_operand(p.l, s.c, h), hid = hidden_operand(p.l, s.c);
     const int64_t row = (int64_t)p.piece * kBlock;  // values of a row of blocks
@@ -1897,12 +1920,12 @@ int run_grad(const gs_vocab_head *h, const LossPlan &p, const LossSaved &s, cons
         wp.p += (int64_t)v0 * w.stride;
         const EpiHiddenPart eh{g.part, p.l.dimp, c > 0};
         const EpiWeightGrad<O> ew{(O *)dw_d + (int64_t)v0 * h->dim, up, h->dim, h->dim % 4 == 0};
-        const Dims de{nv, p.l.rows, p.l.dimp, s.c.n, 0, 1, 0};
-        const Dims dh{want_dh ? h->dim : 0, p.l.rows, nv, s.c.n, 0, 1, 0};
-        const Dims dw{dw_d ? h->dim : 0, nv, p.l.rows, s.c.n, 0, 0, 1}, none{0, 0, 0, s.c.n, 0, 0, 0};
+        const Dims de{nv, p.l.rows, p.l.dimp, n, 0, 1, 0};
+        const Dims dh{want_dh ? h->dim : 0, p.l.rows, nv, n_dh, 0, 1, 0};
+        const Dims dw{dw_d ? h->dim : 0, nv, p.l.rows, n, 0, 0, 1}, none{0, 0, 0, n, 0, 0, 0};
         int rc = GS_OK;
 #define GSV_EPI(SHARES) \
-    EpiLogitGrad<S, SHARES> { s.c.bias, scale, s.lse2, up.scale ? g.factor : nullptr, power, power == 2048.f ? 11.f : 0.f, entries_of(p, s), v0, g.dl, dl.stride, dl.plane, want_db ? g.sums : nullptr, p.l.vocabp }
+    EpiLogitGrad<S, SHARES> { s.c.bias, scale, s.lse2, factor, power, power == 2048.f ? 11.f : 0.f, entries_of(p, s), v0, g.dl, dl.stride, dl.plane, want_db ? g.sums : nullptr, p.l.vocabp }
 #define GSV_GRAD(TL)                                                                              \
     rc = s.share ? launch_product<TL<T, NP, false, false>>(wp, hid, de, GSV_EPI(true), cus, st)   \
                  : launch_product<TL<T, NP, false, false>>(wp, hid, de, GSV_EPI(false), cus, st)
@@ -2036,19 +2059,23 @@ extern "C" int gs_vocab_loss_grad(const gs_vocab_head *h, const gs_vocab_targets
     const hipStream_t s = gs_stream(stream);
     const int rows = p.l.rows;
     const float tau = tau_of(t);
-    const bool per_row = reduction == GS_REDUCE_NONE, f16 = h->type == GS_H_F16;
+    const bool per_row = reduction == GS_REDUCE_NONE, f16 = p.f16;
     if (per_row) {
-        hipLaunchKernelGGL(k_row_factor, dim3(1), dim3(1024), 0, s, grad_d, sv.c.rows, sv.c.n, tau, f16, g.factor, g.scale);
+        hipLaunchKernelGGL(k_row_factor, dim3(1), dim3(1024), 0, s, grad_d, sv.c.rows, sv.c.n, tau, g.rows);
         GS_CHECK_LAUNCH();
     }
     const float power = f16 && !per_row ? 2048.f : 1.f;
-    const Upstream up{grad_d, sv.c.n, reduction == GS_REDUCE_MEAN, tau / power, per_row ? g.scale : nullptr};
+    const Upstream up{grad_d, sv.c.n, reduction == GS_REDUCE_MEAN, tau / power, per_row ? g.rows.scale : nullptr};
     int rc = GS_OK;
     // without a kept row no launch has a tile but dW's, which writes its zeros
-#define GSV_RUN(T, NP, O) rc = run_grad<T, NP, O>(h, p, sv, g, kLog2e / tau, up, power, dhidden_d, dbias_d, dweight_d, cus, s)
-    if (h->type == GS_H_F32) GSV_RUN(Bf16, 3, float);
-    else if (f16) GSV_RUN(F16, 1, _Float16);
-    else GSV_RUN(Bf16, 1, __bf16);
+#define GSV_RUN(T, NP, O, FACTOR, N, N_DH, DB, DW) \
+    rc = run_grad<T, NP, O>(h, p, sv, g, kLog2e / tau, up, FACTOR, N, N_DH, power, dhidden_d, DB, DW, cus, s)
+    const bool own = per_row && f16 && dhidden_d;
+    const float *factor = per_row ? g.rows.factor : nullptr;
+    if (h->type == GS_H_F32) GSV_RUN(Bf16, 3, float, factor, sv.c.n, sv.c.n, dbias_d, dweight_d);
+    else if (f16) GSV_RUN(F16, 1, _Float16, factor, sv.c.n, own ? g.rows.n_own + 1 : sv.c.n, dbias_d, dweight_d);
+    else GSV_RUN(Bf16, 1, __bf16, factor, sv.c.n, sv.c.n, dbias_d, dweight_d);
+    if (own && !rc) GSV_RUN(F16, 1, _Float16, g.rows.own, g.rows.n_own, g.rows.n_own, false, nullptr);
 #undef GSV_RUN
     if (rc) return rc;
     const int64_t items = dhidden_d ? (int64_t)rows * ((h->dim + 255) / 256) : 0;
@@ -2059,7 +2086,7 @@ extern "C" int gs_vocab_loss_grad(const gs_vocab_head *h, const gs_vocab_targets
     const BiasSums bias{g.sums, p.l.vocabp, token_edge(p.l.cls), token_waves(p.l.cls), h->vocab, h->bias_type, dbias_d};
 #define GSV_FG(O, W)                                                                                                       \
     hipLaunchKernelGGL((k_finish_grad<O, W>), dim3(hidden_blocks + bias_blocks), dim3(64 * W), 0, s, g.part, sv.c.inv, sv.c.n, \
-                       g.parts, rows, h->dim, p.l.dimp, up, (O *)dhidden_d, hidden_blocks, bias)
+                       g.parts, rows, h->dim, p.l.dimp, up, own ? g.rows.undo : nullptr, (O *)dhidden_d, hidden_blocks, bias)
 #define GSV_FINISH(O)               \
     if (few) GSV_FG(O, 16);         \
     else GSV_FG(O, 4)

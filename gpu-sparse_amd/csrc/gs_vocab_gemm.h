@@ -427,7 +427,7 @@ struct Pairing {
     int piece;     // most columns of the second product
     int slots;     // workgroups
     int most;      // parts
-    int *parts_d;  // receives the parts; NULL: one, and there is no second product
+    int *parts_d;  // receives the parts (unless there are no rows); NULL: one, and there is no second product
 };
 
 // One or two products in a launch, persistent over their tiles.
@@ -441,14 +441,14 @@ __global__ __launch_bounds__(SA::tile::threads, SA::tile::waves_per_simd) void k
     const int lane = gs_lane(), wave = gs_uniform((int)threadIdx.x >> 6);
     const int wr = wave / TA::WC, wc = wave % TA::WC;
     const int n = A.d.n_d ? gs_uniform(*A.d.n_d) : 0;
-    const Shape a = shape_of<TA>(A.d, n), b = shape_of<TB>(B.d, n);
+    const Shape a = shape_of<TA>(A.d, n), b = shape_of<TB>(B.d, B.d.n_d ? gs_uniform(*B.d.n_d) : 0);
     int parts = 1, nb = 0;
     if (pair.parts_d) {
         nb = b.tr * b.tc;
         // from a whole piece's size, so that every piece has the same parts
         parts = parts_of((pair.piece + kStep - 1) / kStep, a.tr * a.tc, b.steps, b.tr * ((pair.piece + TB::BC - 1) / TB::BC),
                          pair.slots, pair.most);
-        if (blockIdx.x == 0 && threadIdx.x == 0) *pair.parts_d = parts;
+        if (blockIdx.x == 0 && threadIdx.x == 0 && n > 0) *pair.parts_d = parts;
     }
     const int xcds = gridDim.x >= 8 ? 8 : 1, xcd = blockIdx.x % xcds;
     const Share share(a.tr * a.tc * parts, nb, xcd, xcds);

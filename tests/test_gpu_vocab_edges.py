@@ -266,3 +266,32 @@ def test_infinite_hidden_states_and_vocabulary(device, dtype, texts, length, dim
     each = mag * (UT[dtype] * 1.01 + 2 * logit_error(*fine, b).amax() + 256 * U * big.max())
     terms = 6 * (texts * length + 16) * U
     assert_within(dw, dl.t() @ hid, each.t() @ hid.abs() + terms * mag.t() @ hid.abs() + UT[dtype] * 1.01 * (dl.t() @ hid).abs() + TINY[dtype], "dw")
+
+
+# ---------------------------------------------------------------- ranges of types
+
+
+@pytest.mark.parametrize("rows,vocab", [(30, 2000), (200, 2000), (600, 3000)])
+def test_fp16_rows_of_small_upstream_values_keep_their_gradients(device, rows, vocab):
+    """Upstream values of 2^12 to 2^-12, one per row: each row's logit gradients keep fp16's bits next to their own factor, so
+    that dH's error is relative to the row (an absolute part of 2^-36 of its factor), whatever the others' factors are."""
+    h, w, b = inputs(device, (rows, 64), vocab, F16, 93)
+    w = w.detach().abs().requires_grad_()                    # of one sign: what is lost does not cancel
+    t = torch.randint(0, vocab, (rows,), generator=torch.Generator().manual_seed(94)).to(device)
+    f = 2.0 ** torch.linspace(12, -12, rows, device=device)
+    f[1::2] *= -1
+    f[2], f[5] = 0.0, 1e-42
+    dh, dw, db = torch.autograd.grad(gs.vocab_loss(h, w, t, b, reduction="none"), [h, w, b], f)
+    x = logits64(h, w, b)
+    p, f64, one = x.softmax(1), f.double()[:, None], torch.nn.functional.one_hot(t, vocab).double()
+    W, H = w.detach().double(), h.detach().double()
+    ep = 2 * logit_error(h, w, b).amax(1) + 256 * U * (x.abs().amax(1) + math.log(vocab) + 1)
+    dl, mag = (p - one) * f64, (p + one) * f64.abs()
+    each = mag * (UT[F16] * 1.01 + ep[:, None])
+    own = 2.0 ** -36 * f64.abs().expand_as(p)
+    ref = dl @ W
+    assert_within(dh, ref, (each + own) @ W + (vocab + 16) * U * (mag @ W) + UT[F16] * 1.01 * ref.abs() + TINY[F16], "dh")
+    largest = 2.0 ** -36 * f64.abs().max()
+    for name, got, ref, m, e in (("dw", dw, dl.t() @ H, mag.t() @ H.abs(), (each + largest).t() @ H.abs()),
+                                 ("db", db, dl.sum(0), mag.sum(0), (each + largest).sum(0))):
+        assert_within(got, ref, e + (rows + 16) * U * m + UT[F16] * 1.01 * ref.abs() + TINY[F16], name)
