@@ -2055,7 +2055,7 @@ extern "C" int gs_vocab_loss_grad(const gs_vocab_head *h, const gs_vocab_targets
                      scratch_bytes);
         return GS_ENOSPC;
     }
-    if (int rc = check_data(h)) return rc;
+    GS_REQUIRE(h->weight_d, "NULL weight");
     const hipStream_t s = gs_stream(stream);
     const int rows = p.l.rows;
     const float tau = tau_of(t);

@@ -84,10 +84,11 @@ def _bytes(n: int, dev) -> torch.Tensor:
     return torch.empty(int(n), dtype=torch.uint8, device=dev)
 
 
-def _grads(ctx, hidden, weight, bias):
+def _grads(ctx, hidden_shape, weight, bias):
     """Empty gradients of the inputs that need one (hidden, weight, bias)."""
-    return [torch.empty(t.shape, dtype=t.dtype, device=t.device) if need else None
-            for t, need in zip((hidden, weight, bias), ctx.needs_input_grad[:3])]
+    return [torch.empty(shape, dtype=t.dtype, device=t.device) if need else None
+            for t, shape, need in zip((weight, weight, bias), (hidden_shape, weight.shape, None if bias is None else bias.shape),
+                                      ctx.needs_input_grad[:3])]
 
 
 def _kinds(*tensors):
@@ -149,7 +150,7 @@ class _TermWeights(torch.autograd.Function):
         hidden, weight, bias, weights, tokens = _unpack(ctx)
         weights, tokens = weights.contiguous(), tokens.contiguous()
         dev = hidden.device
-        dh, dw, db = _grads(ctx, hidden, weight, bias)
+        dh, dw, db = _grads(ctx, hidden.shape, weight, bias)
         L, head = _lib.lib(), _head(hidden, weight, bias)
         grad = _upstream(grad)
         with _on(dev):
@@ -189,7 +190,7 @@ def term_weights(hidden, weight, bias=None, *, mask=None, return_tokens: bool = 
 
 
 def _losses(hidden, weight, bias, ids, logits, ignore_index, temperature, reduction):
-    """The loss, what a gradient reads of the call (targets struct, saved bytes) and the bytes its workspace takes."""
+    """The loss, what a gradient reads of the call (head and targets structs, saved bytes) and the bytes its workspace takes."""
     dev = hidden.device
     head = _head(hidden, weight, bias)
     if logits is None:
@@ -207,30 +208,37 @@ def _losses(hidden, weight, bias, ids, logits, ignore_index, temperature, reduct
         saved, ws = _bytes(need.value, dev), _bytes(scratch.value, dev)
         _lib.check(L.gs_vocab_loss(C.byref(head), C.byref(targets), reduction, loss.data_ptr(), saved.data_ptr(),
                                    need.value, ws.data_ptr(), scratch.value, _lib.stream_ptr(dev)), "gs_vocab_loss")
-    return loss, targets, saved, grad_need.value
+    return loss, head, targets, saved, grad_need.value
 
 
 def _place(weight):
     return weight.stride(), weight.data_ptr() % SAVED_ALIGN
 
 
-def _as_loss_read_it(hidden, weight, bias, targets, saved_bytes):
+def _weight_to(head, weight):
+    head.weight_d, head.weight_row_stride, head.weight_dim_stride = weight.data_ptr(), weight.stride(0), weight.stride(1)
+
+
+def _as_loss_read_it(head, weight, targets, saved_bytes):
     """The weight as a gradient can read it: where it is, or from the copy among the saved bytes; where the loss made no copy
     and the weight came back in another layout, a contiguous one, as it was then."""
     need, other = C.c_size_t(), C.c_size_t()
-    with _on(hidden.device):
-        _lib.check(_lib.lib().gs_vocab_loss_workspace(C.byref(_head(hidden, weight, bias)), C.byref(targets), C.byref(need),
-                                                      C.byref(other), C.byref(other)), "gs_vocab_loss_workspace")
+    _weight_to(head, weight)
+    with _on(weight.device):
+        _lib.check(_lib.lib().gs_vocab_loss_workspace(C.byref(head), C.byref(targets), C.byref(need), C.byref(other),
+                                                      C.byref(other)), "gs_vocab_loss_workspace")
     return weight if need.value <= saved_bytes else weight.clone(memory_format=torch.contiguous_format)
 
 
 class _VocabLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, bias, ids, logits, ignore_index, temperature, reduction):
-        loss, ctx.targets, saved, ctx.grad_bytes = _losses(hidden, weight, bias, ids, logits, ignore_index, temperature,
-                                                           reduction)
-        ctx.save_for_backward(hidden, weight, bias, ids, logits, saved)
-        ctx.kinds = _kinds(hidden, weight, bias, ids, logits, saved)
+        loss, ctx.head, ctx.targets, saved, ctx.grad_bytes = _losses(hidden, weight, bias, ids, logits, ignore_index,
+                                                                     temperature, reduction)
+        # not the hidden states: what backward reads of them is among the saved bytes
+        ctx.save_for_backward(weight, bias, ids, logits, saved)
+        ctx.kinds = _kinds(weight, bias, ids, logits, saved)
+        ctx.hidden_shape = hidden.shape
         ctx.weight_at = _place(weight)
         ctx.reduction = reduction
         return loss
@@ -238,15 +246,17 @@ class _VocabLoss(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        hidden, weight, bias, _, _, saved = _unpack(ctx)
-        dev = hidden.device
+        weight, bias, _, _, saved = _unpack(ctx)
+        dev = weight.device
         if saved.data_ptr() % SAVED_ALIGN or not saved.is_contiguous():
             saved = saved.clone(memory_format=torch.contiguous_format)
+        head = _lib.GsVocabHead.from_buffer_copy(ctx.head)
+        head.hidden_d = None
         if _place(weight) != ctx.weight_at:
-            weight = _as_loss_read_it(hidden, weight, bias, ctx.targets, saved.numel())
-        dh, dw, db = _grads(ctx, hidden, weight, bias)
-        L, head = _lib.lib(), _head(hidden, weight, bias)
-        grad = _upstream(grad)
+            weight = _as_loss_read_it(head, weight, ctx.targets, saved.numel())
+        _weight_to(head, weight)
+        dh, dw, db = _grads(ctx, ctx.hidden_shape, weight, bias)
+        L, grad = _lib.lib(), _upstream(grad)
         with _on(dev):
             ws = _bytes(ctx.grad_bytes, dev)
             _lib.check(L.gs_vocab_loss_grad(C.byref(head), C.byref(ctx.targets), ctx.reduction, grad.data_ptr(),

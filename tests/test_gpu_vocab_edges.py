@@ -295,3 +295,22 @@ def test_fp16_rows_of_small_upstream_values_keep_their_gradients(device, rows, v
     for name, got, ref, m, e in (("dw", dw, dl.t() @ H, mag.t() @ H.abs(), (each + largest).t() @ H.abs()),
                                  ("db", db, dl.sum(0), mag.sum(0), (each + largest).sum(0))):
         assert_within(got, ref, e + (rows + 16) * U * m + UT[F16] * 1.01 * ref.abs() + TINY[F16], name)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_a_loss_does_not_hold_its_hidden_states(device, dtype):
+    """Its gradient reads its own copy of the kept rows: the hidden states may be freed or written over."""
+    h, w, b = (x.detach() for x in inputs(device, (70, 128), 900, dtype, 77))
+    for name, call in _head_calls(device, 900).items():
+        if name == "term_weights":
+            continue
+        args = [x.clone().requires_grad_() for x in (h, w, b)]
+        want = torch.autograd.grad(call(*args), args)
+        kept = []
+        with torch.autograd.graph.saved_tensors_hooks(lambda x: kept.append(x.data_ptr()) or x, lambda x: x):
+            loss = call(*args)
+        assert args[0].data_ptr() not in kept and args[1].data_ptr() in kept
+        with torch.no_grad():
+            args[0].fill_(NAN)
+        for got, ref in zip(torch.autograd.grad(loss, args), want):
+            assert torch.equal(got, ref), name
