@@ -1687,6 +1687,13 @@ int check_head(const gs_vocab_head *h) {
     return GS_OK;
 }
 
+// Of term weights, which have a grid row per text
+int check_texts(const gs_vocab_head *h) {
+    if (int rc = check_head(h)) return rc;
+    GS_REQUIRE(h->texts <= 65535, "texts=%d exceed 65535", h->texts);
+    return GS_OK;
+}
+
 // What a call that launches reads of a head
 int check_data(const gs_vocab_head *h) {
     GS_REQUIRE(h->weight_d && (h->hidden_d || (int64_t)h->texts * h->length == 0), "NULL hidden states or weight");
@@ -2182,7 +2189,7 @@ int run_entries(const gs_vocab_head *h, const float *grad_d, const float *weight
 }  // namespace gsv
 
 extern "C" int gs_term_weights_workspace(const gs_vocab_head *h, int32_t tokens, size_t *bytes, size_t *grad_bytes) {
-    if (int rc = check_head(h)) return rc;
+    if (int rc = check_texts(h)) return rc;
     GS_REQUIRE(bytes && grad_bytes, "NULL size pointer");
     const Layout l = layout_of(h);
     gs_arena a{nullptr, 0, 0}, b{nullptr, 0, 0};
@@ -2200,7 +2207,7 @@ extern "C" int gs_term_weights_workspace(const gs_vocab_head *h, int32_t tokens,
 
 extern "C" int gs_term_weights(const gs_vocab_head *h, const uint8_t *mask_d, float *weights_d, int32_t *tokens_d,
                                void *workspace_d, size_t workspace_bytes, void *stream) {
-    if (int rc = check_head(h)) return rc;
+    if (int rc = check_texts(h)) return rc;
     int cus = 0;
     if (int rc = cu_count(&cus)) return rc;
     const Layout l = layout_of(h);
@@ -2218,7 +2225,6 @@ extern "C" int gs_term_weights(const gs_vocab_head *h, const uint8_t *mask_d, fl
     if (h->texts == 0) return GS_OK;
     if (int rc = check_data(h)) return rc;
     GS_REQUIRE(weights_d && workspace_d, "NULL weights or workspace");
-    GS_REQUIRE(h->texts <= 65535, "texts=%d exceed 65535", h->texts);
     const hipStream_t s = gs_stream(stream);
     if (l.rows == 0) {  // texts without tokens
         const int64_t n = (int64_t)h->texts * h->vocab;
@@ -2283,8 +2289,7 @@ extern "C" int gs_term_weights(const gs_vocab_head *h, const uint8_t *mask_d, fl
 extern "C" int gs_term_weights_grad(const gs_vocab_head *h, const float *grad_d, const float *weights_d, const int32_t *tokens_d,
                                     void *dhidden_d, void *dweight_d, void *dbias_d, void *workspace_d, size_t workspace_bytes,
                                     void *stream) {
-    if (int rc = check_head(h)) return rc;
-    GS_REQUIRE(h->texts <= 65535, "texts=%d exceed 65535", h->texts);
+    if (int rc = check_texts(h)) return rc;
     gs_arena a{(char *)workspace_d, 0, workspace_bytes};
     EntryPlan p;
     take_entries(a, h, &p);

@@ -406,7 +406,7 @@ int gs_scatter_add(const gs_index *index, const int64_t *lo_d, const int64_t *hi
  *
  * hidden is [texts][length][dim] with any element strides (rows of a loss: texts = 1), weight [vocab][dim] with
  * any element strides; both of `type`.  bias is [vocab] of `bias_type`, or NULL.  Sums are fp32.
- * texts * length <= 2^28, dim <= 32768, vocab <= 2^20. */
+ * texts * length <= 2^28, dim <= 32768, vocab <= 2^20; of term weights, texts <= 65535. */
 #define GS_H_F32 0
 #define GS_H_F16 1
 #define GS_H_BF16 2

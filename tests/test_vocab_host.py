@@ -74,3 +74,16 @@ def test_missing_tensors_are_refused(over, given, match):
     assert L.gs_term_weights_workspace(h, 1, C.byref(a), C.byref(b)) == _lib.GS_OK
     with pytest.raises(ValueError, match=match):
         _lib.check(L.gs_term_weights_grad(h, given, given, given, None, None, None, 8, b.value, None), "gs_term_weights_grad")
+
+
+def test_more_texts_than_a_grid_has_rows_are_refused():
+    """65535 texts of term weights at most, refused before a workspace is asked for; a loss's rows are one text."""
+    L = _lib.lib()
+    a, b, c = C.c_size_t(), C.c_size_t(), C.c_size_t()
+    assert L.gs_term_weights_workspace(C.byref(head(texts=65535)), 0, C.byref(a), C.byref(b)) == _lib.GS_OK
+    many = C.byref(head(texts=65536, length=1))
+    for call in (lambda: L.gs_term_weights_workspace(many, 0, C.byref(a), C.byref(b)),
+                 lambda: L.gs_term_weights(many, None, 8, None, 8, 1 << 40, None),
+                 lambda: L.gs_term_weights_grad(many, 8, 8, 8, 8, 8, 8, 8, 1 << 40, None)):
+        with pytest.raises(ValueError, match="texts=65536 exceed 65535"):
+            _lib.check(call(), "call")
