@@ -314,3 +314,84 @@ def test_a_loss_does_not_hold_its_hidden_states(device, dtype):
             args[0].fill_(NAN)
         for got, ref in zip(torch.autograd.grad(loss, args), want):
             assert torch.equal(got, ref), name
+
+
+PIECES = [
+    # rows, dim, vocab, type, top, reduction: more than 2^30 bytes of logit gradients
+    (33000, 64, 20000, BF16, 7, "mean"),
+    (33000, 64, 20000, F16, 0, "none"),
+    (11000, 64, 20000, F32, 0, "mean"),
+    (11000, 72, 20000, F32, 5, "none"),
+]
+
+
+@pytest.mark.parametrize("rows,dim,vocab,dtype,top,reduction", PIECES)
+def test_a_vocabulary_in_pieces_of_every_kind(device, rows, dim, vocab, dtype, top, reduction):
+    """Entries of a teacher, three planes, fp16's powers of two and factors per row, across the pieces' border."""
+    print(f"pieces rows {rows} {dtype} top {top} {reduction}", flush=True)
+    h, w, b = inputs(device, (rows, dim), vocab, dtype, 97)
+    g = torch.Generator().manual_seed(98)
+    tau = 2.0 if top else 1.0
+    if top:
+        ids = ((torch.randint(0, vocab, (rows, 1), generator=g) + vocab // top * torch.arange(top)) % vocab).to(device)
+        z = torch.randn((rows, top), generator=g).to(device)
+        q = (z.double() / tau).softmax(1)
+        loss = gs.distill_loss(h, w, ids, z, b, temperature=tau, reduction=reduction)
+    else:
+        ids = torch.randint(0, vocab, (rows, 1), generator=g).to(device)
+        q = torch.ones((rows, 1), dtype=torch.float64, device=device)
+        loss = gs.vocab_loss(h, w, ids[:, 0], b, reduction=reduction)
+    up = torch.randn(rows, generator=g).to(device) if reduction == "none" else torch.ones((), device=device)
+    dh, dw, db = torch.autograd.grad(loss, [h, w, b], up)
+    f = (up.double() if reduction == "none" else torch.full((rows,), 1.0 / rows, dtype=torch.float64, device=device)) * tau
+    W, H = w.detach().double(), h.detach().double()
+    rw, rb, ew, eb = torch.zeros_like(W), torch.zeros_like(b, dtype=torch.float64), torch.zeros_like(W), torch.zeros_like(b, dtype=torch.float64)
+    six = 6 if dtype == F32 else 1
+    floor = 2.0 ** -36 * float(f.abs().max()) if dtype == F16 else 0.0
+    for r in range(0, rows, 2048):
+        s = slice(r, r + 2048)
+        x = logits64(h[s], w, b) / tau
+        p = x.softmax(1)
+        d = p.scatter_add(1, ids[s], -q[s]) * f[s, None]
+        m = p.scatter_add(1, ids[s], q[s]) * f[s, None].abs()
+        ep = 2 * logit_error(h[s], w, b).amax(1) / tau + 256 * U * (x.abs().amax(1) + math.log(vocab) + 1)
+        e = m * (UT[dtype] * 1.01 + ep[:, None]) + floor
+        ref = d @ W
+        assert_within(dh[s], ref, e @ W.abs() + (vocab * six + 16) * U * (m @ W.abs()) + UT[dtype] * 1.01 * ref.abs() + TINY[dtype], "dh")
+        rw += d.t() @ H[s]
+        rb += d.sum(0)
+        e += (rows * six + 16) * U * m
+        ew += e.t() @ H[s].abs()
+        eb += e.sum(0)
+    assert_within(dw, rw, ew + UT[dtype] * 1.01 * rw.abs() + TINY[dtype], "dw")
+    assert_within(db, rb, eb + UT[dtype] * 1.01 * rb.abs() + TINY[dtype], "db")
+
+
+def test_two_host_threads(device):
+    """Two threads, each on a stream of its own, get the results of one."""
+    import threading
+    h, w, b = (x.detach() for x in inputs(device, (12, 60, 128), 3000, BF16, 99))
+    t = torch.randint(0, 3000, (12, 60), generator=torch.Generator().manual_seed(100)).to(device)
+
+    def run():
+        args = [x.clone().requires_grad_() for x in (h, w, b)]
+        loss, weights = gs.vocab_loss(args[0], args[1], t, args[2]), gs.term_weights(*args)
+        return [loss.detach(), weights.detach(), *torch.autograd.grad(loss + weights.sum(), args)]
+
+    want = run()
+    torch.cuda.synchronize(device)
+    results = {}
+
+    def work(k):
+        with torch.cuda.stream(torch.cuda.Stream(device)):
+            results[k] = [run() for _ in range(5)]
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for x in threads:
+        x.start()
+    for x in threads:
+        x.join()
+    for k in range(2):
+        for got in results[k]:
+            assert all(torch.equal(x, y) for x, y in zip(got, want))
