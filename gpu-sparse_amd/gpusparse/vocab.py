@@ -236,9 +236,9 @@ class _VocabLoss(torch.autograd.Function):
     def forward(ctx, hidden, weight, bias, ids, logits, ignore_index, temperature, reduction):
         loss, ctx.head, ctx.targets, saved, ctx.grad_bytes = _losses(hidden, weight, bias, ids, logits, ignore_index,
                                                                      temperature, reduction)
-        # not the hidden states: what backward reads of them is among the saved bytes
-        ctx.save_for_backward(weight, bias, ids, logits, saved)
-        ctx.kinds = _kinds(weight, bias, ids, logits, saved)
+        # not the hidden states, nor the targets: what backward reads of them is among the saved bytes
+        ctx.save_for_backward(weight, bias, saved)
+        ctx.kinds = _kinds(weight, bias, saved)
         ctx.hidden_shape = hidden.shape
         ctx.weight_at = _place(weight)
         ctx.reduction = reduction
@@ -247,7 +247,7 @@ class _VocabLoss(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        weight, bias, _, _, saved = _unpack(ctx)
+        weight, bias, saved = _unpack(ctx)
         dev = weight.device
         if saved.data_ptr() % SAVED_ALIGN or not saved.is_contiguous():
             saved = saved.clone(memory_format=torch.contiguous_format)

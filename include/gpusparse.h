@@ -455,9 +455,10 @@ typedef struct gs_vocab_targets {
 
 /* loss = lse(l) - l[target], or temperature^2 sum_k q_k (log q_k - log p[id_k]) with q = softmax(teacher logits /
  * temperature) over the row's ids and p = softmax(l / temperature) over the vocabulary.  saved_d is what the gradient
- * needs besides the weight (it does not read hidden_d, which may be NULL then), and after that the weight again when it is not laid out as the product reads it.  The gradient
- * may be given the weight elsewhere and in other strides; where it could be read in place in gs_vocab_loss and no longer
- * can, saved_bytes is too small and the call is refused. */
+ * needs besides the weight (it reads neither hidden_d, which may be NULL then, nor what targets point to), and after that
+ * the weight again when it is not laid out as the product reads it.  The gradient may be given the weight elsewhere and in
+ * other strides; where it could be read in place in gs_vocab_loss and no longer can, saved_bytes is too small and the call
+ * is refused. */
 int gs_vocab_loss_workspace(const gs_vocab_head *head, const gs_vocab_targets *targets, size_t *saved_bytes,
                             size_t *scratch_bytes, size_t *grad_bytes);
 int gs_vocab_loss(const gs_vocab_head *head, const gs_vocab_targets *targets, int32_t reduction, float *loss_d,

@@ -298,8 +298,8 @@ def test_fp16_rows_of_small_upstream_values_keep_their_gradients(device, rows, v
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
-def test_a_loss_does_not_hold_its_hidden_states(device, dtype):
-    """Its gradient reads its own copy of the kept rows: the hidden states may be freed or written over."""
+def test_a_loss_does_not_hold_its_hidden_states_or_targets(device, dtype):
+    """Its gradient reads its own copy of the kept rows: the hidden states and targets may be freed or written over."""
     h, w, b = (x.detach() for x in inputs(device, (70, 128), 900, dtype, 77))
     for name, call in _head_calls(device, 900).items():
         if name == "term_weights":
@@ -309,7 +309,7 @@ def test_a_loss_does_not_hold_its_hidden_states(device, dtype):
         kept = []
         with torch.autograd.graph.saved_tensors_hooks(lambda x: kept.append(x.data_ptr()) or x, lambda x: x):
             loss = call(*args)
-        assert args[0].data_ptr() not in kept and args[1].data_ptr() in kept
+        assert len(kept) == 3 and args[0].data_ptr() not in kept and args[1].data_ptr() in kept  # weight, bias, its own
         with torch.no_grad():
             args[0].fill_(NAN)
         for got, ref in zip(torch.autograd.grad(loss, args), want):
