@@ -63,21 +63,38 @@ __device__ __forceinline__ uint16_t bits16(float x) {
     return __builtin_bit_cast(uint16_t, (T)x);
 }
 
-// x as bf16 planes, each the nearest to what is left.  A value beyond the largest bf16 value (0x7F7F) takes that for its first,
-// not the infinity that is nearer.  An infinity is (+-1, 0, +-inf): a third plane meets first planes alone, which are 0 where
-// their value is and else have its sign, so that the pair makes the infinity (or NaN) of an fp32 product, and the other
-// pairs finite values that it swallows; as a first plane it would meet 0 and either sign in the other planes.
-__device__ __forceinline__ void split3(float x, uint16_t (&p)[3]) {
-    const bool fin = fabsf(x) < INFINITY;
-    const float most = __uint_as_float(0x7F7F0000u);
-    const __bf16 a = (__bf16)(fin ? fminf(fmaxf(x, -most), most) : x);
-    const float r = x - (float)a;
-    const __bf16 b = (__bf16)r;
-    const __bf16 c = (__bf16)(r - (float)b);
-    const bool nan = x != x;
-    p[0] = fin || nan ? __builtin_bit_cast(uint16_t, a) : (__float_as_uint(x) >> 16 & 0x8000) | 0x3F80;
-    p[1] = fin ? __builtin_bit_cast(uint16_t, b) : 0;
-    p[2] = fin ? __builtin_bit_cast(uint16_t, c) : nan ? 0 : __float_as_uint(x) >> 16;
+// Values as bf16 planes, each the nearest to what is left.  One beyond the largest bf16 value takes that for its first, not the
+// infinity that is nearer.  An infinity is (+-1, 0, +-inf): a third plane meets first planes alone, which are 0 where their
+// value is and else have its sign, so that the pair makes the infinity (or NaN) of an fp32 product, and the other pairs
+// finite values that it swallows; as a first plane it would meet 0 and either sign in the other planes.  (Such values are
+// looked for together: one by one they cost a loss of 77 rows 7 us of 202.)
+template <int N>
+__device__ __forceinline__ void split3(const float (&x)[N], uint16_t (&p)[3][N]) {
+    constexpr float most = 0x1.fep127f;  // 0x7F7F
+    float top = 0.f;
+#pragma unroll
+    for (int e = 0; e < N; e++) {
+        const __bf16 a = (__bf16)x[e];
+        const float r = x[e] - (float)a;
+        const __bf16 b = (__bf16)r;
+        p[0][e] = __builtin_bit_cast(uint16_t, a);
+        p[1][e] = __builtin_bit_cast(uint16_t, b);
+        p[2][e] = __builtin_bit_cast(uint16_t, (__bf16)(r - (float)b));
+        top = fmaxf(top, fabsf(x[e]));
+    }
+    if (__builtin_expect(top > most, 0)) {
+#pragma unroll
+        for (int e = 0; e < N; e++) {
+            if (!(fabsf(x[e]) > most)) continue;
+            const uint32_t sign = __float_as_uint(x[e]) >> 16 & 0x8000;
+            const bool infinite = fabsf(x[e]) == INFINITY;
+            const float r = fabsf(x[e]) - most;  // of at most 16 bits
+            const __bf16 b = (__bf16)r;
+            p[0][e] = sign | (infinite ? 0x3F80 : 0x7F7F);
+            p[1][e] = sign | (infinite ? 0 : __builtin_bit_cast(uint16_t, b));
+            p[2][e] = infinite ? sign | 0x7F80 : sign ^ __builtin_bit_cast(uint16_t, (__bf16)(r - (float)b));
+        }
+    }
 }
 
 template <class T, int NP>
@@ -86,15 +103,12 @@ __device__ __forceinline__ void store_planes4(uint16_t *row, int64_t plane, int 
         *reinterpret_cast<Four<uint16_t> *>(row + d) =
             Four<uint16_t>{{bits16<T>(x[0]), bits16<T>(x[1]), bits16<T>(x[2]), bits16<T>(x[3])}};
     } else {
-        Four<uint16_t> o[3];
+        const float v[4] = {x[0], x[1], x[2], x[3]};
+        uint16_t p[3][4];
+        split3(v, p);
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            uint16_t p[3];
-            split3(x[e], p);
-            o[0].v[e] = p[0], o[1].v[e] = p[1], o[2].v[e] = p[2];
-        }
-#pragma unroll
-        for (int i = 0; i < 3; i++) *reinterpret_cast<Four<uint16_t> *>(row + i * plane + d) = o[i];
+        for (int i = 0; i < 3; i++)
+            *reinterpret_cast<Four<uint16_t> *>(row + i * plane + d) = Four<uint16_t>{{p[i][0], p[i][1], p[i][2], p[i][3]}};
     }
 }
 
@@ -104,16 +118,12 @@ __device__ __forceinline__ void store_planes4(uint16_t *row, int64_t plane, int 
 template <class T, int NP>
 __device__ __forceinline__ void store_blocks(uint16_t *to, int64_t plane, f32x4 a, f32x4 b) {
     uint16_t x[NP][8];
+    const float all[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+    if constexpr (NP == 1) {
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-        const float v = e < 4 ? a[e & 3] : b[e & 3];
-        if constexpr (NP == 1) {
-            x[0][e] = bits16<T>(v);
-        } else {
-            uint16_t s[3];
-            split3(v, s);
-            x[0][e] = s[0], x[1][e] = s[1], x[2][e] = s[2];
-        }
+        for (int e = 0; e < 8; e++) x[0][e] = bits16<T>(all[e]);
+    } else {
+        split3(all, x);
     }
 #pragma unroll
     for (int i = 0; i < NP; i++) {
