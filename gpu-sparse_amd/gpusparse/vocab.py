@@ -85,26 +85,33 @@ def _bytes(n: int, dev) -> torch.Tensor:
     return torch.empty(int(n), dtype=torch.uint8, device=dev)
 
 
-def _grads(ctx, hidden_shape, weight, bias):
+def _grads(ctx, hidden_shape, weight, dev):
     """Empty gradients of the inputs that need one (hidden, weight, bias)."""
-    return [torch.empty(shape, dtype=t.dtype, device=t.device) if need else None
-            for t, shape, need in zip((weight, weight, bias), (hidden_shape, weight.shape, None if bias is None else bias.shape),
-                                      ctx.needs_input_grad[:3])]
+    needs, vocab = ctx.needs_input_grad, weight.shape[0]
+    return (torch.empty(hidden_shape, dtype=weight.dtype, device=dev) if needs[0] else None,
+            torch.empty(weight.shape, dtype=weight.dtype, device=dev) if needs[1] else None,
+            torch.empty(vocab, dtype=ctx.bias_dtype, device=dev) if needs[2] else None)
 
 
-def _kinds(*tensors):
-    return [None if t is None else (t.shape, t.dtype, t.device) for t in tensors]
+def _save(ctx, bias, *tensors):
+    ctx.save_for_backward(*tensors)
+    ctx.at = [(t.data_ptr(), t.shape, t.stride(), t.dtype) for t in tensors]
+    ctx.dev = tensors[0].device
+    ctx.bias_dtype = None if bias is None else bias.dtype
 
 
 def _unpack(ctx):
-    """The saved tensors.  Hooks on them (offloading, packing) may bring them back at other addresses and in other strides,
-    which what reads them has to bear, but not as tensors of another kind, whose memory the kernels would misread."""
+    """The saved tensors, and whether they are where they were.  Hooks on them (offloading, packing) may bring them back at
+    other addresses and in other strides, which what reads them has to bear, but not as tensors of another kind, whose memory
+    the kernels would misread."""
     saved = ctx.saved_tensors
-    for t, kind in zip(saved, ctx.kinds):
-        if t is not None and (t.shape, t.dtype, t.device) != kind:
+    if [(t.data_ptr(), t.shape, t.stride(), t.dtype) for t in saved] == ctx.at:
+        return saved, True
+    for t, (_, shape, _, dtype) in zip(saved, ctx.at):
+        if (t.shape, t.dtype, t.device) != (shape, dtype, ctx.dev):
             raise RuntimeError(f"a saved tensor came back as {t.dtype} {tuple(t.shape)} on {t.device}, not as "
-                               f"{kind[1]} {tuple(kind[0])} on {kind[2]}")
-    return saved
+                               f"{dtype} {tuple(shape)} on {ctx.dev}")
+    return saved, False
 
 
 def _differentiable(*inputs) -> bool:
@@ -117,7 +124,7 @@ def _differentiable(*inputs) -> bool:
 
 
 def _weights(hidden, weight, bias, mask, want_tokens: bool):
-    """Weights, tokens or None, and the bytes that a gradient's workspace takes."""
+    """Weights, tokens or None, the call's head struct, and the bytes that a gradient's workspace takes."""
     dev = hidden.device
     texts, vocab = hidden.shape[0], weight.shape[0]
     weights = torch.empty((texts, vocab), dtype=torch.float32, device=dev)
@@ -130,15 +137,14 @@ def _weights(hidden, weight, bias, mask, want_tokens: bool):
         ws = _bytes(need.value, dev)
         _lib.check(L.gs_term_weights(C.byref(head), _lib.ptr(mask), weights.data_ptr(), _lib.ptr(tokens), ws.data_ptr(),
                                      need.value, _lib.stream_ptr(dev)), "gs_term_weights")
-    return weights, tokens, grad_need.value
+    return weights, tokens, head, grad_need.value
 
 
 class _TermWeights(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, bias, mask):
-        weights, tokens, ctx.grad_bytes = _weights(hidden, weight, bias, mask, True)
-        ctx.save_for_backward(hidden, weight, bias, weights, tokens)
-        ctx.kinds = _kinds(hidden, weight, bias, weights, tokens)
+        weights, tokens, ctx.head, ctx.grad_bytes = _weights(hidden, weight, bias, mask, True)
+        _save(ctx, bias, hidden, weight, weights, tokens)
         ctx.set_materialize_grads(False)
         ctx.mark_non_differentiable(tokens)
         return weights, tokens
@@ -148,12 +154,16 @@ class _TermWeights(torch.autograd.Function):
     def backward(ctx, grad, _):
         if grad is None:
             return None, None, None, None
-        hidden, weight, bias, weights, tokens = _unpack(ctx)
-        weights, tokens = weights.contiguous(), tokens.contiguous()
-        dev = hidden.device
-        dh, dw, db = _grads(ctx, hidden.shape, weight, bias)
-        L, head = _lib.lib(), _head(hidden, weight, bias)
-        grad = _upstream(grad)
+        (hidden, weight, weights, tokens), still = _unpack(ctx)
+        head = ctx.head
+        if not still:
+            weights, tokens = weights.contiguous(), tokens.contiguous()
+            head = _moved(head, weight)
+            head.hidden_d = hidden.data_ptr()
+            head.hidden_text_stride, head.hidden_row_stride, head.hidden_dim_stride = hidden.stride()
+        dev = ctx.dev
+        dh, dw, db = _grads(ctx, hidden.shape, weight, dev)
+        L, grad = _lib.lib(), _upstream(grad)
         with _on(dev):
             ws = _bytes(ctx.grad_bytes, dev)
             _lib.check(L.gs_term_weights_grad(C.byref(head), grad.data_ptr(), weights.data_ptr(), tokens.data_ptr(),
@@ -186,7 +196,7 @@ def term_weights(hidden, weight, bias=None, *, mask=None, return_tokens: bool = 
     if _differentiable(hidden, weight, bias):
         weights, tokens = _TermWeights.apply(hidden, weight, bias, mask)
     else:
-        weights, tokens, _ = _weights(hidden, weight, bias, mask, bool(return_tokens))
+        weights, tokens, _, _ = _weights(hidden, weight, bias, mask, bool(return_tokens))
     return (weights, tokens) if return_tokens else weights
 
 
@@ -212,23 +222,25 @@ def _losses(hidden, weight, bias, ids, logits, ignore_index, temperature, reduct
     return loss, head, targets, saved, grad_need.value
 
 
-def _place(weight):
-    return weight.stride(), weight.data_ptr() % SAVED_ALIGN
-
-
-def _weight_to(head, weight):
+def _moved(head, weight):
+    """The head with its weight where it is now."""
+    head = _lib.GsVocabHead.from_buffer_copy(head)
     head.weight_d, head.weight_row_stride, head.weight_dim_stride = weight.data_ptr(), weight.stride(0), weight.stride(1)
+    return head
 
 
 def _as_loss_read_it(head, weight, targets, saved_bytes):
-    """The weight as a gradient can read it: where it is, or from the copy among the saved bytes; where the loss made no copy
-    and the weight came back in another layout, a contiguous one, as it was then."""
+    """The head and the weight, moved, as a gradient can read it: where it is, or from the copy among the saved bytes; where the
+    loss made no copy and the weight came back in another layout, a contiguous one, as it was then."""
     need, other = C.c_size_t(), C.c_size_t()
-    _weight_to(head, weight)
+    head = _moved(head, weight)
     with _on(weight.device):
         _lib.check(_lib.lib().gs_vocab_loss_workspace(C.byref(head), C.byref(targets), C.byref(need), C.byref(other),
                                                       C.byref(other)), "gs_vocab_loss_workspace")
-    return weight if need.value <= saved_bytes else weight.clone(memory_format=torch.contiguous_format)
+    if need.value > saved_bytes:
+        weight = weight.clone(memory_format=torch.contiguous_format)
+        head = _moved(head, weight)
+    return head, weight
 
 
 class _VocabLoss(torch.autograd.Function):
@@ -237,26 +249,22 @@ class _VocabLoss(torch.autograd.Function):
         loss, ctx.head, ctx.targets, saved, ctx.grad_bytes = _losses(hidden, weight, bias, ids, logits, ignore_index,
                                                                      temperature, reduction)
         # not the hidden states, nor the targets: what backward reads of them is among the saved bytes
-        ctx.save_for_backward(weight, bias, saved)
-        ctx.kinds = _kinds(weight, bias, saved)
+        _save(ctx, bias, weight, saved)
         ctx.hidden_shape = hidden.shape
-        ctx.weight_at = _place(weight)
         ctx.reduction = reduction
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        weight, bias, saved = _unpack(ctx)
-        dev = weight.device
-        if saved.data_ptr() % SAVED_ALIGN or not saved.is_contiguous():
-            saved = saved.clone(memory_format=torch.contiguous_format)
-        head = _lib.GsVocabHead.from_buffer_copy(ctx.head)
-        head.hidden_d = None
-        if _place(weight) != ctx.weight_at:
-            weight = _as_loss_read_it(head, weight, ctx.targets, saved.numel())
-        _weight_to(head, weight)
-        dh, dw, db = _grads(ctx, ctx.hidden_shape, weight, bias)
+        (weight, saved), still = _unpack(ctx)
+        head = ctx.head
+        if not still:
+            if saved.data_ptr() % SAVED_ALIGN or not saved.is_contiguous():
+                saved = saved.clone(memory_format=torch.contiguous_format)
+            head, weight = _as_loss_read_it(head, weight, ctx.targets, saved.numel())
+        dev = ctx.dev
+        dh, dw, db = _grads(ctx, ctx.hidden_shape, weight, dev)
         L, grad = _lib.lib(), _upstream(grad)
         with _on(dev):
             ws = _bytes(ctx.grad_bytes, dev)

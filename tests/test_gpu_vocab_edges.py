@@ -309,7 +309,7 @@ def test_a_loss_does_not_hold_its_hidden_states_or_targets(device, dtype):
         kept = []
         with torch.autograd.graph.saved_tensors_hooks(lambda x: kept.append(x.data_ptr()) or x, lambda x: x):
             loss = call(*args)
-        assert len(kept) == 3 and args[0].data_ptr() not in kept and args[1].data_ptr() in kept  # weight, bias, its own
+        assert len(kept) == 2 and args[0].data_ptr() not in kept and args[1].data_ptr() in kept  # the weight, its own
         with torch.no_grad():
             args[0].fill_(NAN)
         for got, ref in zip(torch.autograd.grad(loss, args), want):
