@@ -395,3 +395,38 @@ def test_two_host_threads(device):
     for k in range(2):
         for got in results[k]:
             assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+def test_calls_in_a_graph(device):
+    """Captured once and replayed between eager calls: losses, weights and gradients of what the inputs hold by then."""
+    h, w, b = (x.detach() for x in inputs(device, (6, 40, 128), 2000, BF16, 101))
+    t = torch.randint(0, 2000, (6, 40), generator=torch.Generator().manual_seed(102)).to(device)
+    ids = torch.randint(0, 2000, (6, 40, 5), generator=torch.Generator().manual_seed(103)).to(device)
+    z = torch.randn((6, 40, 5), generator=torch.Generator().manual_seed(104)).to(device)
+    args = [x.clone().requires_grad_() for x in (h, w, b)]
+    one, ones = torch.ones((), device=device), torch.ones((6, 2000), device=device)
+
+    def run():
+        calls = ((gs.vocab_loss(args[0], args[1], t, args[2]), one), (gs.distill_loss(args[0], args[1], ids, z, args[2]), one),
+                 (gs.term_weights(*args), ones))
+        return [y for x, up in calls for y in (x.detach(), *torch.autograd.grad(x, args, up))]
+
+    side = torch.cuda.Stream(device)
+    side.wait_stream(torch.cuda.current_stream(device))
+    with torch.cuda.stream(side):
+        for _ in range(3):
+            run()
+    torch.cuda.current_stream(device).wait_stream(side)
+    torch.cuda.synchronize(device)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run()
+    for scale in (1.0, -0.5, 0.25, 2.0):
+        with torch.no_grad():
+            args[0].copy_(h * scale)
+        want = run()
+        torch.cuda.synchronize(device)
+        graph.replay()
+        torch.cuda.synchronize(device)
+        for got, ref in zip(out, want):
+            assert torch.equal(got, ref)
