@@ -414,7 +414,7 @@ struct TargetRows {
 
 // Second launch of a call, a wave per row: the kept hidden states and, where the product cannot read it in place
 // (w_rows > 0), the vocabulary as contiguous 16-bit rows (fp32: three planes), zero to a multiple of kStep values; and the
-// kept rows' targets.  Bytes: 77 rows and 30522 terms of 384 fp32 values, 119 MB in 22 us (5.4 TB/s).
+// kept rows' targets.  Bytes: 77 rows and 30522 terms of 384 fp32 values, 117 MB in 22.7 us (5.2 TB/s).
 template <int HT, int NP>
 __global__ __launch_bounds__(256) void k_pack(Source h, const int *rows, const int *n_d, uint16_t *h_out, Source w, int w_rows,
                                               uint16_t *w_out, int dimp, TargetRows targets, TeacherRows teacher) {
@@ -536,7 +536,7 @@ __device__ __forceinline__ void add_row_bias(f32x4 (&acc)[TL::MR][TL::MC], const
 // Softmax sums of a tile: per token the largest scaled logit and the sum of 2^(scaled logit - it), over each wave's
 // terms: part[block of terms][token]; with SHARES also the sum of share * logit: dots[block of terms][token].  An exponent
 // takes four times an addition's cycles, and two waves' epilogues share a SIMD: a fifth of a tile's time at 768 values.
-// 8192 rows, 128003 terms, 1024 values: 1.65 ms (1300 TFLOP/s); 5734 rows, 30522, 768, with entries: 302 us (890).
+// 8192 rows, 128003 terms, 1024 values: 1.65 ms (1300 TFLOP/s); 5734 rows, 30522, 768, with entries: 287 us (940).
 template <bool SHARES>
 struct EpiSums {
     const float *bias;
@@ -598,7 +598,10 @@ struct EpiSums {
 };
 
 // Gradients of a tile's logits: (softmax - target shares) times the row's factor, rounded to 16 bits once (three
-// planes for fp32), in blocks, and their sums over each wave's tokens for the bias.  The rows of a block past the last
+// planes for fp32), in blocks, and their sums over each wave's tokens for the bias.  The rounding is what the products that read
+// them take; with 32 bits they would be six plane pairs.  It costs, of all gradients against float64: distillation in bf16
+// 2.3e-3 where fp32 logit gradients have 1.7e-3, which is the results' own rounding, in fp16 2.9e-4 and 2.1e-4; targets 1.7e-3
+// either way.  The rows of a block past the last
 // kept row are zeros: dW sums over them.  The products are made a second time rather than kept: 8192 rows of 128003
 // logits are 2 GB to write and to read, 0.8 ms, against 1.6 for the product, but in 16 bits they would lose what the losses need.
 // 1.79 ms there, in two pieces (1200 TFLOP/s, 2.1 GB written).
@@ -696,7 +699,7 @@ struct EpiLogitGrad {
 };
 
 // dW: rows are dim, columns terms; out[term][dim] times *scale.  It and dH, one launch: 8192 rows, 128003 terms, 1024 values
-// 4.0 ms (1070 TFLOP/s); 2458 rows, 30522, 768 233 us (990).  What bounds them: loads that two stages do not hide.
+// 4.0 ms (1070 TFLOP/s); 2458 rows, 30522, 768 222 us (1040).  What bounds them: loads that two stages do not hide.
 template <class O>
 struct EpiWeightGrad {
     O *out;
@@ -766,8 +769,8 @@ struct EpiHiddenPart {
 // block w of tokens; for each text b in it the largest logits go to slot w + b (along the blocks and texts one of the
 // two grows with each pair, so slots are distinct, and those of a text lie one after the other), with TOK also the
 // lowest kept row that has it (any number where that is a NaN or -inf).  k_term_weights takes a text's slots together.  The bias is added to the maximum
-// (rounding keeps order).  The product bounds it: 10240 rows, 30522 terms, 768 values, 370 us (1300 TFLOP/s); texts of 20 tokens,
-// whose maxima are joined across lanes and written seven times a wave: 1280 rows 70 us (850).
+// (rounding keeps order).  The product bounds it: 10240 rows, 30522 terms, 768 values, 372 us (1290 TFLOP/s); texts of 20 tokens,
+// whose maxima are joined across lanes and written seven times a wave: 1280 rows 67 us (890).
 template <bool TOK>
 struct EpiTextMax {
     const float *bias;
@@ -988,7 +991,8 @@ struct BiasSums {
 
 // Last launch of a gradient.  dH of every source row from its parts (0 for rows that are not kept): with few rows, and so
 // many parts, a workgroup of W = 16 waves takes 256 values of a row, the waves take parts in turn and are added in order; else
-// (W = 4) a wave does.  undo: a row's own scale, NULL: the upstream value's.  Then workgroups of 32 terms of the bias.  Bytes: 8192 rows of 1024 values, 54 us.
+// (W = 4) a wave does.  undo: a row's own scale, NULL: the upstream value's.  Then workgroups of 32 terms of the bias.
+// Bytes: 8192 rows of 1024 values, 54 us.
 template <class O, int W>
 __global__ __launch_bounds__(64 * W) void k_finish_grad(const float *part, const int *inv, const int *n_d, const int *parts_d,
                                                         int total, int dim, int dimp, Upstream up, const float *undo, O *out,
@@ -1500,7 +1504,7 @@ __device__ __forceinline__ void entries_hidden(int block, int64_t b, const void 
     }
 }
 
-// What k_entries_hidden left open: zeros for tokens without entries, sums of the shares of those in several chunks.
+// What entries_hidden left open: zeros for tokens without entries, sums of the shares of those in several chunks.
 template <int HT>
 __global__ __launch_bounds__(256) void k_entries_join(const int *first, int64_t rows, int length, int dim, int chunk, int chunks,
                                                       const float *part, int dimp, typename HVal<HT>::t *out) {
@@ -1624,8 +1628,9 @@ __global__ __launch_bounds__(256) void k_entry_sums(Source h, Source w, const fl
 // ---------------------------------------------------------------- host
 
 // Tiles.  A tile's operands cross LDS once per wave that shares them, so larger ones feed the matrix units better; but a
-// tile needs work for every CU, and few rows leave the vocabulary's bytes as what takes the time.  30522 terms of 768
-// bf16 values, microseconds of the product alone:
+// tile needs work for every CU, and few rows leave the vocabulary's bytes as what takes the time.  The rule looks at the rows
+// of a call, kept or not, since the host does not know how many are, and not at the terms: it was measured at one number of
+// them.  30522 terms of 768 bf16 values, microseconds of the product alone:
 //   rows    64 x 64   256 x 128   256 x 256
 //     45       11.4        13.0        18.5
 //    128       13.5        13.5        18.7

@@ -12,7 +12,9 @@ product with what follows it, without the ``[tokens, vocab]`` logits in memory:
 
 All three work with autograd (first derivatives, in reverse mode).  Tensors are float32, float16 or
 bfloat16, hidden states and weight of one type; sums and softmaxes are in 32 bits, and
-gradients of 16-bit tensors are rounded to their type.  Hidden states and weight may
+gradients of 16-bit tensors are rounded to their type.  So are a loss's gradients of 16-bit
+logits before the products that make the others of them; float32 tensors keep 32 bits
+throughout, at about six times the products.  Hidden states and weight may
 have any strides, up to 2**28 rows (of term weights, 65535 texts), 32768 values and 2**20
 terms; a 16-bit weight whose rows are 16-byte aligned and a multiple
 of 64 values wide is read where it is, others are laid out once per call.  Work is queued
