@@ -1062,21 +1062,58 @@ __global__ __launch_bounds__(64 * W) void k_finish_grad(const float *part, const
 
 // ---------------------------------------------------------------- term weights' small kernels
 
-// The lowest kept row i in [f0, f1) whose logit of term v is NaN; f0 if the sum has one in another order only.  Comparisons
-// lose a NaN, and to keep it in the tiles' epilogue takes registers that they do not have (step of 32 x 256: 357 -> 569 us),
-// so the logits are made again where a maximum turned out to be NaN.
+// The lowest kept row in [f0, f1) whose logit is NaN; f0 if a sum has one in another order only.  Comparisons lose a NaN, and
+// to keep it in the tiles' epilogue takes registers that they do not have (step of 32 x 256: 357 -> 569 us), so it is looked
+// for where a maximum turned out to be NaN.  A row with a NaN has only NaN logits: a wave finds the text's first (`nan`), and
+// the first with an infinity before it (`inf`), whose logits are made again term by term, as those of an infinite term are.  64
+// texts of 256 tokens, the last one of each a NaN: 2 ms more (1900 with every row's logits made again).
+struct OddRows {
+    int inf, nan;
+};
+template <class T>
+__device__ __forceinline__ const T *source_row(const Source &s, int row) {
+    return (const T *)s.p + (int64_t)(row / s.length) * s.s0 + (int64_t)(row % s.length) * s.s1;
+}
 template <int HT>
-__device__ __forceinline__ int nan_row(const Source &h, const Source &w, float bias, const int *rows, int f0, int f1, int v) {
+__device__ __forceinline__ OddRows odd_rows(const Source &h, const int *rows, int f0, int f1) {
+    using T = typename HVal<HT>::t;
+    OddRows o{f1, f1};
+    for (int i = f0; i < f1; i++) {
+        const T *x = source_row<T>(h, rows[i]);
+        bool nan = false, inf = false;
+#pragma unroll 4
+        for (int d = gs_lane(); d < h.dim; d += 64) {
+            const float y = (float)x[d * h.sd];
+            nan |= y != y, inf |= fabsf(y) == INFINITY;
+        }
+        if (__any(nan)) {
+            o.nan = i;
+            break;
+        }
+        if (__any(inf)) o.inf = min(o.inf, i);
+    }
+    return o;
+}
+template <int HT>
+__device__ __forceinline__ int nan_row(const Source &h, const Source &w, float bias, const int *rows, int f0, int f1, int v,
+                                       const OddRows &o) {
     using T = typename HVal<HT>::t;
     if (bias != bias) return f0;
-    const T *y = (const T *)w.p + (int64_t)v * w.s1;
-    for (int i = f0; i < f1; i++) {
-        const T *x = (const T *)h.p + (int64_t)(rows[i] / h.length) * h.s0 + (int64_t)(rows[i] % h.length) * h.s1;
+    const T *y = source_row<T>(w, v);
+    bool inf = false;
+#pragma unroll 4
+    for (int d = 0; d < h.dim; d++) {
+        const float a = (float)y[d * w.sd];
+        if (a != a) return f0;
+        inf |= fabsf(a) == INFINITY;
+    }
+    for (int i = inf ? f0 : o.inf; i < o.nan; i++) {
+        const T *x = source_row<T>(h, rows[i]);
         float a = 0.f;
         for (int d = 0; d < h.dim && a == a; d++) a = fmaf((float)x[d * h.sd], (float)y[d * w.sd], a);
         if (a + bias != a + bias) return i;
     }
-    return f0;
+    return o.nan < f1 ? o.nan : f0;
 }
 
 // A text's weights from its slots: log(1 + relu(maximum)), and the lowest token that has it (-1 where the weight is 0).  HT:
@@ -1091,7 +1128,8 @@ __global__ __launch_bounds__(256) void k_term_weights(const float *best, const i
     // rows of any length: values of 4 bytes are aligned, groups of four need not be
     typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
     typedef int i4u __attribute__((ext_vector_type(4), aligned(4)));
-    for (int v = (blockIdx.x * 256 + threadIdx.x) * 4; v < vocab; v += gridDim.x * 1024) {
+    for (int v0 = (blockIdx.x * 256 + (int)(threadIdx.x & 192)) * 4; v0 < vocab; v0 += gridDim.x * 1024) {  // whole waves
+        const int v = v0 + gs_lane() * 4;
         const bool four = v + 3 < vocab;
         f32x4 x = f32x4{0.f, 0.f, 0.f, 0.f};
         i4u row = {-1, -1, -1, -1};
@@ -1118,10 +1156,19 @@ __global__ __launch_bounds__(256) void k_term_weights(const float *best, const i
         }
         f4u out;
         i4u tok;
+        if (TOK && __any(x[0] != x[0] || x[1] != x[1] || x[2] != x[2] || x[3] != x[3])) {
+            const OddRows odd = odd_rows<HT>(h, rows, f0, f1);
+#pragma unroll 1
+            for (int e = 0; e < 4; e++) {
+                const float y = e & 2 ? (e & 1 ? x[3] : x[2]) : (e & 1 ? x[1] : x[0]);
+                const int r = y != y ? nan_row<HT>(h, w, bias[v + e], rows, f0, f1, v + e, odd) : -1;
+#pragma unroll
+                for (int k = 0; k < 4; k++) row[k] = r >= 0 && k == e ? r : row[k];
+            }
+        }
 #pragma unroll
         for (int e = 0; e < 4; e++) {
             out[e] = log1pf(x[e]);
-            if (TOK && x[e] != x[e]) row[e] = nan_row<HT>(h, w, bias[v + e], rows, f0, f1, v + e);
             if (TOK) tok[e] = row[e] >= 0 ? rows[row[e]] % length : -1;
         }
         const int64_t to = b * vocab + v;

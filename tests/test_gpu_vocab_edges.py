@@ -430,3 +430,23 @@ def test_calls_in_a_graph(device):
         torch.cuda.synchronize(device)
         for got, ref in zip(out, want):
             assert torch.equal(got, ref)
+
+
+@pytest.mark.parametrize("texts,length,dim", [(3, 12, 64), (3, 50, 64), (3, 300, 70)])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_a_nan_of_infinities_has_its_token(device, dtype, texts, length, dim):
+    """Logits that are NaN by infinities: of two signs in a hidden state, of a term against a 0, beside a later NaN and earlier
+    infinities that make none."""
+    h, w, b = (x.detach().clone() for x in inputs(device, (texts, length, dim), 400, dtype, 105))
+    h[0, 2, 5] = INF                                          # one infinity: infinite logits
+    h[0, 4, 5], h[0, 4, 6] = INF, INF                         # two: NaN where the terms' signs differ
+    h[1, 9, 0] = NAN
+    h[2, 6, 1] = 0.0
+    w[11, 1] = INF                                            # NaN at [2, 6]
+    w[12, 3] = NAN
+    weights, tokens = gs.term_weights(h, w, b, return_tokens=True)
+    x = logits64(h, w, b)
+    nan = torch.isnan(x)
+    some = nan.any(dim=1)
+    assert torch.equal(torch.isnan(weights), some) and 0 < int(some[0].sum()) < 400 and int(some[2].sum()) == 2
+    assert bool((tokens[some] == nan.int().argmax(dim=1)[some]).all())
