@@ -1066,7 +1066,7 @@ __global__ __launch_bounds__(64 * W) void k_finish_grad(const float *part, const
 // to keep it in the tiles' epilogue takes registers that they do not have (step of 32 x 256: 357 -> 569 us), so it is looked
 // for where a maximum turned out to be NaN.  A row with a NaN has only NaN logits: a wave finds the text's first (`nan`), and
 // the first with an infinity before it (`inf`), whose logits are made again term by term, as those of an infinite term are.  64
-// texts of 256 tokens, the last one of each a NaN: 2 ms more (1900 with every row's logits made again).
+// texts of 256 tokens, the last one of each a NaN: 7 ms more (1945 with every row's logits made again).
 struct OddRows {
     int inf, nan;
 };

@@ -450,3 +450,15 @@ def test_a_nan_of_infinities_has_its_token(device, dtype, texts, length, dim):
     some = nan.any(dim=1)
     assert torch.equal(torch.isnan(weights), some) and 0 < int(some[0].sum()) < 400 and int(some[2].sum()) == 2
     assert bool((tokens[some] == nan.int().argmax(dim=1)[some]).all())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_under_activation_checkpoints(device, dtype):
+    """What a call saved is made again before its gradient, elsewhere in memory."""
+    from torch.utils.checkpoint import checkpoint
+    h, w, b = (x.detach() for x in inputs(device, (70, 128), 900, dtype, 107))
+    for name, call in _head_calls(device, 900).items():
+        args = [x.clone().requires_grad_() for x in (h, w, b)]
+        want = torch.autograd.grad(call(*args), args)
+        for got, ref in zip(torch.autograd.grad(checkpoint(call, *args, use_reentrant=False), args), want):
+            assert torch.equal(got, ref), name
