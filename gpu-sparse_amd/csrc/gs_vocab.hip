@@ -5,7 +5,7 @@
 // again, a piece of the vocabulary at a time, as gradients in 16 bits that two more products read.
 #include <math.h>
 
-#include "gs_vocab_gemm.h"
+#include "gs_int8.h"
 
 namespace gsv {
 
@@ -14,49 +14,7 @@ constexpr int kRowPad = 256;           // rows of the vocabulary are padded to t
 constexpr int kMaxTop = 1024;          // teacher logits per row
 constexpr size_t kPieceBytes = 1u << 30;  // logit gradients held at a time
 
-__host__ __device__ inline int64_t round_up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
-
 // ---------------------------------------------------------------- values
-
-template <int HT>
-struct HVal;
-template <>
-struct HVal<GS_H_F32> {
-    using t = float;
-};
-template <>
-struct HVal<GS_H_F16> {
-    using t = _Float16;
-};
-template <>
-struct HVal<GS_H_BF16> {
-    using t = __bf16;
-};
-
-template <class T>
-struct alignas(4 * sizeof(T)) Four {
-    T v[4];
-};
-
-template <class T>
-__device__ __forceinline__ f32x4 load4(const T *p) {
-    const Four<T> x = *reinterpret_cast<const Four<T> *>(p);
-    return f32x4{(float)x.v[0], (float)x.v[1], (float)x.v[2], (float)x.v[3]};
-}
-template <class T>
-__device__ __forceinline__ void store4(T *p, f32x4 x) {
-    *reinterpret_cast<Four<T> *>(p) = Four<T>{{(T)x[0], (T)x[1], (T)x[2], (T)x[3]}};
-}
-
-// Up to four values of a row from d on, 0 beyond its end.  `vec`: rows are contiguous and 4-value aligned.
-template <class T>
-__device__ __forceinline__ f32x4 row4(const T *row, int64_t ds, int d, int dim, bool vec) {
-    if (vec && d + 3 < dim) return load4(row + d);
-    f32x4 x;
-#pragma unroll
-    for (int e = 0; e < 4; e++) x[e] = d + e < dim ? (float)row[(d + e) * ds] : 0.f;
-    return x;
-}
 
 template <class T>
 __device__ __forceinline__ uint16_t bits16(float x) {
@@ -279,13 +237,6 @@ __global__ __launch_bounds__(1024) void k_setup(Keep keep, int length, int *rows
 
 // ---------------------------------------------------------------- packing
 
-struct Source {
-    const void *p;
-    int64_t s0, s1, sd;  // strides of text, row, value
-    int length;          // rows per text
-    int dim, vec;
-};
-
 template <int HT, int NP>
 __device__ __forceinline__ void pack_row(const Source &s, int row, int dimp, uint16_t *dst, int lane) {
     using T = typename HVal<HT>::t;
@@ -433,6 +384,20 @@ __global__ __launch_bounds__(256) void k_pack(Source h, const int *rows, const i
             if (teacher.ids) teacher.take(k, row, lane, ids_s[threadIdx.x >> 6]);
             else targets.take(k, row, lane, h, (const T *)h.p + (int64_t)(row / h.length) * h.s0 + (int64_t)(row % h.length) * h.s1, w);
         }
+    }
+}
+
+// The same for a vocabulary in 8 bits, which is read where it is: the kept hidden states as 8-bit rows of `dimp` values, and
+// their scales.
+template <int HT>
+__global__ __launch_bounds__(256) void k_pack8(Source h, const int *rows, const int *n_d, int dimp, int8_t *out, float *scales) {
+    using T = typename HVal<HT>::t;
+    const int n = *n_d, lane = gs_lane();
+    for (int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); i < n; i += (int64_t)gridDim.x * 4) {
+        const T *const row[1] = {source_row<T>(h, rows[i])};
+        float scale[1];
+        quantize_rows<4, 1>(row, h, dimp, lane, scale, [&](int, int d, uint32_t x) { *reinterpret_cast<uint32_t *>(out + i * dimp + d) = x; });
+        if (lane == 0) scales[i] = scale[0] * kDown;
     }
 }
 
@@ -771,16 +736,21 @@ struct EpiHiddenPart {
 // lowest kept row that has it (any number where that is a NaN or -inf).  k_term_weights takes a text's slots together.  The bias is added to the maximum
 // (rounding keeps order).  The product bounds it: 10240 rows, 30522 terms, 768 values, 372 us (1290 TFLOP/s); texts of 20 tokens,
 // whose maxima are joined across lanes and written seven times a wave: 1280 rows 67 us (890).
-template <bool TOK>
+//
+// Q8: operands in 8 bits.  Sums take their row's scale before they are compared, their column's after.
+template <bool TOK, bool Q8 = false>
 struct EpiTextMax {
     const float *bias;
     const int *seg;   // text of each kept row, -1 for the rest of the last tile
     float *best;      // [slot][vocab]
     int *where;
     int vocab;
-    static constexpr int sides = 2;
+    const float *row_scales, *col_scales;  // of Q8; the rows' times kDown
+    static constexpr int sides = Q8 ? 4 : 2;
     static constexpr bool row_bias = false;
-    __device__ __forceinline__ SideArray side(int a, int r0, int c0, const Shape &) const {
+    __device__ __forceinline__ SideArray side(int a, int r0, int c0, const Shape &s) const {
+        if (a == 2) return {row_scales + r0, s.nr - r0};
+        if (a == 3) return {col_scales + c0, s.nc - c0};
         return a == 0 ? SideArray{bias + c0, 256} : SideArray{seg + r0, 256};
     }
 
@@ -799,7 +769,7 @@ struct EpiTextMax {
     }
     // The column blocks' maxima over the four rows of lanes, each block's in a row of lanes of its own.
     template <int MC>
-    __device__ __forceinline__ void flush(int64_t slot, float (&top)[MC], int (&tok)[MC], float b, const Place &at) const {
+    __device__ __forceinline__ void flush(int64_t slot, float (&top)[MC], int (&tok)[MC], float b, float by, const Place &at) const {
         static_assert(MC == 2 || MC == 4, "a row of lanes writes one column block");
         const auto join = [&](Two<float> x2, Two<int> r2, float &x, int &r) {
             if (TOK) r = x2.b > x2.a || (x2.b == x2.a && r2.b < r2.a) ? r2.b : r2.a;
@@ -815,7 +785,7 @@ struct EpiTextMax {
         join(across<32>(x[0], x[MC / 2 - 1]), TOK ? across<32>(r[0], r[MC / 2 - 1]) : Two<int>{0, 0}, best_x, best_r);
         const int v = at.col0 + at.lane;
         if (at.lane < 16 * MC && v < vocab) {
-            best[slot * vocab + v] = best_x + b;
+            best[slot * vocab + v] = Q8 ? fmaf(best_x * by, kUp, b) : best_x + b;
             if (TOK) where[slot * vocab + v] = best_r;
         }
     }
@@ -829,6 +799,7 @@ struct EpiTextMax {
         if (at.row0 >= at.n_r) return;
         const int64_t block = at.row0 / (TL::MR * 16);
         const float b = at.side(0, at.c_in + (at.lane & (16 * TL::MC - 1)));  // of the column that the lane writes
+        const float by = Q8 ? at.side(3, at.c_in + (at.lane & (16 * TL::MC - 1))) : 1.f;
         float top[TL::MC];
         int tok[TL::MC];
 #pragma unroll
@@ -840,6 +811,11 @@ struct EpiTextMax {
             const f32x4 sf = at.side4(1, at.r_in + 16 * i + 4 * q);
             const int sv[4] = {__float_as_int(sf[0]), __float_as_int(sf[1]), __float_as_int(sf[2]), __float_as_int(sf[3])};
             const int lo = __builtin_amdgcn_readlane(sv[0], 0), hi = __builtin_amdgcn_readlane(sv[3], 48);
+            if (Q8) {
+                const f32x4 sc = at.side4(2, at.r_in + 16 * i + 4 * q);
+#pragma unroll
+                for (int j = 0; j < TL::MC; j++) acc[i][j] = __builtin_convertvector(__builtin_bit_cast(i32x4, acc[i][j]), f32x4) * sc;
+            }
             if (lo == cur && hi == cur) {  // all of one text
 #pragma unroll
                 for (int j = 0; j < TL::MC; j++) take(acc[i][j], row, top[j], tok[j]);
@@ -848,7 +824,7 @@ struct EpiTextMax {
             int now = lo;
             while (now >= 0) {  // rows past the last kept one are -1, and come last
                 if (now != cur) {
-                    flush<TL::MC>(block + cur, top, tok, b, at);
+                    flush<TL::MC>(block + cur, top, tok, b, by, at);
                     cur = now;
 #pragma unroll
                     for (int j = 0; j < TL::MC; j++) top[j] = -INFINITY, tok[j] = 0x7FFFFFFF;
@@ -869,7 +845,7 @@ struct EpiTextMax {
                 now = next == 0x7FFFFFFF ? -1 : next;
             }
         }
-        flush<TL::MC>(block + cur, top, tok, b, at);
+        flush<TL::MC>(block + cur, top, tok, b, by, at);
     }
 };
 
@@ -1070,10 +1046,6 @@ __global__ __launch_bounds__(64 * W) void k_finish_grad(const float *part, const
 struct OddRows {
     int inf, nan;
 };
-template <class T>
-__device__ __forceinline__ const T *source_row(const Source &s, int row) {
-    return (const T *)s.p + (int64_t)(row / s.length) * s.s0 + (int64_t)(row % s.length) * s.s1;
-}
 template <int HT>
 __device__ __forceinline__ OddRows odd_rows(const Source &h, const int *rows, int f0, int f1) {
     using T = typename HVal<HT>::t;
@@ -1295,6 +1267,42 @@ __global__ __launch_bounds__(256, 2) void k_few_rows(Source h, const uint8_t *ma
         }
     }
 }
+
+// What k_few8 makes of a block's sums for texts: lane l holds rows 16 m + 4 (l >> 4) .. + 3 of column v.
+struct EpiFewTerms {
+    const void *bias;
+    int bias_type, texts, length;
+    float *weights;
+    template <int MB>
+    __device__ __forceinline__ void run(const i32x4 (&acc)[MB], int v, const Weight8 &W, const float *scales, int rows, uint64_t kept,
+                                        int q) const {
+        const bool on = v < W.n;
+        const float by = on ? W.scales[v] : 0.f, b = on ? bias_at(bias, bias_type, v) : 0.f;
+        f32x4 x[MB];
+#pragma unroll
+        for (int m = 0; m < MB; m++)
+            x[m] = __builtin_convertvector(acc[m], f32x4) * *reinterpret_cast<const f32x4 *>(scales + 16 * m + 4 * q);
+        for (int text = 0; text < texts; text++) {
+            const int lo = text * length, hi = lo + length;
+            float top = -INFINITY;
+#pragma unroll
+            for (int m = 0; m < MB; m++) {
+                if (16 * m >= hi || 16 * m + 16 <= lo) continue;
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int row = 16 * m + 4 * q + e;
+                    top = row >= lo && row < hi && ((kept >> row) & 1) ? maximum(top, x[m][e], x[m][e]) : top;
+                }
+            }
+            const auto join = [&](Two<float> t) { top = maximum(t.a, t.b, t.b); };
+            join(across<16>(top));
+            join(across<32>(top));
+            // the bias of a text without a kept row is not looked at: it may be infinite or NaN
+            const bool any = (kept >> lo) & (~0ull >> (64 - length));
+            if (q == 0 && on) weights[(int64_t)text * W.n + v] = log1pf(any ? maximum(fmaf(top * by, kUp, b), 0.f, 0.f) : 0.f);
+        }
+    }
+};
 
 __global__ void k_no_tokens(int64_t n, float *weights, int *tokens) {
     for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
@@ -1724,15 +1732,6 @@ int token_block(TileClass c) { return token_edge(c) / 2; }
         case GS_H_F16: CALL(_Float16); break; \
         default: CALL(__bf16); break;        \
     }
-
-int cu_count(int *cus) {
-    int dev = 0;
-    GS_CHECK_HIP(hipGetDevice(&dev));
-    GS_CHECK_HIP(hipDeviceGetAttribute(cus, hipDeviceAttributeMultiprocessorCount, dev));
-    return GS_OK;
-}
-
-bool known(int type) { return type == GS_H_F32 || type == GS_H_F16 || type == GS_H_BF16; }
 
 bool vec_ok(const void *p, int type, int64_t s0, int64_t s1, int64_t sd) {
     return sd == 1 && s0 % 4 == 0 && s1 % 4 == 0 && (uintptr_t)p % (type == GS_H_F32 ? 16 : 8) == 0;
@@ -2316,8 +2315,8 @@ extern "C" int gs_term_weights(const gs_vocab_head *h, const uint8_t *mask_d, fl
     {
         const Dims d{l.rows, h->vocab, l.dimp, c.n, 1, 0, 0};
         const Operand hid = hidden_operand(l, c), w = weight_operand(l, c, h);
-        const EpiTextMax<true> et{c.bias, c.seg, best, where, h->vocab};
-        const EpiTextMax<false> ef{c.bias, c.seg, best, where, h->vocab};
+        const EpiTextMax<true> et{c.bias, c.seg, best, where, h->vocab, nullptr, nullptr};
+        const EpiTextMax<false> ef{c.bias, c.seg, best, where, h->vocab, nullptr, nullptr};
         int rc = GS_OK;
 #define GSV_TILE(TL, T, NP)                                                                  \
     rc = tokens_d ? launch_product<TL<T, NP, false, false>>(hid, w, d, et, cus, s)             \
@@ -2366,4 +2365,103 @@ extern "C" int gs_term_weights_grad(const gs_vocab_head *h, const float *grad_d,
     if (h->type == GS_H_F32) return run_entries<GS_H_F32>(h, grad_d, weights_d, tokens_d, dhidden_d, dweight_d, dbias_d, p, s);
     if (h->type == GS_H_F16) return run_entries<GS_H_F16>(h, grad_d, weights_d, tokens_d, dhidden_d, dweight_d, dbias_d, p, s);
     return run_entries<GS_H_BF16>(h, grad_d, weights_d, tokens_d, dhidden_d, dweight_d, dbias_d, p, s);
+}
+
+// ---------------------------------------------------------------- term weights of a vocabulary in 8 bits
+
+namespace gsv {
+
+// As layout_of, whose unit is 16 bits
+Layout layout8_of(const gs_vocab_head *h) {
+    const int rows = h->texts * h->length;
+    return Layout{rows, (int)round_up(h->dim, kPad8) / 2, 1, (int)round_up(h->vocab, kRowPad), true, class_of(rows)};
+}
+
+int check_texts8(const gs_vocab_head *h) {
+    if (int rc = check_texts(h)) return rc;
+    GS_REQUIRE(h->weight_row_stride % kPad8 == 0 && h->weight_row_stride >= round_up(h->dim, kPad8) && h->weight_row_stride < (1 << 20),
+               "weight_row_stride=%lld of 8-bit rows: a multiple of %d, at least dim rounded up to one, below 2^20",
+               (long long)h->weight_row_stride, kPad8);
+    return GS_OK;
+}
+
+template <int HT>
+int run_terms8(const gs_vocab_head *h, const Layout &l, const float *scales_d, const uint8_t *mask_d, float *weights_d, const Common &c,
+               float *best, float *row_scales, int cus, hipStream_t s) {
+    using T = typename HVal<HT>::t;
+    const Source hs = hidden_source(h);
+    if (few8_ok(l.rows, 2 * l.dimp))
+        return launch_few8<T>(hs, mask_d, l.rows, Weight8{(const int8_t *)h->weight_d, h->weight_row_stride, scales_d, h->vocab}, 2 * l.dimp,
+                              EpiFewTerms{h->bias_d, h->bias_type, h->texts, h->length, weights_d}, cus, s);
+    hipLaunchKernelGGL(k_setup, dim3(1 + gs_blocks(l.vocabp, 1024, 1024)), dim3(1024), 0, s, Keep{mask_d, nullptr, 0, h->vocab, l.rows},
+                       h->length, c.rows, c.inv, c.seg, c.text_first, c.n, h->bias_d, h->bias_type, h->vocab, l.vocabp, c.bias, nullptr,
+                       (int64_t)0);
+    GS_CHECK_LAUNCH();
+    hipLaunchKernelGGL((k_pack8<HT>), dim3(gs_blocks(l.rows, 4, 8192)), dim3(256), 0, s, hs, c.rows, c.n, 2 * l.dimp, (int8_t *)c.hidden,
+                       row_scales);
+    GS_CHECK_LAUNCH();
+    const Dims d{l.rows, h->vocab, l.dimp, c.n, 1, 0, 0};
+    const Operand hid{c.hidden, l.dimp, 0, l.dimp}, w{(const uint16_t *)h->weight_d, h->weight_row_stride / 2, 0, l.dimp};
+    const EpiTextMax<false, true> epi{c.bias, c.seg, best, nullptr, h->vocab, row_scales, scales_d};
+    int rc = GS_OK;
+    switch (l.cls) {
+        case kSmall: rc = launch_product<Small<I8, 1, false, false>>(hid, w, d, epi, cus, s); break;
+        case kWide: rc = launch_product<Flat<I8, 1, false, false>>(hid, w, d, epi, cus, s); break;
+        default: rc = launch_product<Large<I8, 1, false, false>>(hid, w, d, epi, cus, s); break;
+    }
+    if (rc) return rc;
+    hipLaunchKernelGGL((k_term_weights<false, GS_H_F32>), dim3(gs_blocks(h->vocab, 1024, 1024), h->texts), dim3(256), 0, s, best, nullptr,
+                       c.text_first, token_block(l.cls), h->vocab, c.rows, h->length, weights_d, nullptr, hs, hs, c.bias);
+    GS_CHECK_LAUNCH();
+    return GS_OK;
+}
+
+void take_terms8(gs_arena &a, const Layout &l, const gs_vocab_head *h, Common *c, float **best, float **row_scales) {
+    take_common(a, l, h, true, c);
+    *row_scales = a.take<float>(l.rows);
+    *best = a.take<float>(text_slots(h, l) * h->vocab);
+}
+
+}  // namespace gsv
+
+extern "C" int gs_term_weights8_workspace(const gs_vocab_head *h, size_t *bytes) {
+    if (int rc = check_texts8(h)) return rc;
+    GS_REQUIRE(bytes, "NULL size pointer");
+    const Layout l = layout8_of(h);
+    gs_arena a{nullptr, 0, 0};
+    Common c;
+    float *best, *row_scales;
+    if (!few8_ok(l.rows, 2 * l.dimp)) take_terms8(a, l, h, &c, &best, &row_scales);
+    *bytes = a.used;
+    return GS_OK;
+}
+
+extern "C" int gs_term_weights8(const gs_vocab_head *h, const float *scales_d, const uint8_t *mask_d, float *weights_d, void *workspace_d,
+                                size_t workspace_bytes, void *stream) {
+    if (int rc = check_texts8(h)) return rc;
+    const Layout l = layout8_of(h);
+    gs_arena a{(char *)workspace_d, 0, workspace_bytes};
+    Common c{};
+    float *best = nullptr, *row_scales = nullptr;
+    if (!few8_ok(l.rows, 2 * l.dimp)) take_terms8(a, l, h, &c, &best, &row_scales);
+    if (!a.ok()) {
+        gs_set_error("term_weights8 workspace too small: need %zu bytes, got %zu", a.used, workspace_bytes);
+        return GS_ENOSPC;
+    }
+    if (h->texts == 0) return GS_OK;
+    if (int rc = check_data(h)) return rc;
+    GS_REQUIRE(scales_d && weights_d && (workspace_d || a.used == 0), "NULL scales, weights or workspace");
+    GS_REQUIRE((uintptr_t)h->weight_d % 16 == 0, "8-bit rows that are not 16-byte aligned");
+    const hipStream_t s = gs_stream(stream);
+    if (l.rows == 0) {
+        const int64_t n = (int64_t)h->texts * h->vocab;
+        hipLaunchKernelGGL(k_no_tokens, dim3(gs_blocks(n, 256, 8192)), dim3(256), 0, s, n, weights_d, nullptr);
+        GS_CHECK_LAUNCH();
+        return GS_OK;
+    }
+    int cus = 0;
+    if (int rc = cu_count(&cus)) return rc;
+    if (h->type == GS_H_F32) return run_terms8<GS_H_F32>(h, l, scales_d, mask_d, weights_d, c, best, row_scales, cus, s);
+    if (h->type == GS_H_F16) return run_terms8<GS_H_F16>(h, l, scales_d, mask_d, weights_d, c, best, row_scales, cus, s);
+    return run_terms8<GS_H_BF16>(h, l, scales_d, mask_d, weights_d, c, best, row_scales, cus, s);
 }

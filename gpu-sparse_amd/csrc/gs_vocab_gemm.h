@@ -21,7 +21,7 @@
 
 #include <atomic>
 
-#include "gs_common.h"
+#include "gs_values.h"
 
 namespace gsv {
 
@@ -29,7 +29,6 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) char *lds_t;
 
 struct Bf16 {

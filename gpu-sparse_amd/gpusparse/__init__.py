@@ -13,7 +13,9 @@ from .search import (MAX_K, MAX_T, PendingSearch, atomic_fused_score, compacted_
 from .chunked import build_chunk_boundaries, triton_chunked_score, triton_chunked_score_fused
 from .engine import determine_dimension, retrieve, run_engine, to_csr, to_query_tensors, write_run
 from .storage import load_index, save_index
+from .int8 import Int8Rows, int8_linear, quantize_rows
 from .vocab import MAX_TOP, distill_loss, term_weights, vocab_loss
+from .embedding import embed_tokens
 from .verification import compute_recall_exact, prepare_queries_from_meta
 
 __all__ = [
@@ -23,5 +25,5 @@ __all__ = [
     "scatter_add", "search", "search_async", "search_counts", "search_plan", "timing_dict", "topk_rows", "triton_fused_score", "build_chunk_boundaries",
     "triton_chunked_score", "triton_chunked_score_fused", "determine_dimension", "retrieve", "run_engine", "to_csr", "to_query_tensors",
     "write_run", "load_index", "save_index", "compute_recall_exact", "prepare_queries_from_meta",
-    "MAX_TOP", "distill_loss", "term_weights", "vocab_loss",
+    "MAX_TOP", "distill_loss", "term_weights", "vocab_loss", "Int8Rows", "int8_linear", "quantize_rows", "embed_tokens",
 ]

@@ -24,7 +24,7 @@ GS_SEARCH_PHASES = 8
 NOALLOC_SCRATCH_BYTES = 256 << 20   # GS_NOALLOC_SCRATCH_BYTES
 PHASE_NAMES = ("query_prep", "heavy_terms", "threshold_seed", "scoring", "candidate_select", "fp64_rescore",
                "final_sort")
-ABI_VERSION = 11
+ABI_VERSION = 12
 
 WTYPE_OF_DTYPE = {torch.float32: GS_W_F32, torch.float16: GS_W_F16, torch.uint8: GS_W_U8}
 
@@ -124,7 +124,7 @@ class GsSynthSpec(C.Structure):
     ]
 
 
-GS_H_F32, GS_H_F16, GS_H_BF16 = 0, 1, 2
+GS_H_F32, GS_H_F16, GS_H_BF16, GS_H_I8 = 0, 1, 2, 3
 GS_REDUCE_NONE, GS_REDUCE_MEAN, GS_REDUCE_SUM = 0, 1, 2
 HTYPE_OF_DTYPE = {torch.float32: GS_H_F32, torch.float16: GS_H_F16, torch.bfloat16: GS_H_BF16}
 
@@ -161,6 +161,47 @@ class GsVocabTargets(C.Structure):
         ("teacher_type", C.c_int32),
         ("top", C.c_int32),
         ("temperature", C.c_float),
+    ]
+
+
+class GsLinear8(C.Structure):
+    """Mirror of ``struct gs_linear8``."""
+
+    _fields_ = [
+        ("x_d", C.c_void_p),
+        ("x_row_stride", C.c_int64),
+        ("x_dim_stride", C.c_int64),
+        ("values_d", C.c_void_p),
+        ("values_stride", C.c_int64),
+        ("scales_d", C.c_void_p),
+        ("bias_d", C.c_void_p),
+        ("out_d", C.c_void_p),
+        ("type", C.c_int32),
+        ("out_type", C.c_int32),
+        ("bias_type", C.c_int32),
+        ("rows", C.c_int32),
+        ("dim", C.c_int32),
+        ("out", C.c_int32),
+    ]
+
+
+class GsLookup(C.Structure):
+    """Mirror of ``struct gs_lookup``."""
+
+    _fields_ = [
+        ("ids_d", C.c_void_p),
+        ("weight_d", C.c_void_p),
+        ("scales_d", C.c_void_p),
+        ("weight_row_stride", C.c_int64),
+        ("weight_dim_stride", C.c_int64),
+        ("tokens", C.c_int64),
+        ("padding", C.c_int64),
+        ("id_bytes", C.c_int32),
+        ("type", C.c_int32),
+        ("out_type", C.c_int32),
+        ("vocab", C.c_int32),
+        ("dim", C.c_int32),
+        ("scale", C.c_float),
     ]
 
 
@@ -228,6 +269,14 @@ SIGNATURES = {
     "gs_vocab_loss": (C.c_int, [C.POINTER(GsVocabHead), C.POINTER(GsVocabTargets), _I32, _P, _P, _SZ, _P, _SZ, _P]),
     "gs_vocab_loss_grad": (C.c_int, [C.POINTER(GsVocabHead), C.POINTER(GsVocabTargets), _I32, _P, _P, _SZ, _P, _P, _P,
                                      _P, _SZ, _P]),
+    "gs_quantize_rows": (C.c_int, [_P, _I32, _I64, _I32, _I64, _I64, _P, _I64, _P, _P]),
+    "gs_int8_linear_workspace": (C.c_int, [C.POINTER(GsLinear8), C.POINTER(_SZ)]),
+    "gs_int8_linear": (C.c_int, [C.POINTER(GsLinear8), _P, _SZ, _P]),
+    "gs_term_weights8_workspace": (C.c_int, [C.POINTER(GsVocabHead), C.POINTER(_SZ)]),
+    "gs_term_weights8": (C.c_int, [C.POINTER(GsVocabHead), _P, _P, _P, _P, _SZ, _P]),
+    "gs_embed_tokens": (C.c_int, [C.POINTER(GsLookup), _P, _P]),
+    "gs_embed_tokens_grad_workspace": (C.c_int, [C.POINTER(GsLookup), C.POINTER(_SZ)]),
+    "gs_embed_tokens_grad": (C.c_int, [C.POINTER(GsLookup), _P, _I64, _P, _P, _SZ, _P]),
 }
 
 SYNTH_SIGNATURES = {

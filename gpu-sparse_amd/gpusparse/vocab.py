@@ -22,13 +22,12 @@ on the current stream of the tensors' device; results are deterministic.
 """
 from __future__ import annotations
 
-from contextlib import nullcontext
-
 import torch
-from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
+from ._tensors import _bytes, _differentiable, _on, _same_device
+from .int8 import Int8Rows, _check_bias, _gpu, _refuse_gradient
 
 C = _lib.C
 REDUCTIONS = {"none": _lib.GS_REDUCE_NONE, "mean": _lib.GS_REDUCE_MEAN, "sum": _lib.GS_REDUCE_SUM}
@@ -57,12 +56,6 @@ def _check_head(hidden, weight, bias, dims: str) -> torch.device:
     return dev
 
 
-def _same_device(dev, **tensors):
-    for name, t in tensors.items():
-        if t is not None and t.device != dev:
-            raise ValueError(f"{name} is on {t.device}, hidden on {dev}")
-
-
 def _head(hidden, weight, bias) -> _lib.GsVocabHead:
     """The C struct of hidden [texts, length, dim] or [rows, dim], weight [vocab, dim] and a contiguous bias."""
     s, n = hidden.stride(), hidden.shape
@@ -74,17 +67,8 @@ def _head(hidden, weight, bias) -> _lib.GsVocabHead:
                             weight.shape[0])
 
 
-def _on(dev):
-    """The tensors' device as the current one; entering it costs more than asking whether it is."""
-    return nullcontext() if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
-
-
 def _upstream(grad: torch.Tensor) -> torch.Tensor:
     return grad if grad.dtype == torch.float32 and grad.is_contiguous() else grad.to(torch.float32).contiguous()
-
-
-def _bytes(n: int, dev) -> torch.Tensor:
-    return torch.empty(int(n), dtype=torch.uint8, device=dev)
 
 
 def _grads(ctx, hidden_shape, weight, dev):
@@ -114,15 +98,6 @@ def _unpack(ctx):
             raise RuntimeError(f"a saved tensor came back as {t.dtype} {tuple(t.shape)} on {t.device}, not as "
                                f"{dtype} {tuple(shape)} on {ctx.dev}")
     return saved, False
-
-
-def _differentiable(*inputs) -> bool:
-    """Whether a call has to go through autograd: a gradient may be asked for, tensors may carry tangents or belong to a
-    functional transform (both of which autograd refuses here), or a trace records it.  One that need not leaves autograd
-    out (5 us of a query's 21)."""
-    return ((torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in inputs))
-            or forward_ad._current_level >= 0 or torch._C._are_functorch_transforms_active()
-            or torch._C._get_tracing_state() is not None)
 
 
 def _weights(hidden, weight, bias, mask, want_tokens: bool):
@@ -174,11 +149,33 @@ class _TermWeights(torch.autograd.Function):
         return dh, dw, db, None
 
 
+def _weights8(hidden, weight, bias, mask):
+    dev = hidden.device
+    weights = torch.empty((hidden.shape[0], weight.shape[0]), dtype=torch.float32, device=dev)
+    L, head, need = _lib.lib(), _head(hidden, weight.values, bias), C.c_size_t()
+    with _on(dev):
+        _lib.check(L.gs_term_weights8_workspace(C.byref(head), C.byref(need)), "gs_term_weights8_workspace")
+        ws = _bytes(need.value, dev) if need.value else None
+        _lib.check(L.gs_term_weights8(C.byref(head), weight.scales.data_ptr(), _lib.ptr(mask), weights.data_ptr(), _lib.ptr(ws),
+                                      need.value, _lib.stream_ptr(dev)), "gs_term_weights8")
+    return weights
+
+
+def _check_head8(hidden, weight, bias) -> torch.device:
+    if hidden.dtype not in _lib.HTYPE_OF_DTYPE:
+        raise ValueError(f"hidden must be float32, float16 or bfloat16, got {hidden.dtype}")
+    if hidden.shape[-1] != weight.shape[1]:
+        raise ValueError(f"hidden must be [texts, length, dim] with dim {weight.shape[1]}, got {tuple(hidden.shape)}")
+    _check_bias(bias, weight.shape[0])
+    return _gpu(hidden, "hidden", weight=weight, bias=bias)
+
+
 def term_weights(hidden, weight, bias=None, *, mask=None, return_tokens: bool = False):
     """Term weights of texts from an encoder's hidden states: float32 [texts, vocab],
     ``log(1 + relu(max over the text's kept tokens of hidden @ weight.T + bias))``.
 
-    hidden: [texts, length, dim].  weight: [vocab, dim].  bias: [vocab] or None.
+    hidden: [texts, length, dim].  weight: [vocab, dim], or :class:`gpusparse.Int8Rows` of it: then the kept hidden states
+    are taken in 8 bits as well, and there is neither a gradient nor return_tokens.  bias: [vocab] or None.
     mask: [texts, length], nonzero for the tokens that count (None: all do); the hidden
     states of the others are never read, and a text without any has weights 0.
     return_tokens: also the int32 [texts, vocab] lowest token that reaches the maximum
@@ -186,7 +183,10 @@ def term_weights(hidden, weight, bias=None, *, mask=None, return_tokens: bool = 
     flows.  A NaN is the maximum of its text: the weight is NaN, and the gradient where it flows."""
     if not isinstance(hidden, torch.Tensor) or hidden.dim() != 3:
         raise ValueError("hidden must be [texts, length, dim]")
-    dev = _check_head(hidden, weight, bias, "[texts, length, dim]")
+    q8 = isinstance(weight, Int8Rows)
+    if q8 and return_tokens:
+        raise ValueError("return_tokens goes with the gradient, which a vocabulary in 8 bits does not have")
+    dev = _check_head8(hidden, weight, bias) if q8 else _check_head(hidden, weight, bias, "[texts, length, dim]")
     if mask is not None:
         if not isinstance(mask, torch.Tensor) or tuple(mask.shape) != tuple(hidden.shape[:2]):
             raise ValueError(f"mask must be a tensor of shape {tuple(hidden.shape[:2])}")
@@ -195,6 +195,9 @@ def term_weights(hidden, weight, bias=None, *, mask=None, return_tokens: bool = 
             mask = mask != 0
         mask = mask.contiguous()
     bias = None if bias is None else bias.contiguous()
+    if q8:
+        _refuse_gradient(hidden, bias)
+        return _weights8(hidden, weight, bias, mask)
     if _differentiable(hidden, weight, bias):
         weights, tokens = _TermWeights.apply(hidden, weight, bias, mask)
     else:

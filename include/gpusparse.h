@@ -25,7 +25,7 @@
 extern "C" {
 #endif
 
-#define GS_ABI_VERSION 11
+#define GS_ABI_VERSION 12
 
 #define GS_OK 0
 #define GS_EINVAL 1   /* bad argument or layout */
@@ -466,6 +466,60 @@ int gs_vocab_loss(const gs_vocab_head *head, const gs_vocab_targets *targets, in
 int gs_vocab_loss_grad(const gs_vocab_head *head, const gs_vocab_targets *targets, int32_t reduction,
                        const float *grad_d, const void *saved_d, size_t saved_bytes, void *dhidden_d, void *dweight_d,
                        void *dbias_d, void *scratch_d, size_t scratch_bytes, void *stream);
+
+/* ------------------------------------------------------------ rows in 8 bits
+ * No counterpart in the reference.  A row x is kept as whole numbers q = nearest(127 x / max|x|), ties to even, and one
+ * scale max|x| / 127.  A row with an infinity or a NaN has scale NaN (and values 0), one whose largest magnitude is below
+ * 2^-94 counts as zeros.  8-bit rows start 16-byte aligned, a multiple of 128 bytes apart that covers dim rounded up to 128;
+ * what lies between dim and that is read, but counts for nothing. */
+int gs_quantize_rows(const void *x_d, int32_t type, int64_t rows, int32_t dim, int64_t row_stride, int64_t dim_stride,
+                     int8_t *values_d, int64_t values_stride, float *scales_d, void *stream);
+
+/* y[r][o] = sum_d x'[r][d] w[o][d] + bias[o], with x' the row of x in 8 bits (made within the call) and w the 8-bit rows:
+ * sums are exact whole numbers, scaled and rounded at the end.  x [rows][dim] of `type` with any element strides, out_d
+ * [rows][out] of out_type, contiguous.  rows <= 2^28, dim <= 32768, out <= 2^20. */
+typedef struct gs_linear8 {
+    const void *x_d;
+    int64_t x_row_stride, x_dim_stride;
+    const int8_t *values_d;
+    int64_t values_stride;
+    const float *scales_d;
+    const void *bias_d;  /* [out] of bias_type, or NULL */
+    void *out_d;
+    int32_t type, out_type, bias_type;
+    int32_t rows, dim, out;
+} gs_linear8;
+int gs_int8_linear_workspace(const gs_linear8 *linear, size_t *bytes);
+int gs_int8_linear(const gs_linear8 *linear, void *workspace_d, size_t workspace_bytes, void *stream);
+
+/* gs_term_weights of a vocabulary in 8 bits: weight_d are its values (int8, weight_row_stride bytes apart,
+ * weight_dim_stride 1), scales_d its scales; each kept hidden state is taken in 8 bits as well. */
+int gs_term_weights8_workspace(const gs_vocab_head *head, size_t *bytes);
+int gs_term_weights8(const gs_vocab_head *head, const float *scales_d, const uint8_t *mask_d, float *weights_d,
+                     void *workspace_d, size_t workspace_bytes, void *stream);
+
+/* ------------------------------------------------------------ token lookup
+ * No counterpart in the reference.  out_d [tokens][dim] = scale * (the id's row of weight), contiguous; zeros for an id outside
+ * [0, vocab).  weight_d [vocab][dim] with any element strides, of `type`; or 8-bit rows (type GS_H_I8, dim_stride 1, scales_d).
+ * out_type is `type`, or any GS_H_* of values for 8-bit rows.
+ * Its gradient: dweight_d [vocab][dim] of `type`, contiguous and written whole, scale * the sum of grad_d's rows (dim values on
+ * end, grad_row_stride values apart) whose id it is, in a fixed order; ids equal to `padding` have none (no id: negative).
+ * tokens <= 2^28, vocab <= 2^20, dim <= 32768. */
+#define GS_H_I8 3
+typedef struct gs_lookup {
+    const void *ids_d;      /* [tokens], of id_bytes 4 or 8 */
+    const void *weight_d;
+    const float *scales_d;  /* of GS_H_I8 */
+    int64_t weight_row_stride, weight_dim_stride;
+    int64_t tokens, padding;
+    int32_t id_bytes, type, out_type;
+    int32_t vocab, dim;
+    float scale;
+} gs_lookup;
+int gs_embed_tokens(const gs_lookup *lookup, void *out_d, void *stream);
+int gs_embed_tokens_grad_workspace(const gs_lookup *lookup, size_t *bytes);
+int gs_embed_tokens_grad(const gs_lookup *lookup, const void *grad_d, int64_t grad_row_stride, void *dweight_d, void *workspace_d,
+                         size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }
