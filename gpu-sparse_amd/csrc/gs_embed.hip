@@ -86,7 +86,7 @@ __global__ __launch_bounds__(256) void k_embed_strided(Ids ids, const T *table, 
 // how many there are).  The ids are split into kRanges ranges of 2^shift ids.  One workgroup orders a range; it finds its tokens
 // among all ids itself, or, of many tokens, in segments that k_split has sorted by range.
 constexpr int kRanges = 256, kSegs = 1024, kOrderLds = 128 * 1024;
-constexpr int kSplitThreads = 512, kSplitWaves = kSplitThreads / 64, kSplitTile = 4096;
+constexpr int kSplitThreads = 512, kSplitWaves = kSplitThreads / 64, kSplitTile = 1024;
 
 struct Tokens {
     Ids ids;
@@ -209,7 +209,12 @@ __global__ __launch_bounds__(1024) void k_order(Tokens t, int64_t seg_size, int 
     if (SPLIT) {
         for (int s = tid; s < segs; s += 1024) seg_at[s] = counts[(int64_t)g * segs + s];
         int before = 0;
-        for (int i = tid; i < g * segs; i += 1024) before += counts[i];
+        const int cells = g * segs;  // a whole number of fours where that matters
+        for (int i = tid * 4; i + 3 < cells; i += 4096) {
+            const i32x4 c = *reinterpret_cast<const i32x4 *>(counts + i);
+            before += c[0] + c[1] + c[2] + c[3];
+        }
+        if (tid < (cells & 3)) before += counts[(cells & ~3) + tid];
         before = (int)gs_wave_sum((uint32_t)before);
         if (lane == 0) atomicAdd(&before_s, before);
         __syncthreads();
@@ -217,35 +222,52 @@ __global__ __launch_bounds__(1024) void k_order(Tokens t, int64_t seg_size, int 
         if (tid == 0) seg_at[segs] = (int)n;
         __syncthreads();
     }
-    // entry e of the range (SPLIT), or token e: its id within the range, and the token
+    // A wave's entries a to b of the range (SPLIT), or tokens, kRounds of 64 at a time, so that their loads are on their way
+    // together: ids within the range (-1: another's), and tokens.
+    constexpr int kRounds = SPLIT ? 4 : 16;
     const int64_t per = (n + waves - 1) / waves, a = wave < waves ? min(n, wave * per) : n, b = min(n, a + per);
-    const auto take = [&](int64_t e, bool in, int &key, uint32_t &token) {
+    int key[kRounds], below = 0;
+    uint32_t token[kRounds];
+    const auto fetch = [&](int64_t e0, bool count_below) {
         if (SPLIT) {
-            int lo = 0, hi = segs;  // the last segment that starts at or before e
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) >> 1;
-                if (seg_at[mid] <= e) lo = mid;
-                else hi = mid;
+            int64_t at[kRounds];
+#pragma unroll
+            for (int k = 0; k < kRounds; k++) {
+                const int64_t e = e0 + k * 64 + lane;
+                int lo = 0, hi = segs;  // the last segment that starts at or before e
+                while (hi - lo > 1) {
+                    const int mid = (lo + hi) >> 1;
+                    if (seg_at[mid] <= e) lo = mid;
+                    else hi = mid;
+                }
+                at[k] = e < b ? lo * seg_size + begin[(int64_t)g * segs + lo] + (e - seg_at[lo]) : -1;
             }
-            if (!in) return false;
-            const int64_t at = lo * seg_size + begin[(int64_t)g * segs + lo] + (e - seg_at[lo]);
-            key = low[at], token = pos[at];
-            return true;
+#pragma unroll
+            for (int k = 0; k < kRounds; k++) {
+                key[k] = at[k] >= 0 ? low[at[k]] : -1;
+                token[k] = at[k] >= 0 ? pos[at[k]] : 0;
+            }
+        } else {
+            int64_t id[kRounds];
+#pragma unroll
+            for (int k = 0; k < kRounds; k++) {
+                const int64_t e = e0 + k * 64 + lane;
+                id[k] = e < b ? t.ids.at(e) : -1;
+            }
+#pragma unroll
+            for (int k = 0; k < kRounds; k++) {
+                const bool on = t.kept(id[k]);
+                key[k] = on && (int)id[k] >> t.shift == g ? (int)id[k] - id0 : -1;
+                token[k] = (uint32_t)(e0 + k * 64 + lane);
+                below += count_below && on && (int)id[k] < id0;
+            }
         }
-        const int64_t id = in ? t.ids.at(e) : -1;
-        const bool on = t.kept(id) && (int)id >> t.shift == g;
-        key = on ? (int)id - id0 : 0, token = (uint32_t)e;
-        return on;
     };
-    int below = 0;
-    for (int64_t e = a + lane; e < b; e += 64) {
-        int key;
-        uint32_t token;
-        if (take(e, true, key, token)) atomicAdd(&count[wave * width + key], 1);
-        else if (!SPLIT) {
-            const int64_t id = t.ids.at(e);
-            below += t.kept(id) && (int)id < id0;
-        }
+    for (int64_t e0 = a; e0 < b; e0 += kRounds * 64) {
+        fetch(e0, true);
+#pragma unroll
+        for (int k = 0; k < kRounds; k++)
+            if (key[k] >= 0) atomicAdd(&count[wave * width + key[k]], 1);
     }
     if (!SPLIT) {
         below = (int)gs_wave_sum((uint32_t)below);
@@ -269,22 +291,24 @@ __global__ __launch_bounds__(1024) void k_order(Tokens t, int64_t seg_size, int 
     if (tid == 0 && g == t.ranges - 1) o.start[t.vocab] = base + total;
     for (int i = tid; i < waves * width; i += 1024) count[i] += base + first[i & (width - 1)];
     __syncthreads();
-    for (int64_t e0 = a; e0 < b; e0 += 64) {
-        int key = 0;
-        uint32_t token = 0;
-        const bool on = take(e0 + lane, e0 + lane < b, key, token);
-        if (!__any(on)) continue;
-        int rank, all;
-        same_key(key, on, t.shift, rank, all);
-        int *next = &count[wave * width + (on ? key : 0)];
-        const int at = *next;
-        gs_wave_sync();
-        if (on) {
-            o.order[at + rank] = token;
-            o.id[at + rank] = id0 + key;
-            if (rank == 0) *next = at + all;
+    for (int64_t e0 = a; e0 < b; e0 += kRounds * 64) {
+        if (b - a > kRounds * 64) fetch(e0, false);
+#pragma unroll
+        for (int k = 0; k < kRounds; k++) {
+            const bool on = key[k] >= 0;
+            if (!__any(on)) continue;
+            int rank, all;
+            same_key(key[k], on, t.shift, rank, all);
+            int *next = &count[wave * width + (on ? key[k] : 0)];
+            const int at = *next;
+            gs_wave_sync();
+            if (on) {
+                o.order[at + rank] = token[k];
+                o.id[at + rank] = id0 + key[k];
+                if (rank == 0) *next = at + all;
+            }
+            gs_wave_sync();
         }
-        gs_wave_sync();
     }
 }
 
@@ -402,6 +426,115 @@ __global__ __launch_bounds__(256) void k_embed_join(Sorted o, int vocab, int dim
         if (d + e < dim) dw[(int64_t)id * dim + d + e] = (T)(x[e] * scale);
 }
 
+// The whole gradient of at most 1024 tokens, for latency: a workgroup takes a range of ids, looks through all tokens for them
+// (one each per thread), and writes the range's rows: zeros, a wave the sum of an id's tokens, all waves together that of an id with
+// more than kLong of them.  What bounds it is dW, whose rows are mostly zeros.
+constexpr int kFewTokens = 1024, kLong = 32;
+template <class T, int N>
+__global__ __launch_bounds__(1024) void k_embed_few(Tokens t, const T *grad, int64_t stride, int dim, float scale, T *dw) {
+    using P = Piece<T, N>;
+    typedef float acc_t __attribute__((ext_vector_type(N)));
+    __shared__ int list[kFewTokens], sorted[kFewTokens], runs[kFewTokens + 1], wave_n[16];  // key << 10 | token
+    __shared__ uint32_t has[128];
+    __shared__ __align__(16) acc_t part[16][64];
+    const int tid = threadIdx.x, lane = gs_lane(), wave = gs_uniform(tid >> 6);
+    const int width = 1 << t.shift, id0 = blockIdx.x << t.shift, rows = min(width, t.vocab - id0);
+    const int64_t id = tid < t.n ? t.ids.at(tid) : -1;
+    const bool on = t.kept(id) && (int)id >> t.shift == (int)blockIdx.x;
+    const auto place = [&](bool flag) {  // of this thread's among the flags, and how many there are
+        const uint64_t m = __ballot(flag);
+        __syncthreads();
+        if (lane == 0) wave_n[wave] = __popcll(m);
+        __syncthreads();
+        int at = __popcll(m & gs_lanemask_lt()), all = 0;
+        for (int w = 0; w < 16; w++) {
+            if (w < wave) at += wave_n[w];
+            all += wave_n[w];
+        }
+        return make_int2(at, all);
+    };
+    if (tid < 128) has[tid] = 0;
+    const int2 mine = place(on);
+    const int n = mine.y;
+    if (on) {
+        const int key = (int)id - id0;
+        list[mine.x] = key << 10 | tid;
+        atomicOr(&has[key >> 5], 1u << (key & 31));
+    }
+    __syncthreads();
+    const auto put = [&](int row, int d, acc_t x) {
+        P y;
+#pragma unroll
+        for (int e = 0; e < N; e++) y.v[e] = (T)(x[e] * scale);
+        T *to = dw + (int64_t)(id0 + row) * dim + d;
+        if (d + N <= dim) *reinterpret_cast<P *>(to) = y;
+        else
+#pragma unroll
+            for (int e = 0; e < N; e++)
+                if (d + e < dim) to[e] = y.v[e];
+    };
+    for (int r = wave; r < rows; r += 16)
+        if (!(has[r >> 5] >> (r & 31) & 1))
+            for (int d = lane * N; d < dim; d += 64 * N) put(r, d, acc_t{});
+    if (n == 0) return;
+    // the keys differ, since they hold their token
+    if (tid < n) {
+        const int x = list[tid];
+        int at = 0;
+        for (int k = 0; k < n; k++) at += list[k] < x;
+        sorted[at] = x;
+    }
+    __syncthreads();
+    const bool starts = tid < n && (tid == 0 || sorted[tid] >> 10 != sorted[tid - 1] >> 10);
+    const int2 run = place(starts);
+    if (starts) runs[run.x] = tid;
+    if (tid == 0) runs[run.y] = n;
+    __syncthreads();
+    // rows a to b of the sorted list
+    const auto sum = [&](int a, int b, int d) {
+        acc_t x{};
+        constexpr int U = 8;
+        for (int k = a; k < b; k += U) {
+            typename P::vec v[U];
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const T *row = grad + (sorted[min(k + u, b - 1)] & 1023) * stride + d;
+                if (d + N <= dim) v[u] = reinterpret_cast<const P *>(row)->v;
+                else
+#pragma unroll
+                    for (int e = 0; e < N; e++) v[u][e] = d + e < dim ? row[e] : (T)0;
+            }
+#pragma unroll
+            for (int u = 0; u < U; u++)
+                if (k + u < b) {
+#pragma unroll
+                    for (int e = 0; e < N; e++) x[e] += (float)v[u][e];
+                }
+        }
+        return x;
+    };
+    const int slices = (dim + 64 * N - 1) / (64 * N);
+    for (int w = wave; w < run.y * slices; w += 16) {
+        const int r = w / slices, d = (w - r * slices) * 64 * N + lane * N;
+        if (runs[r + 1] - runs[r] <= kLong) put(sorted[runs[r]] >> 10, d, sum(runs[r], runs[r + 1], d));
+    }
+    for (int r = 0; r < run.y; r++) {
+        const int a = runs[r], len = runs[r + 1] - a;
+        if (len <= kLong) continue;
+        for (int s = 0; s < slices; s++) {
+            const int d = s * 64 * N + lane * N;
+            part[wave][lane] = sum(a + len * wave / 16, a + len * (wave + 1) / 16, d);
+            __syncthreads();
+            if (wave == 0) {
+                acc_t x = part[0][lane];
+                for (int k = 1; k < 16; k++) x += part[k][lane];
+                put(sorted[a] >> 10, d, x);
+            }
+            __syncthreads();
+        }
+    }
+}
+
 // ---------------------------------------------------------------- host
 
 int check_lookup(const gs_lookup *l) {
@@ -430,7 +563,7 @@ int run_lookup(const gs_lookup *l, const float *scales, O *out, hipStream_t s) {
 
 struct GradPlan {
     int shift, ranges, segs, chunk, slices, n_vec;
-    bool split;
+    bool few, split;
     int64_t seg_size, chunks, ld;
     Sorted o;
     uint32_t *pos;
@@ -444,7 +577,9 @@ GradPlan plan_grad(gs_arena &a, const gs_lookup *l) {
     GradPlan p{};
     while ((kRanges << p.shift) < l->vocab) p.shift++;
     p.ranges = (l->vocab + (1 << p.shift) - 1) >> p.shift;
+    p.few = l->tokens <= kFewTokens;
     p.split = l->tokens > kDirect;
+    if (p.few) return p;
     p.seg_size = kSplitTile;
     while (p.seg_size * kSegs < l->tokens) p.seg_size *= 2;
     p.segs = (int)((l->tokens + p.seg_size - 1) / p.seg_size);
@@ -470,6 +605,11 @@ GradPlan plan_grad(gs_arena &a, const gs_lookup *l) {
 template <class T, int N>
 int run_grad(const gs_lookup *l, const GradPlan &p, const void *grad_d, int64_t stride, void *dweight_d, hipStream_t s) {
     const Tokens t{Ids{l->ids_d, l->id_bytes}, l->tokens, l->padding, l->vocab, p.shift, p.ranges};
+    if (p.few) {
+        hipLaunchKernelGGL((k_embed_few<T, N>), dim3(p.ranges), dim3(1024), 0, s, t, (const T *)grad_d, stride, l->dim, l->scale, (T *)dweight_d);
+        GS_CHECK_LAUNCH();
+        return GS_OK;
+    }
     const int width = 1 << p.shift, waves = 16 < kOrderLds / 4 / width ? 16 : kOrderLds / 4 / width;
     const int lds = (waves + 1) * width * 4;
     static std::atomic<uint64_t> set{0}, set_split{0};
@@ -547,7 +687,7 @@ extern "C" int gs_embed_tokens_grad(const gs_lookup *l, const void *grad_d, int6
         gs_set_error("embed_tokens_grad workspace too small: need %zu bytes, got %zu", a.used, workspace_bytes);
         return GS_ENOSPC;
     }
-    GS_REQUIRE(workspace_d && dweight_d && ((l->ids_d && grad_d) || l->tokens == 0), "NULL ids, gradient or workspace");
+    GS_REQUIRE((workspace_d || a.used == 0) && dweight_d && ((l->ids_d && grad_d) || l->tokens == 0), "NULL ids, gradient or workspace");
     const hipStream_t s = gs_stream(stream);
     if (l->type == GS_H_F32) return run_grad<float, 4>(l, p, grad_d, grad_row_stride, dweight_d, s);
     if (l->type == GS_H_F16) return run_grad<_Float16, 8>(l, p, grad_d, grad_row_stride, dweight_d, s);

@@ -46,57 +46,95 @@ __device__ __forceinline__ RowScale row_scale(uint32_t bits) {
     r.scale = bits >= 0x7F800000u ? __builtin_nanf("") : none ? 0.f : r.most / 127.f;
     return r;
 }
-// The nearest whole number to 127 x / most.  x * inv is off by less than 2^-15 (three roundings of a value up to 127), so it
-// decides alone except next to a half, where the difference from the quotient is taken in 64 bits, without error: 127 x, n most
-// and their difference are of fewer than 53 bits there.
-__device__ __forceinline__ int quantized(float x, const RowScale &r) {
-    if (r.inv == 0.f) return 0;
-    const float y = x * r.inv;
-    float n = rintf(y);
-    if (__builtin_expect(fabsf(fabsf(y - n) - 0.5f) < 0x1p-10f, 0)) {
-        const double off = fma(-(double)n, (double)r.most, (double)x * 127.0), half = 0.5 * (double)r.most;
-        if (fabs(off) > half || (fabs(off) == half && ((int)n & 1))) n += off > 0 ? 1.f : -1.f;
+// Eight values' nearest whole numbers to 127 x / most, a byte each.  x * inv is off by less than 2^-16 (two roundings of a
+// value up to 127), so it decides alone except next to a half, where the difference from the quotient is taken without error: of
+// 127 x and n most the rounding errors are kept, and their difference and that to most / 2 are of close numbers.
+// Adding 1.5 x 2^23 rounds to a whole number, whose two's complement is then the sum's low byte.
+template <class T>
+struct Raw8 {  // eight values as they lie
+    typedef T vec __attribute__((ext_vector_type(8)));
+    typedef T any __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+    vec v;
+    __device__ __forceinline__ float operator[](int e) const { return (float)v[e]; }
+};
+template <class T>
+__device__ __forceinline__ uint2 quantized8(const Raw8<T> &x, const RowScale &r) {
+    if (r.inv == 0.f) return make_uint2(0, 0);
+    constexpr float kRound = 0x1.8p23f;
+    uint32_t t[8];
+    float far = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        const float y = x[e] * r.inv, s = y + kRound;
+        far = fmaxf(far, fabsf(y - (s - kRound)));
+        t[e] = __float_as_uint(s);
     }
-    return (int)n;
+    if (__builtin_expect(far > 0.5f - 0x1p-15f, 0)) {
+        const float most = r.most * 0x1p-8f, half = 0.5f * most;  // 127 x stays finite
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const int n = (int)(int8_t)t[e];
+            const float v = x[e] * 0x1p-8f, p = v * 127.f, q = (float)n * most;
+            const float d = p - q, low = fmaf(v, 127.f, -p) - fmaf((float)n, most, -q);
+            const float over = d > 0 ? (d - half) + low : (-d - half) - low;  // |127 x - n most| - most / 2, or its sign
+            if (over > 0 || (over == 0 && (n & 1))) t[e] = (uint32_t)(n + (d > 0 ? 1 : -1));
+        }
+    }
+    const auto four = [](uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+        const uint32_t lo = __builtin_amdgcn_perm(b, a, 0x0C0C0400), hi = __builtin_amdgcn_perm(d, c, 0x0C0C0400);
+        return lo | hi << 16;
+    };
+    return make_uint2(four(t[0], t[1], t[2], t[3]), four(t[4], t[5], t[6], t[7]));
 }
-__device__ __forceinline__ uint32_t quantized4(f32x4 x, const RowScale &r) {
-    return (quantized(x[0], r) & 255) | (quantized(x[1], r) & 255) << 8 | (quantized(x[2], r) & 255) << 16 |
-           (uint32_t)quantized(x[3], r) << 24;
-}
-__device__ __forceinline__ uint32_t magnitude(f32x4 x) {
+template <class T>
+__device__ __forceinline__ uint32_t magnitude(const Raw8<T> &x) {
     uint32_t m = 0;
 #pragma unroll
-    for (int e = 0; e < 4; e++) m = max(m, __float_as_uint(x[e]) & 0x7FFFFFFFu);
+    for (int e = 0; e < 8; e++) m = max(m, __float_as_uint(x[e]) & 0x7FFFFFFFu);
     return m;
 }
+// Up to eight values of a row from d on, 0 beyond its end.  UNIT: they lie on end, and are read 16 bytes at a time wherever they
+// start.
+template <bool UNIT, class T>
+__device__ __forceinline__ Raw8<T> row8(const T *row, int64_t ds, int d, int dim) {
+    Raw8<T> x;
+    if (UNIT && d + 8 <= dim) {
+        x.v = *reinterpret_cast<const typename Raw8<T>::any *>(row + d);
+    } else {
+        const T *p = row + (UNIT ? d : d * ds);
+#pragma unroll
+        for (int e = 0; e < 8; e++) x.v[e] = d + e < dim ? p[UNIT ? e : e * ds] : (T)0.f;
+    }
+    return x;
+}
 
-// N rows by one wave: put(u, d, word) takes row u's values d .. d + 3, zeros from dim to dimp (a multiple of 4); returns the
-// scales.  Rows of up to 256 HOLD values are read once, all at a time; longer ones twice.
-template <int HOLD, int N, class T, class Put>
-__device__ __forceinline__ void quantize_rows(const T *const (&row)[N], const Source &s, int dimp, int lane, float (&scale)[N],
-                                              Put &&put) {
-    f32x4 x[N][HOLD];
-    uint32_t most[N];
+// N rows by one wave, those that are `on` (which is uniform): put(u, d, bytes) takes row u's values d .. d + 7, zeros from dim to
+// dimp (a multiple of 8); scale receives the scales.  Rows of up to 512 HOLD values are read once, all at a time; longer ones twice.
+template <bool UNIT, int HOLD, int N, class T, class Put>
+__device__ __forceinline__ void quantize_rows(const T *(&row)[N], const bool (&on)[N], const Source &s, int dimp, int lane,
+                                              float (&scale)[N], Put &&put) {
+    Raw8<T> x[N][HOLD];
 #pragma unroll
     for (int u = 0; u < N; u++) {
+        if (!on[u]) continue;
 #pragma unroll
-        for (int c = 0; c < HOLD; c++) x[u][c] = row4(row[u], s.sd, c * 256 + lane * 4, s.dim, s.vec);
+        for (int c = 0; c < HOLD; c++) x[u][c] = row8<UNIT>(row[u], s.sd, c * 512 + lane * 8, s.dim);
     }
 #pragma unroll
     for (int u = 0; u < N; u++) {
-        most[u] = 0;
+        if (!on[u]) continue;
+        uint32_t most = 0;
 #pragma unroll
-        for (int c = 0; c < HOLD; c++) most[u] = max(most[u], magnitude(x[u][c]));
-        for (int d = HOLD * 256 + lane * 4; d < s.dim; d += 256) most[u] = max(most[u], magnitude(row4(row[u], s.sd, d, s.dim, s.vec)));
-    }
-#pragma unroll
-    for (int u = 0; u < N; u++) {
-        const RowScale r = row_scale(gs_wave_max_u32(most[u]));
+        for (int c = 0; c < HOLD; c++) most = max(most, magnitude(x[u][c]));
+#pragma unroll 2
+        for (int d = HOLD * 512 + lane * 8; d < s.dim; d += 512) most = max(most, magnitude(row8<UNIT>(row[u], s.sd, d, s.dim)));
+        const RowScale r = row_scale(gs_wave_max_u32(most));
         scale[u] = r.scale;
 #pragma unroll
         for (int c = 0; c < HOLD; c++)
-            if (c * 256 + lane * 4 < dimp) put(u, c * 256 + lane * 4, quantized4(x[u][c], r));
-        for (int d = HOLD * 256 + lane * 4; d < dimp; d += 256) put(u, d, quantized4(row4(row[u], s.sd, d, s.dim, s.vec), r));
+            if (c * 512 + lane * 8 < dimp) put(u, c * 512 + lane * 8, quantized8(x[u][c], r));
+#pragma unroll 1
+        for (int d = HOLD * 512 + lane * 8; d < dimp; d += 512) put(u, d, quantized8(row8<UNIT>(row[u], s.sd, d, s.dim), r));
     }
 }
 
@@ -114,7 +152,15 @@ __device__ __forceinline__ float bias_at(const void *bias, int type, int v) {
                             : type == GS_H_F16 ? (float)((const _Float16 *)bias)[v] : (float)((const __bf16 *)bias)[v];
 }
 
-// Products of at most 64 rows in one launch, for latency: a workgroup of eight waves quantises all rows into LDS itself and
+// A column's scale and bias
+struct ColumnScale {
+    float by, bias;
+};
+__device__ __forceinline__ ColumnScale column_scale(int v, const Weight8 &W, const void *bias, int type) {
+    return v < W.n ? ColumnScale{W.scales[v], bias_at(bias, type, v)} : ColumnScale{0.f, 0.f};
+}
+
+// Products of at most 64 rows, their values on end, in one launch, for latency: a workgroup of eight waves quantises all rows into LDS itself and
 // takes blocks of 16 columns, KS of its waves a block, each its part of k.  The weight goes from memory to the operands'
 // registers: a lane takes 32 bytes on end of its column, so that a wave's loads take whole lines, and the first of them are asked
 // for before the rows are quantised.
@@ -141,6 +187,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void k_few8(Source h, const uint
     constexpr int kAhead = 4;  // steps of 128 values in each of two buffers
     i32x4 w[2][2 * kAhead];
     int g = blockIdx.x, c0;
+    ColumnScale next;  // of the lane's column
     __amdgpu_buffer_rsrc_t from;
     const auto load = [&](i32x4 (&b)[2 * kAhead], int k) {
 #pragma unroll
@@ -158,19 +205,27 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void k_few8(Source h, const uint
         from = gs_rsrc(W.p + (int64_t)(n ? c0 : 0) * W.stride, (uint32_t)(n * (int)W.stride));
         load(w[0], k0);
         load(w[1], k0 + kAhead);
+        next = epi.column(c0 + i, W);
     };
     seek();
 
-    for (int r = wave * 2; r < rows; r += 2 * kFewWaves) {
-        const int second = min(r + 1, rows - 1);
-        if (!((kept >> r | kept >> second) & 1)) continue;
-        // a row that is left out is not read
-        const int a = (kept >> r) & 1 ? r : second, b = (kept >> second) & 1 ? second : r;
-        const T *const row[2] = {source_row<T>(h, a), source_row<T>(h, b)};
-        const int at[2] = {a, b};
-        float s[2];
-        quantize_rows<3, 2>(row, h, kp, lane, s, [&](int u, int d, uint32_t x) { *reinterpret_cast<uint32_t *>(smem + at[u] * ls + d) = x; });
-        if (lane == 0) scales[a] = s[0] * kDown, scales[b] = s[1] * kDown;
+    constexpr int kRows = 4;  // of a wave at a time
+    for (int r0 = wave; r0 < rows; r0 += kRows * kFewWaves) {
+        const T *row[kRows];
+        bool on[kRows];  // a row that is left out is not read
+        float s[kRows];
+#pragma unroll
+        for (int u = 0; u < kRows; u++) {
+            const int r = r0 + u * kFewWaves;
+            on[u] = r < rows && ((kept >> r) & 1);
+            row[u] = on[u] ? source_row<T>(h, r) : nullptr;
+        }
+        quantize_rows<true, 2, kRows>(row, on, h, kp, lane, s, [&](int u, int d, uint2 x) {
+            *reinterpret_cast<uint2 *>(smem + (r0 + u * kFewWaves) * ls + d) = x;
+        });
+#pragma unroll
+        for (int u = 0; u < kRows; u++)
+            if (on[u] && lane == 0) scales[r0 + u * kFewWaves] = s[u] * kDown;
     }
     __syncthreads();
 
@@ -199,11 +254,12 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void k_few8(Source h, const uint
             load(w[1], k + 3 * kAhead);
         }
         const int done = c0;
+        const ColumnScale col = next;
         g += gridDim.x;
         const bool more = g < groups;
         if (more) seek();
         if (KS == 1) {
-            epi.template run<MB>(acc, done + i, W, scales, rows, kept, q);
+            epi.template run<MB>(acc, done + i, W, col, scales, rows, kept, q);
         } else {
 #pragma unroll
             for (int m = 0; m < MB; m++) part[(wave * MB + m) * 64 + lane] = acc[m];
@@ -213,7 +269,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void k_few8(Source h, const uint
                 for (int m = 0; m < MB; m++)
 #pragma unroll
                     for (int k = 1; k < kFewWaves; k++) acc[m] += part[(k * MB + m) * 64 + lane];
-                epi.template run<MB>(acc, done + i, W, scales, rows, kept, q);
+                epi.template run<MB>(acc, done + i, W, col, scales, rows, kept, q);
             }
             __syncthreads();
         }
@@ -228,7 +284,7 @@ inline int cu_count(int *cus) {
     return GS_OK;
 }
 
-inline bool few8_ok(int rows, int kp) { return rows <= kFewRows && few_lds(rows, kp, kFewWaves) <= kFewLds; }
+inline bool few8_ok(int rows, int kp, int64_t dim_stride) { return dim_stride == 1 && rows <= kFewRows && few_lds(rows, kp, kFewWaves) <= kFewLds; }
 
 // Once per device and kernel: LDS beyond 64 KiB
 inline int allow_lds(const void *f, int bytes, std::atomic<uint64_t> &set) {

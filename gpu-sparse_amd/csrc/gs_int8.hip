@@ -2,105 +2,151 @@
 //   gs_quantize_rows   a matrix's rows as whole numbers and a scale each
 //   gs_int8_linear     y = x W^T + b; x is quantised per row within the call, sums are whole numbers
 #include "gs_int8.h"
+#include <stdlib.h>
 
 namespace gsv {
 
-// A wave per row.  Bytes bound it (two or four per value in, one out).
-template <int HT>
-__global__ __launch_bounds__(256) void k_quantize_rows(Source x, int64_t rows, int dimp, int8_t *out, int64_t stride, float *scales, float by) {
+// A wave per row; workgroups after those write the bias in fp32.  Bytes bound it (two or four per value in, one out).
+template <int HT, bool UNIT>
+__global__ __launch_bounds__(256) void k_quantize_rows(Source x, int64_t rows, int row_blocks, int dimp, int8_t *out, int64_t stride, float *scales,
+                                                       float by, const void *bias, int bias_type, int n, float *bias_o) {
     using T = typename HVal<HT>::t;
+    if ((int)blockIdx.x >= row_blocks) {
+        const int v = ((int)blockIdx.x - row_blocks) * 256 + (int)threadIdx.x;
+        if (v < n) bias_o[v] = bias_at(bias, bias_type, v);
+        return;
+    }
     const int lane = gs_lane();
-    for (int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); i < rows; i += (int64_t)gridDim.x * 4) {
-        const T *const row[1] = {(const T *)x.p + i * x.s1};
+    for (int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); i < rows; i += (int64_t)row_blocks * 4) {
+        const T *row[1] = {(const T *)x.p + i * x.s1};
+        const bool on[1] = {true};
         float scale[1];
-        quantize_rows<4, 1>(row, x, dimp, lane, scale, [&](int, int d, uint32_t w) { *reinterpret_cast<uint32_t *>(out + i * stride + d) = w; });
+        quantize_rows<UNIT, 2, 1>(row, on, x, dimp, lane, scale, [&](int, int d, uint2 w) { *reinterpret_cast<uint2 *>(out + i * stride + d) = w; });
         if (lane == 0) scales[i] = scale[0] * by;
     }
 }
 
-int quantize(const Source &x, int type, int64_t rows, int dimp, int8_t *out, int64_t stride, float *scales, float by, hipStream_t s) {
-    const dim3 g(gs_blocks(rows, 4, 8192));
-#define GSV_QUANTIZE(HT) hipLaunchKernelGGL((k_quantize_rows<HT>), g, dim3(256), 0, s, x, rows, dimp, out, stride, scales, by)
-    if (type == GS_H_F32) GSV_QUANTIZE(GS_H_F32);
-    else if (type == GS_H_F16) GSV_QUANTIZE(GS_H_F16);
-    else GSV_QUANTIZE(GS_H_BF16);
+int quantize(const Source &x, int type, int64_t rows, int dimp, int8_t *out, int64_t stride, float *scales, float by, const void *bias,
+             int bias_type, int n, float *bias_o, hipStream_t s) {
+    const int row_blocks = (int)gs_blocks(rows, 4, 8192);
+    const dim3 g(row_blocks + (n + 255) / 256);
+#define GSV_QUANTIZE(HT)                                                                                                                   \
+    if (x.sd == 1)                                                                                                                         \
+        hipLaunchKernelGGL((k_quantize_rows<HT, true>), g, dim3(256), 0, s, x, rows, row_blocks, dimp, out, stride, scales, by, bias, bias_type, \
+                           n, bias_o);                                                                                                     \
+    else                                                                                                                                   \
+        hipLaunchKernelGGL((k_quantize_rows<HT, false>), g, dim3(256), 0, s, x, rows, row_blocks, dimp, out, stride, scales, by, bias, bias_type, \
+                           n, bias_o)
+    if (type == GS_H_F32) { GSV_QUANTIZE(GS_H_F32); }
+    else if (type == GS_H_F16) { GSV_QUANTIZE(GS_H_F16); }
+    else { GSV_QUANTIZE(GS_H_BF16); }
 #undef GSV_QUANTIZE
     GS_CHECK_LAUNCH();
     return GS_OK;
 }
 
-// A tile's outputs: rows are columns of y (rows of the weight), columns its rows (tokens), so that a lane holds four values on end.
+// Values on end of an output row, which may start anywhere
+template <class O, int N>
+struct Run {
+    typedef O vec __attribute__((ext_vector_type(N), aligned(sizeof(O))));
+};
+
+// A tile's outputs: rows are columns of y (rows of the weight), columns its rows (tokens), so that a lane holds four values on
+// end.  16-bit ones: lanes of two rows of lanes swap halves, as in store_blocks, so that a lane writes eight.
 template <class O>
 struct EpiLinear {
-    const float *w_scales, *x_scales;  // x's times kDown
-    const void *bias;
-    int bias_type;
+    const float *w_scales, *x_scales, *bias;  // x's times kDown
     O *out;
     int64_t ld;
-    int vec;  // rows of the output are aligned to four values
-    static constexpr int sides = 2;
+    static constexpr int sides = 3;
     static constexpr bool row_bias = false;
     __device__ __forceinline__ SideArray side(int a, int r0, int c0, const Shape &s) const {
-        return a == 0 ? SideArray{w_scales + r0, s.nr - r0} : SideArray{x_scales + c0, s.nc - c0};
+        if (a == 1) return {x_scales + c0, s.nc - c0};
+        return {(a == 0 ? w_scales : bias) + r0, s.nr - r0};
     }
-    struct Bias {
-        f32x4 b[8];
-    };
+    struct None {};
     template <class TL>
-    __device__ __forceinline__ auto before(const Place &at) const {
-        Bias h;
-        const int q = at.lane >> 4;
-#pragma unroll
-        for (int i = 0; i < TL::MR; i++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int v = at.row0 + 16 * i + 4 * q + e;
-                h.b[i][e] = bias_at(bias, bias_type, min(v, at.n_r - 1));
-            }
-        return h;
+    __device__ __forceinline__ None before(const Place &) const {
+        return {};
     }
-    template <class TL, class H>
-    __device__ __forceinline__ void run(f32x4 (&acc)[TL::MR][TL::MC], const Place &at, const H &held) const {
+    template <int N>
+    __device__ __forceinline__ static void put(O *to, const O (&y)[N], int left) {
+        if (left >= N) {
+            typename Run<O, N>::vec v;
+#pragma unroll
+            for (int e = 0; e < N; e++) v[e] = y[e];
+            *reinterpret_cast<typename Run<O, N>::vec *>(to) = v;
+        } else {
+#pragma unroll
+            for (int e = 0; e < N; e++)
+                if (e < left) to[e] = y[e];
+        }
+    }
+    template <class TL>
+    __device__ __forceinline__ void run(f32x4 (&acc)[TL::MR][TL::MC], const Place &at, const None &) const {
+        static_assert(TL::MR % 2 == 0, "blocks of rows go in pairs");
         const int q = at.lane >> 4;
 #pragma unroll
-        for (int i = 0; i < TL::MR; i++) {
-            const f32x4 sw = at.side4(0, at.r_in + 16 * i + 4 * q);
-            const int v = at.row0 + 16 * i + 4 * q;
+        for (int j = 0; j < TL::MC; j++) {
+            const int n = at.col0 + 16 * j + (at.lane & 15);
+            const float sx = at.side(1, at.c_in + 16 * j + (at.lane & 15));
+            O *row = out + n * ld;
 #pragma unroll
-            for (int j = 0; j < TL::MC; j++) {
-                const int n = at.col0 + 16 * j + (at.lane & 15);
-                const float sx = at.side(1, at.c_in + 16 * j + (at.lane & 15));
-                const f32x4 x = __builtin_convertvector(__builtin_bit_cast(i32x4, acc[i][j]), f32x4) * sx * sw;
-                f32x4 y;
+            for (int i = 0; i < TL::MR; i += 2) {
+                O y[8];
 #pragma unroll
-                for (int e = 0; e < 4; e++) y[e] = fmaf(x[e], kUp, held.b[i][e]);
-                if (n >= at.n_c) continue;
-                O *to = out + n * ld + v;
-                if (vec && v + 3 < at.n_r) store4(to, y);
-                else
-                    for (int e = 0; e < 4; e++)
-                        if (v + e < at.n_r) to[e] = (O)y[e];
+                for (int h = 0; h < 2; h++) {
+                    const int in = at.r_in + 16 * (i + h) + 4 * q;
+                    const f32x4 x = __builtin_convertvector(__builtin_bit_cast(i32x4, acc[i + h][j]), f32x4) * sx * at.side4(0, in);
+                    const f32x4 b = at.side4(2, in);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) y[4 * h + e] = (O)fmaf(x[e], kUp, b[e]);
+                }
+                if constexpr (sizeof(O) == 2) {
+                    const auto two = [&](int e) {
+                        return (uint32_t)__builtin_bit_cast(uint16_t, y[e]) | (uint32_t)__builtin_bit_cast(uint16_t, y[e + 1]) << 16;
+                    };
+                    const auto u = __builtin_amdgcn_permlane16_swap(two(0), two(4), false, false);
+                    const auto v = __builtin_amdgcn_permlane16_swap(two(2), two(6), false, false);
+                    const uint32_t w[4] = {u[0], v[0], u[1], v[1]};
+#pragma unroll
+                    for (int e = 0; e < 8; e++) y[e] = __builtin_bit_cast(O, (uint16_t)(w[e / 2] >> 16 * (e & 1)));
+                    const int c = at.row0 + 16 * (i + (q & 1)) + 8 * (q >> 1);
+                    if (n < at.n_c) put<8>(row + c, y, at.n_r - c);
+                } else {
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const int c = at.row0 + 16 * (i + h) + 4 * q;
+                        const O z[4] = {y[4 * h], y[4 * h + 1], y[4 * h + 2], y[4 * h + 3]};
+                        if (n < at.n_c) put<4>(row + c, z, at.n_r - c);
+                    }
+                }
             }
         }
     }
 };
 
 // What k_few8 makes of a block's sums: lane l holds rows 16 m + 4 (l >> 4) .. + 3 of column v.
-template <class O>
 struct EpiFewLinear {
     const void *bias;
-    int bias_type;
-    O *out;
+    void *out;
+    int bias_type, out_type;
+    __device__ __forceinline__ ColumnScale column(int v, const Weight8 &W) const { return column_scale(v, W, bias, bias_type); }
     template <int MB>
-    __device__ __forceinline__ void run(const i32x4 (&acc)[MB], int v, const Weight8 &W, const float *scales, int rows, uint64_t, int q) const {
+    __device__ __forceinline__ void run(const i32x4 (&acc)[MB], int v, const Weight8 &W, const ColumnScale &col, const float *scales, int rows,
+                                        uint64_t, int q) const {
         if (v >= W.n) return;
-        const float by = W.scales[v], b = bias_at(bias, bias_type, v);
 #pragma unroll
         for (int m = 0; m < MB; m++)
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 const int row = 16 * m + 4 * q + e;
-                if (row < rows) out[(int64_t)row * W.n + v] = (O)fmaf((float)acc[m][e] * scales[row] * by, kUp, b);
+                if (row >= rows) continue;
+                const float y = fmaf((float)acc[m][e] * scales[row] * col.by, kUp, col.bias);
+                const int64_t to = (int64_t)row * W.n + v;
+                if (out_type == GS_H_F32) ((float *)out)[to] = y;
+                else if (out_type == GS_H_F16) ((_Float16 *)out)[to] = (_Float16)y;
+                else ((__bf16 *)out)[to] = (__bf16)y;
             }
     }
 };
@@ -124,9 +170,8 @@ int check_stride8(const char *what, const void *p, int64_t stride, int dim) {
     return GS_OK;
 }
 
-Source rows_source(const void *p, int type, int64_t row_stride, int64_t dim_stride, int dim) {
-    const bool vec = dim_stride == 1 && row_stride % 4 == 0 && (uintptr_t)p % (type == GS_H_F32 ? 16 : 8) == 0;
-    return Source{p, 0, row_stride, dim_stride, 0x7FFFFFFF, dim, vec};
+Source rows_source(const void *p, int64_t row_stride, int64_t dim_stride, int dim) {
+    return Source{p, 0, row_stride, dim_stride, 0x7FFFFFFF, dim, 0};
 }
 
 int check_linear(const gs_linear8 *a) {
@@ -141,14 +186,15 @@ int check_linear(const gs_linear8 *a) {
 
 struct Scratch8 {
     int8_t *x;
-    float *scales;
+    float *scales, *bias;
     int dimp;
     bool few;
 };
 Scratch8 scratch_of(gs_arena &a, const gs_linear8 *l) {
-    Scratch8 s{nullptr, nullptr, (int)round_up(l->dim, kPad8), few8_ok(l->rows, (int)round_up(l->dim, kPad8))};
+    Scratch8 s{nullptr, nullptr, nullptr, (int)round_up(l->dim, kPad8), few8_ok(l->rows, (int)round_up(l->dim, kPad8), l->x_dim_stride)};
     if (s.few) return s;
     s.scales = a.take<float>(l->rows);
+    s.bias = a.take<float>(l->out);
     s.x = a.take<int8_t>((size_t)l->rows * s.dimp);
     return s;
 }
@@ -157,11 +203,11 @@ template <class O>
 int run_product(const gs_linear8 *l, const Scratch8 &s, int cus, hipStream_t st) {
     const Operand w{(const uint16_t *)l->values_d, l->values_stride / 2, 0, s.dimp / 2}, x{(const uint16_t *)s.x, s.dimp / 2, 0, s.dimp / 2};
     const Dims d{l->out, l->rows, s.dimp / 2, nullptr, 0, 0, 0};
-    const bool vec = l->out % 4 == 0 && (uintptr_t)l->out_d % (4 * sizeof(O)) == 0;
-    const EpiLinear<O> epi{l->scales_d, s.scales, l->bias_d, l->bias_type, (O *)l->out_d, l->out, vec};
+    const EpiLinear<O> epi{l->scales_d, s.scales, s.bias, (O *)l->out_d, l->out};
     const auto tiles = [&](int e) { return (int64_t)((l->out + e - 1) / e) * ((l->rows + e - 1) / e); };
-    if (tiles(256) >= cus) return launch_product<Large8<I8>>(w, x, d, epi, cus, st);
-    if (tiles(128) >= cus) return launch_product<Mid8<I8>>(w, x, d, epi, cus, st);
+    static const int force = getenv("GSX") ? atoi(getenv("GSX")) : 0;
+    if (force == 1 || (!force && tiles(256) >= cus)) return launch_product<Large8<I8>>(w, x, d, epi, cus, st);
+    if (force == 2 || (!force && tiles(128) >= cus)) return launch_product<Mid8<I8>>(w, x, d, epi, cus, st);
     return launch_product<Small8<I8>>(w, x, d, epi, cus, st);
 }
 
@@ -176,8 +222,8 @@ extern "C" int gs_quantize_rows(const void *x_d, int32_t type, int64_t rows, int
     if (int rc = check_stride8("quantize_rows", values_d, values_stride, dim)) return rc;
     if (rows == 0) return GS_OK;
     GS_REQUIRE(x_d && values_d && scales_d, "NULL rows, values or scales");
-    return quantize(rows_source(x_d, type, row_stride, dim_stride, dim), type, rows, (int)round_up(dim, kPad8), values_d, values_stride,
-                    scales_d, 1.f, gs_stream(stream));
+    return quantize(rows_source(x_d, row_stride, dim_stride, dim), type, rows, (int)round_up(dim, kPad8), values_d, values_stride,
+                    scales_d, 1.f, nullptr, GS_H_F32, 0, nullptr, gs_stream(stream));
 }
 
 extern "C" int gs_int8_linear_workspace(const gs_linear8 *l, size_t *bytes) {
@@ -202,21 +248,15 @@ extern "C" int gs_int8_linear(const gs_linear8 *l, void *workspace_d, size_t wor
     int cus = 0;
     if (int rc = cu_count(&cus)) return rc;
     const hipStream_t st = gs_stream(stream);
-    const Source x = rows_source(l->x_d, l->type, l->x_row_stride, l->x_dim_stride, l->dim);
+    const Source x = rows_source(l->x_d, l->x_row_stride, l->x_dim_stride, l->dim);
     if (s.few) {
         const Weight8 W{l->values_d, l->values_stride, l->scales_d, l->out};
-#define GSV_FEW(HT, O) return launch_few8<typename HVal<HT>::t>(x, nullptr, l->rows, W, s.dimp, EpiFewLinear<O>{l->bias_d, l->bias_type, (O *)l->out_d}, cus, st)
-#define GSV_FEW_OUT(HT)                                   \
-    if (l->out_type == GS_H_F32) GSV_FEW(HT, float);      \
-    if (l->out_type == GS_H_F16) GSV_FEW(HT, _Float16);   \
-    GSV_FEW(HT, __bf16)
-        if (l->type == GS_H_F32) { GSV_FEW_OUT(GS_H_F32); }
-        if (l->type == GS_H_F16) { GSV_FEW_OUT(GS_H_F16); }
-        GSV_FEW_OUT(GS_H_BF16);
-#undef GSV_FEW_OUT
-#undef GSV_FEW
+        const EpiFewLinear epi{l->bias_d, l->out_d, l->bias_type, l->out_type};
+        if (l->type == GS_H_F32) return launch_few8<float>(x, nullptr, l->rows, W, s.dimp, epi, cus, st);
+        if (l->type == GS_H_F16) return launch_few8<_Float16>(x, nullptr, l->rows, W, s.dimp, epi, cus, st);
+        return launch_few8<__bf16>(x, nullptr, l->rows, W, s.dimp, epi, cus, st);
     }
-    if (int rc = quantize(x, l->type, l->rows, s.dimp, s.x, s.dimp, s.scales, kDown, st)) return rc;
+    if (int rc = quantize(x, l->type, l->rows, s.dimp, s.x, s.dimp, s.scales, kDown, l->bias_d, l->bias_type, l->out, s.bias, st)) return rc;
     if (l->out_type == GS_H_F32) return run_product<float>(l, s, cus, st);
     if (l->out_type == GS_H_F16) return run_product<_Float16>(l, s, cus, st);
     return run_product<__bf16>(l, s, cus, st);

@@ -388,17 +388,86 @@ __global__ __launch_bounds__(256) void k_pack(Source h, const int *rows, const i
 }
 
 // The same for a vocabulary in 8 bits, which is read where it is: the kept hidden states as 8-bit rows of `dimp` values, and
-// their scales.
-template <int HT>
+// their scales.  Where k_setup has listed the kept rows:
+template <int HT, bool UNIT>
 __global__ __launch_bounds__(256) void k_pack8(Source h, const int *rows, const int *n_d, int dimp, int8_t *out, float *scales) {
     using T = typename HVal<HT>::t;
     const int n = *n_d, lane = gs_lane();
     for (int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); i < n; i += (int64_t)gridDim.x * 4) {
-        const T *const row[1] = {source_row<T>(h, rows[i])};
+        const T *row[1] = {source_row<T>(h, rows[i])};
+        const bool on[1] = {true};
         float scale[1];
-        quantize_rows<4, 1>(row, h, dimp, lane, scale, [&](int, int d, uint32_t x) { *reinterpret_cast<uint32_t *>(out + i * dimp + d) = x; });
+        quantize_rows<UNIT, 2, 1>(row, on, h, dimp, lane, scale, [&](int, int d, uint2 x) { *reinterpret_cast<uint2 *>(out + i * dimp + d) = x; });
         if (lane == 0) scales[i] = scale[0] * kDown;
     }
+}
+// And where it has not: a workgroup takes kPackRows rows and counts the kept ones before them in the mask itself (a byte per row,
+// from the L2), so that there is one launch for both, and no walk by one workgroup: 64 texts of 256 tokens XXX.  Workgroups after
+// those write the bias.
+constexpr int kPackRows = 16, kPackMost = 1 << 16;
+template <int HT, bool UNIT>
+__global__ __launch_bounds__(256) void k_setup_pack8(Source h, const uint8_t *mask, int total, int texts, int row_blocks, int dimp, int8_t *out,
+                                                     float *scales, int *seg, int *text_first, int *n, const void *bias, int bias_type,
+                                                     int vocab, int padded, float *bias_o) {
+    using T = typename HVal<HT>::t;
+    __shared__ int part[4];
+    const int tid = threadIdx.x, lane = gs_lane(), wave = tid >> 6;
+    if ((int)blockIdx.x >= row_blocks) {
+        const int v = ((int)blockIdx.x - row_blocks) * 256 + tid;
+        if (v < padded) bias_o[v] = v < vocab ? bias_at(bias, bias_type, v) : -INFINITY;
+        return;
+    }
+    const int r0 = blockIdx.x * kPackRows, length = h.length;
+    const auto is_kept = [&](int r) { return r < total && (!mask || mask[r] != 0); };
+    int before = 0;
+    if (!mask) {
+        before = r0;
+    } else {
+        int c = 0;
+        for (int r = tid * 16; r < r0; r += 4096) {  // whole pieces: r0 is a multiple of 16
+            typedef uint32_t words __attribute__((ext_vector_type(4), aligned(1)));
+            const words x = *reinterpret_cast<const words *>(mask + r);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const uint32_t any = ((x[e] & 0x7F7F7F7Fu) + 0x7F7F7F7Fu) | x[e];  // bit 7 of each byte that is not 0
+                c += __popc(any & 0x80808080u);
+            }
+        }
+        c = (int)gs_wave_sum((uint32_t)c);
+        if (lane == 0) part[wave] = c;
+        __syncthreads();
+        before = part[0] + part[1] + part[2] + part[3];
+    }
+    const uint64_t kept = __ballot(lane < kPackRows && is_kept(min(r0 + lane, total)));
+    if (wave == 0 && lane < kPackRows) {
+        const int r = r0 + lane, at = before + __popcll(kept & gs_lanemask_lt());
+        if (r < total) {
+            const int text = r / length;
+            if (r == text * length) text_first[text] = at;
+            if ((kept >> lane) & 1) seg[at] = text;
+        }
+    }
+    if ((int)blockIdx.x == row_blocks - 1) {
+        const int all = before + __popcll(kept);
+        if (tid == 0) *n = all, text_first[texts] = all;
+        for (int i = all + tid; i < (int)round_up(all, kRowPad); i += 256) seg[i] = -1;
+    }
+    constexpr int kRows = 4;  // of a wave
+    const T *row[kRows];
+    bool on[kRows];
+    float s[kRows];
+    int at[kRows];
+#pragma unroll
+    for (int u = 0; u < kRows; u++) {
+        const int in = wave + 4 * u;
+        on[u] = (kept >> in) & 1;
+        at[u] = before + __popcll(kept & ((1ull << in) - 1));
+        row[u] = on[u] ? source_row<T>(h, r0 + in) : nullptr;
+    }
+    quantize_rows<UNIT, 2, kRows>(row, on, h, dimp, lane, s, [&](int u, int d, uint2 x) { *reinterpret_cast<uint2 *>(out + (int64_t)at[u] * dimp + d) = x; });
+#pragma unroll
+    for (int u = 0; u < kRows; u++)
+        if (on[u] && lane == 0) scales[at[u]] = s[u] * kDown;
 }
 
 // One upstream value for all rows is kept out of the rounding of the logit gradients, so that their largest parts, p - 1
@@ -1273,11 +1342,11 @@ struct EpiFewTerms {
     const void *bias;
     int bias_type, texts, length;
     float *weights;
+    __device__ __forceinline__ ColumnScale column(int v, const Weight8 &W) const { return column_scale(v, W, bias, bias_type); }
     template <int MB>
-    __device__ __forceinline__ void run(const i32x4 (&acc)[MB], int v, const Weight8 &W, const float *scales, int rows, uint64_t kept,
-                                        int q) const {
+    __device__ __forceinline__ void run(const i32x4 (&acc)[MB], int v, const Weight8 &W, const ColumnScale &col, const float *scales, int rows,
+                                        uint64_t kept, int q) const {
         const bool on = v < W.n;
-        const float by = on ? W.scales[v] : 0.f, b = on ? bias_at(bias, bias_type, v) : 0.f;
         f32x4 x[MB];
 #pragma unroll
         for (int m = 0; m < MB; m++)
@@ -1299,7 +1368,7 @@ struct EpiFewTerms {
             join(across<32>(top));
             // the bias of a text without a kept row is not looked at: it may be infinite or NaN
             const bool any = (kept >> lo) & (~0ull >> (64 - length));
-            if (q == 0 && on) weights[(int64_t)text * W.n + v] = log1pf(any ? maximum(fmaf(top * by, kUp, b), 0.f, 0.f) : 0.f);
+            if (q == 0 && on) weights[(int64_t)text * W.n + v] = log1pf(any ? maximum(fmaf(top * col.by, kUp, col.bias), 0.f, 0.f) : 0.f);
         }
     }
 };
@@ -2385,21 +2454,37 @@ int check_texts8(const gs_vocab_head *h) {
     return GS_OK;
 }
 
+// The kept hidden states in 8 bits, where they came from, and the bias.
+template <int HT, bool UNIT>
+int prepare8(const gs_vocab_head *h, const Layout &l, const Source &hs, const uint8_t *mask_d, const Common &c, float *row_scales, hipStream_t s) {
+    if (l.rows <= kPackMost) {
+        const int row_blocks = (l.rows + kPackRows - 1) / kPackRows;
+        hipLaunchKernelGGL((k_setup_pack8<HT, UNIT>), dim3(row_blocks + l.vocabp / 256), dim3(256), 0, s, hs, mask_d, l.rows, h->texts,
+                           row_blocks, 2 * l.dimp, (int8_t *)c.hidden, row_scales, c.seg, c.text_first, c.n, h->bias_d, h->bias_type, h->vocab,
+                           l.vocabp, c.bias);
+        GS_CHECK_LAUNCH();
+        return GS_OK;
+    }
+    hipLaunchKernelGGL(k_setup, dim3(1 + gs_blocks(l.vocabp, 1024, 1024)), dim3(1024), 0, s, Keep{mask_d, nullptr, 0, h->vocab, l.rows},
+                       h->length, c.rows, c.inv, c.seg, c.text_first, c.n, h->bias_d, h->bias_type, h->vocab, l.vocabp, c.bias, nullptr,
+                       (int64_t)0);
+    GS_CHECK_LAUNCH();
+    hipLaunchKernelGGL((k_pack8<HT, UNIT>), dim3(gs_blocks(l.rows, 4, 8192)), dim3(256), 0, s, hs, c.rows, c.n, 2 * l.dimp, (int8_t *)c.hidden,
+                       row_scales);
+    GS_CHECK_LAUNCH();
+    return GS_OK;
+}
+
 template <int HT>
 int run_terms8(const gs_vocab_head *h, const Layout &l, const float *scales_d, const uint8_t *mask_d, float *weights_d, const Common &c,
                float *best, float *row_scales, int cus, hipStream_t s) {
     using T = typename HVal<HT>::t;
     const Source hs = hidden_source(h);
-    if (few8_ok(l.rows, 2 * l.dimp))
+    if (few8_ok(l.rows, 2 * l.dimp, h->hidden_dim_stride))
         return launch_few8<T>(hs, mask_d, l.rows, Weight8{(const int8_t *)h->weight_d, h->weight_row_stride, scales_d, h->vocab}, 2 * l.dimp,
                               EpiFewTerms{h->bias_d, h->bias_type, h->texts, h->length, weights_d}, cus, s);
-    hipLaunchKernelGGL(k_setup, dim3(1 + gs_blocks(l.vocabp, 1024, 1024)), dim3(1024), 0, s, Keep{mask_d, nullptr, 0, h->vocab, l.rows},
-                       h->length, c.rows, c.inv, c.seg, c.text_first, c.n, h->bias_d, h->bias_type, h->vocab, l.vocabp, c.bias, nullptr,
-                       (int64_t)0);
-    GS_CHECK_LAUNCH();
-    hipLaunchKernelGGL((k_pack8<HT>), dim3(gs_blocks(l.rows, 4, 8192)), dim3(256), 0, s, hs, c.rows, c.n, 2 * l.dimp, (int8_t *)c.hidden,
-                       row_scales);
-    GS_CHECK_LAUNCH();
+    if (int rc = hs.sd == 1 ? prepare8<HT, true>(h, l, hs, mask_d, c, row_scales, s) : prepare8<HT, false>(h, l, hs, mask_d, c, row_scales, s))
+        return rc;
     const Dims d{l.rows, h->vocab, l.dimp, c.n, 1, 0, 0};
     const Operand hid{c.hidden, l.dimp, 0, l.dimp}, w{(const uint16_t *)h->weight_d, h->weight_row_stride / 2, 0, l.dimp};
     const EpiTextMax<false, true> epi{c.bias, c.seg, best, nullptr, h->vocab, row_scales, scales_d};
@@ -2431,7 +2516,7 @@ extern "C" int gs_term_weights8_workspace(const gs_vocab_head *h, size_t *bytes)
     gs_arena a{nullptr, 0, 0};
     Common c;
     float *best, *row_scales;
-    if (!few8_ok(l.rows, 2 * l.dimp)) take_terms8(a, l, h, &c, &best, &row_scales);
+    if (!few8_ok(l.rows, 2 * l.dimp, h->hidden_dim_stride)) take_terms8(a, l, h, &c, &best, &row_scales);
     *bytes = a.used;
     return GS_OK;
 }
@@ -2443,7 +2528,7 @@ extern "C" int gs_term_weights8(const gs_vocab_head *h, const float *scales_d, c
     gs_arena a{(char *)workspace_d, 0, workspace_bytes};
     Common c{};
     float *best = nullptr, *row_scales = nullptr;
-    if (!few8_ok(l.rows, 2 * l.dimp)) take_terms8(a, l, h, &c, &best, &row_scales);
+    if (!few8_ok(l.rows, 2 * l.dimp, h->hidden_dim_stride)) take_terms8(a, l, h, &c, &best, &row_scales);
     if (!a.ok()) {
         gs_set_error("term_weights8 workspace too small: need %zu bytes, got %zu", a.used, workspace_bytes);
         return GS_ENOSPC;

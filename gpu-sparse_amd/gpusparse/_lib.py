@@ -354,7 +354,7 @@ def require_gpu(device=None) -> torch.device:
 
 def stream_ptr(device: torch.device) -> int:
     """hipStream_t of the current torch stream on `device`."""
-    return torch.cuda.current_stream(device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if device.index is None else device.index)
 
 
 def ptr(t) -> int | None:
