@@ -4,6 +4,7 @@
 // The gradient sorts the tokens by id, stably and without an atomic that decides an order, and sums runs of equal ids: every
 // sum has one order, and each row of dW is written once, zeros included.
 #include "gs_int8.h"
+#include <stdlib.h>
 
 namespace gsv {
 
@@ -24,49 +25,53 @@ struct Ids {
 
 // ---------------------------------------------------------------- lookup
 
-// A thread takes U pieces of N values, 256 apart.  Bytes bound it.
-template <class T, class O, int N, int U>
-__global__ __launch_bounds__(256) void k_embed(Ids ids, const T *table, int64_t stride, const float *scales, int vocab, int dim, int pieces,
+// A thread takes U pieces of N values, 256 apart: all ids first, then all rows, so that their loads are on their way together.
+// TAIL: a row's last piece is not whole.  Bytes bound it.
+template <class T, class O, int N, int U, bool TAIL>
+__global__ __launch_bounds__(256) void k_embed(Ids ids, const T *table, int64_t stride, const float *scales, int vocab, int dim, uint32_t pieces,
                                                int64_t total, float scale, O *out) {
-    const int64_t base = (int64_t)blockIdx.x * (256 * U);
-    const int64_t n0 = base / pieces;
-    const int p0 = (int)(base - n0 * pieces);
+    const int64_t base = (int64_t)blockIdx.x * (256 * U), n0 = base / pieces;
+    const uint32_t p0 = (uint32_t)(base - n0 * pieces), most = (uint32_t)min((int64_t)(256 * U), total - base) - 1;
     typename Piece<T, N>::vec x[U];
     float by[U];
-    int64_t to[U];
-    int left[U];
+    uint32_t row[U], d[U];
+    int64_t id[U];
 #pragma unroll
     for (int u = 0; u < U; u++) {
-        const uint32_t at = p0 + u * 256 + threadIdx.x, r = at / (uint32_t)pieces;
-        const int64_t n = n0 + r;
-        const int d = (int)(at - r * pieces) * N;
-        left[u] = base + u * 256 + threadIdx.x < total ? dim - d : 0;
-        to[u] = n * dim + d;
-        by[u] = scale;
-#pragma unroll
-        for (int e = 0; e < N; e++) x[u][e] = (T)0;
-        if (left[u] <= 0) continue;
-        const int64_t id = ids.at(n);
-        if (id < 0 || id >= vocab) continue;
-        const T *row = table + id * stride + d;
-        if (left[u] >= N) x[u] = reinterpret_cast<const Piece<T, N> *>(row)->v;
-        else
-#pragma unroll
-            for (int e = 0; e < N; e++)
-                if (e < left[u]) x[u][e] = row[e];
-        if (scales) by[u] = scales[id];
+        const uint32_t at = p0 + min(u * 256 + threadIdx.x, most);  // those past the last one take it again, and write nothing
+        row[u] = at / pieces;
+        d[u] = (at - row[u] * pieces) * N;
+        id[u] = ids.at(n0 + row[u]);
     }
 #pragma unroll
     for (int u = 0; u < U; u++) {
-        if (left[u] <= 0) continue;
+        const bool in = id[u] >= 0 && id[u] < vocab;
+        const int64_t v = in ? id[u] : 0;
+        const T *from = table + v * stride + d[u];
+        if (!TAIL || d[u] + N <= dim) {
+            x[u] = reinterpret_cast<const Piece<T, N> *>(from)->v;
+        } else {
+#pragma unroll
+            for (int e = 0; e < N; e++) x[u][e] = d[u] + e < dim ? from[e] : (T)0;
+        }
+        by[u] = scales ? scales[v] : scale;
+        row[u] = in ? row[u] : ~row[u];
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        if (u * 256 + threadIdx.x > most) break;
+        const bool in = (int32_t)row[u] >= 0;
         Piece<O, N> y;
 #pragma unroll
-        for (int e = 0; e < N; e++) y.v[e] = (O)(scales ? (float)x[u][e] * by[u] * scale : (float)x[u][e] * by[u]);
-        if (left[u] >= N) *reinterpret_cast<Piece<O, N> *>(out + to[u]) = y;
-        else
+        for (int e = 0; e < N; e++) y.v[e] = in ? (O)(scales ? (float)x[u][e] * by[u] * scale : (float)x[u][e] * by[u]) : (O)0.f;
+        O *to = out + (n0 + (in ? row[u] : ~row[u])) * dim + d[u];
+        if (!TAIL || d[u] + N <= dim) {
+            *reinterpret_cast<Piece<O, N> *>(to) = y;
+        } else {
 #pragma unroll
             for (int e = 0; e < N; e++)
-                if (e < left[u]) out[to[u] + e] = y.v[e];
+                if (d[u] + e < dim) to[e] = y.v[e];
+        }
     }
 }
 
@@ -86,25 +91,56 @@ __global__ __launch_bounds__(256) void k_embed_strided(Ids ids, const T *table, 
 // how many there are).  The ids are split into kRanges ranges of 2^shift ids.  One workgroup orders a range; it finds its tokens
 // among all ids itself, or, of many tokens, in segments that k_split has sorted by range.
 constexpr int kRanges = 256, kSegs = 1024, kOrderLds = 128 * 1024;
+constexpr int kOrderMost = 160 * 1024 - 12 * 1024;
+constexpr int kDirectWave = 1024, kDirectLds = 64 * 1024;  // tokens that a wave looks through, and what counts may take beside their list
 constexpr int kSplitThreads = 512, kSplitWaves = kSplitThreads / 64, kSplitTile = 1024;
 
 struct Tokens {
     Ids ids;
     int64_t n, padding;
     int vocab, shift, ranges;
-    __device__ __forceinline__ bool kept(int64_t id) const { return id >= 0 && id < vocab && id != padding; }
+    // token n's id, -1 where it is not kept
+    __device__ __forceinline__ int id(int64_t n) const {
+        uint32_t v;
+        bool far = false;
+        if (ids.bytes == 8) {
+            const uint2 x = ((const uint2 *)ids.p)[n];
+            v = x.x, far = x.y != 0;
+        } else {
+            v = ((const uint32_t *)ids.p)[n];
+        }
+        return far || v >= (uint32_t)vocab || v == (uint32_t)padding ? -1 : (int)v;
+    }
 };
 
-// Of the lanes that are on: how many before this one hold the same key, and how many do in all.
+// Of the lanes that are on: how many before this one hold the same key of `bits` bits, and how many do in all.
 __device__ __forceinline__ void same_key(uint32_t key, bool on, int bits, int &rank, int &all) {
-    uint64_t same = __ballot(on);
-    for (int b = 0; b < bits; b++) {
-        const bool one = (key >> b) & 1;
-        const uint64_t m = __ballot(on && one);
-        same &= one ? m : ~m;
+    const uint64_t of = __ballot(on);
+    uint32_t lo = (uint32_t)of, hi = (uint32_t)(of >> 32);
+#pragma unroll
+    for (int b = 0; b < 12; b++) {
+        if (b >= bits) break;
+        const uint32_t mine = 0u - ((key >> b) & 1);
+        const uint64_t m = __ballot(mine != 0);
+        lo &= ~(mine ^ (uint32_t)m), hi &= ~(mine ^ (uint32_t)(m >> 32));
     }
+    const uint64_t same = (uint64_t)hi << 32 | lo;
     rank = __popcll(same & gs_lanemask_lt());
     all = __popcll(same);
+}
+// Adds the lanes that are on to their keys' counts.  A few keys are counted together first, since adds to one place wait for each
+// other (262144 tokens of one id: 790 us in all with an add for each).
+__device__ __forceinline__ void add_keys(int *count, int key, bool on) {
+    uint64_t left = __ballot(on);
+#pragma unroll
+    for (int k = 0; k < 3; k++) {
+        if (!left) return;
+        const int first = __builtin_ctzll(left), its = __builtin_amdgcn_readlane(key, first);
+        const uint64_t same = __ballot(key == its) & left;
+        if (gs_lane() == first) atomicAdd(count + its, __popcll(same));
+        left &= ~same;
+    }
+    if (left >> gs_lane() & 1) atomicAdd(count + key, 1);
 }
 
 // Exclusive prefix sums over `n` ints in LDS by a workgroup of W waves, n at most 64 W * 4; returns their total.
@@ -147,8 +183,8 @@ __global__ __launch_bounds__(kSplitThreads) void k_split(Tokens t, int64_t seg_s
     for (int r = lane; r < kRanges; r += 64) count[wave][r] = 0;
     gs_wave_sync();
     for (int64_t n = a + lane; n < b; n += 64) {
-        const int64_t id = t.ids.at(n);
-        if (t.kept(id)) atomicAdd(&count[wave][(int)id >> t.shift], 1);
+        const int id = t.id(n);
+        add_keys(count[wave], id >> t.shift, id >= 0);
     }
     __syncthreads();
     if (tid < kRanges) {
@@ -170,16 +206,17 @@ __global__ __launch_bounds__(kSplitThreads) void k_split(Tokens t, int64_t seg_s
     }
     __syncthreads();
     for (int64_t n0 = a; n0 < b; n0 += 64) {
-        const int64_t n = n0 + lane, id = n < b ? t.ids.at(n) : -1;
-        const bool on = t.kept(id);
-        const int r = on ? (int)id >> t.shift : 0;
+        const int64_t n = n0 + lane;
+        const int id = n < b ? t.id(n) : -1;
+        const bool on = id >= 0;
+        const int r = on ? id >> t.shift : 0;
         int rank, all;
         same_key(r, on, 8, rank, all);
         const int at = count[wave][r];
         gs_wave_sync();
         if (on) {
             pos[s0 + at + rank] = (uint32_t)n;
-            low[s0 + at + rank] = (uint16_t)((int)id & ((1 << t.shift) - 1));
+            low[s0 + at + rank] = (uint16_t)(id & ((1 << t.shift) - 1));
             if (rank == 0) count[wave][r] = at + all;
         }
         gs_wave_sync();
@@ -197,19 +234,20 @@ template <bool SPLIT>
 __global__ __launch_bounds__(1024) void k_order(Tokens t, int64_t seg_size, int segs, const uint32_t *pos, const uint16_t *low, const int *counts,
                                                 const int *begin, Sorted o) {
     extern __shared__ __align__(16) char smem[];
-    __shared__ int wave_sums[16], seg_at[SPLIT ? kSegs + 1 : 1], before_s;
+    __shared__ int wave_sums[16], seg_at[SPLIT ? kSegs + 1 : 1], seg_from[SPLIT ? kSegs : 1], before_s;
     int *count = reinterpret_cast<int *>(smem);  // [waves][width]
     const int tid = threadIdx.x, lane = gs_lane(), wave = tid >> 6;
     const int g = blockIdx.x, width = 1 << t.shift, id0 = g << t.shift;
-    const int waves = min(16, kOrderLds / 4 / width);
+    const int waves = min(16, (SPLIT ? kOrderLds : kDirectLds) / 4 / width);
     for (int i = tid; i < waves * width; i += 1024) count[i] = 0;
     if (tid == 0) before_s = 0;
     __syncthreads();
     int64_t n = t.n;
     if (SPLIT) {
-        for (int s = tid; s < segs; s += 1024) seg_at[s] = counts[(int64_t)g * segs + s];
+        if (tid < segs) seg_at[tid] = counts[(int64_t)g * segs + tid], seg_from[tid] = begin[(int64_t)g * segs + tid];
         int before = 0;
         const int cells = g * segs;  // a whole number of fours where that matters
+#pragma unroll 8
         for (int i = tid * 4; i + 3 < cells; i += 4096) {
             const i32x4 c = *reinterpret_cast<const i32x4 *>(counts + i);
             before += c[0] + c[1] + c[2] + c[3];
@@ -222,57 +260,84 @@ __global__ __launch_bounds__(1024) void k_order(Tokens t, int64_t seg_size, int 
         if (tid == 0) seg_at[segs] = (int)n;
         __syncthreads();
     }
-    // A wave's entries a to b of the range (SPLIT), or tokens, kRounds of 64 at a time, so that their loads are on their way
-    // together: ids within the range (-1: another's), and tokens.
-    constexpr int kRounds = SPLIT ? 4 : 16;
+    // A wave takes entries a to b of the range (SPLIT), or lists those of its tokens that are of the range: id within the range and
+    // token, in order.
     const int64_t per = (n + waves - 1) / waves, a = wave < waves ? min(n, wave * per) : n, b = min(n, a + per);
-    int key[kRounds], below = 0;
-    uint32_t token[kRounds];
-    const auto fetch = [&](int64_t e0, bool count_below) {
-        if (SPLIT) {
-            int64_t at[kRounds];
+    uint32_t *mine = reinterpret_cast<uint32_t *>(count + (waves + 1) * width) + wave * kDirectWave;
+    int m = 0;
+    if (SPLIT) {
+        m = (int)(b - a);
+    } else if (a < b) {
+        constexpr int kRounds = kDirectWave / 64;
+        int id[kRounds], below = 0;
 #pragma unroll
-            for (int k = 0; k < kRounds; k++) {
-                const int64_t e = e0 + k * 64 + lane;
-                int lo = 0, hi = segs;  // the last segment that starts at or before e
-                while (hi - lo > 1) {
-                    const int mid = (lo + hi) >> 1;
-                    if (seg_at[mid] <= e) lo = mid;
-                    else hi = mid;
-                }
-                at[k] = e < b ? lo * seg_size + begin[(int64_t)g * segs + lo] + (e - seg_at[lo]) : -1;
-            }
+        for (int k = 0; k < kRounds; k++) id[k] = t.id(min(a + k * 64 + lane, b - 1));
 #pragma unroll
-            for (int k = 0; k < kRounds; k++) {
-                key[k] = at[k] >= 0 ? low[at[k]] : -1;
-                token[k] = at[k] >= 0 ? pos[at[k]] : 0;
+        for (int k = 0; k < kRounds; k++) {
+            const int in = k * 64 + lane;
+            if (in >= b - a) id[k] = -1;
+            below += id[k] >= 0 && id[k] < id0;
+            const bool on = id[k] >= 0 && id[k] >> t.shift == g;
+            const uint64_t some = __ballot(on);
+            if (!some) continue;
+            if (on) {
+                const int key = id[k] - id0;
+                mine[m + __popcll(some & gs_lanemask_lt())] = (uint32_t)key << 10 | in;
             }
-        } else {
-            int64_t id[kRounds];
-#pragma unroll
-            for (int k = 0; k < kRounds; k++) {
-                const int64_t e = e0 + k * 64 + lane;
-                id[k] = e < b ? t.ids.at(e) : -1;
-            }
-#pragma unroll
-            for (int k = 0; k < kRounds; k++) {
-                const bool on = t.kept(id[k]);
-                key[k] = on && (int)id[k] >> t.shift == g ? (int)id[k] - id0 : -1;
-                token[k] = (uint32_t)(e0 + k * 64 + lane);
-                below += count_below && on && (int)id[k] < id0;
-            }
+            m += __popcll(some);
         }
-    };
-    for (int64_t e0 = a; e0 < b; e0 += kRounds * 64) {
-        fetch(e0, true);
-#pragma unroll
-        for (int k = 0; k < kRounds; k++)
-            if (key[k] >= 0) atomicAdd(&count[wave * width + key[k]], 1);
-    }
-    if (!SPLIT) {
         below = (int)gs_wave_sum((uint32_t)below);
         if (lane == 0) atomicAdd(&before_s, below);
     }
+    gs_wave_sync();
+    // f(key, token, on) for the wave's entries, 64 at a time, kAhead rounds' loads on their way together.  An entry's
+    // segment is the last that starts at or before it, searched for where ranges hold few entries a segment, else walked to.
+    constexpr int kAhead = SPLIT ? 8 : 1;
+    const bool walk = SPLIT && n >= segs * 32;
+    int key[kAhead], seg;
+    uint32_t token[kAhead];
+    const auto search = [&](int64_t e) {
+        int lo = 0, hi = segs;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (seg_at[mid] <= e) lo = mid;
+            else hi = mid;
+        }
+        return lo;
+    };
+    const auto fetch = [&](int e0) {
+        if constexpr (SPLIT) {
+            int64_t at[kAhead];
+#pragma unroll
+            for (int k = 0; k < kAhead; k++) {
+                const int64_t e = a + min(e0 + k * 64 + lane, m - 1);
+                if (walk) {
+                    while (seg_at[seg + 1] <= e) seg++;
+                } else {
+                    seg = search(e);
+                }
+                at[k] = seg * seg_size + seg_from[seg] + (e - seg_at[seg]);
+            }
+#pragma unroll
+            for (int k = 0; k < kAhead; k++) key[k] = low[at[k]], token[k] = pos[at[k]];
+        } else {
+            const uint32_t x = mine[min(e0 + lane, m - 1)];
+            key[0] = x >> 10, token[0] = (uint32_t)a + (x & 1023);
+        }
+    };
+    const auto each = [&](bool again, auto &&f) {
+        if (SPLIT && walk && m > 0) seg = search(a + min(lane, m - 1));
+        for (int e0 = 0; e0 < m; e0 += kAhead * 64) {
+            if (!again || m > kAhead * 64) fetch(e0);
+#pragma unroll
+            for (int k = 0; k < kAhead; k++) {
+                if (e0 + k * 64 >= m) break;
+                f(key[k], token[k], e0 + k * 64 + lane < m);
+                gs_wave_sync();
+            }
+        }
+    };
+    each(false, [&](int key, uint32_t, bool on) { add_keys(count + wave * width, key, on); });
     __syncthreads();
     // over the waves, then over the ids
     int *first = count + waves * width;
@@ -291,25 +356,18 @@ __global__ __launch_bounds__(1024) void k_order(Tokens t, int64_t seg_size, int 
     if (tid == 0 && g == t.ranges - 1) o.start[t.vocab] = base + total;
     for (int i = tid; i < waves * width; i += 1024) count[i] += base + first[i & (width - 1)];
     __syncthreads();
-    for (int64_t e0 = a; e0 < b; e0 += kRounds * 64) {
-        if (b - a > kRounds * 64) fetch(e0, false);
-#pragma unroll
-        for (int k = 0; k < kRounds; k++) {
-            const bool on = key[k] >= 0;
-            if (!__any(on)) continue;
-            int rank, all;
-            same_key(key[k], on, t.shift, rank, all);
-            int *next = &count[wave * width + (on ? key[k] : 0)];
-            const int at = *next;
-            gs_wave_sync();
-            if (on) {
-                o.order[at + rank] = token[k];
-                o.id[at + rank] = id0 + key[k];
-                if (rank == 0) *next = at + all;
-            }
-            gs_wave_sync();
+    each(true, [&](int key, uint32_t token, bool on) {
+        int rank, all;
+        same_key(key, on, t.shift, rank, all);
+        int *next = &count[wave * width + key];
+        const int at = *next;
+        gs_wave_sync();
+        if (on) {
+            o.order[at + rank] = token;
+            o.id[at + rank] = id0 + key;
+            if (rank == 0) *next = at + all;
         }
-    }
+    });
 }
 
 // ---------------------------------------------------------------- sums
@@ -317,7 +375,13 @@ __global__ __launch_bounds__(1024) void k_order(Tokens t, int64_t seg_size, int 
 // A chunk of entries and a slice of 64 N columns are a wave's: it adds the rows of one id after the other in fp32.  A sum whose
 // id has all its entries in the chunk is a row of dW; the others are parts: part[chunk][0] of the id that came from before,
 // part[chunk][1] of the one that started here.  More waves write the zeros of ids without an entry.
-template <class T, int N>
+//
+// STREAM: rows are read past the caches.  Each is read once, so that those that do not fit the 256 MiB of the last of them only
+// throw others out: 262144 rows of 1024 16-bit values 187 -> 156 us; but 16384 of 768, which are still there from what made them,
+// 17 -> 22.
+constexpr int kZeroRows = 16;
+constexpr int64_t kStreamBytes = 256 << 20;
+template <class T, int N, bool STREAM>
 __global__ __launch_bounds__(256) void k_embed_sums(Sorted o, const T *grad, int64_t stride, int vocab, int dim, int chunk, int slices,
                                                     int64_t sum_waves, float scale, float *part, T *dw) {
     using P = Piece<T, N>;
@@ -335,12 +399,11 @@ __global__ __launch_bounds__(256) void k_embed_sums(Sorted o, const T *grad, int
                 if (d + e < dim) row[d + e] = y.v[e];
     };
     if (w >= sum_waves) {
-        constexpr int kRows = 8;
-        const int64_t v0 = (w - sum_waves) * kRows;
-        for (int r = 0; r < kRows; r++) {
-            const int64_t v = v0 + r;
-            if (v >= vocab || o.start[v] != o.start[v + 1]) continue;
-            for (int d = lane * N; d < dim; d += 64 * N) put(dw + v * dim, d, acc_t{});
+        const int64_t v0 = (w - sum_waves) * kZeroRows, v = v0 + lane;
+        uint64_t none = __ballot(lane < kZeroRows && v < vocab && o.start[v] == o.start[v + 1]);
+        for (; none; none &= none - 1) {
+            T *row = dw + (v0 + __builtin_ctzll(none)) * dim;
+            for (int d = lane * N; d < dim; d += 64 * N) put(row, d, acc_t{});
         }
         return;
     }
@@ -379,7 +442,8 @@ __global__ __launch_bounds__(256) void k_embed_sums(Sorted o, const T *grad, int
             for (int u = 0; u < U; u++) {
                 const uint32_t token = __builtin_amdgcn_readlane(my_token, min(k + u, here - 1));
                 const T *row = grad + token * stride + d;
-                if (d + N <= dim) x[u] = reinterpret_cast<const P *>(row)->v;
+                if (d + N <= dim)
+                    x[u] = STREAM ? __builtin_nontemporal_load(&reinterpret_cast<const P *>(row)->v) : reinterpret_cast<const P *>(row)->v;
                 else
 #pragma unroll
                     for (int q = 0; q < N; q++) x[u][q] = d + q < dim ? row[q] : (T)0;
@@ -439,8 +503,8 @@ __global__ __launch_bounds__(1024) void k_embed_few(Tokens t, const T *grad, int
     __shared__ __align__(16) acc_t part[16][64];
     const int tid = threadIdx.x, lane = gs_lane(), wave = gs_uniform(tid >> 6);
     const int width = 1 << t.shift, id0 = blockIdx.x << t.shift, rows = min(width, t.vocab - id0);
-    const int64_t id = tid < t.n ? t.ids.at(tid) : -1;
-    const bool on = t.kept(id) && (int)id >> t.shift == (int)blockIdx.x;
+    const int id = tid < t.n ? t.id(tid) : -1;
+    const bool on = id >= 0 && id >> t.shift == (int)blockIdx.x;
     const auto place = [&](bool flag) {  // of this thread's among the flags, and how many there are
         const uint64_t m = __ballot(flag);
         __syncthreads();
@@ -457,7 +521,7 @@ __global__ __launch_bounds__(1024) void k_embed_few(Tokens t, const T *grad, int
     const int2 mine = place(on);
     const int n = mine.y;
     if (on) {
-        const int key = (int)id - id0;
+        const int key = id - id0;
         list[mine.x] = key << 10 | tid;
         atomicOr(&has[key >> 5], 1u << (key & 31));
     }
@@ -555,8 +619,12 @@ int run_lookup(const gs_lookup *l, const float *scales, O *out, hipStream_t s) {
     constexpr int U = 4;
     const int64_t blocks = (total + 256 * U - 1) / (256 * U);
     GS_REQUIRE(blocks < (1ll << 31), "%lld tokens of %d values exceed a grid", (long long)l->tokens, l->dim);
-    hipLaunchKernelGGL((k_embed<T, O, N, U>), dim3((unsigned)blocks), dim3(256), 0, s, ids, (const T *)l->weight_d, l->weight_row_stride,
-                       scales, l->vocab, l->dim, pieces, total, l->scale, out);
+#define GSV_EMBED(TAIL)                                                                                                            \
+    hipLaunchKernelGGL((k_embed<T, O, N, U, TAIL>), dim3((unsigned)blocks), dim3(256), 0, s, ids, (const T *)l->weight_d,            \
+                       l->weight_row_stride, scales, l->vocab, l->dim, (uint32_t)pieces, total, l->scale, out)
+    if (l->dim % N) GSV_EMBED(true);
+    else GSV_EMBED(false);
+#undef GSV_EMBED
     GS_CHECK_LAUNCH();
     return GS_OK;
 }
@@ -571,14 +639,16 @@ struct GradPlan {
     int *counts, *begin;
     float *part;
 };
-constexpr int64_t kDirect = 16384;  // tokens that every range's workgroup looks through itself
+// Tokens that every range's workgroup looks through itself, 1024 a wave; where counts leave room for fewer than 16 waves, fewer.
+static const int64_t kDirect = getenv("GSD") ? atoi(getenv("GSD")) : 16384;  // tokens that every range's workgroup looks through itself
 
 GradPlan plan_grad(gs_arena &a, const gs_lookup *l) {
     GradPlan p{};
     while ((kRanges << p.shift) < l->vocab) p.shift++;
     p.ranges = (l->vocab + (1 << p.shift) - 1) >> p.shift;
     p.few = l->tokens <= kFewTokens;
-    p.split = l->tokens > kDirect;
+    const int room = kDirectLds / 4 >> p.shift;
+    p.split = l->tokens > (room < 16 ? room : 16) * kDirectWave || l->tokens > kDirect;
     if (p.few) return p;
     p.seg_size = kSplitTile;
     while (p.seg_size * kSegs < l->tokens) p.seg_size *= 2;
@@ -610,22 +680,26 @@ int run_grad(const gs_lookup *l, const GradPlan &p, const void *grad_d, int64_t 
         GS_CHECK_LAUNCH();
         return GS_OK;
     }
-    const int width = 1 << p.shift, waves = 16 < kOrderLds / 4 / width ? 16 : kOrderLds / 4 / width;
-    const int lds = (waves + 1) * width * 4;
+    const int width = 1 << p.shift, room = (p.split ? kOrderLds : kDirectLds) / 4 / width, waves = room < 16 ? room : 16;
+    const int lds = (waves + 1) * width * 4 + (p.split ? 0 : waves * kDirectWave * 4);
     static std::atomic<uint64_t> set{0}, set_split{0};
     if (p.split) {
         hipLaunchKernelGGL(k_split, dim3(p.segs), dim3(kSplitThreads), 0, s, t, p.seg_size, p.segs, p.pos, p.low, p.counts, p.begin);
         GS_CHECK_LAUNCH();
-        if (int rc = allow_lds(reinterpret_cast<const void *>(&k_order<true>), kOrderLds + kOrderLds / 8, set_split)) return rc;
+        if (int rc = allow_lds(reinterpret_cast<const void *>(&k_order<true>), kOrderMost, set_split)) return rc;
         hipLaunchKernelGGL(k_order<true>, dim3(p.ranges), dim3(1024), lds, s, t, p.seg_size, p.segs, p.pos, p.low, p.counts, p.begin, p.o);
     } else {
-        if (int rc = allow_lds(reinterpret_cast<const void *>(&k_order<false>), kOrderLds + kOrderLds / 8, set)) return rc;
+        if (int rc = allow_lds(reinterpret_cast<const void *>(&k_order<false>), kOrderMost, set)) return rc;
         hipLaunchKernelGGL(k_order<false>, dim3(p.ranges), dim3(1024), lds, s, t, p.seg_size, p.segs, p.pos, p.low, p.counts, p.begin, p.o);
     }
     GS_CHECK_LAUNCH();
-    const int64_t sum_waves = (p.chunks * p.slices + 3) / 4 * 4, zero_waves = ((int64_t)l->vocab + 7) / 8;
-    hipLaunchKernelGGL((k_embed_sums<T, N>), dim3((unsigned)((sum_waves + zero_waves + 3) / 4)), dim3(256), 0, s, p.o, (const T *)grad_d, stride,
-                       l->vocab, l->dim, p.chunk, p.slices, sum_waves, l->scale, p.part, (T *)dweight_d);
+    const int64_t sum_waves = (p.chunks * p.slices + 3) / 4 * 4, zero_waves = ((int64_t)l->vocab + kZeroRows - 1) / kZeroRows;
+#define GSV_SUMS(STREAM)                                                                                                             \
+    hipLaunchKernelGGL((k_embed_sums<T, N, STREAM>), dim3((unsigned)((sum_waves + zero_waves + 3) / 4)), dim3(256), 0, s, p.o,         \
+                       (const T *)grad_d, stride, l->vocab, l->dim, p.chunk, p.slices, sum_waves, l->scale, p.part, (T *)dweight_d)
+    if (l->tokens * l->dim * (int64_t)sizeof(T) > kStreamBytes) GSV_SUMS(true);
+    else GSV_SUMS(false);
+#undef GSV_SUMS
     GS_CHECK_LAUNCH();
     if (p.chunks > 1) {
         hipLaunchKernelGGL((k_embed_join<T>), dim3((unsigned)(p.chunks - 1), (l->dim + 255) / 256), dim3(256), 0, s, p.o, l->vocab, l->dim,

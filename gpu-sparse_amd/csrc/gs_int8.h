@@ -74,8 +74,8 @@ __device__ __forceinline__ uint2 quantized8(const Raw8<T> &x, const RowScale &r)
 #pragma unroll
         for (int e = 0; e < 8; e++) {
             const int n = (int)(int8_t)t[e];
-            const float v = x[e] * 0x1p-8f, p = v * 127.f, q = (float)n * most;
-            const float d = p - q, low = fmaf(v, 127.f, -p) - fmaf((float)n, most, -q);
+            const float w = x[e] * 0x1p-8f, p = w * 127.f, q = (float)n * most;
+            const float d = p - q, low = fmaf(w, 127.f, -p) - fmaf((float)n, most, -q);
             const float over = d > 0 ? (d - half) + low : (-d - half) - low;  // |127 x - n most| - most / 2, or its sign
             if (over > 0 || (over == 0 && (n & 1))) t[e] = (uint32_t)(n + (d > 0 ? 1 : -1));
         }
@@ -108,34 +108,34 @@ __device__ __forceinline__ Raw8<T> row8(const T *row, int64_t ds, int d, int dim
     return x;
 }
 
-// N rows by one wave, those that are `on` (which is uniform): put(u, d, bytes) takes row u's values d .. d + 7, zeros from dim to
-// dimp (a multiple of 8); scale receives the scales.  Rows of up to 512 HOLD values are read once, all at a time; longer ones twice.
-template <bool UNIT, int HOLD, int N, class T, class Put>
-__device__ __forceinline__ void quantize_rows(const T *(&row)[N], const bool (&on)[N], const Source &s, int dimp, int lane,
-                                              float (&scale)[N], Put &&put) {
-    Raw8<T> x[N][HOLD];
+// A row's values d = 512 c + 8 lane .. + 7, c < HOLD
+template <int HOLD, class T>
+struct RowStart {
+    Raw8<T> x[HOLD];
+};
+template <bool UNIT, int HOLD, class T>
+__device__ __forceinline__ RowStart<HOLD, T> row_start(const T *row, const Source &s, int lane) {
+    RowStart<HOLD, T> r;
 #pragma unroll
-    for (int u = 0; u < N; u++) {
-        if (!on[u]) continue;
+    for (int c = 0; c < HOLD; c++) r.x[c] = row8<UNIT>(row, s.sd, c * 512 + lane * 8, s.dim);
+    return r;
+}
+// A row by one wave: put(d, bytes) takes values d .. d + 7, zeros from dim to dimp (a multiple of 8); returns the scale.  Rows of up
+// to 512 HOLD values are read once, by row_start; the rest of longer ones twice.
+template <bool UNIT, int HOLD, class T, class Put>
+__device__ __forceinline__ float quantize_row(const T *row, const RowStart<HOLD, T> &start, const Source &s, int dimp, int lane, Put &&put) {
+    uint32_t most = 0;
 #pragma unroll
-        for (int c = 0; c < HOLD; c++) x[u][c] = row8<UNIT>(row[u], s.sd, c * 512 + lane * 8, s.dim);
-    }
-#pragma unroll
-    for (int u = 0; u < N; u++) {
-        if (!on[u]) continue;
-        uint32_t most = 0;
-#pragma unroll
-        for (int c = 0; c < HOLD; c++) most = max(most, magnitude(x[u][c]));
+    for (int c = 0; c < HOLD; c++) most = max(most, magnitude(start.x[c]));
 #pragma unroll 2
-        for (int d = HOLD * 512 + lane * 8; d < s.dim; d += 512) most = max(most, magnitude(row8<UNIT>(row[u], s.sd, d, s.dim)));
-        const RowScale r = row_scale(gs_wave_max_u32(most));
-        scale[u] = r.scale;
+    for (int d = HOLD * 512 + lane * 8; d < s.dim; d += 512) most = max(most, magnitude(row8<UNIT>(row, s.sd, d, s.dim)));
+    const RowScale r = row_scale(gs_wave_max_u32(most));
 #pragma unroll
-        for (int c = 0; c < HOLD; c++)
-            if (c * 512 + lane * 8 < dimp) put(u, c * 512 + lane * 8, quantized8(x[u][c], r));
+    for (int c = 0; c < HOLD; c++)
+        if (c * 512 + lane * 8 < dimp) put(c * 512 + lane * 8, quantized8(start.x[c], r));
 #pragma unroll 1
-        for (int d = HOLD * 512 + lane * 8; d < dimp; d += 512) put(u, d, quantized8(row8<UNIT>(row[u], s.sd, d, s.dim), r));
-    }
+    for (int d = HOLD * 512 + lane * 8; d < dimp; d += 512) put(d, quantized8(row8<UNIT>(row, s.sd, d, s.dim), r));
+    return r.scale;
 }
 
 // The weight: rows of 8-bit values, and their scales.
@@ -207,26 +207,31 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void k_few8(Source h, const uint
         load(w[1], k0 + kAhead);
         next = epi.column(c0 + i, W);
     };
-    seek();
 
-    constexpr int kRows = 4;  // of a wave at a time
-    for (int r0 = wave; r0 < rows; r0 += kRows * kFewWaves) {
-        const T *row[kRows];
-        bool on[kRows];  // a row that is left out is not read
-        float s[kRows];
-#pragma unroll
-        for (int u = 0; u < kRows; u++) {
-            const int r = r0 + u * kFewWaves;
-            on[u] = r < rows && ((kept >> r) & 1);
-            row[u] = on[u] ? source_row<T>(h, r) : nullptr;
-        }
-        quantize_rows<true, 2, kRows>(row, on, h, kp, lane, s, [&](int u, int d, uint2 x) {
-            *reinterpret_cast<uint2 *>(smem + (r0 + u * kFewWaves) * ls + d) = x;
-        });
+    // The wave's rows, every eighth (those that are left out are not read).  The first kRows are asked for before the weight, whose
+    // loads would have to land before theirs otherwise (24 rows, 30522 columns of 768: XXX).
+    const auto here = [&](int r) { return r < rows && ((kept >> r) & 1); };
+    const auto quantize = [&](int r, const RowStart<2, T> &x) {
+        const float scale = quantize_row<true, 2>(source_row<T>(h, r), x, h, kp, lane,
+                                                  [&](int d, uint2 y) { *reinterpret_cast<uint2 *>(smem + r * ls + d) = y; });
+        if (lane == 0) scales[r] = scale * kDown;
+    };
+    constexpr int kRows = MB > 2 ? 4 : 2 * MB;
+    {
+        RowStart<2, T> x[kRows];
 #pragma unroll
         for (int u = 0; u < kRows; u++)
-            if (on[u] && lane == 0) scales[r0 + u * kFewWaves] = s[u] * kDown;
+            if (here(wave + u * kFewWaves)) x[u] = row_start<true, 2>(source_row<T>(h, wave + u * kFewWaves), h, lane);
+        __builtin_amdgcn_sched_barrier(0);
+        seek();
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int u = 0; u < kRows; u++)
+            if (here(wave + u * kFewWaves)) quantize(wave + u * kFewWaves, x[u]);
     }
+    if (kRows * kFewWaves < 16 * MB)
+        for (int r = wave + kRows * kFewWaves; r < rows; r += kFewWaves)
+            if (here(r)) quantize(r, row_start<true, 2>(source_row<T>(h, r), h, lane));
     __syncthreads();
 
     while (true) {

@@ -18,11 +18,10 @@ __global__ __launch_bounds__(256) void k_quantize_rows(Source x, int64_t rows, i
     }
     const int lane = gs_lane();
     for (int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); i < rows; i += (int64_t)row_blocks * 4) {
-        const T *row[1] = {(const T *)x.p + i * x.s1};
-        const bool on[1] = {true};
-        float scale[1];
-        quantize_rows<UNIT, 2, 1>(row, on, x, dimp, lane, scale, [&](int, int d, uint2 w) { *reinterpret_cast<uint2 *>(out + i * stride + d) = w; });
-        if (lane == 0) scales[i] = scale[0] * by;
+        const T *row = (const T *)x.p + i * x.s1;
+        const float scale = quantize_row<UNIT, 2>(row, row_start<UNIT, 2>(row, x, lane), x, dimp, lane,
+                                                  [&](int d, uint2 w) { *reinterpret_cast<uint2 *>(out + i * stride + d) = w; });
+        if (lane == 0) scales[i] = scale * by;
     }
 }
 

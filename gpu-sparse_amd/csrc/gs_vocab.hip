@@ -394,11 +394,10 @@ __global__ __launch_bounds__(256) void k_pack8(Source h, const int *rows, const 
     using T = typename HVal<HT>::t;
     const int n = *n_d, lane = gs_lane();
     for (int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); i < n; i += (int64_t)gridDim.x * 4) {
-        const T *row[1] = {source_row<T>(h, rows[i])};
-        const bool on[1] = {true};
-        float scale[1];
-        quantize_rows<UNIT, 2, 1>(row, on, h, dimp, lane, scale, [&](int, int d, uint2 x) { *reinterpret_cast<uint2 *>(out + i * dimp + d) = x; });
-        if (lane == 0) scales[i] = scale[0] * kDown;
+        const T *row = source_row<T>(h, rows[i]);
+        const float scale = quantize_row<UNIT, 2>(row, row_start<UNIT, 2>(row, h, lane), h, dimp, lane,
+                                                  [&](int d, uint2 x) { *reinterpret_cast<uint2 *>(out + i * dimp + d) = x; });
+        if (lane == 0) scales[i] = scale * kDown;
     }
 }
 // And where it has not: a workgroup takes kPackRows rows and counts the kept ones before them in the mask itself (a byte per row,
@@ -452,22 +451,27 @@ __global__ __launch_bounds__(256) void k_setup_pack8(Source h, const uint8_t *ma
         if (tid == 0) *n = all, text_first[texts] = all;
         for (int i = all + tid; i < (int)round_up(all, kRowPad); i += 256) seg[i] = -1;
     }
-    constexpr int kRows = 4;  // of a wave
-    const T *row[kRows];
-    bool on[kRows];
-    float s[kRows];
-    int at[kRows];
-#pragma unroll
-    for (int u = 0; u < kRows; u++) {
-        const int in = wave + 4 * u;
-        on[u] = (kept >> in) & 1;
-        at[u] = before + __popcll(kept & ((1ull << in) - 1));
-        row[u] = on[u] ? source_row<T>(h, r0 + in) : nullptr;
+    // a wave's kept rows, one asked for before the one before is done
+    RowStart<2, T> x;
+    const T *row = nullptr;
+    int r = -1;
+    for (int in = wave; in < kPackRows + 4; in += 4) {
+        const bool on = in < kPackRows && ((kept >> in) & 1);
+        if (in < kPackRows && !on) continue;
+        const T *row1 = row;
+        RowStart<2, T> x1;
+        if (on) {
+            row1 = source_row<T>(h, r0 + in);
+            x1 = row_start<UNIT, 2>(row1, h, lane);
+        }
+        if (r >= 0) {
+            const int at = before + __popcll(kept & ((1ull << r) - 1));
+            const float scale = quantize_row<UNIT, 2>(row, x, h, dimp, lane,
+                                                      [&](int d, uint2 y) { *reinterpret_cast<uint2 *>(out + (int64_t)at * dimp + d) = y; });
+            if (lane == 0) scales[at] = scale * kDown;
+        }
+        r = in, row = row1, x = x1;
     }
-    quantize_rows<UNIT, 2, kRows>(row, on, h, dimp, lane, s, [&](int u, int d, uint2 x) { *reinterpret_cast<uint2 *>(out + (int64_t)at[u] * dimp + d) = x; });
-#pragma unroll
-    for (int u = 0; u < kRows; u++)
-        if (on[u] && lane == 0) scales[at[u]] = s[u] * kDown;
 }
 
 // One upstream value for all rows is kept out of the rounding of the logit gradients, so that their largest parts, p - 1
