@@ -4,7 +4,6 @@
 // The gradient sorts the tokens by id, stably and without an atomic that decides an order, and sums runs of equal ids: every
 // sum has one order, and each row of dW is written once, zeros included.
 #include "gs_int8.h"
-#include <stdlib.h>
 
 namespace gsv {
 
@@ -89,11 +88,17 @@ __global__ __launch_bounds__(256) void k_embed_strided(Ids ids, const T *table, 
 
 // Tokens sorted by id: order[e], the token of entry e, ascending within an id, and start[v], the first entry of id v (start[vocab]:
 // how many there are).  The ids are split into kRanges ranges of 2^shift ids.  One workgroup orders a range; it finds its tokens
-// among all ids itself, or, of many tokens, in segments that k_split has sorted by range.
-constexpr int kRanges = 256, kSegs = 1024, kOrderLds = 128 * 1024;
-constexpr int kOrderMost = 160 * 1024 - 12 * 1024;
-constexpr int kDirectWave = 1024, kDirectLds = 64 * 1024;  // tokens that a wave looks through, and what counts may take beside their list
+// among all ids itself (16384 tokens: 14 us, a launch), or, of more, in segments that k_split has sorted by range (17, two; 262144
+// tokens 31).
+constexpr int kRanges = 256, kSegs = 1024;
 constexpr int kSplitThreads = 512, kSplitWaves = kSplitThreads / 64, kSplitTile = 1024;
+// A wave of k_order counts ids on its own, in at most so many bytes of LDS for all waves: fewer waves where ranges are wide.  Beside
+// the counts lie the tokens that a wave has found itself, of 1024 that it looks through.
+constexpr int kOrderLds = 128 * 1024, kDirectLds = 64 * 1024, kOrderMost = 148 * 1024, kDirectWave = 1024;
+__host__ __device__ inline int order_waves(int lds, int shift) {
+    const int room = lds / 4 >> shift;
+    return room < 16 ? room : 16;
+}
 
 struct Tokens {
     Ids ids;
@@ -238,7 +243,7 @@ __global__ __launch_bounds__(1024) void k_order(Tokens t, int64_t seg_size, int 
     int *count = reinterpret_cast<int *>(smem);  // [waves][width]
     const int tid = threadIdx.x, lane = gs_lane(), wave = tid >> 6;
     const int g = blockIdx.x, width = 1 << t.shift, id0 = g << t.shift;
-    const int waves = min(16, (SPLIT ? kOrderLds : kDirectLds) / 4 / width);
+    const int waves = order_waves(SPLIT ? kOrderLds : kDirectLds, t.shift);
     for (int i = tid; i < waves * width; i += 1024) count[i] = 0;
     if (tid == 0) before_s = 0;
     __syncthreads();
@@ -639,16 +644,12 @@ struct GradPlan {
     int *counts, *begin;
     float *part;
 };
-// Tokens that every range's workgroup looks through itself, 1024 a wave; where counts leave room for fewer than 16 waves, fewer.
-static const int64_t kDirect = getenv("GSD") ? atoi(getenv("GSD")) : 16384;  // tokens that every range's workgroup looks through itself
-
 GradPlan plan_grad(gs_arena &a, const gs_lookup *l) {
     GradPlan p{};
     while ((kRanges << p.shift) < l->vocab) p.shift++;
     p.ranges = (l->vocab + (1 << p.shift) - 1) >> p.shift;
     p.few = l->tokens <= kFewTokens;
-    const int room = kDirectLds / 4 >> p.shift;
-    p.split = l->tokens > (room < 16 ? room : 16) * kDirectWave || l->tokens > kDirect;
+    p.split = l->tokens > order_waves(kDirectLds, p.shift) * kDirectWave;
     if (p.few) return p;
     p.seg_size = kSplitTile;
     while (p.seg_size * kSegs < l->tokens) p.seg_size *= 2;
@@ -674,13 +675,14 @@ GradPlan plan_grad(gs_arena &a, const gs_lookup *l) {
 
 template <class T, int N>
 int run_grad(const gs_lookup *l, const GradPlan &p, const void *grad_d, int64_t stride, void *dweight_d, hipStream_t s) {
-    const Tokens t{Ids{l->ids_d, l->id_bytes}, l->tokens, l->padding, l->vocab, p.shift, p.ranges};
+    const int64_t padding = l->padding >= 0 && l->padding < l->vocab ? l->padding : -1;
+    const Tokens t{Ids{l->ids_d, l->id_bytes}, l->tokens, padding, l->vocab, p.shift, p.ranges};
     if (p.few) {
         hipLaunchKernelGGL((k_embed_few<T, N>), dim3(p.ranges), dim3(1024), 0, s, t, (const T *)grad_d, stride, l->dim, l->scale, (T *)dweight_d);
         GS_CHECK_LAUNCH();
         return GS_OK;
     }
-    const int width = 1 << p.shift, room = (p.split ? kOrderLds : kDirectLds) / 4 / width, waves = room < 16 ? room : 16;
+    const int width = 1 << p.shift, waves = order_waves(p.split ? kOrderLds : kDirectLds, p.shift);
     const int lds = (waves + 1) * width * 4 + (p.split ? 0 : waves * kDirectWave * 4);
     static std::atomic<uint64_t> set{0}, set_split{0};
     if (p.split) {

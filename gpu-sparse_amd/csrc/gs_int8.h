@@ -209,7 +209,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void k_few8(Source h, const uint
     };
 
     // The wave's rows, every eighth (those that are left out are not read).  The first kRows are asked for before the weight, whose
-    // loads would have to land before theirs otherwise (24 rows, 30522 columns of 768: XXX).
+    // loads would have to land before theirs otherwise (24 rows, 30522 columns of 768: 12.5 -> 11.5 us).
     const auto here = [&](int r) { return r < rows && ((kept >> r) & 1); };
     const auto quantize = [&](int r, const RowStart<2, T> &x) {
         const float scale = quantize_row<true, 2>(source_row<T>(h, r), x, h, kp, lane,

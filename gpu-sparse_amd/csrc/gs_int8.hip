@@ -2,7 +2,6 @@
 //   gs_quantize_rows   a matrix's rows as whole numbers and a scale each
 //   gs_int8_linear     y = x W^T + b; x is quantised per row within the call, sums are whole numbers
 #include "gs_int8.h"
-#include <stdlib.h>
 
 namespace gsv {
 
@@ -150,6 +149,13 @@ struct EpiFewLinear {
     }
 };
 
+// Tiles: the largest of which there are as many as CUs.  Product alone, us:
+//   rows x dim -> out        256      128      64
+//   16384 x 1024 -> 4096      84       93     151
+//   16384 x 768 -> 768      18.6     18.0      35   (192 tiles of 256: a quarter of the CUs has none)
+//   4099 x 777 -> 1001        37       14      14
+// What bounds the first: 137e9 operations at 1.65e15 a second, of 2.4e15 that a library product of 16384^3 reaches; its 134 MB of
+// output take 26 us of it at the rate of a copy.
 template <class T>
 using Small8 = Tile<T, 1, 64, 64, 2, 2, 4, 2, false, false>;
 template <class T>
@@ -204,9 +210,8 @@ int run_product(const gs_linear8 *l, const Scratch8 &s, int cus, hipStream_t st)
     const Dims d{l->out, l->rows, s.dimp / 2, nullptr, 0, 0, 0};
     const EpiLinear<O> epi{l->scales_d, s.scales, s.bias, (O *)l->out_d, l->out};
     const auto tiles = [&](int e) { return (int64_t)((l->out + e - 1) / e) * ((l->rows + e - 1) / e); };
-    static const int force = getenv("GSX") ? atoi(getenv("GSX")) : 0;
-    if (force == 1 || (!force && tiles(256) >= cus)) return launch_product<Large8<I8>>(w, x, d, epi, cus, st);
-    if (force == 2 || (!force && tiles(128) >= cus)) return launch_product<Mid8<I8>>(w, x, d, epi, cus, st);
+    if (tiles(256) >= cus) return launch_product<Large8<I8>>(w, x, d, epi, cus, st);
+    if (tiles(128) >= cus) return launch_product<Mid8<I8>>(w, x, d, epi, cus, st);
     return launch_product<Small8<I8>>(w, x, d, epi, cus, st);
 }
 

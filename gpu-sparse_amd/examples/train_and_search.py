@@ -3,11 +3,13 @@
 Texts are runs of word ids; a fixed table of word vectors and a moving average stand in for an encoder's body, and a
 linear layer and the vocabulary matrix above it are trained with the library's operators:
 
+  embed_tokens   the words' vectors
   vocab_loss     the word at a position that was hidden from the input
   distill_loss   a teacher's top logits at every position (here: a sharper head with the true word vectors)
   term_weights   texts as sparse vectors: queries against their documents, with a penalty on active terms
 
-Then the documents' term weights become an index, and the queries' are searched on it.
+Then the documents' term weights become an index, and the queries' are searched on it; and again with layer and vocabulary
+in 8 bits, as they would be served (quantize_rows, int8_linear, term_weights).
 
     python gpu-sparse_amd/examples/train_and_search.py --steps 60
 """
@@ -45,7 +47,7 @@ class Texts:
 
     def hidden(self, ids, hide=None):
         """[texts, length, dim], each of unit variance: word vectors with half of their neighbours', hidden words as zeros."""
-        x = self.words[ids]
+        x = gs.embed_tokens(ids, self.words)
         if hide is not None:
             x = x.masked_fill(hide[:, :, None], 0.0)
         return torch.nn.functional.layer_norm(x + 0.5 * (x.roll(1, dims=1) + x.roll(-1, dims=1)), (self.dim,))
@@ -63,6 +65,19 @@ class Head(torch.nn.Module):
 
     def forward(self, x):
         return (x @ self.turn).to(self.dtype), self.weight.to(self.dtype), self.bias.to(self.dtype)
+
+
+class Head8:
+    """A trained head in 8 bits."""
+
+    def __init__(self, head):
+        self.turn = gs.quantize_rows(head.turn.detach().t())
+        self.weight = gs.quantize_rows(head.weight.detach())
+        self.bias = head.bias.detach()
+        self.dtype = head.dtype
+
+    def __call__(self, x):
+        return gs.int8_linear(x, self.turn, dtype=self.dtype), self.weight, self.bias
 
 
 def train(head, texts, steps, batch, top=16, log=print):
@@ -132,8 +147,10 @@ def run(steps=60, n_docs=2000, vocab=4000, dim=128, length=48, batch=64, dtype=t
     before, _ = search(head, texts)
     first, last = train(head, texts, steps, batch, log=log)
     after, per_doc = search(head, texts)
-    log("documents found among the first 10: %.3f before, %.3f after; %.0f terms per document" % (before, after, per_doc))
-    return {"before": before, "after": after, "first": first, "last": last, "terms_per_doc": per_doc}
+    after8, per_doc8 = search(Head8(head), texts)
+    log("documents found among the first 10: %.3f before, %.3f after, %.3f in 8 bits; %.0f terms per document (%.0f)"
+        % (before, after, after8, per_doc, per_doc8))
+    return {"before": before, "after": after, "after8": after8, "first": first, "last": last, "terms_per_doc": per_doc}
 
 
 def main():

@@ -7,6 +7,9 @@ import torch
 from torch.autograd import forward_ad
 
 
+HERE = nullcontext()
+
+
 def _same_device(dev, of="hidden", **tensors):
     for name, t in tensors.items():
         if t is not None and t.device != dev:
@@ -15,7 +18,7 @@ def _same_device(dev, of="hidden", **tensors):
 
 def _on(dev):
     """The tensors' device as the current one; entering it costs more than asking whether it is."""
-    return nullcontext() if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+    return HERE if torch._C._cuda_getDevice() == dev.index else torch.cuda.device(dev)
 
 
 def _bytes(n: int, dev) -> torch.Tensor:
@@ -26,6 +29,9 @@ def _differentiable(*inputs) -> bool:
     """Whether a call has to go through autograd: a gradient may be asked for, tensors may carry tangents or belong to a
     functional transform (both of which autograd refuses here), or a trace records it.  One that need not leaves autograd
     out (5 us of a query's 21)."""
-    return ((torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in inputs))
-            or forward_ad._current_level >= 0 or torch._C._are_functorch_transforms_active()
+    if torch.is_grad_enabled():
+        for t in inputs:
+            if t is not None and t.requires_grad:
+                return True
+    return (forward_ad._current_level >= 0 or torch._C._are_functorch_transforms_active()
             or torch._C._get_tracing_state() is not None)

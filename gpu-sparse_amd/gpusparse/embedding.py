@@ -18,47 +18,63 @@ MAX_SCALE = torch.finfo(torch.float32).max
 
 def _lookup(ids, weight, scale: float, padding: int):
     """The rows, and the C struct of the call."""
-    q8 = isinstance(weight, Int8Rows)
-    table = weight.values if q8 else weight
+    if isinstance(weight, Int8Rows):
+        table, scales, wtype = weight.values, weight.scales.data_ptr(), _lib.GS_H_I8
+    else:
+        table, scales, wtype = weight, None, _lib.HTYPE_OF_DTYPE[weight.dtype]
     vocab, dim = table.shape
-    out = torch.empty(ids.shape + (dim,), dtype=weight.dtype, device=table.device)
-    htype = _lib.HTYPE_OF_DTYPE[weight.dtype]
-    a = _lib.GsLookup(ids.data_ptr(), table.data_ptr(), weight.scales.data_ptr() if q8 else None, table.stride(0), table.stride(1),
-                      ids.numel(), padding, ids.element_size(), _lib.GS_H_I8 if q8 else htype, htype, vocab, dim, scale)
-    with _on(table.device):
-        _lib.check(_lib.lib().gs_embed_tokens(C.byref(a), out.data_ptr(), _lib.stream_ptr(table.device)), "gs_embed_tokens")
+    dev = table.device
+    out = table.new_empty((*ids.shape, dim), dtype=weight.dtype)
+    row, value = table.stride()
+    a = _lib.GsLookup(ids.data_ptr(), table.data_ptr(), scales, row, value, ids.numel(), padding, ids.element_size(), wtype,
+                      _lib.HTYPE_OF_DTYPE[weight.dtype], vocab, dim, scale)
+    with _on(dev):
+        _lib.check(_lib.lib().gs_embed_tokens(C.byref(a), out.data_ptr(), _lib.stream_ptr(dev)), "gs_embed_tokens")
     return out, a
+
+
+def _gradient(ctx, grad):
+    ids, = ctx.saved_tensors
+    a, dev = ctx.lookup, ctx.dev
+    if (ids.data_ptr(), ids.shape, ids.stride(), ids.dtype) != ctx.at:  # hooks on saved tensors may move them, no more
+        if (ids.shape, ids.dtype, ids.device) != (ctx.at[1], ctx.at[3], dev):
+            raise RuntimeError(f"the saved ids came back as {ids.dtype} {tuple(ids.shape)} on {ids.device}")
+        ids = ids.contiguous()
+        a = _lib.GsLookup.from_buffer_copy(a)
+        a.ids_d = ids.data_ptr()
+    row = a.dim
+    if not grad.is_contiguous():
+        grad = grad.reshape(-1, a.dim)
+        if grad.stride(1) != 1:
+            grad = grad.contiguous()
+        row = grad.stride(0)
+    dw = torch.empty((a.vocab, a.dim), dtype=ctx.dtype, device=dev)
+    ws = _bytes(ctx.grad_bytes, dev) if ctx.grad_bytes else None
+    with _on(dev):
+        _lib.check(_lib.lib().gs_embed_tokens_grad(C.byref(a), grad.data_ptr(), row, dw.data_ptr(), _lib.ptr(ws), ctx.grad_bytes,
+                                                   _lib.stream_ptr(dev)), "gs_embed_tokens_grad")
+    return None, dw, None, None
+
+
+_gradient_once = once_differentiable(_gradient)
 
 
 class _Embed(torch.autograd.Function):
     @staticmethod
     def forward(ctx, ids, weight, scale, padding):
         out, ctx.lookup = _lookup(ids, weight, scale, padding)
+        need = C.c_size_t()
+        _lib.check(_lib.lib().gs_embed_tokens_grad_workspace(C.byref(ctx.lookup), C.byref(need)), "gs_embed_tokens_grad_workspace")
+        ctx.grad_bytes = need.value
         ctx.save_for_backward(ids)
-        ctx.kind = (ids.shape, ids.dtype, ids.device)
-        ctx.dtype = weight.dtype
+        ctx.at = (ids.data_ptr(), ids.shape, ids.stride(), ids.dtype)
+        ctx.dev, ctx.dtype = out.device, weight.dtype
         return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad):
-        ids, = ctx.saved_tensors
-        if (ids.shape, ids.dtype, ids.device) != ctx.kind:  # hooks on saved tensors may move them, no more
-            raise RuntimeError(f"the saved ids came back as {ids.dtype} {tuple(ids.shape)} on {ids.device}")
-        ids, dev = ids.contiguous(), ids.device
-        a = _lib.GsLookup.from_buffer_copy(ctx.lookup)
-        a.ids_d = ids.data_ptr()
-        grad = grad.reshape(-1, a.dim)
-        if grad.stride(1) != 1:
-            grad = grad.contiguous()
-        dw = torch.empty((a.vocab, a.dim), dtype=ctx.dtype, device=dev)
-        L, need = _lib.lib(), C.c_size_t()
-        with _on(dev):
-            _lib.check(L.gs_embed_tokens_grad_workspace(C.byref(a), C.byref(need)), "gs_embed_tokens_grad_workspace")
-            ws = _bytes(need.value, dev)
-            _lib.check(L.gs_embed_tokens_grad(C.byref(a), grad.data_ptr(), grad.stride(0), dw.data_ptr(), ws.data_ptr(),
-                                              need.value, _lib.stream_ptr(dev)), "gs_embed_tokens_grad")
-        return None, dw, None, None
+        # what refuses a second derivative has nothing to do where none can be asked for (4 us)
+        return _gradient_once(ctx, grad) if torch.is_grad_enabled() else _gradient(ctx, grad)
 
 
 def embed_tokens(ids, weight, *, scale: float = 1.0, padding_idx: int | None = None):

@@ -137,7 +137,7 @@ def int8_linear(x: torch.Tensor, weight: Int8Rows, bias=None, *, dtype: torch.dt
     _refuse_gradient(x, bias)
     bias = None if bias is None else bias.contiguous()
     rows = x if x.dim() == 2 else x.reshape(-1, dim)
-    y = torch.empty(x.shape[:-1] + (out,), dtype=dtype, device=dev)
+    y = x.new_empty((*x.shape[:-1], out), dtype=dtype)
     L = _lib.lib()
     a = _lib.GsLinear8(rows.data_ptr(), rows.stride(0), rows.stride(1), weight.values.data_ptr(), weight.values.stride(0),
                        weight.scales.data_ptr(), _lib.ptr(bias), y.data_ptr(), _lib.HTYPE_OF_DTYPE[x.dtype],

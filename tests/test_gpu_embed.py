@@ -27,6 +27,8 @@ def words(shape, vocab, device, seed=2, how="words"):
     u = torch.rand(shape, generator=g, dtype=torch.float64)
     if how == "words":
         ids = (torch.exp(u * math.log(vocab + 1)) - 1).long().clamp(0, vocab - 1) * 7919 % vocab
+    elif how == "half":
+        ids = torch.where(u < 0.5, 0, (u * vocab).long())
     elif how == "one":
         ids = torch.full(shape, vocab // 2)
     elif how == "sorted":
@@ -73,6 +75,12 @@ CASES = [
     ((4, 33), 256, 64, F32, 1.0, 0, "words"),
     ((5, 300), 257, 129, F32, -2.0, None, "words"),
     ((2, 2, 50), 30522, 777, F16, 1.0, 17, "words"),
+    ((1024,), 30522, 384, F32, 1.0, 0, "words"),                # the most that are summed where they are sorted
+    ((1025,), 30522, 384, F32, 1.0, 0, "words"),
+    ((1000,), 1 << 20, 12, BF16, 1.0, None, "words"),
+    ((1024,), 300, 600, F16, 0.01, None, "one"),                # one id alone, whose sum the waves share
+    ((700,), 4, 130, BF16, 1.0, 1, "evenly"),
+    ((4, 512), 1 << 20, 20, F32, 1.0, None, "evenly"),
     ((16384,), 1000, 40, BF16, 1.0, None, "words"),             # the most that one launch orders
     ((16385,), 1000, 40, BF16, 1.0, None, "words"),             # and one more
     ((20, 2000), 30522, 72, BF16, 0.125, 0, "words"),
@@ -82,6 +90,8 @@ CASES = [
     ((50000,), 513, 520, BF16, 1.0, None, "words"),             # runs over many chunks
     ((30000,), 5, 260, F32, 1.0, 2, "evenly"),
     ((70000,), 30522, 16, F16, 0.001, None, "one"),             # one id alone
+    ((60, 1000), 30522, 24, BF16, 1.0, None, "half"),           # half of the tokens are one id
+    ((131080,), 3000, 1024, BF16, 1.0, None, "words"),          # more than 256 MiB of upstream values
     ((65536,), 70000, 16, BF16, 1.0, None, "sorted"),
     ((300,), 50, 5000, BF16, 1.0, None, "words"),               # long rows
     ((64,), 10, 32768, F32, 1.0, None, "words"),

@@ -156,6 +156,8 @@ LINEAR = [
     (33, 300, 20000, BF16, BF16, None),       # three blocks of rows, as many columns as go round twice
     (64, 1024, 515, F32, None, BF16),
     (64, 1400, 515, BF16, BF16, None),        # 64 rows too wide for LDS
+    (40, 900, 300, BF16, BF16, None),         # 40 rows: four blocks of them
+    (48, 128, 33000, F16, BF16, None),
     (3, 32768, 65, BF16, None, None),         # long rows
     (1, 32768, 65, F16, F32, None),
     (65, 128, 64, BF16, None, None),
@@ -256,6 +258,10 @@ TERMS = [
     (4, 300, 133, 517, BF16, "holes"),
     (3, 259, 72, 300, F32, "prefix"),
     (90, 33, 64, 260, BF16, "holes"),
+    (5, 30, 640, 300, BF16, None),             # no mask, more than 64 rows
+    (9, 200, 1030, 300, F32, "empty"),         # rows of more than 1024 values
+    (300, 250, 64, 130, BF16, "empty"),        # more than 65536 rows
+    (700, 100, 24, 40, F16, None),
     (5, 8, 5000, 140, BF16, "holes"),          # few rows, too wide for LDS
     (2, 8, 64, 1, F16, None),
     (6, 50, 64, 300, BF16, "none"),
@@ -445,3 +451,34 @@ def test_arguments_are_checked(device):
             gs.term_weights(*bad)
     with pytest.raises(RuntimeError, match="GPU"):
         gs.quantize_rows(torch.zeros((2, 64)))
+
+
+# ---------------------------------------------------------------- together
+
+def test_an_encoder_served_in_8_bits(device):
+    """Tokens looked up, a layer, term weights and a search, all from 8-bit matrices: the same as from what they stand for, taken
+    through the definitions in float64, and the index finds its own texts."""
+    g = torch.Generator().manual_seed(9)
+    vocab, dim, texts, length = 900, 96, 40, 12
+    table = torch.randn((vocab, dim), generator=g).to(device)
+    turn = (torch.eye(dim) + 0.1 * torch.randn((dim, dim), generator=g)).to(device)
+    bias = torch.full((vocab,), -2.0, device=device)
+    ids = torch.randint(0, vocab, (texts, length), generator=g).to(device)
+    lens = torch.randint(3, length + 1, (texts, 1), generator=g).to(device)
+    mask = torch.arange(length, device=device)[None] < lens
+    ids = torch.where(mask, ids, -1)
+    table8, turn8 = gs.quantize_rows(table / math.sqrt(dim)), gs.quantize_rows(turn)
+    x = gs.embed_tokens(ids, table8, scale=math.sqrt(dim))
+    h = gs.int8_linear(x, turn8)
+    weights = gs.term_weights(h, table8, bias, mask=mask)
+    want, l = linear64(x, turn8, None)
+    assert_within(h.view(-1, dim), want, linear_bound(want, l, F32), "layer")
+    want, bound = terms64(h, table8, bias, mask)
+    assert_within(weights, want, bound, "weights")
+    at = weights.nonzero().cpu()
+    csr = gs.CSR(torch.cat([torch.zeros(1, dtype=torch.int64), (weights > 0).sum(1).cumsum(0).cpu()]).numpy(), at[:, 1].int().numpy(),
+                 weights[weights > 0].cpu().numpy(), (texts, vocab))
+    index = gs.build_from_csr(csr, device)
+    top, terms = gs.topk_rows(weights, 16)
+    _, docs = gs.search(index, (torch.where(top > 0, terms, -1).int(), top), 3)
+    assert bool((docs[:, 0] == torch.arange(texts, device=device)).all())

@@ -107,8 +107,11 @@ def test_lookup_types_and_pointers():
         with pytest.raises(ValueError, match=match):
             _lib.check(L.gs_embed_tokens(C.byref(lookup(**over)), 8, None), "call")
     assert L.gs_embed_tokens(C.byref(lookup(tokens=0)), None, None) == _lib.GS_OK
-    assert L.gs_embed_tokens_grad_workspace(C.byref(lookup()), C.byref(n)) == _lib.GS_OK and n.value > 0
-    assert L.gs_embed_tokens_grad(C.byref(lookup()), 8, 100, 8, 256, n.value - 1, None) == _lib.GS_ENOSPC
+    assert L.gs_embed_tokens_grad_workspace(C.byref(lookup(tokens=1024)), C.byref(n)) == _lib.GS_OK and n.value == 0
+    assert L.gs_embed_tokens_grad_workspace(C.byref(lookup(tokens=1025)), C.byref(n)) == _lib.GS_OK and n.value > 1025 * 8
+    assert L.gs_embed_tokens_grad(C.byref(lookup(tokens=1025)), 8, 100, 8, 256, n.value - 1, None) == _lib.GS_ENOSPC
+    with pytest.raises(ValueError, match="NULL"):
+        _lib.check(L.gs_embed_tokens_grad(C.byref(lookup(tokens=1025, ids_d=256)), 256, 100, 256, None, n.value, None), "call")
     for over, stride, match in ((dict(type=_lib.GS_H_I8), 100, "no gradient"), (dict(), -100, "negative stride"), (dict(), 100, "NULL")):
         with pytest.raises(ValueError, match=match):
             _lib.check(L.gs_embed_tokens_grad(C.byref(lookup(**over)), 8, stride, 8, 256, n.value, None), "call")
