@@ -46,10 +46,7 @@ __device__ __forceinline__ RowScale row_scale(uint32_t bits) {
     r.scale = bits >= 0x7F800000u ? __builtin_nanf("") : none ? 0.f : r.most / 127.f;
     return r;
 }
-// Eight values' nearest whole numbers to 127 x / most, a byte each.  x * inv is off by less than 2^-16 (two roundings of a
-// value up to 127), so it decides alone except next to a half, where the difference from the quotient is taken without error: of
-// 127 x and n most the rounding errors are kept, and their difference and that to most / 2 are of close numbers.
-// Adding 1.5 x 2^23 rounds to a whole number, whose two's complement is then the sum's low byte.
+
 template <class T>
 struct Raw8 {  // eight values as they lie
     typedef T vec __attribute__((ext_vector_type(8)));
@@ -57,6 +54,10 @@ struct Raw8 {  // eight values as they lie
     vec v;
     __device__ __forceinline__ float operator[](int e) const { return (float)v[e]; }
 };
+// Eight values' nearest whole numbers to 127 x / most, a byte each.  x * inv is off by less than 2^-16 (two roundings of a
+// value up to 127), so it decides alone except next to a half, where the difference from the quotient is taken without error: of
+// 127 x and n most the rounding errors are kept, and their difference and that to most / 2 are of close numbers.
+// Adding 1.5 x 2^23 rounds to a whole number, whose two's complement is then the sum's low byte.
 template <class T>
 __device__ __forceinline__ uint2 quantized8(const Raw8<T> &x, const RowScale &r) {
     if (r.inv == 0.f) return make_uint2(0, 0);
@@ -160,10 +161,11 @@ __device__ __forceinline__ ColumnScale column_scale(int v, const Weight8 &W, con
     return v < W.n ? ColumnScale{W.scales[v], bias_at(bias, type, v)} : ColumnScale{0.f, 0.f};
 }
 
-// Products of at most 64 rows, their values on end, in one launch, for latency: a workgroup of eight waves quantises all rows into LDS itself and
-// takes blocks of 16 columns, KS of its waves a block, each its part of k.  The weight goes from memory to the operands'
-// registers: a lane takes 32 bytes on end of its column, so that a wave's loads take whole lines, and the first of them are asked
-// for before the rows are quantised.
+// Products of at most 64 rows, their values on end, in one launch, for latency: a workgroup of eight waves quantises all rows into
+// LDS itself and takes blocks of 16 columns, KS of its waves a block, each its part of k.  The weight goes from memory to the
+// operands' registers: a lane takes 32 bytes on end of its column, so that a wave's loads take whole lines, and the first of them
+// are asked for before the rows are quantised.  What bounds it is the weight's bytes and latency: one row of 768 values, 30522
+// columns 6.4 us (3.7 TB/s), 24 rows 13 (in two launches 14); one row of 1024, 4096 columns 5.
 constexpr int kFewRows = 64, kFewLds = 80 * 1024, kFewWaves = 8;
 
 __host__ __device__ inline int few_stride(int kp) { return kp + 16; }  // rows start 4 banks apart

