@@ -35,18 +35,14 @@ struct I8 {
 };
 
 struct RowScale {
-    float most, inv, scale;  // inv: 127 / most; 0 where all values are kept as 0
+    float most, inv, scale;  // largest magnitude times 2^-8; 1 / that, 0 where all values are kept as 0
 };
 // bits: the largest of the values' bits without their signs, above infinity's where one is NaN
 __device__ __forceinline__ RowScale row_scale(uint32_t bits) {
-    RowScale r;
-    r.most = __uint_as_float(bits);
-    const bool none = bits >= 0x7F800000u || r.most < kLeast8;
-    r.inv = none ? 0.f : 127.f / r.most;
-    r.scale = bits >= 0x7F800000u ? __builtin_nanf("") : none ? 0.f : r.most / 127.f;
-    return r;
+    const float most = __uint_as_float(bits);
+    const bool odd = bits >= 0x7F800000u, none = odd || most < kLeast8;
+    return {most * 0x1p-8f, none ? 0.f : __builtin_amdgcn_rcpf(most * 0x1p-8f), odd ? __builtin_nanf("") : none ? 0.f : most / 127.f};
 }
-
 template <class T>
 struct Raw8 {  // eight values as they lie
     typedef T vec __attribute__((ext_vector_type(8)));
@@ -54,31 +50,29 @@ struct Raw8 {  // eight values as they lie
     vec v;
     __device__ __forceinline__ float operator[](int e) const { return (float)v[e]; }
 };
-// Eight values' nearest whole numbers to 127 x / most, a byte each.  x * inv is off by less than 2^-16 (two roundings of a
-// value up to 127), so it decides alone except next to a half, where the difference from the quotient is taken without error: of
-// 127 x and n most the rounding errors are kept, and their difference and that to most / 2 are of close numbers.
-// Adding 1.5 x 2^23 rounds to a whole number, whose two's complement is then the sum's low byte.
+// Eight values' nearest whole numbers to p / most (p = 127 x, both times 2^-8, so that p stays finite), a byte each.
+//
+// y = p inv is off by a few units; y + (p - y most) inv is the quotient to half a unit and, where that is n + 1/2, exactly that.
+// 16-bit values: p has no rounding, and no other quotient is nearer to n + 1/2 than 2^-12 of itself, so rounding y is rounding the
+// quotient.  fp32: p's rounding error `low` is kept; where y is n + 1/2 the sign of p + low - y most, which is exact there, says on which
+// side the quotient is.  Adding 1.5 x 2^23 rounds to the nearest whole number, ties to even, whose two's complement is then the
+// sum's low byte.  (Deciding by x * inv alone except next to a half costs less, but the code for the halves, once for each place where
+// rows are quantised, has to come from memory: 24 rows and 30522 columns of 768 12.9 us instead of 10.5.)
 template <class T>
 __device__ __forceinline__ uint2 quantized8(const Raw8<T> &x, const RowScale &r) {
     if (r.inv == 0.f) return make_uint2(0, 0);
-    constexpr float kRound = 0x1.8p23f;
+    constexpr float kRound = 0x1.8p23f, kMul = 127.f * 0x1p-8f;
     uint32_t t[8];
-    float far = 0.f;
 #pragma unroll
     for (int e = 0; e < 8; e++) {
-        const float y = x[e] * r.inv, s = y + kRound;
-        far = fmaxf(far, fabsf(y - (s - kRound)));
-        t[e] = __float_as_uint(s);
-    }
-    if (__builtin_expect(far > 0.5f - 0x1p-15f, 0)) {
-        const float most = r.most * 0x1p-8f, half = 0.5f * most;  // 127 x stays finite
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const int n = (int)(int8_t)t[e];
-            const float w = x[e] * 0x1p-8f, p = w * 127.f, q = (float)n * most;
-            const float d = p - q, low = fmaf(w, 127.f, -p) - fmaf((float)n, most, -q);
-            const float over = d > 0 ? (d - half) + low : (-d - half) - low;  // |127 x - n most| - most / 2, or its sign
-            if (over > 0 || (over == 0 && (n & 1))) t[e] = (uint32_t)(n + (d > 0 ? 1 : -1));
+        const float p = x[e] * kMul, y0 = p * r.inv;
+        if constexpr (sizeof(T) == 2) {
+            t[e] = __float_as_uint(fmaf(fmaf(-y0, r.most, p), r.inv, y0) + kRound);
+        } else {
+            const float low = fmaf(x[e], kMul, -p);
+            const float y = fmaf(fmaf(-y0, r.most, p) + low, r.inv, y0), n = rintf(y);
+            const float rest = fmaf(-y, r.most, p) + low;
+            t[e] = __float_as_uint((fabsf(y - n) == 0.5f && rest != 0.f ? y + copysignf(0.5f, rest) : n) + kRound);
         }
     }
     const auto four = [](uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
@@ -161,18 +155,26 @@ __device__ __forceinline__ ColumnScale column_scale(int v, const Weight8 &W, con
     return v < W.n ? ColumnScale{W.scales[v], bias_at(bias, type, v)} : ColumnScale{0.f, 0.f};
 }
 
-// Products of at most 64 rows, their values on end, in one launch, for latency: a workgroup of eight waves quantises all rows into
+// Products of at most 128 rows, their values on end, in one launch, for latency: a workgroup of eight waves quantises all rows into
 // LDS itself and takes blocks of 16 columns, KS of its waves a block, each its part of k.  The weight goes from memory to the
 // operands' registers: a lane takes 32 bytes on end of its column, so that a wave's loads take whole lines, and the first of them
 // are asked for before the rows are quantised.  What bounds it is the weight's bytes and latency: one row of 768 values, 30522
-// columns 6.4 us (3.7 TB/s), 24 rows 13 (in two launches 14); one row of 1024, 4096 columns 5.
-constexpr int kFewRows = 64, kFewLds = 80 * 1024, kFewWaves = 8;
+// columns 6.3 us (3.7 TB/s), 24 rows 10.5; one row of 1024, 4096 columns 4.
+constexpr int kFewRows = 128, kFewWaves = 8, kFewLds = 150 * 1024;
+constexpr int kFewPitch = 17;  // of a row of 16 values that an epilogue leaves in LDS
+
+// Rows that count, a bit each
+struct Kept {
+    uint64_t lo, hi;
+    __device__ __forceinline__ bool operator()(int r) const { return (r < 64 ? lo >> r : hi >> (r - 64)) & 1; }
+};
 
 __host__ __device__ inline int few_stride(int kp) { return kp + 16; }  // rows start 4 banks apart
-inline int few_blocks(int rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }  // of 16 rows, that k_few8 is made for
-inline size_t few_lds(int rows, int kp, int ks) {
-    const int blocks = few_blocks(rows);
-    return (size_t)rows * few_stride(kp) + kFewRows * 4 + (ks > 1 ? (size_t)kFewWaves * blocks * 1024 : 0);
+inline int few_blocks(int rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 64 ? 4 : 8; }  // of 16 rows, that k_few8 is made for
+// joins: whether the epilogue passes values through LDS
+inline size_t few_lds(int rows, int kp, int ks, bool joins) {
+    const size_t blocks = few_blocks(rows), values = blocks * 16 * kFewPitch * 4;
+    return (size_t)rows * few_stride(kp) + kFewRows * 4 + (ks > 1 ? kFewWaves * blocks * 1024 + values : joins ? kFewWaves * values : 0);
 }
 
 template <class T, int MB, int KS, class Epi>
@@ -183,7 +185,10 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void k_few8(Source h, const uint
     const int ls = few_stride(kp);
     float *scales = reinterpret_cast<float *>(smem + (size_t)rows * ls);
     i32x4 *part = reinterpret_cast<i32x4 *>(scales + kFewRows);
-    const uint64_t kept = __ballot(lane < rows && (!mask || mask[min(lane, rows - 1)] != 0));
+    constexpr int values = MB * 16 * kFewPitch;  // KS > 1: one set, after the parts; else a wave's own
+    float *left = reinterpret_cast<float *>(part) + (KS > 1 ? kFewWaves * MB * 256 : wave * values);
+    const auto ballot = [&](int r) { return __ballot(r < rows && (!mask || mask[min(r, rows - 1)] != 0)); };
+    const Kept kept{ballot(lane), MB > 4 ? ballot(lane + 64) : 0};
     const int steps = kp / kPad8, k0 = KS == 1 ? 0 : steps * wave / KS, k1 = KS == 1 ? steps : steps * (wave + 1) / KS;
 
     constexpr int kAhead = 4;  // steps of 128 values in each of two buffers
@@ -211,8 +216,8 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void k_few8(Source h, const uint
     };
 
     // The wave's rows, every eighth (those that are left out are not read).  The first kRows are asked for before the weight, whose
-    // loads would have to land before theirs otherwise (24 rows, 30522 columns of 768: 12.5 -> 11.5 us).
-    const auto here = [&](int r) { return r < rows && ((kept >> r) & 1); };
+    // loads would have to land before theirs otherwise (24 rows, 30522 columns of 768: a microsecond).
+    const auto here = [&](int r) { return r < rows && kept(r); };
     const auto quantize = [&](int r, const RowStart<2, T> &x) {
         const float scale = quantize_row<true, 2>(source_row<T>(h, r), x, h, kp, lane,
                                                   [&](int d, uint2 y) { *reinterpret_cast<uint2 *>(smem + r * ls + d) = y; });
@@ -266,19 +271,25 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void k_few8(Source h, const uint
         const bool more = g < groups;
         if (more) seek();
         if (KS == 1) {
-            epi.template run<MB>(acc, done + i, W, col, scales, rows, kept, q);
+#pragma unroll
+            for (int m = 0; m < MB; m++) epi.block(acc[m], m, done + i, W, col, scales, rows, lane, left);
+            if (Epi::joins) {
+                gs_wave_sync();
+                epi.finish(left, done + i, W, col, kept, lane, 0, 1);
+                gs_wave_sync();
+            }
         } else {
 #pragma unroll
             for (int m = 0; m < MB; m++) part[(wave * MB + m) * 64 + lane] = acc[m];
             __syncthreads();
-            if (wave == 0) {
+            if (wave < MB) {  // a wave joins the parts of a block of rows
+                i32x4 sum = part[wave * 64 + lane];
 #pragma unroll
-                for (int m = 0; m < MB; m++)
-#pragma unroll
-                    for (int k = 1; k < kFewWaves; k++) acc[m] += part[(k * MB + m) * 64 + lane];
-                epi.template run<MB>(acc, done + i, W, col, scales, rows, kept, q);
+                for (int k = 1; k < kFewWaves; k++) sum += part[(k * MB + wave) * 64 + lane];
+                epi.block(sum, wave, done + i, W, col, scales, rows, lane, left);
             }
             __syncthreads();
+            if (Epi::joins) epi.finish(left, done + i, W, col, kept, lane, wave, kFewWaves);
         }
         if (!more) break;
     }
@@ -291,7 +302,10 @@ inline int cu_count(int *cus) {
     return GS_OK;
 }
 
-inline bool few8_ok(int rows, int kp, int64_t dim_stride) { return dim_stride == 1 && rows <= kFewRows && few_lds(rows, kp, kFewWaves) <= kFewLds; }
+template <class Epi>
+bool few8_ok(int rows, int kp, int64_t dim_stride) {
+    return dim_stride == 1 && rows <= Epi::most_rows && few_lds(rows, kp, kFewWaves, Epi::joins) <= kFewLds && few_lds(rows, kp, 1, Epi::joins) <= kFewLds;
+}
 
 // Once per device and kernel: LDS beyond 64 KiB
 inline int allow_lds(const void *f, int bytes, std::atomic<uint64_t> &set) {
@@ -311,7 +325,7 @@ int launch_few8(const Source &h, const uint8_t *mask, int rows, const Weight8 &W
     if (int rc = allow_lds(reinterpret_cast<const void *>(&k_few8<T, MB, KS, Epi>), kFewLds, set)) return rc;
     const int columns = KS == 1 ? 16 * kFewWaves : 16, groups = (W.n + columns - 1) / columns;
     hipLaunchKernelGGL((k_few8<T, MB, KS, Epi>), dim3((unsigned)(groups < cus ? groups : cus)), dim3(64 * kFewWaves),
-                       few_lds(rows, kp, KS), s, h, mask, rows, W, kp, groups, epi);
+                       few_lds(rows, kp, KS, Epi::joins), s, h, mask, rows, W, kp, groups, epi);
     GS_CHECK_LAUNCH();
     return GS_OK;
 }
@@ -325,9 +339,14 @@ int launch_few8(const Source &h, const uint8_t *mask, int rows, const Weight8 &W
     switch (few_blocks(rows)) {
         case 1: GSV_FEW8(1);
         case 2: GSV_FEW8(2);
-        default: GSV_FEW8(4);
+        case 4:
+            if constexpr (Epi::most_rows > 32) GSV_FEW8(4);
+            break;
+        default:
+            if constexpr (Epi::most_rows > 64) GSV_FEW8(8);
     }
 #undef GSV_FEW8
+    GS_REQUIRE(false, "%d rows are not few", rows);
 }
 
 }  // namespace gsv

@@ -130,24 +130,25 @@ struct EpiFewLinear {
     const void *bias;
     void *out;
     int bias_type, out_type;
+    static constexpr bool joins = false;
+    // 24 rows of 768, 30522 columns 10.5 us, in two launches 14; 64 rows 19 and 14: a row's outputs are written 32 bytes at a time
+    static constexpr int most_rows = 32;
     __device__ __forceinline__ ColumnScale column(int v, const Weight8 &W) const { return column_scale(v, W, bias, bias_type); }
-    template <int MB>
-    __device__ __forceinline__ void run(const i32x4 (&acc)[MB], int v, const Weight8 &W, const ColumnScale &col, const float *scales, int rows,
-                                        uint64_t, int q) const {
+    __device__ __forceinline__ void block(const i32x4 &sum, int m, int v, const Weight8 &W, const ColumnScale &col, const float *scales, int rows,
+                                          int lane, float *) const {
         if (v >= W.n) return;
 #pragma unroll
-        for (int m = 0; m < MB; m++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int row = 16 * m + 4 * q + e;
-                if (row >= rows) continue;
-                const float y = fmaf((float)acc[m][e] * scales[row] * col.by, kUp, col.bias);
-                const int64_t to = (int64_t)row * W.n + v;
-                if (out_type == GS_H_F32) ((float *)out)[to] = y;
-                else if (out_type == GS_H_F16) ((_Float16 *)out)[to] = (_Float16)y;
-                else ((__bf16 *)out)[to] = (__bf16)y;
-            }
+        for (int e = 0; e < 4; e++) {
+            const int row = 16 * m + 4 * (lane >> 4) + e;
+            if (row >= rows) continue;
+            const float y = fmaf((float)sum[e] * scales[row] * col.by, kUp, col.bias);
+            const int64_t to = (int64_t)row * W.n + v;
+            if (out_type == GS_H_F32) ((float *)out)[to] = y;
+            else if (out_type == GS_H_F16) ((_Float16 *)out)[to] = (_Float16)y;
+            else ((__bf16 *)out)[to] = (__bf16)y;
+        }
     }
+    __device__ __forceinline__ void finish(const float *, int, const Weight8 &, const ColumnScale &, const Kept &, int, int, int) const {}
 };
 
 // Tiles: the largest of which there are as many as CUs.  Product alone, us:
@@ -197,7 +198,7 @@ struct Scratch8 {
     bool few;
 };
 Scratch8 scratch_of(gs_arena &a, const gs_linear8 *l) {
-    Scratch8 s{nullptr, nullptr, nullptr, (int)round_up(l->dim, kPad8), few8_ok(l->rows, (int)round_up(l->dim, kPad8), l->x_dim_stride)};
+    Scratch8 s{nullptr, nullptr, nullptr, (int)round_up(l->dim, kPad8), few8_ok<EpiFewLinear>(l->rows, (int)round_up(l->dim, kPad8), l->x_dim_stride)};
     if (s.few) return s;
     s.scales = a.take<float>(l->rows);
     s.bias = a.take<float>(l->out);

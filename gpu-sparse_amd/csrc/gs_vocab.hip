@@ -1342,38 +1342,45 @@ __global__ __launch_bounds__(256, 2) void k_few_rows(Source h, const uint8_t *ma
     }
 }
 
-// What k_few8 makes of a block's sums for texts: lane l holds rows 16 m + 4 (l >> 4) .. + 3 of column v.
+// What k_few8 makes of a block's sums for texts.  The logits but for their column's scale go to LDS, since a text's rows lie in any
+// lanes: then a row of lanes takes a text (of four or more), or a fourth of its rows.  (21 texts of 3 tokens of 170 fp32 values, 11762 terms: 21 us, 44 with maxima taken from registers
+// text by text; 69 of one token of 512, 27652 terms: 27, and 57 as tiles in three launches; one of 24, 768, 30522: 11.5.)
 struct EpiFewTerms {
     const void *bias;
     int bias_type, texts, length;
     float *weights;
+    static constexpr bool joins = true;
+    static constexpr int most_rows = kFewRows;
     __device__ __forceinline__ ColumnScale column(int v, const Weight8 &W) const { return column_scale(v, W, bias, bias_type); }
-    template <int MB>
-    __device__ __forceinline__ void run(const i32x4 (&acc)[MB], int v, const Weight8 &W, const ColumnScale &col, const float *scales, int rows,
-                                        uint64_t kept, int q) const {
-        const bool on = v < W.n;
-        f32x4 x[MB];
+    __device__ __forceinline__ void block(const i32x4 &sum, int m, int, const Weight8 &, const ColumnScale &, const float *scales, int, int lane,
+                                          float *left) const {
+        const int row = 16 * m + 4 * (lane >> 4);
+        const f32x4 x = __builtin_convertvector(sum, f32x4) * *reinterpret_cast<const f32x4 *>(scales + row);
 #pragma unroll
-        for (int m = 0; m < MB; m++)
-            x[m] = __builtin_convertvector(acc[m], f32x4) * *reinterpret_cast<const f32x4 *>(scales + 16 * m + 4 * q);
-        for (int text = 0; text < texts; text++) {
-            const int lo = text * length, hi = lo + length;
+        for (int e = 0; e < 4; e++) left[(row + e) * kFewPitch + (lane & 15)] = x[e];
+    }
+    // wave `wave` of `waves` that share the values
+    __device__ __forceinline__ void finish(const float *left, int v, const Weight8 &W, const ColumnScale &col, const Kept &kept, int lane, int wave,
+                                           int waves) const {
+        const int q = lane >> 4;
+        const bool apart = texts >= 4;  // a text for each row of lanes
+        for (int t0 = apart ? wave * 4 : wave; t0 < texts; t0 += apart ? waves * 4 : waves) {
+            const int text = apart ? t0 + q : t0, lo = text * length;
             float top = -INFINITY;
-#pragma unroll
-            for (int m = 0; m < MB; m++) {
-                if (16 * m >= hi || 16 * m + 16 <= lo) continue;
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const int row = 16 * m + 4 * q + e;
-                    top = row >= lo && row < hi && ((kept >> row) & 1) ? maximum(top, x[m][e], x[m][e]) : top;
-                }
+            bool any = false;  // the bias of a text without a kept row is not looked at: it may be infinite or NaN
+            for (int r = apart ? 0 : q; r < length; r += apart ? 1 : 4) {
+                if (text >= texts || !kept(lo + r)) continue;
+                const float x = left[(lo + r) * kFewPitch + (lane & 15)];
+                top = maximum(top, x, x), any = true;
             }
-            const auto join = [&](Two<float> t) { top = maximum(t.a, t.b, t.b); };
-            join(across<16>(top));
-            join(across<32>(top));
-            // the bias of a text without a kept row is not looked at: it may be infinite or NaN
-            const bool any = (kept >> lo) & (~0ull >> (64 - length));
-            if (q == 0 && on) weights[(int64_t)text * W.n + v] = log1pf(any ? maximum(fmaf(top * col.by, kUp, col.bias), 0.f, 0.f) : 0.f);
+            if (!apart) {
+                const auto join = [&](Two<float> t) { top = maximum(t.a, t.b, t.b); };
+                join(across<16>(top));
+                join(across<32>(top));
+                any = __any(any);
+            }
+            if (text < texts && v < W.n && (apart || q == 0))
+                weights[(int64_t)text * W.n + v] = log1pf(any ? maximum(fmaf(top * col.by, kUp, col.bias), 0.f, 0.f) : 0.f);
         }
     }
 };
@@ -2485,7 +2492,7 @@ int run_terms8(const gs_vocab_head *h, const Layout &l, const float *scales_d, c
                float *best, float *row_scales, int cus, hipStream_t s) {
     using T = typename HVal<HT>::t;
     const Source hs = hidden_source(h);
-    if (few8_ok(l.rows, 2 * l.dimp, h->hidden_dim_stride))
+    if (few8_ok<EpiFewTerms>(l.rows, 2 * l.dimp, h->hidden_dim_stride))
         return launch_few8<T>(hs, mask_d, l.rows, Weight8{(const int8_t *)h->weight_d, h->weight_row_stride, scales_d, h->vocab}, 2 * l.dimp,
                               EpiFewTerms{h->bias_d, h->bias_type, h->texts, h->length, weights_d}, cus, s);
     if (int rc = hs.sd == 1 ? prepare8<HT, true>(h, l, hs, mask_d, c, row_scales, s) : prepare8<HT, false>(h, l, hs, mask_d, c, row_scales, s))
@@ -2521,7 +2528,7 @@ extern "C" int gs_term_weights8_workspace(const gs_vocab_head *h, size_t *bytes)
     gs_arena a{nullptr, 0, 0};
     Common c;
     float *best, *row_scales;
-    if (!few8_ok(l.rows, 2 * l.dimp, h->hidden_dim_stride)) take_terms8(a, l, h, &c, &best, &row_scales);
+    if (!few8_ok<EpiFewTerms>(l.rows, 2 * l.dimp, h->hidden_dim_stride)) take_terms8(a, l, h, &c, &best, &row_scales);
     *bytes = a.used;
     return GS_OK;
 }
@@ -2533,7 +2540,7 @@ extern "C" int gs_term_weights8(const gs_vocab_head *h, const float *scales_d, c
     gs_arena a{(char *)workspace_d, 0, workspace_bytes};
     Common c{};
     float *best = nullptr, *row_scales = nullptr;
-    if (!few8_ok(l.rows, 2 * l.dimp, h->hidden_dim_stride)) take_terms8(a, l, h, &c, &best, &row_scales);
+    if (!few8_ok<EpiFewTerms>(l.rows, 2 * l.dimp, h->hidden_dim_stride)) take_terms8(a, l, h, &c, &best, &row_scales);
     if (!a.ok()) {
         gs_set_error("term_weights8 workspace too small: need %zu bytes, got %zu", a.used, workspace_bytes);
         return GS_ENOSPC;
