@@ -6,7 +6,7 @@
 namespace gsv {
 
 // A wave per row; workgroups after those write the bias in fp32.  Bytes bound it (two or four per value in, one out): 16384 rows of
-// 768 16-bit values 13.2 us (2.9 TB/s; launch and a row's latency are a third of it).
+// 768 16-bit values 12 us (3.1 TB/s; launch and a row's latency are a third of it).
 template <int HT, bool UNIT>
 __global__ __launch_bounds__(256) void k_quantize_rows(Source x, int64_t rows, int row_blocks, int dimp, int8_t *out, int64_t stride, float *scales,
                                                        float by, const void *bias, int bias_type, int n, float *bias_o) {
@@ -153,11 +153,11 @@ struct EpiFewLinear {
 
 // Tiles: the largest of which there are as many as CUs.  Product alone, us:
 //   rows x dim -> out        256      128      64
-//   16384 x 1024 -> 4096      84       93     151
-//   16384 x 768 -> 768      18.6     18.0      35   (192 tiles of 256: a quarter of the CUs has none)
+//   16384 x 1024 -> 4096      76       93     151
+//   16384 x 768 -> 768      18.6     18.2      35   (192 tiles of 256: a quarter of the CUs has none)
 //   4099 x 777 -> 1001        37       14      14
-// What bounds the first: 137e9 operations at 1.65e15 a second, of 2.4e15 that a library product of 16384^3 reaches; its 134 MB of
-// output take 26 us of it at the rate of a copy.
+// The first runs at 1810 TOP/s, of 2404 that a library product of 16384^3 reaches (and of 1280 that it does at this shape); its 134 MB
+// of output take 26 us of the 76 at the rate of a copy.
 template <class T>
 using Small8 = Tile<T, 1, 64, 64, 2, 2, 4, 2, false, false>;
 template <class T>

@@ -1,7 +1,8 @@
 """The encoder's first layer: rows of the vocabulary by token id, and their gradient.
 
 The matrix is the one that the vocabulary head multiplies with (:mod:`gpusparse.vocab`), where both are tied: autograd adds
-their gradients.  It may be in 8 bits for serving (:class:`gpusparse.Int8Rows`).
+their gradients.  It may be in 8 bits for serving (:class:`gpusparse.Int8Rows`).  Work is queued on the current stream of
+the weight's device.
 """
 from __future__ import annotations
 

@@ -265,6 +265,55 @@ def test_saved_ids_that_come_back_elsewhere(device):
         torch.autograd.grad(out, [w], grad)
 
 
+def test_under_an_activation_checkpoint(device):
+    from torch.utils.checkpoint import checkpoint
+    w = table(200, 16, F32, device).requires_grad_()
+    ids = words((6, 11), 200, device)
+    want, = torch.autograd.grad((gs.embed_tokens(ids, w, scale=0.5) ** 2).sum(), [w])
+    for reentrant in (False, True):
+        out = checkpoint(lambda x: gs.embed_tokens(ids, x, scale=0.5) ** 2, w, use_reentrant=reentrant)
+        w.grad = None
+        out.sum().backward()
+        assert torch.equal(w.grad, want)
+
+
+def test_functional_transforms_and_forward_mode_are_refused(device):
+    w = table(20, 4, F32, device)
+    ids = torch.arange(5, device=device)
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda x: gs.embed_tokens(ids, x).sum())(w)
+    with torch.autograd.forward_ad.dual_level():
+        with pytest.raises(RuntimeError):
+            gs.embed_tokens(ids, torch.autograd.forward_ad.make_dual(w, torch.ones_like(w)))
+    q = gs.quantize_rows(w)
+    with pytest.raises(ValueError, match="no gradient"):
+        torch.vmap(lambda x: gs.int8_linear(x, q))(torch.zeros((3, 2, 4), device=device))
+
+
+def test_two_threads(device):
+    import threading
+    w = table(400, 32, BF16, device).requires_grad_()
+    idss = [words((n,), 400, device, seed=n) for n in (50, 3000)]
+    grads = [torch.randn((i.numel(), 32), generator=torch.Generator().manual_seed(3)).to(BF16).to(device) for i in idss]
+    want = [torch.autograd.grad(gs.embed_tokens(i, w), [w], g)[0] for i, g in zip(idss, grads)]
+    torch.cuda.synchronize()
+    good = [False, False]
+
+    def work(k):
+        with torch.cuda.stream(torch.cuda.Stream(device)):
+            ok = True
+            for _ in range(20):
+                ok &= torch.equal(torch.autograd.grad(gs.embed_tokens(idss[k], w), [w], grads[k])[0], want[k])
+            good[k] = ok
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert all(good)
+
+
 def test_streams_and_two_at_once(device):
     ws = [table(500, 40, BF16, device, seed=k).requires_grad_() for k in range(2)]
     idss = [words((n,), 500, device, seed=k) for k, n in enumerate((400, 30000))]

@@ -253,6 +253,11 @@ TERMS = [
     (2, 32, 64, 257, F32, "prefix"),
     (64, 1, 64, 300, BF16, "holes"),
     (13, 5, 200, 515, F32, "holes"),           # 65 rows
+    (120, 1, 64, 300, BF16, "holes"),          # a token each
+    (1, 128, 300, 17000, F16, "prefix"),       # the most rows of one launch, a wave for each block of terms
+    (16, 8, 200, 16400, BF16, "empty"),
+    (5, 25, 96, 16500, F32, "holes"),
+    (43, 3, 70, 400, BF16, "prefix"),          # 129 rows: several
     (40, 6, 129, 777, BF16, "prefix"),
     (7, 100, 64, 1030, F16, "empty"),          # texts cross tiles
     (4, 300, 133, 517, BF16, "holes"),
@@ -322,7 +327,7 @@ def test_term_weights_of_a_vocabulary_in_8_bits(device, texts, length, dim, voca
         assert torch.equal(gs.term_weights(h, w, None, mask=mask.to(torch.int64) * 3), got)
 
 
-@pytest.mark.parametrize("texts,length", [(3, 5), (4, 40)])
+@pytest.mark.parametrize("texts,length", [(3, 5), (3, 40), (9, 8), (4, 40)])
 def test_odd_tokens_terms_and_biases(device, texts, length):
     """A NaN or infinite token makes its text's weights NaN; a term's NaN row or bias that term's; -inf keeps a term out, +inf is
     infinite; a text without a kept token has weights 0 under any bias."""
