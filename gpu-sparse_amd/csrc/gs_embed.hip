@@ -92,7 +92,7 @@ __global__ __launch_bounds__(256) void k_embed_strided(Ids ids, const T *table, 
 // among all ids itself (16384 tokens: 14 us, a launch), or, of more, in segments that k_split has sorted by range (17, two; 262144
 // tokens 31, and 270 where all hold one id: a range is one workgroup's, at 1 ns a token).
 constexpr int kRanges = 256, kSegs = 1024;
-constexpr int kSplitThreads = 512, kSplitWaves = kSplitThreads / 64, kSplitTile = 1024;
+constexpr int kSplitThreads = 512, kSplitWaves = kSplitThreads / 64, kSegTokens = 1024;  // of a segment, at least
 // A wave of k_order counts ids on its own, in at most so many bytes of LDS for all waves: fewer waves where ranges are wide.  Beside
 // the counts lie the tokens that a wave has found itself, of 1024 that it looks through.
 constexpr int kOrderLds = 128 * 1024, kDirectLds = 64 * 1024, kOrderMost = 148 * 1024, kDirectWave = 1024;
@@ -178,8 +178,7 @@ __device__ __forceinline__ int block_prefix(int *x, int n, int *wave_sums) {
     return total;
 }
 
-// A segment's tokens sorted by range, kSplitTile at a time: a tile's places follow each other within a range.
-// pos[segment]: token; low[segment]: the id's bits within its range; counts[range][segment], begin[range][segment].
+// A segment's tokens sorted by range, in order within a range.  pos[segment]: token; low[segment]: the id's bits within its range; counts[range][segment], begin[range][segment].
 __global__ __launch_bounds__(kSplitThreads) void k_split(Tokens t, int64_t seg_size, int segs, uint32_t *pos, uint16_t *low, int *counts,
                                                          int *begin) {
     __shared__ int count[kSplitWaves][kRanges], first[kRanges], wave_sums[kSplitWaves];
@@ -625,7 +624,7 @@ int run_lookup(const gs_lookup *l, const float *scales, O *out, hipStream_t s) {
     const Ids ids{l->ids_d, l->id_bytes};
     constexpr int U = 4;
     const int64_t blocks = (total + 256 * U - 1) / (256 * U);
-    GS_REQUIRE(blocks < (1ll << 31), "%lld tokens of %d values exceed a grid", (long long)l->tokens, l->dim);
+    GS_REQUIRE(blocks < (1ll << 24), "%lld tokens of %d values exceed a grid", (long long)l->tokens, l->dim);
 #define GSV_EMBED(TAIL)                                                                                                            \
     hipLaunchKernelGGL((k_embed<T, O, N, U, TAIL>), dim3((unsigned)blocks), dim3(256), 0, s, ids, (const T *)l->weight_d,            \
                        l->weight_row_stride, scales, l->vocab, l->dim, (uint32_t)pieces, total, l->scale, out)
@@ -653,7 +652,7 @@ GradPlan plan_grad(gs_arena &a, const gs_lookup *l) {
     p.few = l->tokens <= kFewTokens;
     p.split = l->tokens > order_waves(kDirectLds, p.shift) * kDirectWave;
     if (p.few) return p;
-    p.seg_size = kSplitTile;
+    p.seg_size = kSegTokens;
     while (p.seg_size * kSegs < l->tokens) p.seg_size *= 2;
     p.segs = (int)((l->tokens + p.seg_size - 1) / p.seg_size);
     p.chunk = 16;

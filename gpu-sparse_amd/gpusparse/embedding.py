@@ -98,7 +98,9 @@ def embed_tokens(ids, weight, *, scale: float = 1.0, padding_idx: int | None = N
         raise ValueError(f"scale must be finite in float32, got {scale}")
     if padding_idx is not None and not 0 <= int(padding_idx) < weight.shape[0]:
         raise ValueError(f"padding_idx must be in [0, {weight.shape[0]}), got {padding_idx}")
-    _gpu(weight, "weight", ids=ids)
+    dev = ids.device
+    if dev.type != "cuda" or weight.device != dev:
+        _gpu(weight, "weight", ids=ids)
     padding = -1 if padding_idx is None else int(padding_idx)
     ids = ids.contiguous()
     if q8:

@@ -84,6 +84,7 @@ def _refuse_gradient(*inputs):
 
 
 def _gpu(t, name: str, **others) -> torch.device:
+    """The GPU that a call runs on, which is t's; refuses tensors that are elsewhere."""
     dev = t.device
     if dev.type != "cuda":
         dev = _lib.require_gpu(dev)
@@ -133,7 +134,9 @@ def int8_linear(x: torch.Tensor, weight: Int8Rows, bias=None, *, dtype: torch.dt
     if dtype not in _lib.HTYPE_OF_DTYPE:
         raise ValueError(f"dtype must be float32, float16 or bfloat16, got {dtype}")
     _check_bias(bias, out)
-    dev = _gpu(x, "x", weight=weight, bias=bias)
+    dev = x.device
+    if dev.type != "cuda" or weight.values.device != dev or (bias is not None and bias.device != dev):
+        dev = _gpu(x, "x", weight=weight, bias=bias)
     _refuse_gradient(x, bias)
     bias = None if bias is None else bias.contiguous()
     rows = x if x.dim() == 2 else x.reshape(-1, dim)

@@ -167,7 +167,10 @@ def _check_head8(hidden, weight, bias) -> torch.device:
     if hidden.shape[-1] != weight.shape[1]:
         raise ValueError(f"hidden must be [texts, length, dim] with dim {weight.shape[1]}, got {tuple(hidden.shape)}")
     _check_bias(bias, weight.shape[0])
-    return _gpu(hidden, "hidden", weight=weight, bias=bias)
+    dev = hidden.device
+    if dev.type != "cuda" or weight.values.device != dev or (bias is not None and bias.device != dev):
+        dev = _gpu(hidden, "hidden", weight=weight, bias=bias)
+    return dev
 
 
 def term_weights(hidden, weight, bias=None, *, mask=None, return_tokens: bool = False):
