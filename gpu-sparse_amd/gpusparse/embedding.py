@@ -15,6 +15,7 @@ from .int8 import Int8Rows, _gpu, _refuse_gradient
 
 C = _lib.C
 MAX_SCALE = torch.finfo(torch.float32).max
+FEW_TOKENS = 1024  # whose gradient takes no workspace
 
 
 def _lookup(ids, weight, scale: float, padding: int):
@@ -49,7 +50,7 @@ def _gradient(ctx, grad):
         if grad.stride(1) != 1:
             grad = grad.contiguous()
         row = grad.stride(0)
-    dw = torch.empty((a.vocab, a.dim), dtype=ctx.dtype, device=dev)
+    dw = grad.new_empty((a.vocab, a.dim))
     ws = _bytes(ctx.grad_bytes, dev) if ctx.grad_bytes else None
     with _on(dev):
         _lib.check(_lib.lib().gs_embed_tokens_grad(C.byref(a), grad.data_ptr(), row, dw.data_ptr(), _lib.ptr(ws), ctx.grad_bytes,
@@ -64,12 +65,14 @@ class _Embed(torch.autograd.Function):
     @staticmethod
     def forward(ctx, ids, weight, scale, padding):
         out, ctx.lookup = _lookup(ids, weight, scale, padding)
-        need = C.c_size_t()
-        _lib.check(_lib.lib().gs_embed_tokens_grad_workspace(C.byref(ctx.lookup), C.byref(need)), "gs_embed_tokens_grad_workspace")
-        ctx.grad_bytes = need.value
+        ctx.grad_bytes = 0
+        if ids.numel() > FEW_TOKENS:
+            need = C.c_size_t()
+            _lib.check(_lib.lib().gs_embed_tokens_grad_workspace(C.byref(ctx.lookup), C.byref(need)), "gs_embed_tokens_grad_workspace")
+            ctx.grad_bytes = need.value
         ctx.save_for_backward(ids)
         ctx.at = (ids.data_ptr(), ids.shape, ids.stride(), ids.dtype)
-        ctx.dev, ctx.dtype = out.device, weight.dtype
+        ctx.dev = out.device
         return out
 
     @staticmethod

@@ -107,7 +107,7 @@ def test_lookup_types_and_pointers():
         with pytest.raises(ValueError, match=match):
             _lib.check(L.gs_embed_tokens(C.byref(lookup(**over)), 8, None), "call")
     assert L.gs_embed_tokens(C.byref(lookup(tokens=0)), None, None) == _lib.GS_OK
-    assert L.gs_embed_tokens_grad_workspace(C.byref(lookup(tokens=1024)), C.byref(n)) == _lib.GS_OK and n.value == 0
+    assert L.gs_embed_tokens_grad_workspace(C.byref(lookup(tokens=gs.embedding.FEW_TOKENS)), C.byref(n)) == _lib.GS_OK and n.value == 0
     assert L.gs_embed_tokens_grad_workspace(C.byref(lookup(tokens=1025)), C.byref(n)) == _lib.GS_OK and n.value > 1025 * 8
     assert L.gs_embed_tokens_grad(C.byref(lookup(tokens=1025)), 8, 100, 8, 256, n.value - 1, None) == _lib.GS_ENOSPC
     with pytest.raises(ValueError, match="NULL"):
