@@ -155,6 +155,18 @@ __device__ __forceinline__ ColumnScale column_scale(int v, const Weight8 &W, con
     return v < W.n ? ColumnScale{W.scales[v], bias_at(bias, type, v)} : ColumnScale{0.f, 0.f};
 }
 
+// A maximum over a text's rows is taken of their sums times their own scales, and the column's scale multiplies that alone: as its
+// magnitude, since a scale below zero, which a weight made elsewhere may have, turns the order round, so that its column's
+// values change sign first.  An infinite one makes a NaN of some values, which are maxima.  (Not of NaN scales: all values are NaN.)
+__device__ __forceinline__ bool reorders(float by) { return by < 0.f || by == INFINITY; }
+__device__ __forceinline__ float in_order(float x, const ColumnScale &c) {
+    if (fabsf(c.by) == INFINITY) {
+        const float l = fmaf(x * c.by, kUp, c.bias);
+        if (l != l) return l;
+    }
+    return c.by < 0.f ? -x : x;
+}
+
 // Products of at most 128 rows, their values on end, in one launch, for latency: a workgroup of eight waves quantises all rows into
 // LDS itself and takes blocks of 16 columns, KS of its waves a block, each its part of k.  The weight goes from memory to the
 // operands' registers: a lane takes 32 bytes on end of its column, so that a wave's loads take whole lines, and the first of them

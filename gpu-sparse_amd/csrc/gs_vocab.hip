@@ -812,7 +812,7 @@ struct EpiHiddenPart {
 // (rounding keeps order).  The product bounds it: 10240 rows, 30522 terms, 768 values, 372 us (1290 TFLOP/s); texts of 20 tokens,
 // whose maxima are joined across lanes and written seven times a wave: 1280 rows 67 us (890).
 //
-// Q8: operands in 8 bits.  Sums take their row's scale before they are compared, their column's after: 10240 rows, 30522 terms, 768
+// Q8: operands in 8 bits.  Sums take their row's scale before they are compared, their column's magnitude after (in_order): 10240 rows, 30522 terms, 768
 // values 201 us (2390 TOP/s, what a library product of 16384^3 reaches).
 template <bool TOK, bool Q8 = false>
 struct EpiTextMax {
@@ -861,7 +861,7 @@ struct EpiTextMax {
         join(across<32>(x[0], x[MC / 2 - 1]), TOK ? across<32>(r[0], r[MC / 2 - 1]) : Two<int>{0, 0}, best_x, best_r);
         const int v = at.col0 + at.lane;
         if (at.lane < 16 * MC && v < vocab) {
-            best[slot * vocab + v] = Q8 ? fmaf(best_x * by, kUp, b) : best_x + b;
+            best[slot * vocab + v] = Q8 ? fmaf(best_x * fabsf(by), kUp, b) : best_x + b;
             if (TOK) where[slot * vocab + v] = best_r;
         }
     }
@@ -876,6 +876,7 @@ struct EpiTextMax {
         const int64_t block = at.row0 / (TL::MR * 16);
         const float b = at.side(0, at.c_in + (at.lane & (16 * TL::MC - 1)));  // of the column that the lane writes
         const float by = Q8 ? at.side(3, at.c_in + (at.lane & (16 * TL::MC - 1))) : 1.f;
+        const bool some = Q8 && __any(reorders(by));
         float top[TL::MC];
         int tok[TL::MC];
 #pragma unroll
@@ -891,6 +892,15 @@ struct EpiTextMax {
                 const f32x4 sc = at.side4(2, at.r_in + 16 * i + 4 * q);
 #pragma unroll
                 for (int j = 0; j < TL::MC; j++) acc[i][j] = __builtin_convertvector(__builtin_bit_cast(i32x4, acc[i][j]), f32x4) * sc;
+                if (__builtin_expect(some, 0)) {
+#pragma unroll
+                    for (int j = 0; j < TL::MC; j++) {
+                        const int c = at.c_in + 16 * j + (at.lane & 15);
+                        const ColumnScale col{at.side(3, c), at.side(0, c)};
+#pragma unroll
+                        for (int e = 0; e < 4; e++) acc[i][j][e] = in_order(acc[i][j][e], col);
+                    }
+                }
             }
             if (lo == cur && hi == cur) {  // all of one text
 #pragma unroll
@@ -1354,10 +1364,14 @@ struct EpiFewTerms {
     static constexpr bool joins = true;
     static constexpr int most_rows = kFewRows;
     __device__ __forceinline__ ColumnScale column(int v, const Weight8 &W) const { return column_scale(v, W, bias, bias_type); }
-    __device__ __forceinline__ void block(const i32x4 &sum, int m, int, const Weight8 &, const ColumnScale &, const float *scales, int, int lane,
+    __device__ __forceinline__ void block(const i32x4 &sum, int m, int, const Weight8 &, const ColumnScale &col, const float *scales, int, int lane,
                                           float *left) const {
         const int row = 16 * m + 4 * (lane >> 4);
-        const f32x4 x = __builtin_convertvector(sum, f32x4) * *reinterpret_cast<const f32x4 *>(scales + row);
+        f32x4 x = __builtin_convertvector(sum, f32x4) * *reinterpret_cast<const f32x4 *>(scales + row);
+        if (__builtin_expect(__any(reorders(col.by)), 0)) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) x[e] = in_order(x[e], col);
+        }
 #pragma unroll
         for (int e = 0; e < 4; e++) left[(row + e) * kFewPitch + (lane & 15)] = x[e];
     }
@@ -1382,7 +1396,7 @@ struct EpiFewTerms {
                 any = __any(any);
             }
             if (text < texts && v < W.n && (apart || q == 0))
-                weights[(int64_t)text * W.n + v] = log1pf(any ? maximum(fmaf(top * col.by, kUp, col.bias), 0.f, 0.f) : 0.f);
+                weights[(int64_t)text * W.n + v] = log1pf(any ? maximum(fmaf(top * fabsf(col.by), kUp, col.bias), 0.f, 0.f) : 0.f);
         }
     }
 };

@@ -470,7 +470,7 @@ int gs_vocab_loss_grad(const gs_vocab_head *head, const gs_vocab_targets *target
 /* ------------------------------------------------------------ rows in 8 bits
  * No counterpart in the reference.  A row x is kept as whole numbers q = nearest(127 x / max|x|), ties to even, and one
  * scale max|x| / 127.  A row with an infinity or a NaN has scale NaN (and values 0), one whose largest magnitude is below
- * 2^-94 counts as zeros.  8-bit rows start 16-byte aligned, a multiple of 128 bytes apart that covers dim rounded up to 128;
+ * 2^-94 counts as zeros.  Scales that come from elsewhere may have either sign.  8-bit rows start 16-byte aligned, a multiple of 128 bytes apart that covers dim rounded up to 128;
  * what lies between dim and that is read, but counts for nothing. */
 int gs_quantize_rows(const void *x_d, int32_t type, int64_t rows, int32_t dim, int64_t row_stride, int64_t dim_stride,
                      int8_t *values_d, int64_t values_stride, float *scales_d, void *stream);

@@ -380,6 +380,81 @@ def test_padded_memory_of_a_weight_counts_for_nothing(device):
         assert torch.equal(gs.term_weights(x[None], w), gs.term_weights(x[None], copy))
 
 
+SIGNED = [
+    # texts, length, dim, vocab: one launch (waves that share a block of terms; a wave for each), tiles of each size
+    (3, 5, 64, 300), (2, 17, 96, 16500), (30, 4, 64, 300), (4, 40, 64, 517), (9, 50, 128, 1030), (20, 100, 64, 700),
+]
+
+
+@pytest.mark.parametrize("bias_type", [None, F32, F16, BF16])
+@pytest.mark.parametrize("texts,length,dim,vocab", SIGNED)
+def test_scales_of_either_sign(device, texts, length, dim, vocab, bias_type):
+    """A weight made elsewhere may have scales below zero: the largest logit is that of the smallest sum."""
+    print(f"signed scales {texts}x{length} dim {dim} vocab {vocab} bias {bias_type}", flush=True)
+    h = rows((texts, length, dim), F32, 40, device, spread=False)
+    q = gs.quantize_rows(rows((vocab, dim), F32, 41, device, spread=False) / math.sqrt(dim))
+    sign = torch.where(torch.rand(vocab, generator=torch.Generator().manual_seed(42)) < 0.5, -1.0, 1.0).to(device)
+    w = gs.Int8Rows(q.values, q.scales * sign, F32)
+    bias = None if bias_type is None else rows((vocab,), bias_type, 43, device, spread=False) * 0.5
+    mask = mask_of("holes" if texts == 3 else "empty", texts, length, device)
+    want, bound = terms64(h, w, bias, mask)
+    got = gs.term_weights(h, w, bias, mask=mask)
+    assert_within(got, want, bound, "weights")
+    # the sign in the values' place is the same matrix, bit for bit
+    turned = gs.Int8Rows(q.values * sign.to(torch.int8)[:, None], q.scales, F32)
+    assert torch.equal(gs.term_weights(h, turned, bias, mask=mask), got)
+    x = h.view(-1, dim)
+    assert torch.equal(gs.int8_linear(x, w, bias), gs.int8_linear(x, turned, bias))
+    if bool((sign < 0).all() | (sign > 0).all()):
+        pytest.fail("scales of one sign alone")
+
+
+@pytest.mark.parametrize("texts,length,dim,vocab", SIGNED)
+def test_scales_that_are_not_finite(device, texts, length, dim, vocab):
+    """A term whose scale is infinite has infinite logits, and a NaN where a token's sum is 0 or the bias an infinity of the other
+    sign: that is its text's maximum.  One whose scale is NaN has NaN everywhere."""
+    h = rows((texts, length, dim), F32, 44, device, spread=False)
+    h[1, 0] = 0                                                 # every sum of it is 0
+    q = gs.quantize_rows(rows((vocab, dim), F32, 45, device, spread=False) / math.sqrt(dim))
+    scales = q.scales.clone()
+    scales[1], scales[2], scales[3], scales[4] = float("inf"), -float("inf"), float("nan"), -0.0
+    scales[5], scales[6], scales[7] = float("inf"), -float("inf"), -scales[7]
+    scales[vocab - 1] = -float("inf")
+    w = gs.Int8Rows(q.values, scales, F32)
+    bias = torch.zeros(vocab, device=device)
+    bias[5], bias[6] = -float("inf"), float("inf")
+    mask = torch.ones((texts, length), dtype=torch.bool, device=device)
+    mask[2:][-1:] = False                                       # the last of three texts or more has no token
+    l = (values64(h.view(-1, dim))[0].to(device) @ w.values.double().t()) * values64(h.view(-1, dim))[1].to(device).double()[:, None]
+    x = (l * scales.double() + bias.double()).view(texts, length, vocab)
+    top = torch.where(torch.isnan(x).any(dim=1), float("nan"), x.nan_to_num(nan=0, posinf=float("inf"), neginf=-float("inf")).amax(dim=1))
+    want = torch.log1p(top.clamp(min=0))
+    want[2:][-1:] = 0
+    got = gs.term_weights(h, w, bias, mask=mask)
+    assert bool(torch.isnan(want[1, [1, 2, 3, 5, 6, vocab - 1]]).all()) and bool(torch.isinf(want).any())
+    assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(torch.isinf(got), torch.isinf(want))
+    _, bound = terms64(h, gs.Int8Rows(q.values, torch.where(torch.isfinite(scales), scales, 0), F32), None, mask)
+    fine = torch.isfinite(want)
+    assert_within(torch.where(fine, got, 0), torch.where(fine, want, 0), bound, "weights")
+
+
+@pytest.mark.parametrize("texts,length,dim,vocab", [(2, 10, 64, 301), (5, 60, 64, 301), (30, 90, 64, 1030)])
+def test_a_vocabulary_cut_in_parts(device, texts, length, dim, vocab):
+    """Scales that start anywhere in a buffer."""
+    h = rows((texts, length, dim), BF16, 46, device)
+    x = h.view(-1, dim)
+    w = gs.quantize_rows(rows((vocab, dim), BF16, 47, device) / math.sqrt(dim))
+    whole, lin = gs.term_weights(h, w), gs.int8_linear(x, w)
+    at = 0
+    for n in (1, 2, 3, vocab // 2, vocab - vocab // 2 - 6):
+        part = gs.Int8Rows(w.values[at:at + n], w.scales[at:at + n], BF16)
+        assert part.scales.data_ptr() == w.scales.data_ptr() + 4 * at
+        assert torch.equal(gs.term_weights(h, part), whole[:, at:at + n])
+        assert torch.equal(gs.int8_linear(x, part), lin[:, at:at + n])
+        at += n
+    assert at == vocab
+
+
 # ---------------------------------------------------------------- streams, graphs
 
 def test_another_stream_and_two_at_once(device):
