@@ -8,6 +8,14 @@ from torch.autograd import forward_ad
 
 
 HERE = nullcontext()
+MAX_ROWS, MAX_DIM, MAX_TERMS = 1 << 28, 1 << 15, 1 << 20
+
+
+def _check_sizes(rows: int, dim: int, terms: int = 1):
+    """The C entries' limits.  They are checked here as well since ctypes cuts a size that is beyond its field's 32 bits, so
+    that those entries would see another, smaller one."""
+    if rows > MAX_ROWS or dim > MAX_DIM or terms > MAX_TERMS:
+        raise ValueError(f"{rows} rows, {dim} values, {terms} terms: at most {MAX_ROWS}, {MAX_DIM} and {MAX_TERMS} are supported")
 
 
 def _same_device(dev, of="hidden", **tensors):

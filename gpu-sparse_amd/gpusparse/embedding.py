@@ -10,7 +10,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._tensors import _bytes, _differentiable, _on
+from ._tensors import _bytes, _check_sizes, _differentiable, _on
 from .int8 import Int8Rows, _gpu, _refuse_gradient
 
 C = _lib.C
@@ -101,6 +101,7 @@ def embed_tokens(ids, weight, *, scale: float = 1.0, padding_idx: int | None = N
         raise ValueError(f"scale must be finite in float32, got {scale}")
     if padding_idx is not None and not 0 <= int(padding_idx) < weight.shape[0]:
         raise ValueError(f"padding_idx must be in [0, {weight.shape[0]}), got {padding_idx}")
+    _check_sizes(ids.numel(), weight.shape[1], weight.shape[0])
     dev = ids.device
     if dev.type != "cuda" or weight.device != dev:
         _gpu(weight, "weight", ids=ids)

@@ -17,7 +17,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from ._tensors import _bytes, _differentiable, _on, _same_device
+from ._tensors import _bytes, _check_sizes, _differentiable, _on, _same_device
 
 C = _lib.C
 PAD = 128  # bytes that 8-bit rows are padded to
@@ -98,6 +98,7 @@ def quantize_rows(x: torch.Tensor) -> Int8Rows:
         raise ValueError("x must be a float32, float16 or bfloat16 tensor [rows, dim]")
     if x.shape[1] < 1:
         raise ValueError("x must have at least one column")
+    _check_sizes(*x.shape)
     dev = _gpu(x, "x")
     x = x.detach()
     values = torch.empty((x.shape[0], -(-x.shape[1] // PAD) * PAD), dtype=torch.int8, device=dev)
@@ -134,6 +135,7 @@ def int8_linear(x: torch.Tensor, weight: Int8Rows, bias=None, *, dtype: torch.dt
     if dtype not in _lib.HTYPE_OF_DTYPE:
         raise ValueError(f"dtype must be float32, float16 or bfloat16, got {dtype}")
     _check_bias(bias, out)
+    _check_sizes(x.shape[:-1].numel(), dim, out)
     dev = x.device
     if dev.type != "cuda" or weight.values.device != dev or (bias is not None and bias.device != dev):
         dev = _gpu(x, "x", weight=weight, bias=bias)

@@ -26,13 +26,18 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._tensors import _bytes, _differentiable, _on, _same_device
+from ._tensors import _bytes, _check_sizes, _differentiable, _on, _same_device
 from .int8 import Int8Rows, _check_bias, _gpu, _refuse_gradient
 
 C = _lib.C
 REDUCTIONS = {"none": _lib.GS_REDUCE_NONE, "mean": _lib.GS_REDUCE_MEAN, "sum": _lib.GS_REDUCE_SUM}
 MAX_TOP = 1024  # most teacher logits per row
 SAVED_ALIGN = 256  # of what a loss saves for its gradient
+
+
+def _check_head_sizes(hidden, weight):
+    lead = hidden.shape[:-1]
+    _check_sizes(max(lead.numel(), *lead) if lead else 1, weight.shape[1], weight.shape[0])  # a side may be long and another 0
 
 
 def _check_head(hidden, weight, bias, dims: str) -> torch.device:
@@ -49,6 +54,7 @@ def _check_head(hidden, weight, bias, dims: str) -> torch.device:
         raise ValueError(f"hidden must be {dims} with dim {weight.shape[1]}, got {tuple(hidden.shape)}")
     if bias is not None and tuple(bias.shape) != (weight.shape[0],):
         raise ValueError(f"bias must be [{weight.shape[0]}], got {tuple(bias.shape)}")
+    _check_head_sizes(hidden, weight)
     dev = hidden.device
     if dev.type != "cuda":
         dev = _lib.require_gpu(dev)
@@ -167,6 +173,7 @@ def _check_head8(hidden, weight, bias) -> torch.device:
     if hidden.shape[-1] != weight.shape[1]:
         raise ValueError(f"hidden must be [texts, length, dim] with dim {weight.shape[1]}, got {tuple(hidden.shape)}")
     _check_bias(bias, weight.shape[0])
+    _check_head_sizes(hidden, weight)
     dev = hidden.device
     if dev.type != "cuda" or weight.values.device != dev or (bias is not None and bias.device != dev):
         dev = _gpu(hidden, "hidden", weight=weight, bias=bias)

@@ -127,6 +127,44 @@ def test_int8_rows_are_checked():
             gs.Int8Rows(*args)
 
 
+FAR = 2 ** 32 + 5  # 5, cut to 32 bits
+
+
+def wide(*shape, dtype=torch.bfloat16):
+    """A tensor of any size in one value's memory."""
+    return torch.zeros((1,) * len(shape), dtype=dtype).expand(*shape)
+
+
+def test_sizes_beyond_32_bits_are_refused():
+    """Not cut to what is left of them in 32 bits.  Sizes are checked before the device is, so that this needs none."""
+    r = gs.Int8Rows(torch.zeros((3, 64), dtype=torch.int8), torch.ones(3))
+    ids, few = torch.zeros(2, dtype=torch.int64), torch.zeros((1, 2, 64), dtype=torch.bfloat16)
+    for call in (lambda: gs.int8_linear(wide(FAR, 64), r), lambda: gs.int8_linear(wide(2, FAR, 64), r),
+                 lambda: gs.quantize_rows(wide(FAR, 1)), lambda: gs.quantize_rows(wide(1, FAR)),
+                 lambda: gs.embed_tokens(ids, wide(FAR, 1)), lambda: gs.embed_tokens(ids, wide(1, FAR)),
+                 lambda: gs.embed_tokens(wide(FAR, dtype=torch.int64), few[0]),
+                 lambda: gs.term_weights(wide(FAR, 1, 64), r), lambda: gs.term_weights(wide(FAR, 0, 64), r),
+                 lambda: gs.term_weights(wide(1, FAR, 64), few[0]), lambda: gs.term_weights(few, wide(FAR, 64)),
+                 lambda: gs.term_weights(wide(1, 2, FAR), wide(1, FAR)),
+                 lambda: gs.vocab_loss(few[0], wide(FAR, 64), ids), lambda: gs.vocab_loss(wide(FAR, 64), few[0], wide(FAR, dtype=torch.int64)),
+                 lambda: gs.distill_loss(few[0], wide(FAR, 64), ids[:, None], ids[:, None].float())):
+        with pytest.raises(ValueError, match=f"{FAR} (rows|values|terms)|{2 * FAR} rows"):
+            call()
+
+
+@pytest.mark.parametrize("over", [1, 2 ** 32])
+def test_the_largest_sizes(over):
+    """The limits themselves are refused for the GPU that is missing here alone, or would be too large for one."""
+    ids = torch.zeros(2, dtype=torch.int64)
+    with pytest.raises(ValueError, match="terms: at most"):
+        gs.embed_tokens(ids, wide(2 ** 20 + over, 8))
+    with pytest.raises(ValueError, match="values, 5 terms"):
+        gs.embed_tokens(ids, wide(5, 2 ** 15 + over))
+    if not torch.cuda.is_available():
+        with pytest.raises(RuntimeError, match="GPU"):
+            gs.embed_tokens(ids, wide(2 ** 20, 2 ** 15))
+
+
 @pytest.mark.skipif(torch.cuda.is_available(), reason="needs a machine without a GPU")
 def test_without_a_gpu_calls_raise():
     r = gs.Int8Rows(torch.zeros((3, 5), dtype=torch.int8), torch.ones(3))
