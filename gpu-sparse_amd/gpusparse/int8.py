@@ -21,6 +21,7 @@ from ._tensors import _bytes, _check_sizes, _differentiable, _on, _same_device
 
 C = _lib.C
 PAD = 128  # bytes that 8-bit rows are padded to
+MAX_STRIDE = 1 << 20  # rows lie nearer than this, in bytes
 
 
 def _padded(rows: int, dim: int, device) -> torch.Tensor:
@@ -29,10 +30,11 @@ def _padded(rows: int, dim: int, device) -> torch.Tensor:
 
 
 def _in_place(values: torch.Tensor) -> bool:
-    """Whether 8-bit rows can be read where they are: each starts 16-byte aligned and may be read up to its padding's end."""
+    """Whether 8-bit rows can be read where they are: each starts 16-byte aligned, may be read up to its padding's end, and
+    lies as near to the next as the kernels' offsets reach."""
     rows, dim = values.shape
     width = -(-dim // PAD) * PAD
-    if values.stride(1) != 1 or values.stride(0) % PAD or values.stride(0) < width or values.data_ptr() % 16:
+    if values.stride(1) != 1 or values.stride(0) % PAD or not width <= values.stride(0) < MAX_STRIDE or values.data_ptr() % 16:
         return False
     return values.storage_offset() + (rows - 1) * values.stride(0) + width <= values.untyped_storage().nbytes()
 

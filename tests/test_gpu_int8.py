@@ -143,6 +143,20 @@ def test_int8_rows_made_from_parts(device):
     assert gs.Int8Rows(cut, w.scales).values.data_ptr() != cut.data_ptr()
 
 
+def test_int8_rows_that_lie_far_apart(device):
+    """Every 8192nd row of a table of 128-byte rows: 2^20 bytes apart."""
+    table = torch.zeros((3 * 8192, 128), dtype=torch.int8, device=device)
+    w = gs.quantize_rows(rows((3, 100), BF16, 48, device))
+    table[::8192, :100] = w.values
+    far = gs.Int8Rows(table[::8192, :100], w.scales, BF16)
+    for m in (2, 300):
+        x = rows((m, 100), BF16, 49, device)
+        assert torch.equal(gs.int8_linear(x, far), gs.int8_linear(x, w))
+        assert torch.equal(gs.term_weights(x[None], far), gs.term_weights(x[None], w))
+    ids = torch.arange(3, device=device)
+    assert torch.equal(gs.embed_tokens(ids, far), gs.embed_tokens(ids, w))
+
+
 # ---------------------------------------------------------------- int8_linear
 
 LINEAR = [

@@ -127,6 +127,17 @@ def test_int8_rows_are_checked():
             gs.Int8Rows(*args)
 
 
+def test_int8_rows_that_lie_far_apart_are_copied():
+    """Rows of a much wider matrix, or a few rows of a large table: 2^20 bytes and more apart, which no call takes in place."""
+    for rows, stride in ((2, 1 << 20), (3, 3 << 20), (1, 1 << 20)):
+        base = torch.randint(-127, 128, ((rows - 1) * stride + 128,), dtype=torch.int8, generator=torch.Generator().manual_seed(rows))
+        v = base.as_strided((rows, 100), (stride, 1))
+        r = gs.Int8Rows(v, torch.ones(rows))
+        assert r.values.stride(0) == 128 and torch.equal(r.values, v)
+    near = torch.zeros((1 << 20) + 128, dtype=torch.int8).as_strided((2, 100), ((1 << 20) - 128, 1))
+    assert gs.Int8Rows(near, torch.ones(2)).values.data_ptr() == near.data_ptr()
+
+
 FAR = 2 ** 32 + 5  # 5, cut to 32 bits
 
 
