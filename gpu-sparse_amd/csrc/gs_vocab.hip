@@ -2479,6 +2479,7 @@ int check_texts8(const gs_vocab_head *h) {
     GS_REQUIRE(h->weight_row_stride % kPad8 == 0 && h->weight_row_stride >= round_up(h->dim, kPad8) && h->weight_row_stride < (1 << 20),
                "weight_row_stride=%lld of 8-bit rows: a multiple of %d, at least dim rounded up to one, below 2^20",
                (long long)h->weight_row_stride, kPad8);
+    GS_REQUIRE(h->weight_dim_stride == 1, "weight_dim_stride=%lld of 8-bit rows, which lie on end", (long long)h->weight_dim_stride);
     return GS_OK;
 }
 

@@ -76,6 +76,15 @@ def test_heads_in_8_bits_are_checked(over, match):
             _lib.check(call(), "call")
 
 
+@pytest.mark.parametrize("stride", [0, 2, -1, 128])
+def test_heads_in_8_bits_have_their_values_on_end(stride):
+    L, n = _lib.lib(), C.c_size_t()
+    for call in (lambda: L.gs_term_weights8_workspace(C.byref(head(weight_dim_stride=stride)), C.byref(n)),
+                 lambda: L.gs_term_weights8(C.byref(head(weight_dim_stride=stride)), 256, None, 256, 256, 1 << 30, None)):
+        with pytest.raises(ValueError, match=f"weight_dim_stride={stride}"):
+            _lib.check(call(), "call")
+
+
 def test_term_weights8_workspace_and_pointers():
     L, n = _lib.lib(), C.c_size_t()
     assert L.gs_term_weights8_workspace(C.byref(head()), C.byref(n)) == _lib.GS_OK and n.value > 600 * 128
