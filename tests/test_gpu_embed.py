@@ -233,6 +233,30 @@ def test_lookup_in_8_bits(device, dtype, dim):
     assert torch.equal(gs.embed_tokens(ids.int(), q), gs.embed_tokens(ids, q)) or bool(torch.isnan(got).any())
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("kind", [None, "rows", "columns", "8 bits"])
+@pytest.mark.parametrize("n,vocab,dim", [(1, 1, 1), (155, 200, 64), (1500, 300, 129)])
+def test_rows_by_32_bit_ids(device, dtype, kind, n, vocab, dim):
+    """Every id of the table, some below 0 and some past its end, the type's lowest and largest among them."""
+    print(f"32-bit ids {n} of {vocab} x {dim} {dtype} {kind}", flush=True)
+    w = table(vocab, dim, dtype, device)
+    ids = words((n,), vocab, device, how="evenly")
+    if n > 1:
+        ids[:6] = torch.tensor([-2 ** 31, 2 ** 31 - 1, -1, vocab, vocab - 1, 0], device=device)
+    small = ids.int()
+    if kind == "8 bits":
+        q = gs.quantize_rows(w)
+        rows, by = q.values.float() * q.scales[:, None], torch.tensor(1.5, dtype=F32, device=device)
+        inside = (ids >= 0) & (ids < vocab)
+        want = torch.where(inside[:, None], (rows[ids.clamp(0, vocab - 1)] * by).to(dtype), torch.zeros((), dtype=dtype, device=device))
+        got = gs.embed_tokens(small, q, scale=1.5)
+    else:
+        want = looked_up(w, ids, 1.5)
+        got = gs.embed_tokens(small, strided(w, kind), scale=1.5)
+    assert got.dtype == dtype and torch.equal(got, want)
+    assert torch.equal(gs.embed_tokens(small[::2], q if kind == "8 bits" else w, scale=1.5), want[::2])
+
+
 def test_a_table_tied_to_the_vocabulary_head(device):
     """The same matrix looked up and multiplied with: autograd adds both gradients."""
     w = table(300, 64, F32, device).requires_grad_()
