@@ -4,8 +4,9 @@
 // What a product of such rows needs is exact until its end: sums of q_x q_w fit 32 bits (32768 x 128^2 = 2^29), and
 //     l = (sum of q_x q_w) * scale_x * scale_w + bias
 // takes one rounding of the sum to fp32, one per scale and one with the bias.  The scales of x are multiplied by 2^-24 where
-// they are made and the 2^24 is part of the last fma: so neither factor overflows or falls below the normal range before
-// l itself does (scales are 0 or 2^-101 to 2^121).
+// they are made and the 2^24 is part of the last fma, so that nothing overflows before l itself does (scales are 0 or 2^-101 to
+// 2^121).  Its price is at the other end: what the fma multiplies is l 2^-24, below the normal range where l (without its bias) is
+// below 2^-102, and l is then off by up to 2^-126 more.
 //
 // A row with an infinity or a NaN has scale NaN, and everything made from it is NaN.  One whose largest magnitude is below
 // 2^-94 counts as zeros.
@@ -53,7 +54,8 @@ struct Raw8 {  // eight values as they lie
 // Eight values' nearest whole numbers to p / most (p = 127 x, both times 2^-8, so that p stays finite), a byte each.
 //
 // y = p inv is off by a few units; y + (p - y most) inv is the quotient to half a unit and, where that is n + 1/2, exactly that.
-// 16-bit values: p has no rounding, and no other quotient is nearer to n + 1/2 than 2^-12 of itself, so rounding y is rounding the
+// 16-bit values: p has no rounding, and no other quotient is nearer to n + 1/2 than 2^-19 of itself (2 p and (2n + 1) most are both
+// whole multiples of x's last place, 2 p of less than 254 x 2^11), far beyond y's error, so rounding y is rounding the
 // quotient.  fp32: p's rounding error `low` is kept; where y is n + 1/2 the sign of p + low - y most, which is exact there, says on which
 // side the quotient is.  Adding 1.5 x 2^23 rounds to the nearest whole number, ties to even, whose two's complement is then the
 // sum's low byte.  (Deciding by x * inv alone except next to a half costs less, but the code for the halves, once for each place where

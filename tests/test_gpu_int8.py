@@ -251,6 +251,18 @@ def test_int8_linear_of_large_small_and_odd_rows(device, m):
     assert bool((got[2, [0, 1, 2]] == 0).all())
 
 
+@pytest.mark.parametrize("m", [5, 400])
+@pytest.mark.parametrize("power", [-50, -56, -62, -66])
+def test_int8_linear_of_results_near_zero(device, m, power):
+    """Results of about 2^-85 to 2^-117.  Those below 2^-102 are rounded once more, where the product with the scales is 2^-24 of them and below
+    the normal range: half of 2^-149, times 2^24."""
+    x = rows((m, 96), F32, 50, device, spread=False) * 2.0 ** power
+    w = gs.quantize_rows(rows((80, 96), F32, 51, device, spread=False) * 2.0 ** (power + 12))
+    want, l = linear64(x, w, None)
+    bound = 3 * l * U * (1 + 2.0 ** -6) + 2.0 ** -126 * (l.abs() < 2.0 ** -101) + TINY[F32]
+    assert_within(gs.int8_linear(x, w), want, bound, "linear")
+
+
 @pytest.mark.parametrize("shape", [(0, 64), (2, 0, 64)])
 def test_int8_linear_without_rows(device, shape):
     w = gs.quantize_rows(rows((30, 64), BF16, 1, device))
