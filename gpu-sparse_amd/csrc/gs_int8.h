@@ -173,7 +173,8 @@ __device__ __forceinline__ float in_order(float x, const ColumnScale &c) {
 // LDS itself and takes blocks of 16 columns, KS of its waves a block, each its part of k.  The weight goes from memory to the
 // operands' registers: a lane takes 32 bytes on end of its column, so that a wave's loads take whole lines, and the first of them
 // are asked for before the rows are quantised.  What bounds it is the weight's bytes and latency: one row of 768 values, 30522
-// columns 6.3 us (3.7 TB/s), 24 rows 10.5; one row of 1024, 4096 columns 4.
+// columns 6.3 us (3.7 TB/s), 24 rows 10.5; one row of 1024, 4096 columns 4.  How many rows fit LDS depends on their width (few8_ok, which
+// asks for both ways of sharing columns): 128 of up to 512 values for term weights, 100 of 768, 75 of 1024; 32 of up to 4096 for linear layers.
 constexpr int kFewRows = 128, kFewWaves = 8, kFewLds = 150 * 1024;
 constexpr int kFewPitch = 17;  // of a row of 16 values that an epilogue leaves in LDS
 

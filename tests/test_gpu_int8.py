@@ -213,6 +213,15 @@ def test_int8_linear(device, m, dim, n, dtype, bias_type, out_type):
     assert torch.equal(gs.int8_linear(x, w, bias, dtype=out_type), got)
 
 
+@pytest.mark.parametrize("m,dim,n,dtype", [
+    (32, 4096, 1024, BF16), (33, 4096, 1024, BF16), (31, 4097, 300, F16), (32, 4097, 300, F16), (16, 8192, 130, F32), (17, 8192, 130, F32),
+    (500, 4096, 1024, BF16), (2100, 4096, 4096, BF16), (300, 32768, 260, BF16),
+])
+def test_int8_linear_of_long_rows(device, m, dim, n, dtype):
+    """The second layer of a feed-forward block, and either side of what one launch takes."""
+    test_int8_linear(device, m, dim, n, dtype, BF16, None)
+
+
 @pytest.mark.parametrize("m", [3, 200])
 @pytest.mark.parametrize("kind", ["rows", "columns"])
 def test_int8_linear_reads_any_strides(device, m, kind):
@@ -351,6 +360,14 @@ def test_term_weights_of_a_vocabulary_in_8_bits(device, texts, length, dim, voca
     if mask is not None:                        # what is left out is not looked at, whatever it holds
         assert torch.equal(gs.term_weights(h.masked_fill(~mask[:, :, None], float("nan")), w, None, mask=mask), got)
         assert torch.equal(gs.term_weights(h, w, None, mask=mask.to(torch.int64) * 3), got)
+
+
+@pytest.mark.parametrize("texts,length,dim,vocab", [
+    (128, 1, 512, 300), (1, 120, 513, 300), (1, 121, 513, 300), (20, 5, 768, 30522), (1, 101, 768, 30522), (25, 3, 1024, 500), (2, 38, 1024, 500),
+    (8, 7, 2048, 300), (57, 1, 2048, 300), (2, 16, 4096, 200), (3, 11, 4096, 200),
+])
+def test_term_weights_either_side_of_one_launch(device, texts, length, dim, vocab):
+    test_term_weights_of_a_vocabulary_in_8_bits(device, texts, length, dim, vocab, BF16, "holes")
 
 
 @pytest.mark.parametrize("texts,length", [(3, 5), (3, 40), (9, 8), (4, 40)])

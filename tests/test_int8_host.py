@@ -54,6 +54,33 @@ def test_linear_workspace_and_pointers():
     assert L.gs_int8_linear_workspace(C.byref(linear(rows=5)), C.byref(n)) == _lib.GS_OK and n.value == 0
 
 
+@pytest.mark.parametrize("dim,terms_rows,linear_rows", [
+    (64, 128, 32), (512, 128, 32), (513, 120, 32), (768, 100, 32), (1024, 75, 32), (2048, 56, 32), (4096, 32, 32), (4097, 31, 31), (8192, 16, 16),
+    (32768, 4, 4),
+])
+def test_rows_of_one_launch(dim, terms_rows, linear_rows):
+    """As many as are documented take no workspace, one more does."""
+    L, n, padded = _lib.lib(), C.c_size_t(), -(-dim // 128) * 128
+    for rows, none in ((terms_rows, True), (terms_rows + 1, False)):
+        h = head(texts=1, length=rows, dim=dim, weight_row_stride=padded, hidden_row_stride=dim)
+        assert L.gs_term_weights8_workspace(C.byref(h), C.byref(n)) == _lib.GS_OK and (n.value == 0) == none
+    for rows, none in ((linear_rows, True), (linear_rows + 1, False)):
+        l = linear(rows=rows, dim=dim, x_row_stride=dim, values_stride=padded)
+        assert L.gs_int8_linear_workspace(C.byref(l), C.byref(n)) == _lib.GS_OK and (n.value == 0) == none
+
+
+@pytest.mark.parametrize("vocab,tokens", [(30522, 16384), (1 << 18, 16384), ((1 << 18) + 1, 8192), (1 << 19, 8192), ((1 << 19) + 1, 4096), (1 << 20, 4096)])
+def test_bytes_a_token_of_a_gradient(vocab, tokens):
+    """8 up to a number of tokens that depends on the ids, 16 beyond, besides 4 an id and the parts of sums."""
+    L, n = _lib.lib(), C.c_size_t()
+    for t, each in ((tokens, 8), (tokens + 1, 16)):
+        chunk = 16 if t <= 16384 else 32
+        parts = -(-t // chunk) * 2 * 512 * 4                   # rows of 100 16-bit values, in slices of 512
+        assert L.gs_embed_tokens_grad_workspace(C.byref(lookup(tokens=t, vocab=vocab)), C.byref(n)) == _lib.GS_OK
+        left = n.value - parts - 4 * vocab
+        assert each * t <= left <= each * t + 8192             # a segment's counts, and alignment
+
+
 @pytest.mark.parametrize("args,match", [
     ((8, 7, 3, 100, 100, 1, 16, 128, 8), "unknown type 7"), ((8, 0, -1, 100, 100, 1, 16, 128, 8), "rows"),
     ((8, 0, 3, 0, 100, 1, 16, 128, 8), "dim=0"), ((8, 0, 3, 100, 100, 1, 16, 120, 8), "row stride 120"),
