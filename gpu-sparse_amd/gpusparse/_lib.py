@@ -15,6 +15,7 @@ import torch
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libgpusparse.so")
+AUTOGRAD_PATH = os.path.join(_HERE, "_autograd.so")
 SYNTH_PATH = os.path.join(_HERE, "libgs_synth.so")
 
 GS_OK, GS_EINVAL, GS_EHIP, GS_ENOSPC = 0, 1, 2, 3
@@ -288,6 +289,7 @@ SYNTH_SIGNATURES = {
 
 _lock = threading.Lock()
 _lib = None
+_autograd = None
 _synth = None
 
 
@@ -316,6 +318,28 @@ def lib():
                     raise RuntimeError(f"libgpusparse ABI version {v}, expected {ABI_VERSION}")
                 _lib = L
     return _lib
+
+
+def autograd():
+    """The module of the lookup's autograd node, which calls the same library.  Raises if it has not been built for both."""
+    global _autograd
+    if _autograd is None:
+        lib()
+        with _lock:
+            if _autograd is None:
+                if not os.path.exists(AUTOGRAD_PATH):
+                    raise RuntimeError(f"{AUTOGRAD_PATH} is missing: build it first (make -C gpu-sparse_amd/csrc, or "
+                                       "__graft_entry__.build()).")
+                try:
+                    from . import _autograd as module
+                except ImportError as e:
+                    raise RuntimeError(f"{AUTOGRAD_PATH} does not load with torch {torch.__version__}: build it again "
+                                       "(make -B -C gpu-sparse_amd/csrc)") from e
+                if module.ABI_VERSION != ABI_VERSION or not torch.__version__.startswith(module.TORCH_VERSION):
+                    raise RuntimeError(f"{AUTOGRAD_PATH} is of ABI version {module.ABI_VERSION} and torch {module.TORCH_VERSION}, "
+                                       f"expected {ABI_VERSION} and {torch.__version__}: build it again")
+                _autograd = module
+    return _autograd
 
 
 def synth_lib():

@@ -33,6 +33,11 @@ def _bytes(n: int, dev) -> torch.Tensor:
     return torch.empty(int(n), dtype=torch.uint8, device=dev)
 
 
+def _beyond_reverse_mode() -> bool:
+    return (forward_ad._current_level >= 0 or torch._C._are_functorch_transforms_active()
+            or torch._C._get_tracing_state() is not None)
+
+
 def _differentiable(*inputs) -> bool:
     """Whether a call has to go through autograd: a gradient may be asked for, tensors may carry tangents or belong to a
     functional transform (both of which autograd refuses here), or a trace records it.  One that need not leaves autograd
@@ -41,5 +46,4 @@ def _differentiable(*inputs) -> bool:
         for t in inputs:
             if t is not None and t.requires_grad:
                 return True
-    return (forward_ad._current_level >= 0 or torch._C._are_functorch_transforms_active()
-            or torch._C._get_tracing_state() is not None)
+    return _beyond_reverse_mode()

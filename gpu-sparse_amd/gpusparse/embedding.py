@@ -2,7 +2,7 @@
 
 The matrix is the one that the vocabulary head multiplies with (:mod:`gpusparse.vocab`), where both are tied: autograd adds
 their gradients.  It may be in 8 bits for serving (:class:`gpusparse.Int8Rows`).  Work is queued on the current stream of
-the weight's device.
+the weight's device.  What autograd records is a node in C++ (csrc/gs_autograd.cpp).
 """
 from __future__ import annotations
 
@@ -10,7 +10,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._tensors import _bytes, _check_sizes, _differentiable, _on
+from ._tensors import _beyond_reverse_mode, _check_sizes, _on
 from .int8 import Int8Rows, _gpu, _refuse_gradient
 
 C = _lib.C
@@ -18,67 +18,36 @@ MAX_SCALE = torch.finfo(torch.float32).max
 FEW_TOKENS = 1024  # whose gradient takes no workspace
 
 
-def _lookup(ids, weight, scale: float, padding: int):
-    """The rows, and the C struct of the call."""
-    if isinstance(weight, Int8Rows):
-        table, scales, wtype = weight.values, weight.scales.data_ptr(), _lib.GS_H_I8
-    else:
-        table, scales, wtype = weight, None, _lib.HTYPE_OF_DTYPE[weight.dtype]
-    vocab, dim = table.shape
-    dev = table.device
-    out = table.new_empty((*ids.shape, dim), dtype=weight.dtype)
-    row, value = table.stride()
-    a = _lib.GsLookup(ids.data_ptr(), table.data_ptr(), scales, row, value, ids.numel(), padding, ids.element_size(), wtype,
-                      _lib.HTYPE_OF_DTYPE[weight.dtype], vocab, dim, scale)
+def _lookup8(ids, weight, scale: float):
+    vocab, dim = weight.values.shape
+    dev = weight.values.device
+    out = weight.values.new_empty((*ids.shape, dim), dtype=weight.dtype)
+    row, value = weight.values.stride()
+    a = _lib.GsLookup(ids.data_ptr(), weight.values.data_ptr(), weight.scales.data_ptr(), row, value, ids.numel(), -1, ids.element_size(),
+                      _lib.GS_H_I8, _lib.HTYPE_OF_DTYPE[weight.dtype], vocab, dim, scale)
     with _on(dev):
         _lib.check(_lib.lib().gs_embed_tokens(C.byref(a), out.data_ptr(), _lib.stream_ptr(dev)), "gs_embed_tokens")
-    return out, a
-
-
-def _gradient(ctx, grad):
-    ids, = ctx.saved_tensors
-    a, dev = ctx.lookup, ctx.dev
-    if (ids.data_ptr(), ids.shape, ids.stride(), ids.dtype) != ctx.at:  # hooks on saved tensors may move them, no more
-        if (ids.shape, ids.dtype, ids.device) != (ctx.at[1], ctx.at[3], dev):
-            raise RuntimeError(f"the saved ids came back as {ids.dtype} {tuple(ids.shape)} on {ids.device}")
-        ids = ids.contiguous()
-        a = _lib.GsLookup.from_buffer_copy(a)
-        a.ids_d = ids.data_ptr()
-    row = a.dim
-    if not grad.is_contiguous():
-        grad = grad.reshape(-1, a.dim)
-        if grad.stride(1) != 1:
-            grad = grad.contiguous()
-        row = grad.stride(0)
-    dw = grad.new_empty((a.vocab, a.dim))
-    ws = _bytes(ctx.grad_bytes, dev) if ctx.grad_bytes else None
-    with _on(dev):
-        _lib.check(_lib.lib().gs_embed_tokens_grad(C.byref(a), grad.data_ptr(), row, dw.data_ptr(), _lib.ptr(ws), ctx.grad_bytes,
-                                                   _lib.stream_ptr(dev)), "gs_embed_tokens_grad")
-    return None, dw, None, None
-
-
-_gradient_once = once_differentiable(_gradient)
+    return out
 
 
 class _Embed(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, ids, weight, scale, padding):
-        out, ctx.lookup = _lookup(ids, weight, scale, padding)
-        ctx.grad_bytes = 0
-        if ids.numel() > FEW_TOKENS:
-            need = C.c_size_t()
-            _lib.check(_lib.lib().gs_embed_tokens_grad_workspace(C.byref(ctx.lookup), C.byref(need)), "gs_embed_tokens_grad_workspace")
-            ctx.grad_bytes = need.value
-        ctx.save_for_backward(ids)
-        ctx.at = (ids.data_ptr(), ids.shape, ids.stride(), ids.dtype)
-        ctx.dev = out.device
-        return out
+    """For what knows functions of Python alone: a trace, which records this one, and dual tensors and functional transforms, which
+    refuse it."""
 
     @staticmethod
+    def forward(ctx, ids, weight, scale, padding):
+        ctx.save_for_backward(ids)
+        ctx.call = ids.shape, ids.dtype, weight.device, weight.shape[0], scale, padding
+        return _lib.autograd().embed_tokens(ids, weight, scale, padding)
+
+    @staticmethod
+    @once_differentiable
     def backward(ctx, grad):
-        # what refuses a second derivative has nothing to do where none can be asked for (4 us)
-        return _gradient_once(ctx, grad) if torch.is_grad_enabled() else _gradient(ctx, grad)
+        ids, = ctx.saved_tensors
+        shape, dtype, dev, vocab, scale, padding = ctx.call
+        if (ids.shape, ids.dtype, ids.device) != (shape, dtype, dev):  # hooks on saved tensors may move them, no more
+            raise RuntimeError(f"the saved ids came back as {ids.dtype} {tuple(ids.shape)} on {ids.device}")
+        return None, _lib.autograd().embed_tokens_grad(ids.contiguous(), grad, vocab, scale, padding), None, None
 
 
 def embed_tokens(ids, weight, *, scale: float = 1.0, padding_idx: int | None = None):
@@ -99,16 +68,17 @@ def embed_tokens(ids, weight, *, scale: float = 1.0, padding_idx: int | None = N
     scale = float(scale)
     if not abs(scale) <= MAX_SCALE:
         raise ValueError(f"scale must be finite in float32, got {scale}")
-    if padding_idx is not None and not 0 <= int(padding_idx) < weight.shape[0]:
-        raise ValueError(f"padding_idx must be in [0, {weight.shape[0]}), got {padding_idx}")
-    _check_sizes(ids.numel(), weight.shape[1], weight.shape[0])
-    dev = ids.device
-    if dev.type != "cuda" or weight.device != dev:
-        _gpu(weight, "weight", ids=ids)
+    vocab, dim = weight.shape
     padding = -1 if padding_idx is None else int(padding_idx)
+    if padding_idx is not None and not 0 <= padding < vocab:
+        raise ValueError(f"padding_idx must be in [0, {vocab}), got {padding_idx}")
+    _check_sizes(ids.numel(), dim, vocab)
+    if not ids.is_cuda or weight.device != ids.device:
+        _gpu(weight, "weight", ids=ids)
     ids = ids.contiguous()
     if q8:
         _refuse_gradient()
-    elif _differentiable(weight):
+        return _lookup8(ids, weight, scale)
+    if _beyond_reverse_mode():
         return _Embed.apply(ids, weight, scale, padding)
-    return _lookup(ids, weight, scale, padding)[0]
+    return _lib.autograd().embed_tokens(ids, weight, scale, padding)

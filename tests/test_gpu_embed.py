@@ -314,6 +314,94 @@ def test_functional_transforms_and_forward_mode_are_refused(device):
         torch.vmap(lambda x: gs.int8_linear(x, q))(torch.zeros((3, 2, 4), device=device))
 
 
+class Dropped(torch.autograd.Function):
+    """Passes its input on, and nothing back."""
+
+    @staticmethod
+    def forward(ctx, x):
+        return x.view_as(x)
+
+    @staticmethod
+    def backward(ctx, grad):
+        return None
+
+
+@pytest.mark.parametrize("n", [40, 3000])
+def test_the_node_that_autograd_records(device, n):
+    """It is not a function of Python, whose backward pass waits for the interpreter in autograd's own thread; and hooks, retained
+    gradients, leaves that are left out and accumulation are as with any other."""
+    w = table(200, 16, F32, device).requires_grad_()
+    ids = words((n,), 200, device)
+    grad = torch.randn((n, 16), generator=torch.Generator().manual_seed(3)).to(device)
+    out = gs.embed_tokens(ids, w, scale=0.5, padding_idx=7)
+    assert not isinstance(out.grad_fn, torch.autograd.function.BackwardCFunction) and out.grad_fn.name() == "EmbedTokensBackward"
+    assert out.requires_grad and not out.is_leaf and out.grad_fn.next_functions[0][0].variable is w
+    want, = torch.autograd.grad(out, [w], grad, retain_graph=True)
+    with torch.autograd.set_multithreading_enabled(False):
+        assert torch.equal(torch.autograd.grad(out, [w], grad, retain_graph=True)[0], want)
+    seen = []
+    out.register_hook(lambda g: seen.append(g) or 2 * g)
+    out.retain_grad()
+    w.register_post_accumulate_grad_hook(lambda p: seen.append(p.grad.clone()))
+    out.backward(grad)
+    assert torch.equal(seen[0], grad) and torch.equal(out.grad, 2 * grad) and torch.equal(w.grad, 2 * want) and torch.equal(seen[1], w.grad)
+    with pytest.raises(RuntimeError, match="second time"):
+        out.backward(grad)
+    gs.embed_tokens(ids, w, scale=0.5, padding_idx=7).backward(grad)
+    assert torch.equal(w.grad, 2 * want + want)
+    # the table left out, and another input asked for
+    b = torch.ones(16, device=device, requires_grad=True)
+    rows = gs.embed_tokens(ids, w)
+    assert torch.equal(torch.autograd.grad((rows * b).sum(), [b])[0], (rows.detach()).sum(0))
+    # a table that is not a leaf, a view of one
+    part, = torch.autograd.grad(gs.embed_tokens(ids, (w * 1.0)[:100]), [w], grad)
+    assert torch.equal(part[:100], gradient_of(ids, w.detach()[:100], grad)) and not bool(part[100:].any())
+    # no gradient comes back
+    zero, = torch.autograd.grad(Dropped.apply(gs.embed_tokens(ids, w)).sum() + w.sum() * 0, [w])
+    assert zero.shape == w.shape and not bool(zero.any())
+    for off in (torch.no_grad, torch.inference_mode):
+        with off():
+            plain = gs.embed_tokens(ids, w)
+        assert not plain.requires_grad and torch.equal(plain, rows.detach())
+
+
+def gradient_of(ids, w, grad):
+    w = w.clone().requires_grad_()
+    return torch.autograd.grad(gs.embed_tokens(ids, w), [w], grad)[0]
+
+
+def test_what_is_beyond_first_derivatives_in_reverse_mode(device):
+    w = table(60, 8, F32, device).requires_grad_()
+    ids = words((30,), 60, device)
+    grad = torch.randn((30, 8), generator=torch.Generator().manual_seed(3)).to(device)
+    want = gradient_of(ids, w.detach(), grad)
+    dw, = torch.autograd.grad(gs.embed_tokens(ids, w), [w], grad.clone().requires_grad_(), create_graph=True)
+    assert torch.equal(dw.detach(), want) and dw.requires_grad
+    with pytest.raises(RuntimeError, match="first derivatives only"):
+        dw.sum().backward()
+    dw, = torch.autograd.grad(gs.embed_tokens(ids, w), [w], grad, create_graph=True)
+    assert torch.equal(dw, want) and not dw.requires_grad
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(gs.embed_tokens(ids, w), [w], torch.stack([grad, grad]), is_grads_batched=True)
+    # a dual level without a dual tensor changes nothing
+    with torch.autograd.forward_ad.dual_level():
+        assert torch.equal(torch.autograd.grad(gs.embed_tokens(ids, w), [w], grad)[0], want)
+    # a trace records the call, not its result
+    traced = torch.jit.trace(lambda i, x: gs.embed_tokens(i, x, scale=3.0), (ids, w))
+    other = words((30,), 60, device, seed=9)
+    assert torch.equal(traced(other, w).detach(), looked_up(w, other, 3.0))
+    assert torch.equal(torch.autograd.grad(traced(other, w), [w], grad)[0],
+                       torch.autograd.grad(gs.embed_tokens(other, w, scale=3.0), [w], grad)[0])
+
+
+def test_tables_without_rows_or_values_are_refused(device):
+    ids = torch.zeros(3, dtype=torch.int64, device=device)
+    for shape, match in (((0, 8), "vocab=0"), ((8, 0), "dim=0")):
+        for grad in (False, True):
+            with pytest.raises(ValueError, match=match):
+                gs.embed_tokens(ids, torch.zeros(shape, device=device, requires_grad=grad))
+
+
 def test_two_threads(device):
     import threading
     w = table(400, 32, BF16, device).requires_grad_()

@@ -212,6 +212,23 @@ def test_the_largest_sizes(over):
             gs.embed_tokens(ids, wide(2 ** 20, 2 ** 15))
 
 
+def test_the_autograd_module_is_checked(monkeypatch, tmp_path):
+    """Missing, of another ABI or another torch: told, not passed over."""
+    module = _lib.autograd()
+    assert module.ABI_VERSION == _lib.ABI_VERSION and torch.__version__.startswith(module.TORCH_VERSION)
+    monkeypatch.setattr(_lib, "_autograd", None)
+    for name, value in (("ABI_VERSION", _lib.ABI_VERSION - 1), ("TORCH_VERSION", "1.0.0")):
+        with monkeypatch.context() as m:
+            m.setattr(module, name, value)
+            with pytest.raises(RuntimeError, match="build it again"):
+                _lib.autograd()
+    with monkeypatch.context() as m:
+        m.setattr(_lib, "AUTOGRAD_PATH", str(tmp_path / "none.so"))
+        with pytest.raises(RuntimeError, match="missing: build it first"):
+            _lib.autograd()
+    assert _lib.autograd() is module
+
+
 @pytest.mark.skipif(torch.cuda.is_available(), reason="needs a machine without a GPU")
 def test_without_a_gpu_calls_raise():
     r = gs.Int8Rows(torch.zeros((3, 5), dtype=torch.int8), torch.ones(3))
