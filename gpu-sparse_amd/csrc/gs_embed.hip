@@ -25,8 +25,9 @@ struct Ids {
 // ---------------------------------------------------------------- lookup
 
 // A thread takes U pieces of N values, 256 apart: all ids first, then all rows, so that their loads are on their way together.
-// TAIL: a row's last piece is not whole.  Bytes bound it: 16384 rows of 768 16-bit values 8.6 us, from 8 bits 9.4; 262144 rows of 1024
-// 154 (537 MB written, as many read, a quarter of them from memory).
+// TAIL: a row's last piece is not whole.  Bytes bound it: 16384 rows of 768 16-bit values 8.5 us, from 8 bits 9.0; 262144 rows of 1024,
+// 128003 ids, 170 (537 MB written; of 537 read, 108 of different rows, 329 come from beyond the L2 caches), or 154 where the kernel before
+// it leaves the caches alone.
 template <class T, class O, int N, int U, bool TAIL>
 __global__ __launch_bounds__(256) void k_embed(Ids ids, const T *table, int64_t stride, const float *scales, int vocab, int dim, uint32_t pieces,
                                                int64_t total, float scale, O *out) {
@@ -178,7 +179,8 @@ __device__ __forceinline__ int block_prefix(int *x, int n, int *wave_sums) {
     return total;
 }
 
-// A segment's tokens sorted by range, in order within a range.  pos[segment]: token; low[segment]: the id's bits within its range; counts[range][segment], begin[range][segment].
+// A segment's tokens sorted by range, in order within a range.  pos[segment]: token; low[segment]: the id's bits within its range;
+// counts[range][segment], begin[range][segment].
 __global__ __launch_bounds__(kSplitThreads) void k_split(Tokens t, int64_t seg_size, int segs, uint32_t *pos, uint16_t *low, int *counts,
                                                          int *begin) {
     __shared__ int count[kSplitWaves][kRanges], first[kRanges], wave_sums[kSplitWaves];
@@ -382,7 +384,7 @@ __global__ __launch_bounds__(1024) void k_order(Tokens t, int64_t seg_size, int 
 // part[chunk][1] of the one that started here.  More waves write the zeros of ids without an entry.
 //
 // STREAM: rows are read past the caches.  Each is read once, so that those that do not fit the 256 MiB of the last of them only
-// throw others out: 262144 rows of 1024 16-bit values 187 -> 157 us (5.1 TB/s), of which a lookup after it gives back 15; but 16384
+// throw others out: 262144 rows of 1024 16-bit values 187 -> 160 us (5.1 TB/s), of which a lookup after it gives back 15; but 16384
 // of 768, which are still there from what made them, 17 -> 22.
 constexpr int kZeroRows = 16;
 constexpr int64_t kStreamBytes = 256 << 20;

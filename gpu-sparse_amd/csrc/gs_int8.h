@@ -344,7 +344,13 @@ int launch_few8(const Source &h, const uint8_t *mask, int rows, const Weight8 &W
     GS_CHECK_LAUNCH();
     return GS_OK;
 }
-// A block of columns is shared by a workgroup's waves where there would be too few of them for the GPU otherwise.
+// A block of columns is shared by a workgroup's waves where there would be too few of them for the GPU otherwise, below 16384 columns on
+// 256 CUs.  us, shared and not:
+//   columns                     1024        8192       12288       16384       20480       30522
+//   linear, 1 x 768         3.7   5.5   4.6   5.8   5.4   5.8   6.2   5.9   7.0   5.9   9.5   5.9
+//   1 x 1024                3.7   6.2   4.7   6.4   5.4   6.5   6.3   6.5   7.1   6.7  10.0   6.8
+//   32 x 768                8.1  10.5   9.6  10.9  10.7  11.0  11.9  11.0  13.1  11.0  17.1  11.5
+//   term weights, 24 x 768  8.0  10.1   9.8  10.4  11.4  10.5  13.0  10.5  14.8  10.5  19.4  10.5
 template <class T, class Epi>
 int launch_few8(const Source &h, const uint8_t *mask, int rows, const Weight8 &W, int kp, const Epi &epi, int cus, hipStream_t s) {
     const bool split = (int64_t)W.n < (int64_t)64 * cus;

@@ -813,7 +813,17 @@ struct EpiHiddenPart {
 // whose maxima are joined across lanes and written seven times a wave: 1280 rows 67 us (890).
 //
 // Q8: operands in 8 bits.  Sums take their row's scale before they are compared, their column's magnitude after (in_order): 10240 rows, 30522 terms, 768
-// values 201 us (2390 TOP/s, what a library product of 16384^3 reaches).
+// values 201 us (2390 TOP/s, what a library product of 16384^3 reaches; the matrix units are busy half of that time).  Tiles are chosen as
+// for 16 bits (class_of); us for terms in 30522 columns of 768, by the edge of a tile's rows:
+//   rows                   32    64    80   128   160   256   320   512   768
+//   texts of 16    64    18.0  18.3  20.2  20.7  24.8  29.0  33.2  42.5  57.9
+//                 128    19.1  20.0  20.1  20.9  21.6  22.5  30.4  31.8  40.5
+//                 256    22.3  23.1  23.5  24.5  24.7  27.0  27.9  29.8  42.7
+//              k_few8    12.8  19.6  25.8
+//   texts of 4     64    20.6  21.9  25.4  27.0  32.9  39.9  46.4  60.8  85.2
+//                 128    20.9  24.1  24.7  28.2  29.9  32.9  45.0  47.9  63.5
+//                 256    23.8  27.0  28.6  33.4  34.4  41.3  42.6  46.2  69.6
+//              k_few8    12.3  20.4  25.4
 template <bool TOK, bool Q8 = false>
 struct EpiTextMax {
     const float *bias;
@@ -1355,8 +1365,9 @@ __global__ __launch_bounds__(256, 2) void k_few_rows(Source h, const uint8_t *ma
 }
 
 // What k_few8 makes of a block's sums for texts.  The logits but for their column's scale go to LDS, since a text's rows lie in any
-// lanes: then a row of lanes takes a text (of four or more), or a fourth of its rows.  (21 texts of 3 tokens of 170 fp32 values, 11762 terms: 21 us, 44 with maxima taken from registers
-// text by text; 69 of one token of 512, 27652 terms: 27, and 57 as tiles in three launches; one of 24, 768, 30522: 11.5.)
+// lanes: then a row of lanes takes a text (of four or more), or a fourth of its rows.  (21 texts of 3 tokens of 170 fp32 values, 11762
+// terms: 20 us, 44 with maxima taken from registers text by text; 69 of one token of 512, 27652 terms: 27, and 57 as tiles in three
+// launches; one of 24, 768, 30522: 11.)
 struct EpiFewTerms {
     const void *bias;
     int bias_type, texts, length;

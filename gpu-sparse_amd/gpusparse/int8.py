@@ -41,8 +41,8 @@ def _in_place(values: torch.Tensor) -> bool:
 
 class Int8Rows:
     """A matrix [rows, dim] in 8 bits: ``values`` int8 [rows, dim], ``scales`` float32 [rows], and ``dtype``, the type it
-    came from, which lookups give back.  Scales may have either sign.  Values that are not laid out as the kernels read
-    them (rows padded to 128 bytes) are copied once, here."""
+    came from, which lookups give back.  Scales may have either sign; a gradient that they ask for is left out.  Values
+    that are not laid out as the kernels read them (rows padded to 128 bytes, less than 2**20 bytes apart) are copied once, here."""
 
     def __init__(self, values: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = torch.bfloat16):
         if not isinstance(values, torch.Tensor) or values.dtype != torch.int8 or values.dim() != 2:
